@@ -35,6 +35,7 @@ extern "C" {
 #define TGS_DTYPE_FLOAT32 0
 #define TGS_DTYPE_FLOAT16 1
 #define TGS_DTYPE_UINT8 2   /* images only: tgs_image_* and tgs_convert */
+#define TGS_DTYPE_BFLOAT16 3   /* matrices (tgs_matrix) only */
 
 /* SoA Gaussian parameters (or their gradients), as GPUGaussian3d
  * (tinygs/include/tinygs/core/gpu_gaussian.hpp:9-73): means[3n], scales[3n]
@@ -471,6 +472,111 @@ int tgs_image_to_hwc_u8(const void* src, int32_t src_dtype, uint32_t width, uint
 /* Elementwise: half_to_float_gpu / float_to_half_gpu (image_format.cu:117-139),
  * convert_u8_float / convert_u8_half (dataloader.cu:26-95), and u8 <- float. */
 int tgs_convert(const void* src, int32_t src_dtype, void* dst, int32_t dst_dtype, int64_t n, void* stream);
+
+/* ---- attribute network: the operators of a network that maps per-Gaussian
+ * features to Gaussian attributes, and of its training. No counterpart in the
+ * reference.
+ *
+ * A tgs_matrix is `rows` rows of `cols` elements of dtype (TGS_DTYPE_FLOAT32,
+ * _FLOAT16 or _BFLOAT16), a row's elements next to each other and row r at
+ * data + r * stride elements (stride >= cols, below 2^21; rows below 2^31).
+ * data is aligned to its element. The elements between cols and stride are
+ * neither read into a result nor written. Vectors (bias, gamma, beta, their
+ * gradients, means and reciprocal deviations) are packed float32.
+ * The matrices of one call are of one dtype. Products and sums are held in
+ * 32 bits; every stored element is rounded once to its dtype.
+ * An output may not overlap an input unless its entry says so.
+ * A call reads and writes nothing after its last kernel on `stream`; it does
+ * not wait for the device, except to grow the handle's workspace. The
+ * workspace is shared by the calls on a handle: calls on one handle run on one
+ * stream, or the caller orders them. A captured call must not grow it: run one
+ * with the same sizes before capturing. */
+typedef struct tgs_matrix {
+    void* data;
+    int64_t rows;
+    int64_t cols;
+    int64_t stride;
+    int32_t dtype;
+} tgs_matrix;
+typedef struct tgs_network tgs_network;
+typedef struct tgs_muon tgs_muon;
+
+#define TGS_ACTIVATION_NONE 0
+#define TGS_ACTIVATION_RELU 1
+#define TGS_ACTIVATION_SILU 2   /* z / (1 + exp(-z)) */
+#define TGS_ACTIVATION_GELU 3   /* z / 2 (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+
+/* A handle owns the workspace of the layer operators. */
+int tgs_network_create(tgs_network** out);
+int tgs_network_destroy(tgs_network* n);
+/* z = x w^T + bias, y = act(z) + residual. x [rows, in], w [out, in]; bias
+ * [out], residual [rows, out] and preact [rows, out] (receives z) may be NULL.
+ * y may be residual's own matrix. */
+int tgs_linear_forward(tgs_network* n, const tgs_matrix* x, const tgs_matrix* w, const float* bias,
+                       int32_t activation, const tgs_matrix* residual, const tgs_matrix* preact, const tgs_matrix* y,
+                       void* stream);
+/* The gradients of tgs_linear_forward for grad_y = dL/dy: with
+ * dz = grad_y act'(z), grad_x = dz w, grad_w = dz^T x and grad_bias = the
+ * column sums of dz; the residual's gradient is grad_y itself. preact is the
+ * forward's z (may be NULL for TGS_ACTIVATION_NONE). Each of grad_x, grad_w
+ * and grad_bias is assigned, or left out when NULL. For 16-bit matrices and an
+ * activation, dz is rounded to the dtype ahead of the two products (its column
+ * sums are not). The sums over the rows run in an order that depends on the
+ * sizes alone: the same inputs give the same bits. */
+int tgs_linear_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_matrix* x, const tgs_matrix* w,
+                        const tgs_matrix* preact, int32_t activation, const tgs_matrix* grad_x,
+                        const tgs_matrix* grad_w, float* grad_bias, void* stream);
+/* y = (x - mean) rstd gamma + beta over each row's cols elements, with
+ * rstd = 1 / sqrt(variance + epsilon) and the variance over cols. gamma, beta
+ * [cols] may be NULL (one, zero); mean and rstd [rows] are written when not
+ * NULL. y may be x's own matrix. */
+int tgs_layer_norm_forward(tgs_network* n, const tgs_matrix* x, const float* gamma, const float* beta, float epsilon,
+                           const tgs_matrix* y, float* mean, float* rstd, void* stream);
+/* The gradients of tgs_layer_norm_forward from its mean and rstd: with
+ * h = (x - mean) rstd and g = grad_y gamma, grad_x = rstd (g - avg(g) -
+ * h avg(g h)) + residual_grad (may be NULL: the gradient that reaches x by
+ * another path), grad_gamma = the column sums of grad_y h, grad_beta those of
+ * grad_y. Outputs are assigned, or left out when NULL. grad_x may be grad_y's
+ * or residual_grad's own matrix. Sums in a fixed order. */
+int tgs_layer_norm_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_matrix* x, const float* gamma,
+                            const float* mean, const float* rstd, const tgs_matrix* residual_grad,
+                            const tgs_matrix* grad_x, float* grad_gamma, float* grad_beta, void* stream);
+
+/* ---- Muon: the optimiser of the network's matrices. A step, for each matrix
+ * W [rows, cols] with momentum M and gradient G (s = scale):
+ *   M <- mu M + (1 - mu) s G;  U = (1 - mu) s G + mu M (nesterov), or M
+ *   X = U / max(|U|, epsilon), |.| the root of the sum of squares
+ *   iterations times: A = X X^T, X <- a X + (b A + c A^2) X
+ *   W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) X
+ * with a, b, c = 3.4445, -4.7750, 2.0315, which bring the singular values of X
+ * near one.
+ * lr is params.lr times the learning rate of tgs_muon_set_lr (1 at creation). */
+typedef struct tgs_muon_params {
+    float lr;             /* 0.02 at creation */
+    float momentum;       /* 0.95 */
+    float weight_decay;   /* 0 */
+    float epsilon;        /* 1e-12 */
+    int32_t nesterov;     /* 1 */
+    int32_t iterations;   /* 5; 0 to 32 */
+} tgs_muon_params;
+/* weights, momenta: float32 matrices, updated in place; grads: of one dtype;
+ * copies (NULL, or one per matrix): matrices of one dtype that receive the
+ * updated weights rounded to it. All of the matrix's shape, none empty, no two
+ * of them overlapping. The pointers are kept. */
+int tgs_muon_create(const tgs_matrix* weights, const tgs_matrix* grads, const tgs_matrix* momenta,
+                    const tgs_matrix* copies, int32_t count, tgs_muon** out);
+int tgs_muon_destroy(tgs_muon* m);
+/* Rebinds the pointers; count, shapes and dtypes as at creation. Waits for the
+ * device. */
+int tgs_muon_set_matrices(tgs_muon* m, const tgs_matrix* weights, const tgs_matrix* grads, const tgs_matrix* momenta,
+                          const tgs_matrix* copies, int32_t count);
+int tgs_muon_set_params(tgs_muon* m, const tgs_muon_params* p);
+int tgs_muon_get_params(tgs_muon* m, tgs_muon_params* p);
+int tgs_muon_set_lr(tgs_muon* m, float global_lr);
+float tgs_muon_get_lr(tgs_muon* m);
+int tgs_muon_step(tgs_muon* m, float scale, void* stream);
+/* Zero momenta, as after creation with zero ones. */
+int tgs_muon_reset(tgs_muon* m, void* stream);
 
 /* ---- measurement (no counterpart in the reference, which uses NVTX ranges,
  * tinygs/src/rasterizer/fastgs_ours/nvtx_gs.h): HIP events recorded on the

@@ -9,6 +9,11 @@ mirrors tinygs's plugin interfaces on top of it:
   create_loss("l1" | "fused_ssim")                  (loss.cu:13-27)
   create_optimizer("simple_adam", params, grads)    (optim.cu:86-105)
 
+and adds the operators of a network whose outputs are Gaussian attributes:
+
+  LayerOps, AttributeNetwork                        (linear layers, layer norm)
+  create_optimizer("muon", matrices, grads)
+
 Importing the package does not load the library; the first rasterizer /
 loss / optimizer call does, and raises if it has not been built.
 """
@@ -29,7 +34,10 @@ def __getattr__(name):
     if name in ("L1Loss", "FusedSSIMLoss", "LossBase", "create_loss"):
         from . import loss
         return getattr(loss, name)
-    if name in ("SimpleAdam", "OptimizerBase", "create_optimizer"):
+    if name in ("LayerOps", "AttributeNetwork"):
+        from . import network
+        return getattr(network, name)
+    if name in ("SimpleAdam", "Muon", "OptimizerBase", "create_optimizer"):
         from . import optim
         return getattr(optim, name)
     if name in ("GPUGaussian3d", "Image", "GPUBatchInput", "GPUBatchOutput", "RasterizeContext", "LossContext",

@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(HERE, "libtinygs_amd.so")
 TGS_DTYPE_FLOAT32 = 0
 TGS_DTYPE_FLOAT16 = 1
 TGS_DTYPE_UINT8 = 2
+TGS_DTYPE_BFLOAT16 = 3
 TGS_ADAM_DEVICE_STEP = 1
 TGS_ADAM_ROWS_UNMARKED = 2
 TGS_ADAM_ROWS_MARKED = 4
@@ -27,6 +28,10 @@ TGS_BACKWARD_SPARSE = 2
 TGS_BACKWARD_POSE = 4
 TGS_BACKWARD_KEEP_2D = 8
 TGS_FORWARD_NO_SYNC = 1
+TGS_ACTIVATION_NONE = 0
+TGS_ACTIVATION_RELU = 1
+TGS_ACTIVATION_SILU = 2
+TGS_ACTIVATION_GELU = 3
 TGS_OK = 0
 TGS_ERR_INVALID = 1
 TGS_ERR_HIP = 2
@@ -81,8 +86,19 @@ class tgs_ply_info(C.Structure):
                 ("has_colors", C.c_int32)]
 
 
+class tgs_matrix(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("stride", C.c_int64),
+                ("dtype", C.c_int32)]
+
+
+class tgs_muon_params(C.Structure):
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("epsilon", C.c_float),
+                ("nesterov", C.c_int32), ("iterations", C.c_int32)]
+
+
 P = C.c_void_p
 PP = C.POINTER(C.c_void_p)
+MP = C.POINTER(tgs_matrix)
 
 SIGNATURES = {
     "tgs_last_error": ([], C.c_char_p),
@@ -145,6 +161,21 @@ SIGNATURES = {
     "tgs_image_from_hwc_u8": ([P, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int32, P, C.c_int32, P], C.c_int),
     "tgs_image_to_hwc_u8": ([P, C.c_int32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int32, P, P], C.c_int),
     "tgs_convert": ([P, C.c_int32, P, C.c_int32, C.c_int64, P], C.c_int),
+    "tgs_network_create": ([PP], C.c_int),
+    "tgs_network_destroy": ([P], C.c_int),
+    "tgs_linear_forward": ([P, MP, MP, P, C.c_int32, MP, MP, MP, P], C.c_int),
+    "tgs_linear_backward": ([P, MP, MP, MP, MP, C.c_int32, MP, MP, P, P], C.c_int),
+    "tgs_layer_norm_forward": ([P, MP, P, P, C.c_float, MP, P, P, P], C.c_int),
+    "tgs_layer_norm_backward": ([P, MP, MP, P, P, P, MP, MP, P, P, P], C.c_int),
+    "tgs_muon_create": ([MP, MP, MP, MP, C.c_int32, PP], C.c_int),
+    "tgs_muon_destroy": ([P], C.c_int),
+    "tgs_muon_set_matrices": ([P, MP, MP, MP, MP, C.c_int32], C.c_int),
+    "tgs_muon_set_params": ([P, C.POINTER(tgs_muon_params)], C.c_int),
+    "tgs_muon_get_params": ([P, C.POINTER(tgs_muon_params)], C.c_int),
+    "tgs_muon_set_lr": ([P, C.c_float], C.c_int),
+    "tgs_muon_get_lr": ([P], C.c_float),
+    "tgs_muon_step": ([P, C.c_float, P], C.c_int),
+    "tgs_muon_reset": ([P, P], C.c_int),
     "tgs_profiling_set": ([C.c_uint32], C.c_int),
     "tgs_profiling_read": ([C.c_int32, C.POINTER(C.c_double), C.POINTER(C.c_int64), C.c_int32], C.c_int),
     "tgs_stage_name": ([C.c_int32], C.c_char_p),

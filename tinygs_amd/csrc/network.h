@@ -1,0 +1,153 @@
+// What the attribute network's operators share: element types, activations,
+// matrix views and the launchers of linear.hip, layer_norm.hip and muon.hip.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "status.h"
+
+namespace tgs {
+
+// A matrix of a launch: row r at p + r * stride, `cols` elements.
+struct Mat {
+    void* p = nullptr;
+    int64_t rows = 0;
+    int64_t cols = 0;
+    int64_t stride = 0;
+};
+
+template <class T>
+struct Elem;
+template <>
+struct Elem<float> {
+    static constexpr int kDtype = TGS_DTYPE_FLOAT32;
+};
+template <>
+struct Elem<_Float16> {
+    static constexpr int kDtype = TGS_DTYPE_FLOAT16;
+};
+template <>
+struct Elem<__bf16> {
+    static constexpr int kDtype = TGS_DTYPE_BFLOAT16;
+};
+
+// Calls f with a value of the element type / with an integral constant.
+template <class F>
+void by_dtype(int dtype, F f) {
+    if (dtype == TGS_DTYPE_FLOAT32) f(float{});
+    else if (dtype == TGS_DTYPE_FLOAT16) f(_Float16{});
+    else f(__bf16{});
+}
+template <int N>
+struct Constant {
+    static constexpr int value = N;
+};
+template <class F>
+void by_activation(int activation, F f) {
+    if (activation == 1) f(Constant<1>{});
+    else if (activation == 2) f(Constant<2>{});
+    else if (activation == 3) f(Constant<3>{});
+    else f(Constant<0>{});
+}
+
+enum Activation { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
+
+// logistic(v) = 1 / (1 + 2^(-v log2 e)). The exponent's rounding error, up to
+// 2^-24 |v log2 e|, is put back to first order (2^(t + d) = 2^t (1 + d ln 2)),
+// so the result is good to a few units of the last place for every v. Where
+// 2^-t overflows the reciprocal is 0, the limit.
+__device__ __forceinline__ float logistic(float v) {
+    constexpr float kLog2e = 0x1.715476p+0f;        // log2(e) = kLog2e + kLog2eTail
+    constexpr float kLog2eTail = 0x1.4ae0bep-26f;
+    constexpr float kLn2 = 0x1.62e430p-1f;
+    const float t = -v * kLog2e;
+    const float d = fmaf(-v, kLog2e, -t) - v * kLog2eTail;
+    float e = __builtin_amdgcn_exp2f(t);
+    const float c = e * (d * kLn2);
+    e = fabsf(t) < 126.0f ? e + c : e;
+    return __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+constexpr float kGelu1 = 1.5957691216057308f;    // 2 sqrt(2 / pi): 1 + tanh(u) = 2 logistic(2 u)
+constexpr float kGelu3 = 0.071354816272600256f;  // 2 sqrt(2 / pi) 0.044715
+
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == kActRelu) return z < 0.0f ? 0.0f : z;   // NaN stays NaN
+    if constexpr (ACT == kActSilu) return z * logistic(z);
+    if constexpr (ACT == kActGelu) return z * logistic(z * fmaf(kGelu3 * z, z, kGelu1));
+    return z;
+}
+
+// act'(z) = p + z p (1 - p) (d/dz of p's argument). The second term is zero in
+// 32 bits well inside the clamps, which keep it from becoming 0 * infinity.
+template <int ACT>
+__device__ __forceinline__ float activate_slope(float z) {
+    if constexpr (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
+    if constexpr (ACT == kActSilu) {
+        const float p = logistic(z);
+        const float c = fminf(fmaxf(z, -100.0f), 100.0f);
+        return fmaf(c * p, 1.0f - p, p);
+    }
+    if constexpr (ACT == kActGelu) {
+        const float c = fminf(fmaxf(z, -30.0f), 30.0f);
+        const float p = logistic(z * fmaf(kGelu3 * z, z, kGelu1));
+        return fmaf(c * p * (1.0f - p), fmaf(3.0f * kGelu3 * c, c, kGelu1), p);
+    }
+    return 1.0f;
+}
+
+// ---- linear.hip
+struct LinearForward {
+    Mat x, w, residual, preact, y;   // residual.p, preact.p may be NULL
+    const float* bias;               // may be NULL
+    int activation;
+    int dtype;
+};
+struct LinearBackward {
+    Mat grad_y, x, w, preact, grad_x, grad_w;   // grad_x.p, grad_w.p may be NULL
+    float* grad_bias;                           // may be NULL
+    int activation;
+    int dtype;
+};
+size_t linear_backward_workspace(const LinearBackward& a);
+int launch_linear_forward(const LinearForward& a, hipStream_t s);
+int launch_linear_backward(const LinearBackward& a, void* workspace, hipStream_t s);
+
+// ---- layer_norm.hip
+struct LayerNormForward {
+    Mat x, y;
+    const float *gamma, *beta;   // may be NULL
+    float eps;
+    float *mean, *rstd;          // may be NULL
+    int dtype;
+};
+struct LayerNormBackward {
+    Mat grad_y, x, residual, grad_x;            // residual.p, grad_x.p may be NULL
+    const float *gamma, *mean, *rstd;           // gamma may be NULL
+    float *grad_gamma, *grad_beta;              // may be NULL
+    int dtype;
+};
+size_t layer_norm_backward_workspace(const LayerNormBackward& a);
+int launch_layer_norm_forward(const LayerNormForward& a, hipStream_t s);
+int launch_layer_norm_backward(const LayerNormBackward& a, void* workspace, hipStream_t s);
+
+// ---- muon.hip
+constexpr float kNewtonSchulzA = 3.4445f, kNewtonSchulzB = -4.7750f, kNewtonSchulzC = 2.0315f;
+
+struct MuonMatrix {
+    Mat w, g, m, c;   // weights, gradient, momentum, copy (c.p may be NULL)
+};
+struct MuonStep {
+    float momentum, grad_scale;   // grad_scale = (1 - momentum) scale
+    float keep, lr;               // 1 - lr weight_decay; lr
+    float epsilon;
+    int nesterov, iterations;
+    int grad_dtype, copy_dtype;
+};
+size_t muon_workspace(const MuonMatrix* mats, int count);
+int launch_muon_step(const MuonMatrix* mats, int count, const MuonStep& p, void* workspace, hipStream_t s);
+int launch_zero_matrix(const Mat& m, hipStream_t s);
+
+}  // namespace tgs

@@ -1,4 +1,4 @@
-"""SimpleAdam over the C ABI.
+"""SimpleAdam, and Muon for an attribute network's matrices, over the C ABI.
 
 Mirrors tinygs's OptimizerBase / SimpleAdam / create_optimizer
 (tinygs/include/tinygs/optim/optim.hpp:39-106,
@@ -169,8 +169,102 @@ class SimpleAdam(OptimizerBase):
         return m1, m2
 
 
-def create_optimizer(optimizer_type: str, gaussians: GPUGaussian3d, gaussians_grad: GPUGaussian3d):
+class Muon:
+    """Muon on a network's matrices: momentum, the update orthogonalised by Newton-Schulz products, decoupled weight
+    decay. weights and momenta (zeros when not given) are float32 and updated in place; grads are of one dtype;
+    copies, when given, receive the updated weights rounded to their dtype (the network's half-precision matrices).
+    The tensors are kept: a step reads what they hold then. Steps run on one stream, or the caller orders them."""
+
+    def __init__(self, weights, grads, momenta=None, copies=None):
+        self._lib = _lib.load()
+        self._h = None
+        count = len(weights)
+        if momenta is None:
+            torch = __import__("torch")
+            momenta = [torch.zeros(w.shape, dtype=torch.float32, device=w.device) for w in weights]
+        if len(grads) != count or len(momenta) != count or (copies is not None and len(copies) != count):
+            raise RuntimeError("Muon: weights, grads, momenta and copies must have the same count")
+        self.m_weights, self.m_grads, self.m_momenta = list(weights), list(grads), list(momenta)
+        self.m_copies = None if copies is None else list(copies)
+        h = C.c_void_p()
+        _lib.check(self._lib.tgs_muon_create(*self._arrays(), count, C.byref(h)), "create_optimizer")
+        self._h = h
+
+    def _arrays(self):
+        from .network import matrix
+
+        def array(tensors, name):
+            if tensors is None:
+                return None
+            return (_lib.tgs_matrix * len(tensors))(*[matrix(t, f"{name}[{i}]") for i, t in enumerate(tensors)])
+
+        return (array(self.m_weights, "weights"), array(self.m_grads, "grads"), array(self.m_momenta, "momenta"),
+                array(self.m_copies, "copies"))
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            try:
+                self._lib.tgs_muon_destroy(h)
+            except Exception:
+                pass
+            self._h = None
+
+    def get_weights(self):
+        return self.m_weights
+
+    def get_grads(self):
+        return self.m_grads
+
+    def momenta(self):
+        return self.m_momenta
+
+    def set_grads(self, grads):
+        """Other gradient tensors of the same shapes and dtype. Waits for the device."""
+        if len(grads) != len(self.m_weights):
+            raise RuntimeError("Muon: weights and grads must have the same count")
+        kept, self.m_grads = self.m_grads, list(grads)
+        try:
+            _lib.check(self._lib.tgs_muon_set_matrices(self._h, *self._arrays(), len(grads)), "Muon::set_grads")
+        except Exception:
+            self.m_grads = kept
+            raise
+
+    def step(self, scale: float, stream=None):
+        """One step on gradients multiplied by scale."""
+        _lib.check(self._lib.tgs_muon_step(self._h, float(scale), stream_ptr(stream)), "Muon::step")
+
+    def reset(self, stream=None):
+        _lib.check(self._lib.tgs_muon_reset(self._h, stream_ptr(stream)), "Muon::reset")
+
+    def set_lr(self, lr: float):
+        _lib.check(self._lib.tgs_muon_set_lr(self._h, float(lr)), "set_lr")
+
+    def get_lr(self) -> float:
+        return float(self._lib.tgs_muon_get_lr(self._h))
+
+    def get_params(self) -> dict:
+        p = _lib.tgs_muon_params()
+        _lib.check(self._lib.tgs_muon_get_params(self._h, C.byref(p)), "get_params")
+        return {f: getattr(p, f) for f, _ in p._fields_}
+
+    def set_params(self, config: dict):
+        p = _lib.tgs_muon_params()
+        _lib.check(self._lib.tgs_muon_get_params(self._h, C.byref(p)), "get_params")
+        alias = {"eps": "epsilon"}
+        for k, v in config.items():
+            k = alias.get(k, k)
+            if not hasattr(p, k):
+                raise RuntimeError(f"Muon: unknown parameter {k}")
+            setattr(p, k, int(v) if k in ("nesterov", "iterations") else float(v))
+        _lib.check(self._lib.tgs_muon_set_params(self._h, C.byref(p)), "set_params")
+
+
+def create_optimizer(optimizer_type: str, gaussians, gaussians_grad):
+    """"simple_adam" on Gaussians and their gradients, or "muon" on lists of matrices and of theirs."""
     t = optimizer_type.lower()
     if t == "simple_adam":
         return SimpleAdam(gaussians, gaussians_grad)
+    if t == "muon":
+        return Muon(gaussians, gaussians_grad)
     raise RuntimeError(f"Unknown optimizer type: {optimizer_type}")
