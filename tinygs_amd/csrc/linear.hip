@@ -1,135 +1,339 @@
-// Linear layers: y = act(x w^T + bias) + residual and its gradients.
+// Linear layers: z = x w^T + bias, y = act(z) + residual, and their gradients
+// dx = dz w, dw = dz^T x, db = the column sums of dz, dz = dy act'(z).
 //
-// One tiled product serves all three: C(i, j) = sum over k of A(i, k) B(j, k)
-// with the operands read through strides, 64 x 64 outputs and 16 of k per step,
-// 4 x 4 outputs per thread, products and sums in float.
-#include "network.h"
+// The three products are tiles of mfma_tile.h with the contiguous axis of the
+// output as i. Forward: A = w, B = x, both K-contiguous, bias, activation and
+// residual on the sums. dx: A = w R-contiguous, B = dz. dw: A = x, B = dz, both
+// R-contiguous; its long axis (the rows) is split over workgroups whose float
+// sums a second kernel joins in order. An activation's dz is written once, by
+// the pass that also sums its columns, and read by both products.
+#include "mfma_tile.h"
 
 namespace tgs {
 
 namespace {
 
-constexpr int kTileEdge = 64;
-constexpr int kDepth = 16;
-
-// An operand element (r, k) at p + r * sr + k * sk; with a second array (z of
-// the same strides) it is p's element times act'(z's).
-struct Operand {
-    const void* p;
-    const void* z;
-    int64_t sr, sk;
-    int64_t r_size;
+template <class T>
+struct Packed {   // 8 elements of a row, at any element's address
+    typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
-template <class T, int ACT>
-__device__ __forceinline__ float operand_at(const Operand& o, int64_t r, int64_t k, int64_t k_size) {
-    if (r >= o.r_size || k >= k_size) return 0.0f;
-    const float v = (float)((const T*)o.p)[r * o.sr + k * o.sk];
-    if constexpr (ACT != kActNone) return v * activate_slope<ACT>((float)((const T*)o.z)[r * o.sr + k * o.sk]);
-    return v;
-}
-
-struct Epilogue {
-    const float* bias;   // per j
-    Mat residual, preact, y;
-};
-
-// ACT applies to the output; ACT_A to operand A (its slope).
-template <class T, int ACT, int ACT_A>
-__global__ void __launch_bounds__(256) product_kernel(Operand a, Operand b, int64_t k_size, Epilogue e) {
-    __shared__ float sa[kDepth][kTileEdge + 4], sb[kDepth][kTileEdge + 4];
-    const int t = threadIdx.x, ti = t >> 4, tj = t & 15;
-    const int64_t i0 = (int64_t)blockIdx.x * kTileEdge, j0 = (int64_t)blockIdx.y * kTileEdge;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < k_size; k0 += kDepth) {
-        for (int q = t; q < kTileEdge * kDepth; q += 256) {
-            const int r = q / kDepth, k = q % kDepth;
-            float v = operand_at<T, ACT_A>(a, i0 + r, k0 + k, k_size);
-            if constexpr (ACT_A != kActNone) v = (float)(T)v;
-            sa[k][r] = v;
-            sb[k][r] = operand_at<T, kActNone>(b, j0 + r, k0 + k, k_size);
-        }
-        __syncthreads();
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+    if (n >= 8) {
+        const auto u = *(const typename Packed<T>::type*)p;
 #pragma unroll
-        for (int k = 0; k < kDepth; ++k)
-            for (int u = 0; u < 4; ++u)
-                for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(sa[k][ti * 4 + u], sb[k][tj * 4 + v], acc[u][v]);
-        __syncthreads();
+        for (int e = 0; e < 8; ++e) v[e] = (float)u[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < n ? (float)p[e] : 0.0f;
     }
-    for (int u = 0; u < 4; ++u)
-        for (int v = 0; v < 4; ++v) {
-            const int64_t i = i0 + ti * 4 + u, j = j0 + tj * 4 + v;
-            if (i >= e.y.rows || j >= e.y.cols) continue;
-            float z = acc[u][v] + (e.bias ? e.bias[j] : 0.0f);
-            if (e.preact.p) ((T*)e.preact.p)[i * e.preact.stride + j] = (T)z;
-            z = activate<ACT>(z);
-            if (e.residual.p) z += (float)((const T*)e.residual.p)[i * e.residual.stride + j];
-            ((T*)e.y.p)[i * e.y.stride + j] = (T)z;
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
+    if (n >= 8) {
+        typename Packed<T>::type u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = (T)v[e];
+        *(typename Packed<T>::type*)p = u;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < n) p[e] = (T)v[e];
+    }
+}
+
+// Calls f(i, j, n, v) for each run of 8 outputs (i .. i + 7, j) that a lane
+// holds; n of them exist.
+template <class Shape, int TI, int TJ, class F>
+__device__ __forceinline__ void for_outputs(const f32x4 (&acc)[TI][TJ], int64_t i0, int64_t j0, int64_t ni, int64_t nj,
+                                            F f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wi = wave / Shape::kWavesJ, wj = wave % Shape::kWavesJ;
+#pragma unroll
+    for (int u = 0; u < TI; u += 2) {
+        const int64_t i = i0 + (wi * TI + u) * 16 + neighbours_at(lane);
+#pragma unroll
+        for (int t = 0; t < TJ; ++t) {
+            const int64_t j = j0 + (wj * TJ + t) * 16 + (lane & 15);
+            float v[8];
+            neighbours(acc[u][t], acc[u + 1][t], v);
+            if (i < ni && j < nj) f(i, j, (int)(ni - i < 8 ? ni - i : 8), v);
         }
+    }
 }
 
-template <class T, int ACT>
-__global__ void __launch_bounds__(256) bias_gradient_kernel(Mat gy, Mat z, float* out) {
-    const int64_t j = blockIdx.x;
-    double acc = 0.0;
-    for (int64_t r = threadIdx.x; r < gy.rows; r += 256) {
-        float v = (float)((const T*)gy.p)[r * gy.stride + j];
-        if constexpr (ACT != kActNone) v *= activate_slope<ACT>((float)((const T*)z.p)[r * z.stride + j]);
-        acc += v;
+// Tile shapes, as waves and squares of 16 a wave on each axis.
+template <int WI_, int WJ_, int TI_, int TJ_>
+struct Shape {
+    static constexpr int kWavesI = WI_, kWavesJ = WJ_, kSquaresI = TI_, kSquaresJ = TJ_;
+    static constexpr int kI = WI_ * TI_ * 16, kJ = WJ_ * TJ_ * 16, kThreads = 64 * WI_ * WJ_;
+    template <class T, bool A_RC, bool B_RC>
+    using Product = Tile<T, WI_, WJ_, TI_, TJ_, A_RC, B_RC>;
+};
+using Large = Shape<2, 4, 8, 4>;    // 256 x 256, 8 waves, 128 KB of LDS: one workgroup a compute unit
+using Middle = Shape<2, 2, 4, 4>;   // 128 x 128, 4 waves, 64 KB
+using Narrow = Shape<1, 4, 4, 4>;   // 64 x 256, 4 waves, 80 KB: few columns
+using Small = Shape<2, 2, 2, 2>;    // 64 x 64, 4 waves, 32 KB: few tiles
+
+template <class F>
+void by_shape(int64_t ni, int64_t nj, int64_t splits_most, F f) {
+    const auto tiles = [&](int64_t bi, int64_t bj) { return ((ni + bi - 1) / bi) * ((nj + bj - 1) / bj) * splits_most; };
+    if (ni > 128 && nj > 128 && tiles(256, 256) >= 256) f(Large{});
+    else if (ni > 64 && nj > 64 && tiles(128, 128) >= 256) f(Middle{});
+    else if (ni <= 64 && nj > 64 && tiles(64, 256) >= 256) f(Narrow{});
+    else f(Small{});
+}
+
+template <class T, int ACT, class S>
+__device__ __forceinline__ void forward_outputs(const LinearForward& a, const f32x4 (&acc)[S::kSquaresI][S::kSquaresJ],
+                                                int64_t i0, int64_t j0) {
+    for_outputs<S>(acc, i0, j0, a.y.cols, a.y.rows, [&](int64_t i, int64_t j, int n, float (&v)[8]) {
+        if (a.bias) {
+            float b[8];
+            load8(a.bias + i, n, b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += b[e];
+        }
+        if (a.preact.p) store8((T*)a.preact.p + j * a.preact.stride + i, n, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = activate<ACT>(v[e]);
+        if (a.residual.p) {
+            float r[8];
+            load8((const T*)a.residual.p + j * a.residual.stride + i, n, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r[e];
+        }
+        store8((T*)a.y.p + j * a.y.stride + i, n, v);
+    });
+}
+
+template <class T, class S>
+__global__ void __launch_bounds__(S::kThreads) forward_kernel(LinearForward a, uint32_t ni, uint32_t nj) {
+    using P = typename S::template Product<T, false, false>;
+    __shared__ __align__(1024) unsigned char lds[P::kLds];
+    uint32_t ti, tj;
+    tile_of(xcd_contiguous_index(blockIdx.x, ni * nj), ni, nj, ti, tj);
+    const int64_t i0 = (int64_t)ti * S::kI, j0 = (int64_t)tj * S::kJ;
+    f32x4 acc[S::kSquaresI][S::kSquaresJ];
+    P::run(lds, {a.w.p, a.w.rows, a.w.cols, a.w.stride}, {a.x.p, a.x.rows, a.x.cols, a.x.stride}, i0, j0, 0, a.x.cols,
+           acc, [](auto&) {});
+    if (a.activation == kActGelu) forward_outputs<T, kActGelu, S>(a, acc, i0, j0);
+    else if (a.activation == kActSilu) forward_outputs<T, kActSilu, S>(a, acc, i0, j0);
+    else if (a.activation == kActRelu) forward_outputs<T, kActRelu, S>(a, acc, i0, j0);
+    else forward_outputs<T, kActNone, S>(a, acc, i0, j0);
+}
+
+// grad_x = dz w
+template <class T, class S>
+__global__ void __launch_bounds__(S::kThreads) grad_x_kernel(Mat dz, Mat w, Mat gx, uint32_t ni, uint32_t nj) {
+    using P = typename S::template Product<T, true, false>;
+    __shared__ __align__(1024) unsigned char lds[P::kLds];
+    uint32_t ti, tj;
+    tile_of(xcd_contiguous_index(blockIdx.x, ni * nj), ni, nj, ti, tj);
+    const int64_t i0 = (int64_t)ti * S::kI, j0 = (int64_t)tj * S::kJ;
+    f32x4 acc[S::kSquaresI][S::kSquaresJ];
+    P::run(lds, {w.p, w.rows, w.cols, w.stride}, {dz.p, dz.rows, dz.cols, dz.stride}, i0, j0, 0, w.rows, acc,
+           [](auto&) {});
+    for_outputs<S>(acc, i0, j0, gx.cols, gx.rows, [&](int64_t i, int64_t j, int n, float (&v)[8]) {
+        store8((T*)gx.p + j * gx.stride + i, n, v);
+    });
+}
+
+// grad_w = dz^T x over the rows of split blockIdx.y: to grad_w, or its float
+// sums to partial + blockIdx.y * (out * in).
+template <class T, class S>
+__global__ void __launch_bounds__(S::kThreads) grad_w_kernel(Mat dz, Mat x, Mat gw, float* partial, int64_t split_rows,
+                                                             uint32_t ni, uint32_t nj) {
+    using P = typename S::template Product<T, true, true>;
+    __shared__ __align__(1024) unsigned char lds[P::kLds];
+    uint32_t ti, tj;
+    tile_of(xcd_contiguous_index(blockIdx.x, ni * nj), ni, nj, ti, tj);
+    const int64_t i0 = (int64_t)ti * S::kI, j0 = (int64_t)tj * S::kJ;
+    const int64_t k0 = (int64_t)blockIdx.y * split_rows, k1 = min(k0 + split_rows, x.rows);
+    f32x4 acc[S::kSquaresI][S::kSquaresJ];
+    P::run(lds, {x.p, x.rows, x.cols, x.stride}, {dz.p, dz.rows, dz.cols, dz.stride}, i0, j0, k0, k1, acc,
+           [](auto&) {});
+    float* out = partial ? partial + (int64_t)blockIdx.y * gw.rows * gw.cols : nullptr;
+    for_outputs<S>(acc, i0, j0, gw.cols, gw.rows, [&](int64_t i, int64_t j, int n, float (&v)[8]) {
+        if (out) store8(out + j * gw.cols + i, n, v);
+        else store8((T*)gw.p + j * gw.stride + i, n, v);
+    });
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) join_kernel(const float* partial, int splits, Mat out) {
+    const int64_t n = out.rows * out.cols;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
+        float v = partial[q];
+        for (int k = 1; k < splits; ++k) v += partial[k * n + q];
+        ((T*)out.p)[q / out.cols * out.stride + q % out.cols] = (T)v;
     }
-    __shared__ double s[256];
-    s[threadIdx.x] = acc;
+}
+
+// dz = dy act'(z) rounded to T (when dz.p), and the workgroup's column sums of
+// the float dz at sums + blockIdx.x * cols (when sums). A thread keeps 8
+// columns; `across` (a power of two) threads share a row, the others of the
+// 256 take further rows.
+template <class T, int ACT>
+__global__ void __launch_bounds__(256) slope_kernel(Mat gy, Mat z, Mat dz, float* sums, int across) {
+    const int lane = threadIdx.x & (across - 1), group = threadIdx.x / across, groups = 256 / across;
+    const int64_t c = ((int64_t)blockIdx.y * across + lane) * 8;
+    const int n = (int)(gy.cols - c < 8 ? gy.cols - c : 8);
+    float sum[8] = {};
+    if (n > 0)
+        for (int64_t r = (int64_t)blockIdx.x * groups + group; r < gy.rows; r += (int64_t)gridDim.x * groups) {
+            float v[8];
+            load8((const T*)gy.p + r * gy.stride + c, n, v);
+            if constexpr (ACT != kActNone) {
+                float u[8];
+                load8((const T*)z.p + r * z.stride + c, n, u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= activate_slope<ACT>(u[e]);
+                if (dz.p) store8((T*)dz.p + r * dz.stride + c, n, v);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += v[e];
+        }
+    if (!sums) return;
+    __shared__ float s[256][9];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[threadIdx.x][e] = sum[e];
     __syncthreads();
-    for (int n = 128; n > 0; n >>= 1) {
-        if ((int)threadIdx.x < n) s[threadIdx.x] += s[threadIdx.x + n];
-        __syncthreads();
+    for (int q = threadIdx.x; q < across * 8; q += 256) {
+        const int64_t k = (int64_t)blockIdx.y * across * 8 + q;
+        float v = 0.0f;
+        for (int w = 0; w < groups; ++w) v += s[w * across + q / 8][q % 8];
+        if (k < gy.cols) sums[(int64_t)blockIdx.x * gy.cols + k] = v;
     }
-    if (threadIdx.x == 0) out[j] = (float)s[0];
 }
 
-dim3 grid_of(int64_t i, int64_t j) {
-    return dim3((unsigned)((i + kTileEdge - 1) / kTileEdge), (unsigned)((j + kTileEdge - 1) / kTileEdge));
+// out[k] = the sum of the workgroups' sums of column k: 16 threads a column,
+// each over every 16th workgroup, joined in order.
+__global__ void __launch_bounds__(1024) column_sums_kernel(const float* partial, int blocks, int64_t n, float* out) {
+    __shared__ float s[16][64];
+    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int64_t k = (int64_t)blockIdx.x * 64 + lane;
+    float v = 0.0f;
+    if (k < n)
+        for (int b = part; b < blocks; b += 16) v += partial[b * n + k];
+    s[part][lane] = v;
+    __syncthreads();
+    if (part == 0 && k < n) {
+        for (int q = 1; q < 16; ++q) v += s[q][lane];
+        out[k] = v;
+    }
 }
 
-template <class T, int ACT>
-void forward(const LinearForward& a, hipStream_t s) {
-    Operand x{a.x.p, nullptr, a.x.stride, 1, a.x.rows}, w{a.w.p, nullptr, a.w.stride, 1, a.w.rows};
-    product_kernel<T, ACT, kActNone><<<grid_of(a.y.rows, a.y.cols), 256, 0, s>>>(x, w, a.x.cols,
-                                                                               {a.bias, a.residual, a.preact, a.y});
-}
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <class T, int ACT>
-void backward(const LinearBackward& a, hipStream_t s) {
-    const Mat& g = a.grad_y;
-    if (a.grad_x.p && a.grad_x.rows) {
-        Operand dz{g.p, a.preact.p, g.stride, 1, g.rows}, w{a.w.p, nullptr, 1, a.w.stride, a.w.cols};
-        product_kernel<T, kActNone, ACT><<<grid_of(a.grad_x.rows, a.grad_x.cols), 256, 0, s>>>(
-            dz, w, g.cols, {nullptr, {}, {}, a.grad_x});
+// ---- the backward's plan: what it keeps in the workspace
+struct BackwardPlan {
+    bool dz = false;             // an activation's dz is written
+    int64_t dz_stride = 0;
+    int across = 1;              // threads on a row of the slope pass
+    int64_t slope_x = 0, slope_y = 0;   // its grid; 0: no pass
+    int64_t splits = 1, split_rows = 0;
+    size_t dz_bytes = 0, sums_bytes = 0, partial_bytes = 0;
+};
+
+constexpr int64_t kSplitRows = 1024;   // rows a split is worth at least
+
+BackwardPlan plan_backward(const LinearBackward& a) {
+    BackwardPlan p;
+    const int64_t rows = a.grad_y.rows, out = a.grad_y.cols, in = a.x.cols;
+    p.dz = a.activation != kActNone && (a.grad_x.p || a.grad_w.p) && rows > 0;
+    if (p.dz || a.grad_bias) {
+        while (p.across < 256 && p.across * 8 < out) p.across *= 2;
+        p.slope_y = ceil_div(out, (int64_t)p.across * 8);
+        const int64_t by_rows = ceil_div(rows, 256 / p.across);
+        const int64_t most = ceil_div(2048, p.slope_y);
+        p.slope_x = by_rows < most ? by_rows : most;
+        if (a.grad_bias) p.sums_bytes = sizeof(float) * (size_t)(p.slope_x * out + 64);
+    }
+    if (p.dz) {
+        p.dz_stride = ceil_div(out, 8) * 8;
+        p.dz_bytes = (size_t)(rows * p.dz_stride) * (a.dtype == TGS_DTYPE_FLOAT32 ? 4 : 2);
     }
     if (a.grad_w.p) {
-        Operand dz{g.p, a.preact.p, 1, g.stride, g.cols}, x{a.x.p, nullptr, 1, a.x.stride, a.x.cols};
-        product_kernel<T, kActNone, ACT><<<grid_of(a.grad_w.rows, a.grad_w.cols), 256, 0, s>>>(
-            dz, x, g.rows, {nullptr, {}, {}, a.grad_w});
+        const int64_t most = ceil_div(rows, kSplitRows) > 1 ? ceil_div(rows, kSplitRows) : 1;
+        by_shape(in, out, most, [&](auto shape) {
+            using S = decltype(shape);
+            const int64_t tiles = ceil_div(in, S::kI) * ceil_div(out, S::kJ);
+            const int64_t want = ceil_div(512, tiles);
+            p.splits = want < most ? want : most;
+        });
+        p.split_rows = ceil_div(ceil_div(rows, p.splits), 64) * 64;
+        if (p.split_rows < 64) p.split_rows = 64;
+        p.splits = ceil_div(rows, p.split_rows);
+        if (p.splits < 1) p.splits = 1;
+        if (p.splits > 1) p.partial_bytes = sizeof(float) * (size_t)(p.splits * in * out);
     }
-    if (a.grad_bias) bias_gradient_kernel<T, ACT><<<(unsigned)g.cols, 256, 0, s>>>(g, a.preact, a.grad_bias);
+    const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
+    p.dz_bytes = round(p.dz_bytes);
+    p.sums_bytes = round(p.sums_bytes);
+    p.partial_bytes = round(p.partial_bytes);
+    return p;
+}
+
+template <class T>
+void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) {
+    const BackwardPlan p = plan_backward(a);
+    const int64_t rows = a.grad_y.rows, out = a.grad_y.cols, in = a.x.cols;
+    Mat dz = a.grad_y;
+    float* sums = (float*)(workspace + p.dz_bytes);
+    float* partial = (float*)(workspace + p.dz_bytes + p.sums_bytes);
+    if (p.dz) dz = Mat{workspace, rows, out, p.dz_stride};
+    if (p.slope_x)
+        by_activation(a.activation, [&](auto act) {
+            slope_kernel<T, decltype(act)::value><<<dim3((unsigned)p.slope_x, (unsigned)p.slope_y), 256, 0, s>>>(
+                a.grad_y, a.preact, p.dz ? dz : Mat{}, a.grad_bias ? sums : nullptr, p.across);
+        });
+    if (a.grad_bias)
+        column_sums_kernel<<<(unsigned)ceil_div(out, 64), 1024, 0, s>>>(sums, (int)p.slope_x, out, a.grad_bias);
+    if (a.grad_x.p && rows)
+        by_shape(in, rows, 1, [&](auto shape) {
+            using S = decltype(shape);
+            const uint32_t ni = (uint32_t)ceil_div(in, S::kI), nj = (uint32_t)ceil_div(rows, S::kJ);
+            grad_x_kernel<T, S><<<ni * nj, S::kThreads, 0, s>>>(dz, a.w, a.grad_x, ni, nj);
+        });
+    if (a.grad_w.p) {
+        const int64_t most = ceil_div(rows, kSplitRows) > 1 ? ceil_div(rows, kSplitRows) : 1;
+        by_shape(in, out, most, [&](auto shape) {
+            using S = decltype(shape);
+            const uint32_t ni = (uint32_t)ceil_div(in, S::kI), nj = (uint32_t)ceil_div(out, S::kJ);
+            grad_w_kernel<T, S><<<dim3(ni * nj, (unsigned)p.splits), S::kThreads, 0, s>>>(
+                dz, a.x, a.grad_w, p.splits > 1 ? partial : nullptr, p.split_rows, ni, nj);
+        });
+        if (p.splits > 1) {
+            const int64_t blocks = ceil_div(in * out, 256);
+            join_kernel<T><<<(unsigned)(blocks < 2048 ? blocks : 2048), 256, 0, s>>>(partial, (int)p.splits, a.grad_w);
+        }
+    }
 }
 
 }  // namespace
 
-size_t linear_backward_workspace(const LinearBackward&) { return 0; }
+size_t linear_backward_workspace(const LinearBackward& a) {
+    const BackwardPlan p = plan_backward(a);
+    return p.dz_bytes + p.sums_bytes + p.partial_bytes;
+}
 
 int launch_linear_forward(const LinearForward& a, hipStream_t s) {
     by_dtype(a.dtype, [&](auto t) {
-        by_activation(a.activation, [&](auto act) { forward<decltype(t), decltype(act)::value>(a, s); });
+        using T = decltype(t);
+        by_shape(a.y.cols, a.y.rows, 1, [&](auto shape) {
+            using S = decltype(shape);
+            const uint32_t ni = (uint32_t)ceil_div(a.y.cols, S::kI), nj = (uint32_t)ceil_div(a.y.rows, S::kJ);
+            forward_kernel<T, S><<<ni * nj, S::kThreads, 0, s>>>(a, ni, nj);
+        });
     });
     TGS_CHECK_LAUNCH();
     return TGS_OK;
 }
 
-int launch_linear_backward(const LinearBackward& a, void*, hipStream_t s) {
-    by_dtype(a.dtype, [&](auto t) {
-        by_activation(a.activation, [&](auto act) { backward<decltype(t), decltype(act)::value>(a, s); });
-    });
+int launch_linear_backward(const LinearBackward& a, void* workspace, hipStream_t s) {
+    by_dtype(a.dtype, [&](auto t) { backward<decltype(t)>(a, (unsigned char*)workspace, s); });
     TGS_CHECK_LAUNCH();
     return TGS_OK;
 }
