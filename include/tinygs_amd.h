@@ -549,7 +549,8 @@ int tgs_layer_norm_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_
  *   iterations times: A = X X^T, X <- a X + (b A + c A^2) X
  *   W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) X
  * with a, b, c = 3.4445, -4.7750, 2.0315, which bring the singular values of X
- * near one.
+ * near one. The products are of matrices held to 22 bits (two halves each), with
+ * float sums; the sum of squares is held in 64 bits.
  * lr is params.lr times the learning rate of tgs_muon_set_lr (1 at creation). */
 typedef struct tgs_muon_params {
     float lr;             /* 0.02 at creation */
@@ -566,14 +567,15 @@ typedef struct tgs_muon_params {
 int tgs_muon_create(const tgs_matrix* weights, const tgs_matrix* grads, const tgs_matrix* momenta,
                     const tgs_matrix* copies, int32_t count, tgs_muon** out);
 int tgs_muon_destroy(tgs_muon* m);
-/* Rebinds the pointers; count, shapes and dtypes as at creation. Waits for the
- * device. */
+/* Rebinds the pointers; count, shapes and dtypes as at creation. */
 int tgs_muon_set_matrices(tgs_muon* m, const tgs_matrix* weights, const tgs_matrix* grads, const tgs_matrix* momenta,
                           const tgs_matrix* copies, int32_t count);
 int tgs_muon_set_params(tgs_muon* m, const tgs_muon_params* p);
 int tgs_muon_get_params(tgs_muon* m, tgs_muon_params* p);
 int tgs_muon_set_lr(tgs_muon* m, float global_lr);
 float tgs_muon_get_lr(tgs_muon* m);
+/* The first step, and the first after a rebinding, place the matrices' table on
+ * the device and wait for it: capture only later ones. */
 int tgs_muon_step(tgs_muon* m, float scale, void* stream);
 /* Zero momenta, as after creation with zero ones. */
 int tgs_muon_reset(tgs_muon* m, void* stream);

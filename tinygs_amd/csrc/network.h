@@ -136,8 +136,25 @@ int launch_layer_norm_backward(const LayerNormBackward& a, void* workspace, hipS
 // ---- muon.hip
 constexpr float kNewtonSchulzA = 3.4445f, kNewtonSchulzB = -4.7750f, kNewtonSchulzC = 2.0315f;
 
-struct MuonMatrix {
-    Mat w, g, m, c;   // weights, gradient, momentum, copy (c.p may be NULL)
+// A matrix of the step as the kernels read it, and where its work starts in
+// the launches over all matrices (first, by phase).
+enum { kMuonPatches = 0, kMuonGram = 1, kMuonUpdate = 2, kMuonSquare = 3 };
+struct MuonPart {
+    Mat w, g, m, c;              // weights, gradient, momentum, copy (c.p may be NULL)
+    int64_t side, length;        // X is side x length, side <= length
+    int64_t x_stride, x_plane;   // of X's two planes (elements)
+    int64_t g_stride, g_plane;   // of the Gram matrix's and the polynomial's
+    _Float16 *x[2], *gram, *poly;
+    float shape;                 // sqrt(max(1, rows / cols))
+    int tall;                    // X is the transpose
+    uint32_t first[3];
+};
+struct MuonPlan {
+    uint32_t patches;      // workgroups of the element passes
+    uint32_t tiles[2];     // of the products with side x side and side x length outputs
+    bool large[2];         // whether those are the large tiles
+    bool fits;             // whether the counts fit a launch
+    int64_t sums_at, parts_at, bytes;   // in the workspace
 };
 struct MuonStep {
     float momentum, grad_scale;   // grad_scale = (1 - momentum) scale
@@ -146,8 +163,11 @@ struct MuonStep {
     int nesterov, iterations;
     int grad_dtype, copy_dtype;
 };
-size_t muon_workspace(const MuonMatrix* mats, int count);
-int launch_muon_step(const MuonMatrix* mats, int count, const MuonStep& p, void* workspace, hipStream_t s);
+// Fills the parts' shapes and places (offsets from the workspace's start,
+// which place_muon turns into addresses) from their matrices.
+MuonPlan plan_muon(MuonPart* parts, int count);
+void place_muon(MuonPart* parts, int count, unsigned char* workspace);
+int launch_muon_step(const MuonPlan& plan, int count, const MuonStep& p, unsigned char* workspace, hipStream_t s);
 int launch_zero_matrix(const Mat& m, hipStream_t s);
 
 }  // namespace tgs

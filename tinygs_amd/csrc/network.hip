@@ -15,7 +15,9 @@ struct tgs_network {
 };
 
 struct tgs_muon {
-    std::vector<MuonMatrix> mats;
+    std::vector<MuonPart> mats;
+    bool on_device = false;   // the workspace holds the matrices' table
+    MuonPlan plan{};
     int grad_dtype = TGS_DTYPE_FLOAT32;
     int copy_dtype = TGS_DTYPE_FLOAT32;
     tgs_muon_params p{};
@@ -129,9 +131,15 @@ int check_muon(const tgs_matrix* weights, const tgs_matrix* grads, const tgs_mat
 
 void bind_muon(tgs_muon* m, const tgs_matrix* weights, const tgs_matrix* grads, const tgs_matrix* momenta,
                const tgs_matrix* copies, int32_t count) {
-    for (int32_t i = 0; i < count; ++i)
-        m->mats[(size_t)i] = MuonMatrix{view(&weights[i]), view(&grads[i]), view(&momenta[i]),
-                                        view(copies ? &copies[i] : nullptr)};
+    for (int32_t i = 0; i < count; ++i) {
+        MuonPart& a = m->mats[(size_t)i];
+        a.w = view(&weights[i]);
+        a.g = view(&grads[i]);
+        a.m = view(&momenta[i]);
+        a.c = view(copies ? &copies[i] : nullptr);
+    }
+    m->plan = plan_muon(m->mats.data(), count);
+    m->on_device = false;
     m->grad_dtype = grads[0].dtype;
     m->copy_dtype = copies ? copies[0].dtype : TGS_DTYPE_FLOAT32;
 }
@@ -291,6 +299,10 @@ int tgs_muon_create(const tgs_matrix* weights, const tgs_matrix* grads, const tg
     }
     m->p = tgs_muon_params{0.02f, 0.95f, 0.0f, 1e-12f, 1, 5};
     bind_muon(m, weights, grads, momenta, copies, count);
+    if (!m->plan.fits) {
+        delete m;
+        return fail(TGS_ERR_INVALID, "the matrices are too large for one step");
+    }
     *out = m;
     return TGS_OK;
 }
@@ -358,13 +370,24 @@ int tgs_muon_step(tgs_muon* m, float scale, void* stream) {
     p.grad_dtype = m->grad_dtype;
     p.copy_dtype = m->copy_dtype;
     hipStream_t s = (hipStream_t)stream;
-    TGS_TRY(ensure(m->workspace, muon_workspace(m->mats.data(), (int)m->mats.size()), s));
-    return launch_muon_step(m->mats.data(), (int)m->mats.size(), p, m->workspace.p, s);
+    const int count = (int)m->mats.size();
+    if (!m->on_device) {   // the first step, or the first after a rebinding
+        const MuonPlan plan = plan_muon(m->mats.data(), count);
+        TGS_TRY(ensure(m->workspace, (size_t)plan.bytes, s));
+        unsigned char* at = m->workspace.as<unsigned char>();
+        place_muon(m->mats.data(), count, at);
+        TGS_HIP(hipMemcpyAsync(at + plan.parts_at, m->mats.data(), sizeof(MuonPart) * (size_t)count,
+                               hipMemcpyHostToDevice, s));
+        TGS_HIP(hipStreamSynchronize(s));
+        m->plan = plan;
+        m->on_device = true;
+    }
+    return launch_muon_step(m->plan, count, p, m->workspace.as<unsigned char>(), s);
 }
 
 int tgs_muon_reset(tgs_muon* m, void* stream) {
     if (!m) return fail(TGS_ERR_INVALID, "optimizer is NULL");
-    for (const MuonMatrix& a : m->mats) TGS_TRY(launch_zero_matrix(a.m, (hipStream_t)stream));
+    for (const MuonPart& a : m->mats) TGS_TRY(launch_zero_matrix(a.m, (hipStream_t)stream));
     return TGS_OK;
 }
 

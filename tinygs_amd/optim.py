@@ -220,7 +220,7 @@ class Muon:
         return self.m_momenta
 
     def set_grads(self, grads):
-        """Other gradient tensors of the same shapes and dtype. Waits for the device."""
+        """Other gradient tensors of the same shapes and dtype."""
         if len(grads) != len(self.m_weights):
             raise RuntimeError("Muon: weights and grads must have the same count")
         kept, self.m_grads = self.m_grads, list(grads)
