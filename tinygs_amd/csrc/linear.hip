@@ -66,6 +66,7 @@ __device__ __forceinline__ void for_outputs(const f32x4 (&acc)[TI][TJ], int64_t 
 // Tile shapes, as waves and squares of 16 a wave on each axis.
 template <int WI_, int WJ_, int TI_, int TJ_>
 struct Shape {
+    static constexpr int kResident = 160 * 1024 / (2 * 128 * 16 * (WI_ * TI_ + WJ_ * TJ_));   // workgroups a compute unit
     static constexpr int kWavesI = WI_, kWavesJ = WJ_, kSquaresI = TI_, kSquaresJ = TJ_;
     static constexpr int kI = WI_ * TI_ * 16, kJ = WJ_ * TJ_ * 16, kThreads = 64 * WI_ * WJ_;
     template <class T, bool A_RC, bool B_RC>
@@ -161,14 +162,39 @@ __global__ void __launch_bounds__(S::kThreads) grad_w_kernel(Mat dz, Mat x, Mat 
     });
 }
 
+// The splits' sums joined in a fixed order: 256 neighbouring outputs a
+// workgroup, four a lane; each of its four waves takes every fourth split, with
+// eight loads in flight.
 template <class T>
 __global__ void __launch_bounds__(256) join_kernel(const float* partial, int splits, Mat out) {
-    const int64_t n = out.rows * out.cols;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
-        float v = partial[q];
-        for (int k = 1; k < splits; ++k) v += partial[k * n + q];
-        ((T*)out.p)[q / out.cols * out.stride + q % out.cols] = (T)v;
+    __shared__ f32x4 s[4][64];
+    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int64_t n = out.rows * out.cols, q = ((int64_t)blockIdx.x * 64 + lane) * 4;
+    typedef float loose4 __attribute__((ext_vector_type(4), aligned(4)));
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (q + 4 <= n) {
+        int k = part;
+        for (; k + 28 < splits; k += 32) {
+            f32x4 u[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[e] = *(const loose4*)(partial + (k + 4 * e) * n + q);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v += u[e];
+        }
+        for (; k < splits; k += 4) v += *(const loose4*)(partial + k * n + q);
+    } else {
+        for (int k = part; k < splits; k += 4)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (q + e < n) v[e] += partial[k * n + q + e];
     }
+    s[part][lane] = v;
+    __syncthreads();
+    if (part != 0) return;
+    v = ((v + s[1][lane]) + s[2][lane]) + s[3][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (q + e < n) ((T*)out.p)[(q + e) / out.cols * out.stride + (q + e) % out.cols] = (T)v[e];
 }
 
 // dz = dy act'(z) rounded to T (when dz.p), and the workgroup's column sums of
@@ -208,23 +234,6 @@ __global__ void __launch_bounds__(256) slope_kernel(Mat gy, Mat z, Mat dz, float
     }
 }
 
-// out[k] = the sum of the workgroups' sums of column k: 16 threads a column,
-// each over every 16th workgroup, joined in order.
-__global__ void __launch_bounds__(1024) column_sums_kernel(const float* partial, int blocks, int64_t n, float* out) {
-    __shared__ float s[16][64];
-    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
-    const int64_t k = (int64_t)blockIdx.x * 64 + lane;
-    float v = 0.0f;
-    if (k < n)
-        for (int b = part; b < blocks; b += 16) v += partial[b * n + k];
-    s[part][lane] = v;
-    __syncthreads();
-    if (part == 0 && k < n) {
-        for (int q = 1; q < 16; ++q) v += s[q][lane];
-        out[k] = v;
-    }
-}
-
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- the backward's plan: what it keeps in the workspace
@@ -247,7 +256,7 @@ BackwardPlan plan_backward(const LinearBackward& a) {
         while (p.across < 256 && p.across * 8 < out) p.across *= 2;
         p.slope_y = ceil_div(out, (int64_t)p.across * 8);
         const int64_t by_rows = ceil_div(rows, 256 / p.across);
-        const int64_t most = ceil_div(2048, p.slope_y);
+        const int64_t most = ceil_div(1024, p.slope_y);
         p.slope_x = by_rows < most ? by_rows : most;
         if (a.grad_bias) p.sums_bytes = sizeof(float) * (size_t)(p.slope_x * out + 64);
     }
@@ -260,7 +269,8 @@ BackwardPlan plan_backward(const LinearBackward& a) {
         by_shape(in, out, most, [&](auto shape) {
             using S = decltype(shape);
             const int64_t tiles = ceil_div(in, S::kI) * ceil_div(out, S::kJ);
-            const int64_t want = ceil_div(512, tiles);
+            // as many workgroups as fit the card at once (LDS: one to five a compute unit)
+            const int64_t want = ceil_div(256 * S::kResident, tiles);
             p.splits = want < most ? want : most;
         });
         p.split_rows = ceil_div(ceil_div(rows, p.splits), 64) * 64;
@@ -290,7 +300,7 @@ void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) 
                 a.grad_y, a.preact, p.dz ? dz : Mat{}, a.grad_bias ? sums : nullptr, p.across);
         });
     if (a.grad_bias)
-        column_sums_kernel<<<(unsigned)ceil_div(out, 64), 1024, 0, s>>>(sums, (int)p.slope_x, out, a.grad_bias);
+        launch_column_sums(sums, (int)p.slope_x, out, out, a.grad_bias, nullptr, s);
     if (a.grad_x.p && rows)
         by_shape(in, rows, 1, [&](auto shape) {
             using S = decltype(shape);
@@ -306,8 +316,7 @@ void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) 
                 dz, a.x, a.grad_w, p.splits > 1 ? partial : nullptr, p.split_rows, ni, nj);
         });
         if (p.splits > 1) {
-            const int64_t blocks = ceil_div(in * out, 256);
-            join_kernel<T><<<(unsigned)(blocks < 2048 ? blocks : 2048), 256, 0, s>>>(partial, (int)p.splits, a.grad_w);
+            join_kernel<T><<<(unsigned)ceil_div(in * out, 256), 256, 0, s>>>(partial, (int)p.splits, a.grad_w);
         }
     }
 }

@@ -130,6 +130,10 @@ struct LayerNormBackward {
     int dtype;
 };
 size_t layer_norm_backward_workspace(const LayerNormBackward& a);
+// Column sums of `blocks` rows of `width` floats: the first n to `first`, the
+// others to `second` (each may be NULL), in a fixed order.
+void launch_column_sums(const float* partial, int blocks, int64_t n, int64_t width, float* first, float* second,
+                        hipStream_t s);
 int launch_layer_norm_forward(const LayerNormForward& a, hipStream_t s);
 int launch_layer_norm_backward(const LayerNormBackward& a, void* workspace, hipStream_t s);
 

@@ -33,13 +33,14 @@ def _dtypes():
 
 def matrix(t, name: str) -> _lib.tgs_matrix:
     """The C ABI's view of a 2-D tensor; raises for tensors that it cannot address."""
-    if t.dim() != 2:
-        raise RuntimeError(f"{name}: a matrix has two dimensions, not {t.dim()}")
-    rows, cols = t.shape
+    shape = t.shape
+    if len(shape) != 2:
+        raise RuntimeError(f"{name}: a matrix has two dimensions, not {len(shape)}")
+    rows, cols = shape
     step, unit = t.stride()
-    if cols > 1 and unit != 1:
+    if unit != 1 and cols > 1:
         raise RuntimeError(f"{name}: the elements of a row must lie next to each other")
-    dtype = _dtypes().get(t.dtype)
+    dtype = (_DTYPES or _dtypes()).get(t.dtype)
     if dtype is None:
         raise RuntimeError(f"{name}: only float32, float16 and bfloat16 are supported")
     if not t.is_cuda:
@@ -57,9 +58,15 @@ def _vector(t, n: int, name: str):
     return t.data_ptr()
 
 
+_FLOAT32 = None
+
+
 def _float32():
-    import torch
-    return torch.float32
+    global _FLOAT32
+    if _FLOAT32 is None:
+        import torch
+        _FLOAT32 = torch.float32
+    return _FLOAT32
 
 
 class LayerOps:
@@ -72,6 +79,7 @@ class LayerOps:
         self._lib = _lib.load()
         _lib.check(self._lib.tgs_network_create(C.byref(h)), "LayerOps")
         self._h = h
+        self._current = None
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -83,17 +91,22 @@ class LayerOps:
             self._h = None
 
     @staticmethod
-    def _empty(stream, shape, dtype, device):
-        import torch
+    def _empty(stream, like, shape, dtype=None):
         if stream is None:
-            return torch.empty(shape, dtype=dtype, device=device)
-        with torch.cuda.stream(stream):
-            return torch.empty(shape, dtype=dtype, device=device)
-
-    @staticmethod
-    def _stream(stream):
+            return like.new_empty(shape, dtype=dtype)
         import torch
-        return (stream if stream is not None else torch.cuda.current_stream()).cuda_stream
+        with torch.cuda.stream(stream):
+            return like.new_empty(shape, dtype=dtype)
+
+    def _stream(self, stream, like):
+        if stream is not None:
+            return stream.cuda_stream
+        if self._current is None:
+            import torch
+            # the stream's address without the Stream object around it: 0.1 us a call against 2.8
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+            self._current = raw or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        return self._current(like.device.index)
 
     def linear(self, x, weight, bias=None, activation: str = "none", residual=None, keep_preact: bool = False,
                out=None, preact=None, stream=None):
@@ -101,16 +114,16 @@ class LayerOps:
         activation, which linear_backward takes. out may be residual itself."""
         rows, outs = x.shape[0], weight.shape[0]
         if out is None:
-            out = self._empty(stream, (rows, outs), x.dtype, x.device)
+            out = self._empty(stream, x, (rows, outs))
         if preact is None and keep_preact:
-            preact = self._empty(stream, (rows, outs), x.dtype, x.device)
+            preact = self._empty(stream, x, (rows, outs))
         act = ACTIVATIONS.get(activation)
         if act is None:
             raise RuntimeError(f"linear: unknown activation: {activation}")
         rc = self._lib.tgs_linear_forward(
             self._h, matrix(x, "x"), matrix(weight, "weight"), _vector(bias, outs, "bias"), act,
             None if residual is None else matrix(residual, "residual"),
-            None if preact is None else matrix(preact, "preact"), matrix(out, "out"), self._stream(stream))
+            None if preact is None else matrix(preact, "preact"), matrix(out, "out"), self._stream(stream, x))
         if rc:
             _lib.check(rc, "linear")
         return out if preact is None else (out, preact)
@@ -121,11 +134,11 @@ class LayerOps:
         """(grad_x, grad_weight, grad_bias) of linear for grad_y; None where not needed. The residual's gradient is
         grad_y itself. Gradients are assigned, not accumulated."""
         if need_x and grad_x is None:
-            grad_x = self._empty(stream, x.shape, x.dtype, x.device)
+            grad_x = self._empty(stream, x, x.shape)
         if need_weight and grad_weight is None:
-            grad_weight = self._empty(stream, weight.shape, weight.dtype, weight.device)
+            grad_weight = self._empty(stream, weight, weight.shape)
         if need_bias and grad_bias is None:
-            grad_bias = self._empty(stream, (weight.shape[0],), _float32(), x.device)
+            grad_bias = self._empty(stream, x, (weight.shape[0],), _float32())
         act = ACTIVATIONS.get(activation)
         if act is None:
             raise RuntimeError(f"linear_backward: unknown activation: {activation}")
@@ -135,7 +148,7 @@ class LayerOps:
             self._h, matrix(grad_y, "grad_y"), matrix(x, "x"), matrix(weight, "weight"),
             matrix(preact, "preact") if act else None, act, None if grad_x is None else matrix(grad_x, "grad_x"),
             None if grad_weight is None else matrix(grad_weight, "grad_weight"),
-            _vector(grad_bias, weight.shape[0], "grad_bias"), self._stream(stream))
+            _vector(grad_bias, weight.shape[0], "grad_bias"), self._stream(stream, x))
         if rc:
             _lib.check(rc, "linear_backward")
         return grad_x, grad_weight, grad_bias
@@ -144,14 +157,14 @@ class LayerOps:
         """((x - mean) rstd gamma + beta, mean, rstd) over each row. out may be x itself."""
         rows, n = x.shape
         if out is None:
-            out = self._empty(stream, (rows, n), x.dtype, x.device)
+            out = self._empty(stream, x, (rows, n))
         if mean is None:
-            mean = self._empty(stream, (rows,), _float32(), x.device)
+            mean = self._empty(stream, x, (rows,), _float32())
         if rstd is None:
-            rstd = self._empty(stream, (rows,), _float32(), x.device)
+            rstd = self._empty(stream, x, (rows,), _float32())
         rc = self._lib.tgs_layer_norm_forward(
             self._h, matrix(x, "x"), _vector(gamma, n, "gamma"), _vector(beta, n, "beta"), eps, matrix(out, "out"),
-            _vector(mean, rows, "mean"), _vector(rstd, rows, "rstd"), self._stream(stream))
+            _vector(mean, rows, "mean"), _vector(rstd, rows, "rstd"), self._stream(stream, x))
         if rc:
             _lib.check(rc, "layer_norm")
         return out, mean, rstd
@@ -162,16 +175,16 @@ class LayerOps:
         reaches x past the norm. grad_x may be grad_y or residual_grad itself."""
         rows, n = x.shape
         if grad_x is None:
-            grad_x = self._empty(stream, (rows, n), x.dtype, x.device)
+            grad_x = self._empty(stream, x, (rows, n))
         if grad_gamma is None:
-            grad_gamma = self._empty(stream, (n,), _float32(), x.device)
+            grad_gamma = self._empty(stream, x, (n,), _float32())
         if grad_beta is None:
-            grad_beta = self._empty(stream, (n,), _float32(), x.device)
+            grad_beta = self._empty(stream, x, (n,), _float32())
         rc = self._lib.tgs_layer_norm_backward(
             self._h, matrix(grad_y, "grad_y"), matrix(x, "x"), _vector(gamma, n, "gamma"),
             _vector(mean, rows, "mean"), _vector(rstd, rows, "rstd"),
             None if residual_grad is None else matrix(residual_grad, "residual_grad"), matrix(grad_x, "grad_x"),
-            _vector(grad_gamma, n, "grad_gamma"), _vector(grad_beta, n, "grad_beta"), self._stream(stream))
+            _vector(grad_gamma, n, "grad_gamma"), _vector(grad_beta, n, "grad_beta"), self._stream(stream, x))
         if rc:
             _lib.check(rc, "layer_norm_backward")
         return grad_x, grad_gamma, grad_beta
