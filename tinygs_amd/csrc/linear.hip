@@ -162,39 +162,46 @@ __global__ void __launch_bounds__(S::kThreads) grad_w_kernel(Mat dz, Mat x, Mat 
     });
 }
 
-// The splits' sums joined in a fixed order: 256 neighbouring outputs a
+// The splits' float sums joined in a fixed order: 256 neighbouring ones a
 // workgroup, four a lane; each of its four waves takes every fourth split, with
-// eight loads in flight.
+// eight loads in flight. A split holds out's elements and, after them, those
+// of `bias` (either may be left out); `width` is the distance between splits.
 template <class T>
-__global__ void __launch_bounds__(256) join_kernel(const float* partial, int splits, Mat out) {
+__global__ void __launch_bounds__(256) join_kernel(const float* partial, int splits, int64_t width, Mat out, float* bias,
+                                                   int64_t biases) {
     __shared__ f32x4 s[4][64];
     const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
-    const int64_t n = out.rows * out.cols, q = ((int64_t)blockIdx.x * 64 + lane) * 4;
+    const int64_t n = out.rows * out.cols, end = n + biases, q = ((int64_t)blockIdx.x * 64 + lane) * 4;
     typedef float loose4 __attribute__((ext_vector_type(4), aligned(4)));
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (q + 4 <= n) {
+    if (q + 4 <= end) {
         int k = part;
         for (; k + 28 < splits; k += 32) {
             f32x4 u[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) u[e] = *(const loose4*)(partial + (k + 4 * e) * n + q);
+            for (int e = 0; e < 8; ++e) u[e] = *(const loose4*)(partial + (k + 4 * e) * width + q);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v += u[e];
         }
-        for (; k < splits; k += 4) v += *(const loose4*)(partial + k * n + q);
+        for (; k < splits; k += 4) v += *(const loose4*)(partial + k * width + q);
     } else {
         for (int k = part; k < splits; k += 4)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (q + e < n) v[e] += partial[k * n + q + e];
+                if (q + e < end) v[e] += partial[k * width + q + e];
     }
     s[part][lane] = v;
     __syncthreads();
     if (part != 0) return;
     v = ((v + s[1][lane]) + s[2][lane]) + s[3][lane];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (q + e < n) ((T*)out.p)[(q + e) / out.cols * out.stride + (q + e) % out.cols] = (T)v[e];
+    for (int e = 0; e < 4; ++e) {
+        if (q + e < n) {
+            if (out.p) ((T*)out.p)[(q + e) / out.cols * out.stride + (q + e) % out.cols] = (T)v[e];
+        } else if (q + e < end) {
+            bias[q + e - n] = v[e];
+        }
+    }
 }
 
 // dz = dy act'(z) rounded to T (when dz.p), and the workgroup's column sums of
@@ -238,6 +245,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ---- the backward's plan: what it keeps in the workspace
 struct BackwardPlan {
+    bool narrow = false;         // one pass over the rows (linear_narrow.hip)
     bool dz = false;             // an activation's dz is written
     int64_t dz_stride = 0;
     int across = 1;              // threads on a row of the slope pass
@@ -251,6 +259,12 @@ constexpr int64_t kSplitRows = 1024;   // rows a split is worth at least
 BackwardPlan plan_backward(const LinearBackward& a) {
     BackwardPlan p;
     const int64_t rows = a.grad_y.rows, out = a.grad_y.cols, in = a.x.cols;
+    if (linear_backward_is_narrow(a)) {
+        p.narrow = true;
+        p.splits = narrow_backward_splits(a);
+        p.partial_bytes = sizeof(float) * (size_t)(p.splits * (in * out + out));
+        return p;
+    }
     p.dz = a.activation != kActNone && (a.grad_x.p || a.grad_w.p) && rows > 0;
     if (p.dz || a.grad_bias) {
         while (p.across < 256 && p.across * 8 < out) p.across *= 2;
@@ -290,6 +304,19 @@ template <class T>
 void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) {
     const BackwardPlan p = plan_backward(a);
     const int64_t rows = a.grad_y.rows, out = a.grad_y.cols, in = a.x.cols;
+    if (p.narrow) {
+        float* split = (float*)workspace;
+        launch_narrow_backward(a, split, s);
+        const Mat gw{a.grad_w.p, out, in, a.grad_w.p ? a.grad_w.stride : in};
+        const int64_t biases = a.grad_bias ? out : 0;
+        if (gw.p)
+            join_kernel<T><<<(unsigned)ceil_div(in * out + biases, 256), 256, 0, s>>>(split, (int)p.splits, in * out + out,
+                                                                                      gw, a.grad_bias, biases);
+        else if (biases)
+            join_kernel<T><<<(unsigned)ceil_div(out, 256), 256, 0, s>>>(split + in * out, (int)p.splits, in * out + out,
+                                                                        Mat{nullptr, 0, 1, 1}, a.grad_bias, biases);
+        return;
+    }
     Mat dz = a.grad_y;
     float* sums = (float*)(workspace + p.dz_bytes);
     float* partial = (float*)(workspace + p.dz_bytes + p.sums_bytes);
@@ -316,7 +343,8 @@ void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) 
                 dz, a.x, a.grad_w, p.splits > 1 ? partial : nullptr, p.split_rows, ni, nj);
         });
         if (p.splits > 1) {
-            join_kernel<T><<<(unsigned)ceil_div(in * out, 256), 256, 0, s>>>(partial, (int)p.splits, a.grad_w);
+            join_kernel<T><<<(unsigned)ceil_div(in * out, 256), 256, 0, s>>>(partial, (int)p.splits, in * out, a.grad_w,
+                                                                             nullptr, 0);
         }
     }
 }

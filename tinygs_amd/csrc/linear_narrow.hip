@@ -1,0 +1,309 @@
+// The gradients of a narrow linear layer (rows of x and of dy up to 512 bytes:
+// 256 halves, 128 floats) in one pass over the rows: dz = dy act'(z) once from
+// memory, then dx = dz w and the workgroup's share of dw = dz^T x and db from
+// LDS. Bound by the bytes: dy, z and x are read once and dx is written once,
+// where a pass for dz and a product each for dx and dw would move 7 arrays of
+// the rows instead of 4.
+//
+// A workgroup of eight waves, one a compute unit, walks over blocks of 32 rows.
+// w stays in LDS (up to 128 KB), dw's float sums in the registers of the waves
+// (128 x 64 a wave for halves); a block's dz and x take 16 KB each. The next
+// block's dy, z and x are on their way into registers while a block is
+// multiplied. The workgroups' sums are joined by a second kernel in a fixed
+// order.
+//
+// LDS holds rows of 512 bytes whose 16-byte chunks are permuted by the row, so
+// that both reads are free of bank conflicts: 16 rows at one chunk
+// (K-contiguous: dz for dx), and runs of 16 elements of 4 rows at a time
+// (R-contiguous: w for dx, x and dz for dw).
+#include "mfma_tile.h"
+
+namespace tgs {
+
+namespace {
+
+constexpr int kPitch = 512;
+constexpr int kRows = 32;    // of a block
+constexpr int kThreads = 512;
+// Past the end of every block (32 rows of less than 2^23 bytes), also with an
+// offset within the block added, and that below 2^32.
+constexpr uint32_t kNowhere = 0xe0000000u;
+
+template <class T>
+struct Narrow {
+    static constexpr int V = 16 / (int)sizeof(T);          // elements of a chunk
+    static constexpr int kCols = kPitch / (int)sizeof(T);
+    static constexpr int kHalf = 64 / (int)sizeof(T);      // k of one multiply()
+    static constexpr int TI = kCols / 32, TJ = kCols / 64;   // dw squares of a wave: two waves on in, four on out
+    static constexpr int DI = kCols / 128;                 // dx squares of a wave on in
+    static constexpr int kWeights = kCols * kPitch;        // bytes of w
+    static constexpr int kLds = kWeights + 2 * kRows * kPitch;
+    typedef T loose __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+
+    // Sixteen rows take all sixteen chunk slots; the rows of one
+    // R-contiguous read (halves: 8 g + q, floats: 4 g + e) different runs.
+    static __device__ __forceinline__ int turn(int r) {
+        if constexpr (sizeof(T) == 4) return r & 15;
+        return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8);
+    }
+    static __device__ __forceinline__ int at(int r, int chunk) { return r * kPitch + ((chunk ^ turn(r)) << 4); }
+
+    // n (0 to V) elements at p, zeros after them; p is readable where n is 0.
+    static __device__ __forceinline__ loose gather(const T* p, int n) {
+        loose v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const T u = p[min(e, max(n - 1, 0))];
+            v[e] = e < n ? u : (T)0.0f;
+        }
+        return v;
+    }
+
+    static __device__ __forceinline__ typename Frag<T>::type k_fragment(const unsigned char* rows, int r0, int s, int lane) {
+        const int a = lane & 15, g = lane >> 4;
+        return *(const typename Frag<T>::type*)(rows + at(r0 + a, 4 * s + g));
+    }
+
+    // Columns c0 .. c0 + 15 of rows kHalf s .. + kHalf - 1.
+    static __device__ __forceinline__ typename Frag<T>::type r_fragment(const unsigned char* rows, int c0, int s, int lane) {
+        const int a = lane & 15, g = lane >> 4;
+        if constexpr (sizeof(T) == 2) {
+            const int q = a >> 2, k = 32 * s + 8 * g + q, chunk = c0 / 8 + ((a & 3) >> 1), in = (a & 1) * 8;
+            typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+            union {
+                i16x4 half[2];
+                typename Frag<T>::type whole;
+            } u;
+            u.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_byte*)(rows + at(k, chunk) + in));
+            u.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_byte*)(rows + at(k + 4, chunk) + in));
+            return u.whole;
+        } else {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[e] = *(const float*)(rows + at(16 * s + 4 * g + e, c0 / 4 + (a >> 2)) + (a & 3) * 4);
+            return v;
+        }
+    }
+};
+
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// partial + blockIdx.x * (out * in + out): the workgroup's dw and db.
+// RAGGED: in or out is no multiple of a chunk, so that chunks can be partial:
+// rows are gathered element by element. Else buffer loads give zeros where
+// nothing is, and stores there are dropped.
+template <class T, int ACT, bool RAGGED>
+__global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, float* partial, int blocks) {
+    using N = Narrow<T>;
+    constexpr int V = N::V;
+    __shared__ __align__(1024) unsigned char lds[N::kLds];
+    unsigned char *const w = lds, *const dz = lds + N::kWeights, *const xs = dz + kRows * kPitch;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int in = (int)a.x.cols, out = (int)a.grad_y.cols;
+    const int64_t rows = a.grad_y.rows;
+
+    // a thread's chunk of the columns, and its rows of a block: r and r + 16
+    const int chunk = tid & 31, r = tid >> 5;
+    const int n_in = min(max(in - chunk * V, 0), V), n_out = min(max(out - chunk * V, 0), V);
+
+    // A matrix's 32 rows (from `first` on) as this thread's two chunks.
+    const auto fetch = [&](const Mat& m, int64_t first, int n, typename N::loose(&to)[2]) {
+        const T* base = (const T*)m.p + first * m.stride;
+        if constexpr (RAGGED) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = r + 16 * h;
+                const bool exists = first + row < m.rows && n > 0;
+                to[h] = N::gather(exists ? base + row * m.stride + chunk * V : (const T*)m.p, exists ? n : 0);
+            }
+            return;
+        }
+        const int64_t pitch = m.stride * (int64_t)sizeof(T);
+        const auto buffer = resource_of(base, (min(m.rows - first, (int64_t)kRows) - 1) * pitch + m.cols * (int64_t)sizeof(T));
+        const uint32_t from = (n > 0 ? 0u : kNowhere) + (uint32_t)chunk * 16u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            to[h] = __builtin_bit_cast(typename N::loose, __builtin_amdgcn_raw_buffer_load_b128(
+                                                              buffer, (int)(from + (uint32_t)(r + 16 * h) * (uint32_t)pitch), 0, 0));
+    };
+
+    if (a.grad_x.p)
+        for (int n = 0; n < (out > 4 * N::kHalf ? N::kCols : N::kCols / 2); n += kRows) {   // zeros past out
+            typename N::loose v[2];
+            fetch(a.w, n, n_in, v);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) *(typename N::loose*)(w + N::at(n + r + 16 * h, chunk)) = v[h];
+        }
+
+    typename N::loose dy[2], z[2], x[2];
+    const auto fetch_block = [&](int block) {
+        const int64_t first = (int64_t)block * kRows;
+        fetch(a.grad_y, first, n_out, dy);
+        if constexpr (ACT != kActNone) fetch(a.preact, first, n_out, z);
+        if (a.grad_w.p) fetch(a.x, first, n_in, x);
+    };
+
+    f32x4 acc[N::TI][N::TJ];
+#pragma unroll
+    for (int u = 0; u < N::TI; ++u)
+#pragma unroll
+        for (int v = 0; v < N::TJ; ++v) acc[u][v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float sum[V] = {};
+    const int wi = wave >> 2, wj = wave & 3;
+    const bool dw_here = a.grad_w.p && wi * N::TI * 16 < in && wj * N::TJ * 16 < out;
+    const bool dx_here = a.grad_x.p && wave * N::DI * 16 < in;
+    const bool deep = out > 4 * N::kHalf;
+
+    fetch_block(blockIdx.x);
+    for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
+        lds_barrier();   // the last block's reads are done
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (ACT != kActNone) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float d = (float)dy[h][e] * activate_slope<ACT>((float)z[h][e]);
+                    sum[e] += d;
+                    dy[h][e] = (T)d;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[e] += (float)dy[h][e];
+            }
+            *(typename N::loose*)(dz + N::at(r + 16 * h, chunk)) = dy[h];
+            if (a.grad_w.p) *(typename N::loose*)(xs + N::at(r + 16 * h, chunk)) = x[h];
+        }
+        lds_barrier();
+        if (block + (int)gridDim.x < blocks) fetch_block(block + gridDim.x);
+
+        // The addresses below are formed anew for each block: kept over the
+        // blocks they would take the registers of the sums.
+        int near = lane;
+        asm volatile("" : "+v"(near));
+        if (dx_here) {
+            f32x4 d[N::DI][2];
+#pragma unroll
+            for (int u = 0; u < N::DI; ++u) d[u][0] = d[u][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            typename Frag<T>::type fw[2][N::DI], fz[2][2];
+            const auto read = [&](int s, int to) {
+#pragma unroll
+                for (int u = 0; u < N::DI; ++u) fw[to][u] = N::r_fragment(w, (wave * N::DI + u) * 16, s, near);
+#pragma unroll
+                for (int v = 0; v < 2; ++v) fz[to][v] = N::k_fragment(dz, 16 * v, s, near);
+            };
+            const auto four = [&](int s0) {
+                read(s0, 0);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    if (s < 3) read(s0 + s + 1, (s + 1) & 1);
+#pragma unroll
+                    for (int u = 0; u < N::DI; ++u)
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) d[u][v] = multiply(fw[s & 1][u], fz[s & 1][v], d[u][v]);
+                }
+            };
+            four(0);
+            if (deep) four(4);
+            const int64_t first = (int64_t)block * kRows, pitch = a.grad_x.stride * (int64_t)sizeof(T);
+            T* const base = (T*)a.grad_x.p + first * a.grad_x.stride;
+            const auto buffer = resource_of(base, (min(rows - first, (int64_t)kRows) - 1) * pitch + in * (int64_t)sizeof(T));
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const int row = 16 * v + (lane & 15);
+                int i;
+                typename N::loose y;
+                if constexpr (N::DI == 2) {
+                    float f[8];
+                    neighbours(d[0][v], d[1][v], f);
+                    i = wave * 32 + neighbours_at(lane);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) y[e] = (T)f[e];
+                } else {
+                    i = wave * 16 + 4 * (lane >> 4);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) y[e] = (T)d[0][v][e];
+                }
+                if constexpr (!RAGGED) {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), buffer,
+                                                           (int)((i < in ? 0u : kNowhere) + (uint32_t)row * (uint32_t)pitch + (uint32_t)i * (uint32_t)sizeof(T)),
+                                                           0, 0);
+                } else if (first + row < rows) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (i + e < in) base[row * a.grad_x.stride + i + e] = y[e];
+                }
+            }
+        }
+        if (dw_here) {
+#pragma unroll
+            for (int s = 0; s < kRows / N::kHalf; ++s) {
+                typename Frag<T>::type fz[N::TJ];
+#pragma unroll
+                for (int v = 0; v < N::TJ; ++v) fz[v] = N::r_fragment(dz, (wj * N::TJ + v) * 16, s, near);
+#pragma unroll
+                for (int u = 0; u < N::TI; ++u) {
+                    const auto fx = N::r_fragment(xs, (wi * N::TI + u) * 16, s, near);
+#pragma unroll
+                    for (int v = 0; v < N::TJ; ++v) acc[u][v] = multiply(fx, fz[v], acc[u][v]);
+                }
+            }
+        }
+    }
+
+    float* to = partial + (int64_t)blockIdx.x * ((int64_t)out * in + out);
+    if (dw_here) {
+#pragma unroll
+        for (int u = 0; u < N::TI; ++u) {
+            const int i = (wi * N::TI + u) * 16 + 4 * (lane >> 4);
+#pragma unroll
+            for (int v = 0; v < N::TJ; ++v) {
+                const int j = (wj * N::TJ + v) * 16 + (lane & 15);
+                if (j >= out) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + e < in) to[j * in + i + e] = acc[u][v][e];
+            }
+        }
+    }
+    if (a.grad_bias) {   // the sixteen threads of a chunk, in order
+        float* s = (float*)lds;
+        lds_barrier();
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[r * N::kCols + chunk * V + e] = sum[e];
+        lds_barrier();
+        for (int k = tid; k < out; k += kThreads) {
+            float v = s[k];
+            for (int q = 1; q < 16; ++q) v += s[q * N::kCols + k];
+            to[(int64_t)out * in + k] = v;
+        }
+    }
+}
+
+}  // namespace
+
+bool linear_backward_is_narrow(const LinearBackward& a) {
+    const int64_t most = kPitch / (a.dtype == TGS_DTYPE_FLOAT32 ? 4 : 2);
+    return a.x.cols <= most && a.grad_y.cols <= most && a.grad_y.rows > 0 && a.grad_y.rows < ((int64_t)1 << 35);
+}
+
+int narrow_backward_splits(const LinearBackward& a) {
+    const int64_t blocks = (a.grad_y.rows + kRows - 1) / kRows;
+    return (int)(blocks < 256 ? blocks : 256);
+}
+
+void launch_narrow_backward(const LinearBackward& a, float* partial, hipStream_t s) {
+    const int blocks = (int)((a.grad_y.rows + kRows - 1) / kRows);
+    by_dtype(a.dtype, [&](auto t) {
+        by_activation(a.activation, [&](auto act) {
+            using T = decltype(t);
+            constexpr int kAct = decltype(act)::value;
+            if (a.x.cols % Narrow<T>::V || a.grad_y.cols % Narrow<T>::V)
+                backward_kernel<T, kAct, true><<<narrow_backward_splits(a), kThreads, 0, s>>>(a, partial, blocks);
+            else
+                backward_kernel<T, kAct, false><<<narrow_backward_splits(a), kThreads, 0, s>>>(a, partial, blocks);
+        });
+    });
+}
+
+}  // namespace tgs

@@ -86,6 +86,14 @@ __device__ __forceinline__ i32x4 buffer_of(const void* p, int64_t bytes) {
     return r;
 }
 
+// The same for the compiler's own buffer loads and stores. A load past the end
+// gives zeros and a store there is dropped, so that edges need no branches.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource_of(const void* p, int64_t bytes) {
+    const uint32_t n = bytes <= 0 ? 0u : bytes < (int64_t)kPastEnd ? (uint32_t)bytes : kPastEnd;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)n, 0x00020000);
+}
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 // One operand's side of a tile: R rows (i or j), loaded by WAVES waves, STEP
 // bytes of k a step.
 template <class T, int R, int WAVES, bool RC, int STEP = 128>

@@ -53,47 +53,40 @@ void by_activation(int activation, F f) {
 
 enum Activation { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
 
-// logistic(v) = 1 / (1 + 2^(-v log2 e)). The exponent's rounding error, up to
-// 2^-24 |v log2 e|, is put back to first order (2^(t + d) = 2^t (1 + d ln 2)),
-// so the result is good to a few units of the last place for every v. Where
-// 2^-t overflows the reciprocal is 0, the limit.
-__device__ __forceinline__ float logistic(float v) {
-    constexpr float kLog2e = 0x1.715476p+0f;        // log2(e) = kLog2e + kLog2eTail
-    constexpr float kLog2eTail = 0x1.4ae0bep-26f;
-    constexpr float kLn2 = 0x1.62e430p-1f;
-    const float t = -v * kLog2e;
-    const float d = fmaf(-v, kLog2e, -t) - v * kLog2eTail;
-    float e = __builtin_amdgcn_exp2f(t);
-    const float c = e * (d * kLn2);
-    e = fabsf(t) < 126.0f ? e + c : e;
-    return __builtin_amdgcn_rcpf(1.0f + e);
+// 1 / (1 + 2^t): the logistic of v for t = -v log2 e. Off by |t| 2^-24 of
+// itself (t's rounding) and a few units of the last place; where 2^t overflows
+// the reciprocal is 0, the limit. A step that put t's rounding back made the
+// activations half as long again and moved no stored half.
+__device__ __forceinline__ float logistic2(float t) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
 }
 
+constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kGelu1 = 1.5957691216057308f;    // 2 sqrt(2 / pi): 1 + tanh(u) = 2 logistic(2 u)
 constexpr float kGelu3 = 0.071354816272600256f;  // 2 sqrt(2 / pi) 0.044715
 
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
     if constexpr (ACT == kActRelu) return z < 0.0f ? 0.0f : z;   // NaN stays NaN
-    if constexpr (ACT == kActSilu) return z * logistic(z);
-    if constexpr (ACT == kActGelu) return z * logistic(z * fmaf(kGelu3 * z, z, kGelu1));
+    if constexpr (ACT == kActSilu) return z * logistic2(-kLog2E * z);
+    if constexpr (ACT == kActGelu) return z * logistic2(z * fmaf(-kLog2E * kGelu3, z * z, -kLog2E * kGelu1));
     return z;
 }
 
 // act'(z) = p + z p (1 - p) (d/dz of p's argument). The second term is zero in
-// 32 bits well inside the clamps, which keep it from becoming 0 * infinity.
+// 32 bits well inside the bounds on z and z^2, which keep it from becoming
+// 0 * infinity; p itself keeps a NaN.
 template <int ACT>
 __device__ __forceinline__ float activate_slope(float z) {
     if constexpr (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
     if constexpr (ACT == kActSilu) {
-        const float p = logistic(z);
-        const float c = fminf(fmaxf(z, -100.0f), 100.0f);
-        return fmaf(c * p, 1.0f - p, p);
+        const float p = logistic2(-kLog2E * z);
+        return fmaf(fmaxf(z, -100.0f) * p, 1.0f - p, p);
     }
     if constexpr (ACT == kActGelu) {
-        const float c = fminf(fmaxf(z, -30.0f), 30.0f);
-        const float p = logistic(z * fmaf(kGelu3 * z, z, kGelu1));
-        return fmaf(c * p * (1.0f - p), fmaf(3.0f * kGelu3 * c, c, kGelu1), p);
+        const float q = fminf(z * z, 900.0f);
+        const float p = logistic2(z * fmaf(-kLog2E * kGelu3, q, -kLog2E * kGelu1));
+        return fmaf(fmaxf(z, -30.0f) * (p * (1.0f - p)), fmaf(3.0f * kGelu3, q, kGelu1), p);
     }
     return 1.0f;
 }
@@ -114,6 +107,13 @@ struct LinearBackward {
 size_t linear_backward_workspace(const LinearBackward& a);
 int launch_linear_forward(const LinearForward& a, hipStream_t s);
 int launch_linear_backward(const LinearBackward& a, void* workspace, hipStream_t s);
+
+// ---- linear_narrow.hip: the gradients of a layer whose rows are at most 512
+// bytes. Leaves `splits` sets of float sums, each out x in of grad_w and then
+// out of grad_bias.
+bool linear_backward_is_narrow(const LinearBackward& a);
+int narrow_backward_splits(const LinearBackward& a);
+void launch_narrow_backward(const LinearBackward& a, float* partial, hipStream_t s);
 
 // ---- layer_norm.hip
 struct LayerNormForward {
