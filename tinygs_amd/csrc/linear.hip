@@ -357,6 +357,11 @@ size_t linear_backward_workspace(const LinearBackward& a) {
 }
 
 int launch_linear_forward(const LinearForward& a, hipStream_t s) {
+    if (linear_forward_by_rows(a)) {
+        launch_linear_rows(a, s);
+        TGS_CHECK_LAUNCH();
+        return TGS_OK;
+    }
     by_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
         by_shape(a.y.cols, a.y.rows, 1, [&](auto shape) {

@@ -11,83 +11,24 @@
 // block's dy, z and x are on their way into registers while a block is
 // multiplied. The workgroups' sums are joined by a second kernel in a fixed
 // order.
-//
-// LDS holds rows of 512 bytes whose 16-byte chunks are permuted by the row, so
-// that both reads are free of bank conflicts: 16 rows at one chunk
-// (K-contiguous: dz for dx), and runs of 16 elements of 4 rows at a time
-// (R-contiguous: w for dx, x and dz for dw).
-#include "mfma_tile.h"
+#include "narrow_rows.h"
 
 namespace tgs {
 
 namespace {
 
 constexpr int kPitch = 512;
-constexpr int kRows = 32;    // of a block
+constexpr int kRows = 32;   // of a block
 constexpr int kThreads = 512;
-// Past the end of every block (32 rows of less than 2^23 bytes), also with an
-// offset within the block added, and that below 2^32.
-constexpr uint32_t kNowhere = 0xe0000000u;
 
 template <class T>
-struct Narrow {
-    static constexpr int V = 16 / (int)sizeof(T);          // elements of a chunk
-    static constexpr int kCols = kPitch / (int)sizeof(T);
-    static constexpr int kHalf = 64 / (int)sizeof(T);      // k of one multiply()
-    static constexpr int TI = kCols / 32, TJ = kCols / 64;   // dw squares of a wave: two waves on in, four on out
-    static constexpr int DI = kCols / 128;                 // dx squares of a wave on in
-    static constexpr int kWeights = kCols * kPitch;        // bytes of w
+struct Narrow : NarrowRows<T, kPitch> {
+    using N = NarrowRows<T, kPitch>;
+    static constexpr int TI = N::kCols / 32, TJ = N::kCols / 64;   // dw squares of a wave: two waves on in, four on out
+    static constexpr int DI = N::kCols / 128;                      // dx squares of a wave on in
+    static constexpr int kWeights = N::kCols * kPitch;             // bytes of w
     static constexpr int kLds = kWeights + 2 * kRows * kPitch;
-    typedef T loose __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-
-    // Sixteen rows take all sixteen chunk slots; the rows of one
-    // R-contiguous read (halves: 8 g + q, floats: 4 g + e) different runs.
-    static __device__ __forceinline__ int turn(int r) {
-        if constexpr (sizeof(T) == 4) return r & 15;
-        return ((r & 3) << 1) | ((r >> 2) & 1) | (r & 8);
-    }
-    static __device__ __forceinline__ int at(int r, int chunk) { return r * kPitch + ((chunk ^ turn(r)) << 4); }
-
-    // n (0 to V) elements at p, zeros after them; p is readable where n is 0.
-    static __device__ __forceinline__ loose gather(const T* p, int n) {
-        loose v;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const T u = p[min(e, max(n - 1, 0))];
-            v[e] = e < n ? u : (T)0.0f;
-        }
-        return v;
-    }
-
-    static __device__ __forceinline__ typename Frag<T>::type k_fragment(const unsigned char* rows, int r0, int s, int lane) {
-        const int a = lane & 15, g = lane >> 4;
-        return *(const typename Frag<T>::type*)(rows + at(r0 + a, 4 * s + g));
-    }
-
-    // Columns c0 .. c0 + 15 of rows kHalf s .. + kHalf - 1.
-    static __device__ __forceinline__ typename Frag<T>::type r_fragment(const unsigned char* rows, int c0, int s, int lane) {
-        const int a = lane & 15, g = lane >> 4;
-        if constexpr (sizeof(T) == 2) {
-            const int q = a >> 2, k = 32 * s + 8 * g + q, chunk = c0 / 8 + ((a & 3) >> 1), in = (a & 1) * 8;
-            typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-            union {
-                i16x4 half[2];
-                typename Frag<T>::type whole;
-            } u;
-            u.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_byte*)(rows + at(k, chunk) + in));
-            u.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_byte*)(rows + at(k + 4, chunk) + in));
-            return u.whole;
-        } else {
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[e] = *(const float*)(rows + at(16 * s + 4 * g + e, c0 / 4 + (a >> 2)) + (a & 3) * 4);
-            return v;
-        }
-    }
 };
-
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // partial + blockIdx.x * (out * in + out): the workgroup's dw and db.
 // RAGGED: in or out is no multiple of a chunk, so that chunks can be partial:
@@ -128,14 +69,6 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
                                                               buffer, (int)(from + (uint32_t)(r + 16 * h) * (uint32_t)pitch), 0, 0));
     };
 
-    if (a.grad_x.p)
-        for (int n = 0; n < (out > 4 * N::kHalf ? N::kCols : N::kCols / 2); n += kRows) {   // zeros past out
-            typename N::loose v[2];
-            fetch(a.w, n, n_in, v);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) *(typename N::loose*)(w + N::at(n + r + 16 * h, chunk)) = v[h];
-        }
-
     typename N::loose dy[2], z[2], x[2];
     const auto fetch_block = [&](int block) {
         const int64_t first = (int64_t)block * kRows;
@@ -143,6 +76,24 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
         if constexpr (ACT != kActNone) fetch(a.preact, first, n_out, z);
         if (a.grad_w.p) fetch(a.x, first, n_in, x);
     };
+
+    fetch_block(blockIdx.x);
+    const bool deep = out > 4 * N::kHalf;
+    if (a.grad_x.p) {   // zeros past out, up to the half that dx reads
+        constexpr int kQuarters = N::kCols / kRows / 2;
+        const auto place = [&](int n0) {
+            typename N::loose v[kQuarters][2];
+#pragma unroll
+            for (int q = 0; q < kQuarters; ++q) fetch(a.w, n0 + kRows * q, n_in, v[q]);
+#pragma unroll
+            for (int q = 0; q < kQuarters; ++q)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *(typename N::loose*)(w + N::at(n0 + kRows * q + r + 16 * h, chunk)) = v[q][h];
+        };
+        place(0);
+        if (deep) place(N::kCols / 2);
+    }
 
     f32x4 acc[N::TI][N::TJ];
 #pragma unroll
@@ -153,9 +104,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
     const int wi = wave >> 2, wj = wave & 3;
     const bool dw_here = a.grad_w.p && wi * N::TI * 16 < in && wj * N::TJ * 16 < out;
     const bool dx_here = a.grad_x.p && wave * N::DI * 16 < in;
-    const bool deep = out > 4 * N::kHalf;
 
-    fetch_block(blockIdx.x);
     for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
         lds_barrier();   // the last block's reads are done
 #pragma unroll
@@ -253,16 +202,26 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
 
     float* to = partial + (int64_t)blockIdx.x * ((int64_t)out * in + out);
     if (dw_here) {
+        const auto buffer = resource_of(to, (int64_t)out * in * 4);   // at most 256 KB
+        const bool fours = in % 4 == 0;
 #pragma unroll
         for (int u = 0; u < N::TI; ++u) {
             const int i = (wi * N::TI + u) * 16 + 4 * (lane >> 4);
 #pragma unroll
             for (int v = 0; v < N::TJ; ++v) {
                 const int j = (wj * N::TJ + v) * 16 + (lane & 15);
-                if (j >= out) continue;
+                const uint32_t at = (uint32_t)(j * in + i) * 4u;
+                if (fours) {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[u][v]), buffer,
+                                                           (int)(at + (i < in ? 0u : kNowhere)), 0, 0);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (i + e < in) to[j * in + i + e] = acc[u][v][e];
+                    for (int e = 0; e < 4; ++e) {
+                        const float f = acc[u][v][e];
+                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, f), buffer,
+                                                              (int)(at + 4u * e + (i + e < in ? 0u : kNowhere)), 0, 0);
+                    }
+                }
             }
         }
     }
@@ -288,8 +247,9 @@ bool linear_backward_is_narrow(const LinearBackward& a) {
 }
 
 int narrow_backward_splits(const LinearBackward& a) {
-    const int64_t blocks = (a.grad_y.rows + kRows - 1) / kRows;
-    return (int)(blocks < 256 ? blocks : 256);
+    // a workgroup's sums are worth four blocks
+    const int64_t want = (a.grad_y.rows + 4 * kRows - 1) / (4 * kRows);
+    return (int)(want < 256 ? want : 256);
 }
 
 void launch_narrow_backward(const LinearBackward& a, float* partial, hipStream_t s) {

@@ -108,6 +108,10 @@ size_t linear_backward_workspace(const LinearBackward& a);
 int launch_linear_forward(const LinearForward& a, hipStream_t s);
 int launch_linear_backward(const LinearBackward& a, void* workspace, hipStream_t s);
 
+// ---- linear_rows.hip: many rows of a narrow layer
+bool linear_forward_by_rows(const LinearForward& a);
+void launch_linear_rows(const LinearForward& a, hipStream_t s);
+
 // ---- linear_narrow.hip: the gradients of a layer whose rows are at most 512
 // bytes. Leaves `splits` sets of float sums, each out x in of grad_w and then
 // out of grad_bias.
