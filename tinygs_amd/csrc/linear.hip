@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(S::kThreads) forward_kernel(LinearForward a, u
     const int64_t i0 = (int64_t)ti * S::kI, j0 = (int64_t)tj * S::kJ;
     f32x4 acc[S::kSquaresI][S::kSquaresJ];
     P::run(lds, {a.w.p, a.w.rows, a.w.cols, a.w.stride}, {a.x.p, a.x.rows, a.x.cols, a.x.stride}, i0, j0, 0, a.x.cols,
-           acc, [](auto&) {});
+           acc);
     if (a.activation == kActGelu) forward_outputs<T, kActGelu, S>(a, acc, i0, j0);
     else if (a.activation == kActSilu) forward_outputs<T, kActSilu, S>(a, acc, i0, j0);
     else if (a.activation == kActRelu) forward_outputs<T, kActRelu, S>(a, acc, i0, j0);
@@ -134,8 +134,7 @@ __global__ void __launch_bounds__(S::kThreads) grad_x_kernel(Mat dz, Mat w, Mat 
     tile_of(xcd_contiguous_index(blockIdx.x, ni * nj), ni, nj, ti, tj);
     const int64_t i0 = (int64_t)ti * S::kI, j0 = (int64_t)tj * S::kJ;
     f32x4 acc[S::kSquaresI][S::kSquaresJ];
-    P::run(lds, {w.p, w.rows, w.cols, w.stride}, {dz.p, dz.rows, dz.cols, dz.stride}, i0, j0, 0, w.rows, acc,
-           [](auto&) {});
+    P::run(lds, {w.p, w.rows, w.cols, w.stride}, {dz.p, dz.rows, dz.cols, dz.stride}, i0, j0, 0, w.rows, acc);
     for_outputs<S>(acc, i0, j0, gx.cols, gx.rows, [&](int64_t i, int64_t j, int n, float (&v)[8]) {
         store8((T*)gx.p + j * gx.stride + i, n, v);
     });
@@ -153,8 +152,7 @@ __global__ void __launch_bounds__(S::kThreads) grad_w_kernel(Mat dz, Mat x, Mat 
     const int64_t i0 = (int64_t)ti * S::kI, j0 = (int64_t)tj * S::kJ;
     const int64_t k0 = (int64_t)blockIdx.y * split_rows, k1 = min(k0 + split_rows, x.rows);
     f32x4 acc[S::kSquaresI][S::kSquaresJ];
-    P::run(lds, {x.p, x.rows, x.cols, x.stride}, {dz.p, dz.rows, dz.cols, dz.stride}, i0, j0, k0, k1, acc,
-           [](auto&) {});
+    P::run(lds, {x.p, x.rows, x.cols, x.stride}, {dz.p, dz.rows, dz.cols, dz.stride}, i0, j0, k0, k1, acc);
     float* out = partial ? partial + (int64_t)blockIdx.y * gw.rows * gw.cols : nullptr;
     for_outputs<S>(acc, i0, j0, gw.cols, gw.rows, [&](int64_t i, int64_t j, int n, float (&v)[8]) {
         if (out) store8(out + j * gw.cols + i, n, v);

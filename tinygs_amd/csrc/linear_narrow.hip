@@ -17,17 +17,65 @@ namespace tgs {
 
 namespace {
 
-constexpr int kPitch = 512;
+template <class T>
+struct Plane {
+    using type = T;
+};
+template <>
+struct Plane<float> {
+    using type = __bf16;
+};
+
 constexpr int kRows = 32;   // of a block
 constexpr int kThreads = 512;
 
+// Matrices in LDS: halves as they are, in rows of 512 bytes; floats as the
+// three bfloat16 planes of split3, each of rows of 256 bytes, split once as
+// they are placed.
 template <class T>
-struct Narrow : NarrowRows<T, kPitch> {
-    using N = NarrowRows<T, kPitch>;
-    static constexpr int TI = N::kCols / 32, TJ = N::kCols / 64;   // dw squares of a wave: two waves on in, four on out
-    static constexpr int DI = N::kCols / 128;                      // dx squares of a wave on in
-    static constexpr int kWeights = N::kCols * kPitch;             // bytes of w
-    static constexpr int kLds = kWeights + 2 * kRows * kPitch;
+struct Narrow {
+    using C = Chunk<T>;
+    static constexpr int V = C::V;
+    static constexpr int kCols = 512 / (int)sizeof(T);
+    static constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1, kPitch = sizeof(T) == 4 ? 256 : 512;
+    using E = typename Plane<T>::type;
+    using R = NarrowRows<E, kPitch>;
+    static constexpr int kSteps = kCols / 32;               // of dx's k
+    static constexpr int TI = kCols / 32, TJ = kCols / 64;  // dw squares of a wave: two waves on in, four on out
+    static constexpr int DI = kCols / 128;                  // dx squares of a wave on in
+    static constexpr int kWeightPlane = kCols * kPitch, kBlockPlane = kRows * kPitch;
+    static constexpr int kWeights = kPlanes * kWeightPlane, kBlock = kPlanes * kBlockPlane;
+    static constexpr int kLds = kWeights + 2 * kBlock;
+    typedef typename C::type chunk;
+    typedef typename Frag<T>::type frag;
+
+    // A chunk of row r at its place: 16 bytes, or 8 in each plane.
+    static __device__ __forceinline__ void place(unsigned char* rows, int plane, int r, int c, const chunk& v) {
+        if constexpr (sizeof(T) == 2) {
+            *(chunk*)(rows + R::at(r, c)) = v;
+        } else {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            u32x2 p[3];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = v[2 * e], y = v[2 * e + 1];
+#pragma unroll
+                for (int q = 0; q < 3; ++q) p[q][e] = take_bf16(x, y);
+            }
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *(u32x2*)(rows + q * plane + R::at(r, c / 2) + (c & 1) * 8) = p[q];
+        }
+    }
+    static __device__ __forceinline__ frag k_fragment(const unsigned char* rows, int plane, int r0, int s, int lane) {
+        if constexpr (sizeof(T) == 2) return R::k_fragment(rows, r0, s, lane);
+        else return frag{R::k_fragment(rows, r0, s, lane), R::k_fragment(rows + plane, r0, s, lane),
+                         R::k_fragment(rows + 2 * plane, r0, s, lane)};
+    }
+    static __device__ __forceinline__ frag r_fragment(const unsigned char* rows, int plane, int c0, int s, int lane) {
+        if constexpr (sizeof(T) == 2) return R::r_fragment(rows, c0, s, lane);
+        else return frag{R::r_fragment(rows, c0, s, lane), R::r_fragment(rows + plane, c0, s, lane),
+                         R::r_fragment(rows + 2 * plane, c0, s, lane)};
+    }
 };
 
 // partial + blockIdx.x * (out * in + out): the workgroup's dw and db.
@@ -39,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
     using N = Narrow<T>;
     constexpr int V = N::V;
     __shared__ __align__(1024) unsigned char lds[N::kLds];
-    unsigned char *const w = lds, *const dz = lds + N::kWeights, *const xs = dz + kRows * kPitch;
+    unsigned char *const w = lds, *const dz = lds + N::kWeights, *const xs = dz + N::kBlock;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int in = (int)a.x.cols, out = (int)a.grad_y.cols;
     const int64_t rows = a.grad_y.rows;
@@ -49,14 +97,14 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
     const int n_in = min(max(in - chunk * V, 0), V), n_out = min(max(out - chunk * V, 0), V);
 
     // A matrix's 32 rows (from `first` on) as this thread's two chunks.
-    const auto fetch = [&](const Mat& m, int64_t first, int n, typename N::loose(&to)[2]) {
+    const auto fetch = [&](const Mat& m, int64_t first, int n, typename N::chunk(&to)[2]) {
         const T* base = (const T*)m.p + first * m.stride;
         if constexpr (RAGGED) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int row = r + 16 * h;
                 const bool exists = first + row < m.rows && n > 0;
-                to[h] = N::gather(exists ? base + row * m.stride + chunk * V : (const T*)m.p, exists ? n : 0);
+                to[h] = N::C::gather(exists ? base + row * m.stride + chunk * V : (const T*)m.p, exists ? n : 0);
             }
             return;
         }
@@ -65,11 +113,11 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
         const uint32_t from = (n > 0 ? 0u : kNowhere) + (uint32_t)chunk * 16u;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            to[h] = __builtin_bit_cast(typename N::loose, __builtin_amdgcn_raw_buffer_load_b128(
+            to[h] = __builtin_bit_cast(typename N::chunk, __builtin_amdgcn_raw_buffer_load_b128(
                                                               buffer, (int)(from + (uint32_t)(r + 16 * h) * (uint32_t)pitch), 0, 0));
     };
 
-    typename N::loose dy[2], z[2], x[2];
+    typename N::chunk dy[2], z[2], x[2];
     const auto fetch_block = [&](int block) {
         const int64_t first = (int64_t)block * kRows;
         fetch(a.grad_y, first, n_out, dy);
@@ -78,18 +126,18 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
     };
 
     fetch_block(blockIdx.x);
-    const bool deep = out > 4 * N::kHalf;
+    const bool deep = out > N::kCols / 2;
     if (a.grad_x.p) {   // zeros past out, up to the half that dx reads
         constexpr int kQuarters = N::kCols / kRows / 2;
         const auto place = [&](int n0) {
-            typename N::loose v[kQuarters][2];
+            typename N::chunk v[kQuarters][2];
 #pragma unroll
             for (int q = 0; q < kQuarters; ++q) fetch(a.w, n0 + kRows * q, n_in, v[q]);
 #pragma unroll
             for (int q = 0; q < kQuarters; ++q)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    *(typename N::loose*)(w + N::at(n0 + kRows * q + r + 16 * h, chunk)) = v[q][h];
+                    N::place(w, N::kWeightPlane, n0 + kRows * q + r + 16 * h, chunk, v[q][h]);
         };
         place(0);
         if (deep) place(N::kCols / 2);
@@ -120,8 +168,8 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
 #pragma unroll
                 for (int e = 0; e < V; ++e) sum[e] += (float)dy[h][e];
             }
-            *(typename N::loose*)(dz + N::at(r + 16 * h, chunk)) = dy[h];
-            if (a.grad_w.p) *(typename N::loose*)(xs + N::at(r + 16 * h, chunk)) = x[h];
+            N::place(dz, N::kBlockPlane, r + 16 * h, chunk, dy[h]);
+            if (a.grad_w.p) N::place(xs, N::kBlockPlane, r + 16 * h, chunk, x[h]);
         }
         lds_barrier();
         if (block + (int)gridDim.x < blocks) fetch_block(block + gridDim.x);
@@ -134,26 +182,26 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
             f32x4 d[N::DI][2];
 #pragma unroll
             for (int u = 0; u < N::DI; ++u) d[u][0] = d[u][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            typename Frag<T>::type fw[2][N::DI], fz[2][2];
+            typename N::frag fw[2][N::DI], fz[2][2];
             const auto read = [&](int s, int to) {
 #pragma unroll
-                for (int u = 0; u < N::DI; ++u) fw[to][u] = N::r_fragment(w, (wave * N::DI + u) * 16, s, near);
+                for (int u = 0; u < N::DI; ++u) fw[to][u] = N::r_fragment(w, N::kWeightPlane, (wave * N::DI + u) * 16, s, near);
 #pragma unroll
-                for (int v = 0; v < 2; ++v) fz[to][v] = N::k_fragment(dz, 16 * v, s, near);
+                for (int v = 0; v < 2; ++v) fz[to][v] = N::k_fragment(dz, N::kBlockPlane, 16 * v, s, near);
             };
-            const auto four = [&](int s0) {
+            const auto half = [&](int s0) {
                 read(s0, 0);
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    if (s < 3) read(s0 + s + 1, (s + 1) & 1);
+                for (int s = 0; s < N::kSteps / 2; ++s) {
+                    if (s < N::kSteps / 2 - 1) read(s0 + s + 1, (s + 1) & 1);
 #pragma unroll
                     for (int u = 0; u < N::DI; ++u)
 #pragma unroll
                         for (int v = 0; v < 2; ++v) d[u][v] = multiply(fw[s & 1][u], fz[s & 1][v], d[u][v]);
                 }
             };
-            four(0);
-            if (deep) four(4);
+            half(0);
+            if (deep) half(N::kSteps / 2);
             const int64_t first = (int64_t)block * kRows, pitch = a.grad_x.stride * (int64_t)sizeof(T);
             T* const base = (T*)a.grad_x.p + first * a.grad_x.stride;
             const auto buffer = resource_of(base, (min(rows - first, (int64_t)kRows) - 1) * pitch + in * (int64_t)sizeof(T));
@@ -161,7 +209,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
             for (int v = 0; v < 2; ++v) {
                 const int row = 16 * v + (lane & 15);
                 int i;
-                typename N::loose y;
+                typename N::chunk y;
                 if constexpr (N::DI == 2) {
                     float f[8];
                     neighbours(d[0][v], d[1][v], f);
@@ -185,17 +233,14 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
             }
         }
         if (dw_here) {
+            typename N::frag fz[N::TJ];
 #pragma unroll
-            for (int s = 0; s < kRows / N::kHalf; ++s) {
-                typename Frag<T>::type fz[N::TJ];
+            for (int v = 0; v < N::TJ; ++v) fz[v] = N::r_fragment(dz, N::kBlockPlane, (wj * N::TJ + v) * 16, 0, near);
 #pragma unroll
-                for (int v = 0; v < N::TJ; ++v) fz[v] = N::r_fragment(dz, (wj * N::TJ + v) * 16, s, near);
+            for (int u = 0; u < N::TI; ++u) {
+                const auto fx = N::r_fragment(xs, N::kBlockPlane, (wi * N::TI + u) * 16, 0, near);
 #pragma unroll
-                for (int u = 0; u < N::TI; ++u) {
-                    const auto fx = N::r_fragment(xs, (wi * N::TI + u) * 16, s, near);
-#pragma unroll
-                    for (int v = 0; v < N::TJ; ++v) acc[u][v] = multiply(fx, fz[v], acc[u][v]);
-                }
+                for (int v = 0; v < N::TJ; ++v) acc[u][v] = multiply(fx, fz[v], acc[u][v]);
             }
         }
     }
@@ -242,7 +287,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
 }  // namespace
 
 bool linear_backward_is_narrow(const LinearBackward& a) {
-    const int64_t most = kPitch / (a.dtype == TGS_DTYPE_FLOAT32 ? 4 : 2);
+    const int64_t most = 512 / (a.dtype == TGS_DTYPE_FLOAT32 ? 4 : 2);
     return a.x.cols <= most && a.grad_y.cols <= most && a.grad_y.rows > 0 && a.grad_y.rows < ((int64_t)1 << 35);
 }
 
@@ -258,7 +303,7 @@ void launch_narrow_backward(const LinearBackward& a, float* partial, hipStream_t
         by_activation(a.activation, [&](auto act) {
             using T = decltype(t);
             constexpr int kAct = decltype(act)::value;
-            if (a.x.cols % Narrow<T>::V || a.grad_y.cols % Narrow<T>::V)
+            if (a.x.cols % Chunk<T>::V || a.grad_y.cols % Chunk<T>::V)
                 backward_kernel<T, kAct, true><<<narrow_backward_splits(a), kThreads, 0, s>>>(a, partial, blocks);
             else
                 backward_kernel<T, kAct, false><<<narrow_backward_splits(a), kThreads, 0, s>>>(a, partial, blocks);

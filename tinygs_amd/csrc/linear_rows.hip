@@ -3,11 +3,11 @@
 // preact and y.
 //
 // w stays in registers: each of a workgroup's eight waves holds the fragments
-// of its columns (32 halves or 16 floats wide) for all of k, and the workgroup
+// of its 32 columns for all of k, and the workgroup
 // walks over blocks of 64 rows, so that w is read once a workgroup and not once
-// a tile. x and the residual come to LDS without passing registers, the next
-// block's while the current one is multiplied; the wait for them leaves the
-// stores of the block before in flight. 1e6 x 256 -> 256 halves with gelu,
+// a tile. x and the residual come to LDS without passing registers, one to three
+// blocks ahead; the wait for a block leaves the loads and stores that were
+// started after it in flight. 1e6 x 256 -> 256 halves with gelu,
 // residual and preact: 2.05 GB.
 #include "narrow_rows.h"
 
@@ -18,20 +18,28 @@ namespace {
 constexpr int kRows = 64;
 constexpr int kThreads = 512;
 
+// Workgroups a compute unit holds: two where w's registers allow it.
+constexpr int resident(int size, int pitch, int cw) { return size == 2 && pitch == 256 && cw <= 4 ? 2 : 1; }
+
 // PITCH: bytes of a row of x in LDS. CW waves share the columns (COLS of them
 // a workgroup), 8 / CW the rows.
 template <class T, int PITCH, int CW, bool RESIDUAL>
 struct RowsKernel {
     using X = NarrowRows<T, PITCH>;
-    static constexpr int V = X::V;
-    static constexpr int kSquares = 32 / (int)sizeof(T) / 8;      // of columns a wave: 2 (halves), 1 (floats)
-    static constexpr int kCols = CW * kSquares * 16;
-    static constexpr int kResidualPitch = CW * 64;                // bytes of kCols elements
+    using C = Chunk<T>;
+    static constexpr int V = C::V;
+    static constexpr int kCols = CW * 32;                         // two squares a wave
+    static constexpr int kResidualPitch = kCols * (int)sizeof(T) < 256 ? 256 : kCols * (int)sizeof(T);
     using R = NarrowRows<T, kResidualPitch>;
     static constexpr int kRowSquares = 4 * CW / 8;                // of rows a wave
-    static constexpr int kSteps = PITCH / 64;
+    static constexpr int kStores = kRowSquares * 8 / V;           // of y a wave and block
+    static constexpr int kSteps = X::kCols / 32;
     static constexpr int kXBytes = kRows * PITCH, kStage = kXBytes + (RESIDUAL ? kRows * kResidualPitch : 0);
-    static constexpr int kLds = 2 * kStage;
+    static constexpr int kResident = resident((int)sizeof(T), PITCH, CW);
+    static constexpr int kStages = 160 * 1024 / kResident / kStage < 4 ? 160 * 1024 / kResident / kStage : 4;
+    static_assert(kStages >= 2, "two stages at least");
+    static constexpr int kLds = kStages * kStage;
+    static constexpr int kLoads = kStage / 1024 / 8;              // a wave and block
 
     // Rows `first` .. + 63 of m from column c0 on, as rows of PITCH2 bytes in
     // LDS. Chunks past m's columns are filled from what follows in memory,
@@ -55,8 +63,7 @@ struct RowsKernel {
             const uint32_t offset = (c * V < cols ? 0u : kNowhere) + (uint32_t)r * (uint32_t)pitch + (uint32_t)c * 16u;
             if (tail && last && c == cols / V) {
                 const T* p = base + (r < rows ? r : 0) * m.stride + c * V;
-                const auto v = F::gather(p, r < rows ? tail : 0);
-                *(typename F::loose*)(lds + slot * 16) = v;
+                *(typename C::type*)(lds + slot * 16) = C::gather(p, r < rows ? tail : 0);
             } else {
                 load_to_lds(to + (n * 8 + wave) * 1024, offset, buffer);
             }
@@ -65,14 +72,27 @@ struct RowsKernel {
 };
 
 template <int ACT>
-__device__ __forceinline__ void activate_all(float (&v)[8], int n) {
+__device__ __forceinline__ void activate_all(float (&v)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < n) v[e] = activate<ACT>(v[e]);
+    for (int e = 0; e < 8; ++e) v[e] = activate<ACT>(v[e]);
+}
+
+// Waits until at most n of the wave's memory operations are in flight (rounded
+// down to what there is an instruction for), then for the workgroup.
+__device__ __forceinline__ void wait_but_for(int n) {
+#define TGS_WAIT(N) \
+    case N / 4: asm volatile("s_waitcnt vmcnt(" #N ") lgkmcnt(0)" ::: "memory"); break;
+    switch (n / 4) {
+        TGS_WAIT(0) TGS_WAIT(4) TGS_WAIT(8) TGS_WAIT(12) TGS_WAIT(16) TGS_WAIT(20) TGS_WAIT(24) TGS_WAIT(28)
+        TGS_WAIT(32) TGS_WAIT(36) TGS_WAIT(40) TGS_WAIT(44) TGS_WAIT(48) TGS_WAIT(52) TGS_WAIT(56)
+        default: asm volatile("s_waitcnt vmcnt(60) lgkmcnt(0)" ::: "memory");
+    }
+#undef TGS_WAIT
+    asm volatile("s_barrier" ::: "memory");
 }
 
 template <class T, int PITCH, int CW, bool RESIDUAL>
-__global__ void __launch_bounds__(kThreads) rows_kernel(LinearForward a, int blocks) {
+__global__ void __launch_bounds__(kThreads, 2 * resident((int)sizeof(T), PITCH, CW)) rows_kernel(LinearForward a, int blocks) {
     using K = RowsKernel<T, PITCH, CW, RESIDUAL>;
     using X = typename K::X;
     constexpr int V = K::V;
@@ -83,77 +103,104 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(LinearForward a, int blo
     const int64_t out = a.y.cols, rows = a.y.rows, c0 = (int64_t)blockIdx.y * K::kCols;
     const Mat residual = a.residual;
 
+    int filled = 0;   // the stage that the next load fills
     const auto load = [&](int block) {
         const int64_t first = (int64_t)block * kRows;
-        unsigned char* stage = lds + ((block / gridDim.x) & 1) * K::kStage;
+        unsigned char* stage = lds + filled * K::kStage;
+        filled = filled + 1 < K::kStages ? filled + 1 : 0;
         const bool last = first + kRows >= rows;
         K::template load<X>(a.x, first, 0, stage, last, wave, lane);
         if constexpr (RESIDUAL) K::template load<typename K::R>(residual, first, c0, stage + K::kXBytes, last, wave, lane);
     };
-    load(blockIdx.x);
+#pragma unroll
+    for (int n = 0; n < K::kStages - 1; ++n)
+        if ((int)(blockIdx.x + n * gridDim.x) < blocks) load(blockIdx.x + n * gridDim.x);
 
     // w's fragments: columns c of y are rows of w
-    const int64_t column0 = c0 + wc * K::kSquares * 16;
-    typename Frag<T>::type fw[K::kSquares][K::kSteps];
+    const int64_t column0 = c0 + wc * 32;
+    typename Frag<T>::type fw[2][K::kSteps];
 #pragma unroll
-    for (int u = 0; u < K::kSquares; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int s = 0; s < K::kSteps; ++s) {
             const int64_t n = column0 + 16 * u + (lane & 15);
-            const int k = s * X::kHalf + (lane >> 4) * V;
-            const int left = n < out ? min(max(in - k, 0), V) : 0;
-            const T* p = (const T*)a.w.p + (n < out ? n : 0) * a.w.stride + (left > 0 ? k : 0);
-            if (in % V == 0) {
-                const auto v = *(const typename X::loose*)p;   // left is 0 or V; a whole chunk of row n or 0 is there
+            T x[8];
 #pragma unroll
-                for (int e = 0; e < V; ++e) fw[u][s][e] = left > 0 ? v[e] : (T)0.0f;
+            for (int h = 0; h < 8 / V; ++h) {
+                const int k = 32 * s + 8 * (lane >> 4) + V * h;
+                const int left = n < out ? min(max(in - k, 0), V) : 0;
+                const T* p = (const T*)a.w.p + (n < out ? n : 0) * a.w.stride + (left > 0 ? k : 0);
+                typename K::C::type v;
+                if (in % V == 0) {   // left is 0 or V, and row n or 0 has a whole chunk
+                    v = *(const typename K::C::type*)p;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[e] = left > 0 ? v[e] : (T)0.0f;
+                } else {
+                    v = K::C::gather(p, left);
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[V * h + e] = v[e];
+            }
+            if constexpr (sizeof(T) == 4) {
+                fw[u][s] = split3(x);
             } else {
-                const auto v = X::gather(p, left);
 #pragma unroll
-                for (int e = 0; e < V; ++e) fw[u][s][e] = v[e];
+                for (int e = 0; e < 8; ++e) fw[u][s][e] = x[e];
             }
         }
-    // a lane's run of V outputs: columns at .. at + V - 1 of y
-    const int64_t at = column0 + (K::kSquares == 2 ? neighbours_at(lane) : 4 * (lane >> 4));
-    const int exist = (int)min(max(out - at, (int64_t)0), (int64_t)V);
-    float bias[V];
+    // a lane's run of 8 outputs: columns at .. at + 7 of y
+    const int64_t at = column0 + neighbours_at(lane);
+    const int exist = (int)min(max(out - at, (int64_t)0), (int64_t)8);
+    float bias[8];
 #pragma unroll
-    for (int e = 0; e < V; ++e) bias[e] = a.bias && e < exist ? a.bias[at + e] : 0.0f;
-    // The chunk of x that ends k: lanes that hold it clear what follows.
-    const int tail = in % V, tail_step = in / X::kHalf;
-    const bool clears = tail && (lane >> 4) == in % X::kHalf / V;
+    for (int e = 0; e < 8; ++e) bias[e] = a.bias && e < exist ? a.bias[at + e] : 0.0f;
+    // Elements of x past k in the chunk that ends it are whatever follows in
+    // memory: they are cleared in the step that holds them.
+    const int tail_step = in % V ? in / 32 : -1, tail = in % 32 - 8 * (lane >> 4);
+    const auto clear = [&](auto& f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = e < tail ? f[e] : 0;
+    };
 
     const bool ragged = out % V != 0;
-    // a block's stores: these many at least are issued after the next block's loads
-    const int stores = ragged ? 0 : K::kRowSquares * (a.preact.p ? 2 : 1);
-    bool stored = false;
-    for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
-        // this block's loads are done when no more are in flight than the stores after them
-        if (!stored || stores == 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        else if (stores == K::kRowSquares) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(K::kRowSquares) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * K::kRowSquares) : "memory");
-        stored = true;
-        if (block + (int)gridDim.x < blocks) load(block + gridDim.x);
+    // A block's vector stores; ragged columns add some. Between a block's loads
+    // and its use: the stores of the kStages - 1 blocks before it (as far as
+    // there were any) and the loads of the kStages - 2 blocks after it.
+    const int stores = K::kStores * (a.preact.p ? 2 : 1);
+    const int step = (int)gridDim.x;
+    int before = 0, after = blocks > (int)blockIdx.x ? (blocks - 1 - (int)blockIdx.x) / step : 0, now = 0;
+    for (int block = blockIdx.x; block < blocks; block += step) {
+        wait_but_for(min(after, K::kStages - 2) * K::kLoads + before * stores);
+        before = before < K::kStages - 1 ? before + 1 : before;
+        if (after >= K::kStages - 1) load(block + (K::kStages - 1) * step);
+        --after;
 
-        const unsigned char* stage = lds + ((block / gridDim.x) & 1) * K::kStage;
-        f32x4 acc[K::kSquares][K::kRowSquares];
+        const unsigned char* stage = lds + now * K::kStage;
+        now = now + 1 < K::kStages ? now + 1 : 0;
+        f32x4 acc[2][K::kRowSquares];
 #pragma unroll
-        for (int u = 0; u < K::kSquares; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int v = 0; v < K::kRowSquares; ++v) acc[u][v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < K::kSteps; ++s) {
-            if (s == K::kSteps / 2 && in <= s * X::kHalf) break;   // w is zero there
+            if (s >= K::kSteps / 2 && in <= 32 * s) break;   // w is zero there
             typename Frag<T>::type fx[K::kRowSquares];
 #pragma unroll
             for (int v = 0; v < K::kRowSquares; ++v) {
                 fx[v] = X::k_fragment(stage, (wr * K::kRowSquares + v) * 16, s, lane);
-                if (s == tail_step && tail)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) fx[v][e] = clears && e >= tail ? (T)0.0f : fx[v][e];
+                if (s == tail_step) {
+                    if constexpr (sizeof(T) == 4) {
+                        clear(fx[v].high);
+                        clear(fx[v].middle);
+                        clear(fx[v].low);
+                    } else {
+                        clear(fx[v]);
+                    }
+                }
             }
 #pragma unroll
-            for (int u = 0; u < K::kSquares; ++u)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int v = 0; v < K::kRowSquares; ++v) acc[u][v] = multiply(fw[u][s], fx[v], acc[u][v]);
         }
@@ -169,36 +216,37 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(LinearForward a, int blo
         for (int v = 0; v < K::kRowSquares; ++v) {
             const int r = (wr * K::kRowSquares + v) * 16 + (lane & 15);
             float f[8];
-            if constexpr (K::kSquares == 2) {
-                neighbours(acc[0][v], acc[1][v], f);
-            } else {
+            neighbours(acc[0][v], acc[1][v], f);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] = acc[0][v][e];
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) f[e] += bias[e];
+            for (int e = 0; e < 8; ++e) f[e] += bias[e];
             const auto store = [&](const __amdgpu_buffer_rsrc_t& buffer, T* p, int64_t stride, int64_t pitch) {
-                typename X::loose o;
 #pragma unroll
-                for (int e = 0; e < V; ++e) o[e] = (T)f[e];
-                if (!ragged) {
-                    __builtin_amdgcn_raw_buffer_store_b128(
-                        __builtin_bit_cast(u32x4, o), buffer,
-                        (int)((exist > 0 ? 0u : kNowhere) + (uint32_t)r * (uint32_t)pitch + (uint32_t)at * (uint32_t)sizeof(T)), 0, 0);
-                } else if (r <= held) {
+                for (int h = 0; h < 8 / V; ++h) {
+                    typename K::C::type o;
 #pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (e < exist) p[r * stride + e] = o[e];
+                    for (int e = 0; e < V; ++e) o[e] = (T)f[V * h + e];
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), buffer,
+                                                           (int)((exist >= V * (h + 1) ? 0u : kNowhere) + (uint32_t)r * (uint32_t)pitch +
+                                                                 (uint32_t)(at + V * h) * (uint32_t)sizeof(T)),
+                                                           0, 0);
+                    if (ragged && exist > V * h && exist < V * (h + 1) && r <= held) {
+#pragma unroll
+                        for (int e = 0; e < V; ++e)
+                            if (V * h + e < exist) p[r * stride + V * h + e] = o[e];
+                    }
                 }
             };
             if (a.preact.p) store(z_buffer, z0, a.preact.stride, z_pitch);
-            if (a.activation == kActGelu) activate_all<kActGelu>(f, V);
-            else if (a.activation == kActSilu) activate_all<kActSilu>(f, V);
-            else if (a.activation == kActRelu) activate_all<kActRelu>(f, V);
+            if (a.activation == kActGelu) activate_all<kActGelu>(f);
+            else if (a.activation == kActSilu) activate_all<kActSilu>(f);
+            else if (a.activation == kActRelu) activate_all<kActRelu>(f);
             if constexpr (RESIDUAL) {
-                const auto q = *(const typename X::loose*)(stage + K::kXBytes + K::R::at(r, (int)(at - c0) / V));
 #pragma unroll
-                for (int e = 0; e < V; ++e) f[e] += (float)q[e];
+                for (int h = 0; h < 8 / V; ++h) {
+                    const auto q = *(const typename K::C::type*)(stage + K::kXBytes + K::R::at(r, (int)(at - c0) / V + h));
+#pragma unroll
+                    for (int e = 0; e < V; ++e) f[V * h + e] += (float)q[e];
+                }
             }
             store(y_buffer, y0, a.y.stride, y_pitch);
         }
@@ -221,10 +269,8 @@ void launch_linear_rows(const LinearForward& a, hipStream_t s) {
             constexpr int P = decltype(pitch)::value, CW = decltype(cw)::value;
             constexpr bool kResidual = decltype(residual)::value != 0;
             using K = RowsKernel<T, P, CW, kResidual>;
-            // as many workgroups as the card holds at once
-            constexpr int kResident = 160 * 1024 / K::kLds < 2 ? 1 : 2;
             const int across = (int)((a.y.cols + K::kCols - 1) / K::kCols);
-            const int want = 256 * kResident / across, down = blocks < want ? blocks : want;
+            const int want = 256 * K::kResident / across, down = blocks < want ? blocks : want;   // what the card holds at once
             rows_kernel<T, P, CW, kResidual><<<dim3((unsigned)down, (unsigned)across), kThreads, 0, s>>>(a, blocks);
         };
         const auto by_residual = [&](auto pitch, auto cw) {
@@ -232,8 +278,9 @@ void launch_linear_rows(const LinearForward& a, hipStream_t s) {
             else launch(pitch, cw, Constant<0>{});
         };
         const auto by_columns = [&](auto pitch) {
-            if (a.y.cols <= kMost / 2) by_residual(pitch, Constant<4>{});
-            else by_residual(pitch, Constant<8>{});
+            if (a.y.cols <= 64) by_residual(pitch, Constant<2>{});
+            else if (sizeof(T) == 4 || a.y.cols <= 128) by_residual(pitch, Constant<4>{});
+            else if constexpr (sizeof(T) == 2) by_residual(pitch, Constant<8>{});
         };
         if (a.x.cols <= kMost / 2) by_columns(Constant<256>{});
         else by_columns(Constant<512>{});

@@ -34,25 +34,58 @@ template <>
 struct Frag<__bf16> {
     typedef __bf16 type __attribute__((ext_vector_type(8)));
 };
+// A float is held as three bfloat16, high + middle + low: 24 bits in all, each
+// the nearest to what the ones before leave. Floats of 2^128 (1 - 2^-9) and
+// more count as infinite.
 template <>
 struct Frag<float> {
-    typedef f32x4 type;
+    typedef __bf16 plane __attribute__((ext_vector_type(8)));
+    struct type {
+        plane high, middle, low;
+    };
 };
 
-// One step's products of a 16 x 16 square: 32 of k for halves, 16 for floats
-// (four instructions, element e of each lane's chunk at a time; both operands
-// are read in the same order of k). Row 4 (lane / 16) + r of the square is in
-// register r, column lane % 16.
+// Two floats to their nearest bfloat16 (in one word: one conversion makes
+// both), and what is left of them.
+__device__ __forceinline__ uint32_t take_bf16(float& x, float& y) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const uint32_t u = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+    x -= __builtin_bit_cast(float, u << 16);
+    y -= __builtin_bit_cast(float, u & 0xffff0000u);
+    return u;
+}
+
+__device__ __forceinline__ Frag<float>::type split3(const float (&v)[8]) {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    words p[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float x = v[2 * e], y = v[2 * e + 1];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) p[q][e] = take_bf16(x, y);
+    }
+    return {__builtin_bit_cast(Frag<float>::plane, p[0]), __builtin_bit_cast(Frag<float>::plane, p[1]),
+            __builtin_bit_cast(Frag<float>::plane, p[2])};
+}
+
+// Products of a 16 x 16 square over 32 of k. Row 4 (lane / 16) + r of the
+// square is in register r, column lane % 16. Floats: six of the nine plane
+// products (the others are below 2^-25 of the whole), 96 cycles where the
+// matrix cores' float instructions take 256.
 __device__ __forceinline__ f32x4 multiply(Frag<_Float16>::type a, Frag<_Float16>::type b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x4 multiply(Frag<__bf16>::type a, Frag<__bf16>::type b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 multiply(f32x4 a, f32x4 b, f32x4 c) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
-    return c;
+__device__ __forceinline__ f32x4 multiply(const Frag<float>::type& a, const Frag<float>::type& b, f32x4 c) {
+    c = multiply(a.low, b.high, c);
+    c = multiply(a.high, b.low, c);
+    c = multiply(a.middle, b.middle, c);
+    c = multiply(a.middle, b.high, c);
+    c = multiply(a.high, b.middle, c);
+    return multiply(a.high, b.high, c);
 }
 
 // An operand of a launch. K-contiguous: `rows` of `cols` = k elements;
@@ -111,10 +144,10 @@ struct TileSide {
     // K-contiguous: lanes 0..15 read rows r .. r + 15 at one chunk, so chunks
     // are turned by the row (by every fourth where four rows fill the banks). R-contiguous: a read takes 4 (halves: 8) rows at
     // one run of 16 elements, so the runs are turned by what tells the rows
-    // apart; rows of 128 bytes already alternate between the banks' halves.
+    // (8 g + q, floats: 8 g + e at one e) apart; rows of 128 bytes already alternate between the banks' halves.
     static __device__ __forceinline__ int turn(int r) {
         if constexpr (!RC) return STEP == 128 ? r & 7 : (r >> 2) & 3;
-        if constexpr (sizeof(T) == 4) return ((r >> 2) & 3) << 2;
+        if constexpr (sizeof(T) == 4) return ((r >> 3) & 3) << 2;
         if constexpr (kRowBytes == 128) return (((r >> 1) & 1) | (((r >> 3) & 1) << 1)) << 1;
         return ((r & 3) | (((r >> 3) & 1) << 2)) << 1;
     }
@@ -181,12 +214,31 @@ struct TileSide {
         end -= step_bytes;
     }
 
-    // The fragment of rows r0 .. r0 + 15 (r0 a multiple of 16) at half step s.
+    static constexpr int kSubs = kDepth / 32;   // multiply()s of a step
+
+    // The fragment of rows r0 .. r0 + 15 (r0 a multiple of 16) at part s of a step.
     static __device__ __forceinline__ typename Frag<T>::type fragment(const unsigned char* lds, int r0, int s, int lane) {
         const int a = lane & 15, g = lane >> 4;
-        if constexpr (!RC) {
+        if constexpr (sizeof(T) == 4) {
+            float x[8];
+            if constexpr (!RC) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4 v = *(const f32x4*)(lds + (r0 + a) * STEP + (((2 * g + h) ^ turn(a)) << 4));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[4 * h + e] = v[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int k = 8 * g + e;
+                    x[e] = *(const float*)(lds + k * kRowBytes + (((r0 >> 4) ^ (turn(k) >> 2)) << 6) + a * 4);
+                }
+            }
+            return split3(x);
+        } else if constexpr (!RC) {
             return *(const typename Frag<T>::type*)(lds + (r0 + a) * STEP + (((4 * s + g) ^ turn(a)) << 4));
-        } else if constexpr (sizeof(T) == 2) {
+        } else {
             // the transposing read: lanes 4 q .. 4 q + 3 of 16 name row q's
             // four runs of 8 bytes, and lane l receives column l of the rows
             const int q = a >> 2, k = 32 * s + 8 * g + q;
@@ -200,14 +252,6 @@ struct TileSide {
             const int at4 = ((r0 >> 4) ^ (turn(8 * g + q + 4) >> 1)) * 32 + (a & 3) * 8;
             u.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds_byte*)(lds + (k + 4) * kRowBytes + at4));
             return u.whole;
-        } else {
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int k = 16 * s + 4 * g + e;
-                v[e] = *(const float*)(lds + k * kRowBytes + (((r0 >> 4) ^ (turn(k) >> 2)) << 6) + a * 4);
-            }
-            return v;
         }
     }
 };
@@ -240,9 +284,8 @@ struct Tile {
     static constexpr int kStage = A::kBytes + B::kBytes;
     static constexpr int kLds = 2 * kStage;
 
-    template <class F>
     static __device__ __forceinline__ void run(unsigned char* lds, const TileOperand& a, const TileOperand& b, int64_t i0,
-                                               int64_t j0, int64_t k0, int64_t k1, f32x4 (&acc)[TI][TJ], F also) {
+                                               int64_t j0, int64_t k0, int64_t k1, f32x4 (&acc)[TI][TJ]) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wi = wave / WJ, wj = wave % WJ;
         A sa;
@@ -268,17 +311,26 @@ struct Tile {
                 sb.load(next + A::kBytes, left, wave, lane);
             }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                typename Frag<T>::type fa[TI], fb[TJ];
+            for (int s = 0; s < A::kSubs; ++s) {
+                typename Frag<T>::type fb[TJ];
 #pragma unroll
                 for (int v = 0; v < TJ; ++v) fb[v] = B::fragment(now + A::kBytes, (wj * TJ + v) * 16, s, lane);
+                if constexpr (sizeof(T) == 4) {   // twelve registers a fragment: one of A at a time
 #pragma unroll
-                for (int u = 0; u < TI; ++u) fa[u] = A::fragment(now, (wi * TI + u) * 16, s, lane);
+                    for (int u = 0; u < TI; ++u) {
+                        const auto fa = A::fragment(now, (wi * TI + u) * 16, s, lane);
 #pragma unroll
-                for (int u = 0; u < TI; ++u)
+                        for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa, fb[v], acc[u][v]);
+                    }
+                } else {
+                    typename Frag<T>::type fa[TI];
 #pragma unroll
-                    for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[u], fb[v], acc[u][v]);
-                also(fb);
+                    for (int u = 0; u < TI; ++u) fa[u] = A::fragment(now, (wi * TI + u) * 16, s, lane);
+#pragma unroll
+                    for (int u = 0; u < TI; ++u)
+#pragma unroll
+                        for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[u], fb[v], acc[u][v]);
+                }
             }
         }
     }
