@@ -9,8 +9,11 @@
 // Operand tiles go from memory to LDS without passing registers: lane l of a
 // wave's load writes the 16 bytes at its LDS base + 16 l, from any byte
 // address and zeros when the address is past the buffer's end, which is how
-// edges are filled. Two stages: the loads of step t + 1 are in flight while
-// step t is multiplied; one barrier a step. LDS is read without conflicts
+// edges are filled. A ring of stages: the loads of the next steps are in
+// flight while a step is multiplied; one barrier a step. A step's fragments
+// are read into registers while the step before it is multiplied: read at its
+// own start, the matrix cores waited for LDS (16384 x 2048 -> 1024 gradients:
+// 75 us). LDS is read without conflicts
 // because the 16-byte chunks of a row are permuted by the row's number: the
 // lanes choose which chunk they fetch.
 #pragma once
@@ -103,7 +106,9 @@ __device__ __forceinline__ uint32_t lds_address(void* p) { return (uint32_t)(uin
 
 // 16 bytes a lane from buffer + offset to LDS at base + 16 lane.
 __device__ __forceinline__ void load_to_lds(uint32_t base, uint32_t offset, i32x4 buffer) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(base), "v"(offset),
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                     __builtin_amdgcn_readfirstlane(base)),
+                 "v"(offset),
                  "s"(buffer)
                  : "memory");
 }
@@ -256,9 +261,18 @@ struct TileSide {
     }
 };
 
-__device__ __forceinline__ void wait_all_and_barrier() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// Waits until at most n (0 to 3) groups of L of the wave's loads are in
+// flight and its LDS accesses are done, then for the workgroup.
+template <int L>
+__device__ __forceinline__ void wait_for_stage(int n) {
+    static_assert(3 * L < 64, "what the counter holds");
+    if (n > 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(3 * L) : "memory");
+    else if (n == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * L) : "memory");
+    else if (n == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(L) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
+
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Rows (4 registers) of squares t and t + 1 of a lane, exchanged between the
 // 16-lane rows so that the lane holds 8 neighbouring outputs: squares t, t + 1
@@ -274,15 +288,17 @@ __device__ __forceinline__ void neighbours(const f32x4& a, const f32x4& b, float
 __device__ __forceinline__ int neighbours_at(int lane) { return 8 * (lane >> 5) + 16 * ((lane >> 4) & 1); }
 
 // The tile at (i0, j0) over k in [k0, k1): acc[ti][tj] of each wave. `lds`
-// holds two stages. k0 is a multiple of a step.
-template <class T, int WI, int WJ, int TI, int TJ, bool A_RC, bool B_RC>
+// holds the stages. k0 is a multiple of a step.
+template <class T, int WI, int WJ, int TI, int TJ, bool A_RC, bool B_RC, int STEP, int STAGES>
 struct Tile {
     static constexpr int kWaves = WI * WJ, kThreads = 64 * kWaves;
     static constexpr int BI = WI * TI * 16, BJ = WJ * TJ * 16;
-    using A = TileSide<T, BI, kWaves, A_RC>;
-    using B = TileSide<T, BJ, kWaves, B_RC>;
+    using A = TileSide<T, BI, kWaves, A_RC, STEP>;
+    using B = TileSide<T, BJ, kWaves, B_RC, STEP>;
     static constexpr int kStage = A::kBytes + B::kBytes;
-    static constexpr int kLds = 2 * kStage;
+    static constexpr int kLds = STAGES * kStage;
+    static constexpr int kLoads = A::kLoads + B::kLoads;   // at least these many a wave and stage (gathers add some)
+    static_assert(STAGES >= 2 && STAGES <= 5, "");
 
     static __device__ __forceinline__ void run(unsigned char* lds, const TileOperand& a, const TileOperand& b, int64_t i0,
                                                int64_t j0, int64_t k0, int64_t k1, f32x4 (&acc)[TI][TJ]) {
@@ -297,41 +313,73 @@ struct Tile {
 #pragma unroll
             for (int v = 0; v < TJ; ++v) acc[u][v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         const int steps = (int)((k1 - k0 + A::kDepth - 1) / A::kDepth);
-        if (steps > 0) {
-            sa.load(lds, k1 - k0, wave, lane);
-            sb.load(lds + A::kBytes, k1 - k0, wave, lane);
-        }
-        for (int t = 0; t < steps; ++t) {
-            const unsigned char* now = lds + (t & 1) * kStage;
-            wait_all_and_barrier();
-            if (t + 1 < steps) {
-                unsigned char* next = lds + ((t + 1) & 1) * kStage;
-                const int64_t left = k1 - k0 - (int64_t)(t + 1) * A::kDepth;
-                sa.load(next, left, wave, lane);
-                sb.load(next + A::kBytes, left, wave, lane);
-            }
-#pragma unroll
-            for (int s = 0; s < A::kSubs; ++s) {
+        if (steps <= 0) return;
+        int64_t left = k1 - k0;   // of k from the next load on
+        unsigned char* fill = lds;
+        const auto load = [&] {
+            sa.load(fill, left, wave, lane);
+            sb.load(fill + A::kBytes, left, wave, lane);
+            left -= A::kDepth;
+            fill = fill + kStage < lds + kLds ? fill + kStage : lds;
+        };
+        const unsigned char* from = lds;   // the stage of the next read
+        if constexpr (sizeof(T) == 4) {
+            static_assert(STAGES == 2 && A::kSubs == 1, "");
+            load();
+            for (int t = 0; t < steps; ++t) {
+                wait_for_stage<kLoads>(0);
+                if (t + 1 < steps) load();
                 typename Frag<T>::type fb[TJ];
 #pragma unroll
-                for (int v = 0; v < TJ; ++v) fb[v] = B::fragment(now + A::kBytes, (wj * TJ + v) * 16, s, lane);
-                if constexpr (sizeof(T) == 4) {   // twelve registers a fragment: one of A at a time
+                for (int v = 0; v < TJ; ++v) fb[v] = B::fragment(from + A::kBytes, (wj * TJ + v) * 16, 0, lane);
 #pragma unroll
-                    for (int u = 0; u < TI; ++u) {
-                        const auto fa = A::fragment(now, (wi * TI + u) * 16, s, lane);
+                for (int u = 0; u < TI; ++u) {   // twelve registers a fragment: one of A at a time
+                    const auto fa = A::fragment(from, (wi * TI + u) * 16, 0, lane);
 #pragma unroll
-                        for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa, fb[v], acc[u][v]);
-                    }
-                } else {
-                    typename Frag<T>::type fa[TI];
-#pragma unroll
-                    for (int u = 0; u < TI; ++u) fa[u] = A::fragment(now, (wi * TI + u) * 16, s, lane);
-#pragma unroll
-                    for (int u = 0; u < TI; ++u)
-#pragma unroll
-                        for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[u], fb[v], acc[u][v]);
+                    for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa, fb[v], acc[u][v]);
                 }
+                from = from + kStage < lds + kLds ? from + kStage : lds;
             }
+        } else {
+#pragma unroll
+            for (int n = 0; n < STAGES; ++n)
+                if (n < steps) load();
+            typename Frag<T>::type fa[TI], fb[TJ], next[TJ];
+            const auto multiply_row = [&](int u) {
+#pragma unroll
+                for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[u], fb[v], acc[u][v]);
+            };
+            // The products of the fragments held, and the reads of part s of stage `from` in their place.
+            const auto pass = [&](int s) {
+#pragma unroll
+                for (int v = 0; v < TJ; ++v) next[v] = B::fragment(from + A::kBytes, (wj * TJ + v) * 16, s, lane);
+#pragma unroll
+                for (int u = 0; u < TI; ++u) {   // A's fragments are replaced one by one as their products are done
+                    multiply_row(u);
+                    fa[u] = A::fragment(from, (wi * TI + u) * 16, s, lane);
+                    __builtin_amdgcn_sched_barrier(0);   // read earlier, they would take registers of their own
+                }
+#pragma unroll
+                for (int v = 0; v < TJ; ++v) fb[v] = next[v];
+            };
+            wait_for_stage<kLoads>(min(steps - 1, STAGES - 1));
+#pragma unroll
+            for (int v = 0; v < TJ; ++v) fb[v] = B::fragment(from + A::kBytes, (wj * TJ + v) * 16, 0, lane);
+#pragma unroll
+            for (int u = 0; u < TI; ++u) fa[u] = A::fragment(from, (wi * TI + u) * 16, 0, lane);
+            for (int t = 0; t + 1 < steps; ++t) {
+#pragma unroll
+                for (int s = 1; s < A::kSubs; ++s) pass(s);
+                // the next stage is there, and every wave has read this one, which the load fills anew
+                wait_for_stage<kLoads>(min(steps - 2 - t, STAGES - 2));
+                if (t + STAGES < steps) load();
+                from = from + kStage < lds + kLds ? from + kStage : lds;
+                pass(0);
+            }
+#pragma unroll
+            for (int s = 1; s < A::kSubs; ++s) pass(s);
+#pragma unroll
+            for (int u = 0; u < TI; ++u) multiply_row(u);
         }
     }
 };

@@ -9,9 +9,13 @@
 // 2^-25 of one, in the range of halves (|X|, |G| < 2, |P| < 3: the singular
 // values of X stay below 1.3). A product is then three of halves, hi hi + hi lo
 // + lo hi with float sums (lo lo is 2^-22 of it), at the matrix cores' half
-// rate: 5.4 times the float products' (1.42 and 0.153 PFLOP/s measured), over
-// three. Halves alone (11 bits) would leave the update's small singular
+// rate. Halves alone (11 bits) would leave the update's small singular
 // directions, which the steps lift up to 485 times, wrong by several percent.
+// A row holds 32 hi and then their 32 lo in turn, so that a step of 32 of k is
+// one cache line of it.
+//
+// G and P are symmetric: only the tiles on and below the diagonal are made, and
+// each is stored a second time transposed, through LDS.
 #include <math.h>
 
 #include "mfma_tile.h"
@@ -23,16 +27,34 @@ namespace {
 constexpr float kScale = 4096.0f;
 constexpr int kPatch = 64;   // edge of the element passes' patches
 
+constexpr int kPatchThreads = 1024;
+constexpr int kPatchWaves = kPatchThreads / 64;
+
 // The matrix that number `n` of a launch's work belongs to: the last whose
-// first number is not above it.
-__device__ __forceinline__ int part_of(const MuonPart* parts, int count, int phase, uint32_t n) {
-    int lo = 0, hi = count;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (parts[mid].first[phase] <= n) lo = mid;
-        else hi = mid;
+// first number is not above it. `firsts` are the matrices' first numbers; a
+// wave looks at 64 of them at a time.
+__device__ __forceinline__ int part_of(const uint32_t* firsts, int count, uint32_t n) {
+    const int lane = threadIdx.x & 63;
+    int part = -1;
+    for (int k = 0; k < count; k += 64) {
+        const uint64_t below = ballot(k + lane < count && firsts[min(k + lane, count - 1)] <= n);
+        part += __popcll(below);
+        if (below != ~0ull) break;
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(part);
+}
+
+// Where column c of a row is: its hi, and 32 elements on its lo.
+__device__ __forceinline__ int64_t column(int64_t c) { return (c >> 5) * 64 + (c & 31); }
+
+__device__ __forceinline__ double workgroup_sum(double v) {
+    __shared__ double s[kPatchWaves];
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_down(v, d, 64);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = s[0];
+    for (int k = 1; k < kPatchWaves; ++k) v += s[k];
+    return v;
 }
 
 __device__ __forceinline__ float update_of(float g, float m, const MuonStep& p) {
@@ -41,32 +63,28 @@ __device__ __forceinline__ float update_of(float g, float m, const MuonStep& p) 
 
 // M <- mu M + (1 - mu) s G, and the patch's sum of squares of U.
 template <class G>
-__global__ void __launch_bounds__(256) momentum_kernel(const MuonPart* parts, int count, MuonStep p, double* sums) {
-    const MuonPart& a = parts[part_of(parts, count, kMuonPatches, blockIdx.x)];
+__global__ void __launch_bounds__(kPatchThreads) momentum_kernel(const MuonPart* parts, const uint32_t* firsts, int count,
+                                                                 MuonStep p, double* sums) {
+    const MuonPart& a = parts[part_of(firsts, count, blockIdx.x)];
     const uint32_t n = blockIdx.x - a.first[kMuonPatches];
     const int64_t across = (a.w.cols + kPatch - 1) / kPatch;
-    const int64_t r0 = n / across * kPatch, c0 = n % across * kPatch;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t r0 = n / across * kPatch, c = n % across * kPatch + (threadIdx.x & 63);
+    const int wave = threadIdx.x >> 6;
     double sum = 0.0;
-#pragma unroll 4
-    for (int k = wave; k < kPatch; k += 4) {
-        const int64_t r = r0 + k, c = c0 + lane;
-        if (r >= a.w.rows || c >= a.w.cols) continue;
-        const float g = (float)((const G*)a.g.p)[r * a.g.stride + c] * p.grad_scale;
-        float* at = (float*)a.m.p + r * a.m.stride + c;
-        const float m = fmaf(p.momentum, *at, g);
-        *at = m;
-        const double u = (double)update_of(g, m, p);
-        sum += u * u;
+#pragma unroll
+    for (int k = 0; k < kPatch / kPatchWaves; ++k) {
+        const int64_t r = r0 + wave + k * kPatchWaves;
+        if (r < a.w.rows && c < a.w.cols) {
+            const float g = (float)((const G*)a.g.p)[r * a.g.stride + c] * p.grad_scale;
+            float* at = (float*)a.m.p + r * a.m.stride + c;
+            const float m = fmaf(p.momentum, *at, g);
+            *at = m;
+            const double u = (double)update_of(g, m, p);
+            sum += u * u;
+        }
     }
-    __shared__ double s[256];
-    s[threadIdx.x] = sum;
-    __syncthreads();
-    for (int k = 128; k > 0; k >>= 1) {
-        if ((int)threadIdx.x < k) s[threadIdx.x] += s[threadIdx.x + k];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) sums[blockIdx.x] = s[0];
+    sum = workgroup_sum(sum);
+    if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
 
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
@@ -75,203 +93,236 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
 }
 
 // X = U / max(|U|, epsilon), scaled and split; a tall matrix through LDS into
-// its transpose. Columns up to the stride are zeros.
+// its transpose. Columns up to a multiple of 32 are zeros.
 template <class G>
-__global__ void __launch_bounds__(256) normalise_kernel(const MuonPart* parts, int count, MuonStep p,
-                                                        const double* sums) {
-    const MuonPart& a = parts[part_of(parts, count, kMuonPatches, blockIdx.x)];
+__global__ void __launch_bounds__(kPatchThreads) normalise_kernel(const MuonPart* parts, const uint32_t* firsts, int count,
+                                                                  MuonStep p, const double* sums) {
+    const MuonPart& a = parts[part_of(firsts, count, blockIdx.x)];
     const uint32_t n = blockIdx.x - a.first[kMuonPatches];
     const int64_t across = (a.w.cols + kPatch - 1) / kPatch, down = (a.w.rows + kPatch - 1) / kPatch;
-    __shared__ double s[256];
     double sum = 0.0;
-    for (int64_t k = threadIdx.x; k < across * down; k += 256) sum += sums[a.first[kMuonPatches] + k];
-    s[threadIdx.x] = sum;
-    __syncthreads();
-    for (int k = 128; k > 0; k >>= 1) {
-        if ((int)threadIdx.x < k) s[threadIdx.x] += s[threadIdx.x + k];
-        __syncthreads();
-    }
-    const double norm = sqrt(s[0]);
+    for (int64_t k = threadIdx.x; k < across * down; k += kPatchThreads) sum += sums[a.first[kMuonPatches] + k];
+    const double norm = sqrt(workgroup_sum(sum));
     const double inv = (double)kScale / (norm < (double)p.epsilon ? (double)p.epsilon : norm);   // NaN stays
     const int64_t r0 = n / across * kPatch, c0 = n % across * kPatch;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    _Float16* const x = a.x[0];
     __shared__ float t[kPatch][kPatch + 1];
-#pragma unroll 4
-    for (int k = wave; k < kPatch; k += 4) {
-        const int64_t r = r0 + k, c = c0 + lane;
+#pragma unroll
+    for (int k = 0; k < kPatch / kPatchWaves; ++k) {
+        const int q = wave + k * kPatchWaves;
+        const int64_t r = r0 + q, c = c0 + lane;
         float v = 0.0f;
         if (r < a.w.rows && c < a.w.cols) {
             const float g = (float)((const G*)a.g.p)[r * a.g.stride + c] * p.grad_scale;
             v = (float)((double)update_of(g, ((const float*)a.m.p)[r * a.m.stride + c], p) * inv);
         }
-        if (a.tall) t[k][lane] = v;
-        else if (r < a.side && c < a.x_stride) split(v, a.x[0][r * a.x_stride + c], a.x[0][a.x_plane + r * a.x_stride + c]);
+        if (a.tall) t[q][lane] = v;
+        else if (r < a.side && 2 * c < a.x_stride) split(v, x[r * a.x_stride + column(c)], x[r * a.x_stride + column(c) + 32]);
     }
     if (!a.tall) return;
     __syncthreads();
-#pragma unroll 4
-    for (int k = wave; k < kPatch; k += 4) {
-        const int64_t r = c0 + k, c = r0 + lane;   // of X
-        if (r < a.side && c < a.x_stride)
-            split(t[lane][k], a.x[0][r * a.x_stride + c], a.x[0][a.x_plane + r * a.x_stride + c]);
+#pragma unroll
+    for (int k = 0; k < kPatch / kPatchWaves; ++k) {
+        const int q = wave + k * kPatchWaves;
+        const int64_t r = c0 + q, c = r0 + lane;   // of X
+        if (r < a.side && 2 * c < a.x_stride)
+            split(t[lane][q], x[r * a.x_stride + column(c)], x[r * a.x_stride + column(c) + 32]);
     }
 }
 
 // W <- keep W - lr shape X, and the copy.
 template <class C>
-__global__ void __launch_bounds__(256) apply_kernel(const MuonPart* parts, int count, MuonStep p) {
-    const MuonPart& a = parts[part_of(parts, count, kMuonPatches, blockIdx.x)];
+__global__ void __launch_bounds__(kPatchThreads) apply_kernel(const MuonPart* parts, const uint32_t* firsts, int count,
+                                                              MuonStep p) {
+    const MuonPart& a = parts[part_of(firsts, count, blockIdx.x)];
     const uint32_t n = blockIdx.x - a.first[kMuonPatches];
     const int64_t across = (a.w.cols + kPatch - 1) / kPatch;
     const int64_t r0 = n / across * kPatch, c0 = n % across * kPatch;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const _Float16* x = a.x[p.iterations & 1];
+    const _Float16* const x = a.x[p.iterations & 1];
     const float step = p.lr * a.shape * (1.0f / kScale);
     __shared__ float t[kPatch][kPatch + 1];
     if (a.tall) {
-#pragma unroll 4
-        for (int k = wave; k < kPatch; k += 4) {
-            const int64_t r = c0 + k, c = r0 + lane;
+#pragma unroll
+        for (int k = 0; k < kPatch / kPatchWaves; ++k) {
+            const int q = wave + k * kPatchWaves;
+            const int64_t r = c0 + q, c = r0 + lane;
             if (r < a.side && c < a.length)
-                t[lane][k] = (float)x[r * a.x_stride + c] + (float)x[a.x_plane + r * a.x_stride + c];
+                t[lane][q] = (float)x[r * a.x_stride + column(c)] + (float)x[r * a.x_stride + column(c) + 32];
         }
         __syncthreads();
     }
-#pragma unroll 4
-    for (int k = wave; k < kPatch; k += 4) {
-        const int64_t r = r0 + k, c = c0 + lane;
-        if (r >= a.w.rows || c >= a.w.cols) continue;
-        const float v = a.tall ? t[k][lane]
-                               : (float)x[r * a.x_stride + c] + (float)x[a.x_plane + r * a.x_stride + c];
-        float* w = (float*)a.w.p + r * a.w.stride + c;
-        const float u = fmaf(-step, v, p.keep * *w);
-        *w = u;
-        if (a.c.p) ((C*)a.c.p)[r * a.c.stride + c] = (C)u;
+#pragma unroll
+    for (int k = 0; k < kPatch / kPatchWaves; ++k) {
+        const int q = wave + k * kPatchWaves;
+        const int64_t r = r0 + q, c = c0 + lane;
+        if (r < a.w.rows && c < a.w.cols) {
+            const float v = a.tall ? t[q][lane]
+                                   : (float)x[r * a.x_stride + column(c)] + (float)x[r * a.x_stride + column(c) + 32];
+            float* w = (float*)a.w.p + r * a.w.stride + c;
+            const float u = fmaf(-step, v, p.keep * *w);
+            *w = u;
+            if (a.c.p) ((C*)a.c.p)[r * a.c.stride + c] = (C)u;
+        }
     }
 }
 
 // ---- the products
 
-// A tile of the three-product sum. Steps of 64 bytes of k: four planes of
-// 128 rows twice are 64 KB, two workgroups a compute unit.
-template <int WI, int WJ, int TI, int TJ, bool A_RC>
+// A tile of the three-product sum, in steps of 32 of k. K-contiguous operands
+// are matrices of twice the columns, whose steps of 128 bytes are a row's 32 hi
+// and 32 lo; the R-contiguous X has tiles of twice the rows and steps of 32 k.
+template <int WI, int WJ, int TI, int TJ, int STAGES, bool A_RC>
 struct SplitTile {
     static constexpr int kWavesI = WI, kWavesJ = WJ;
     static constexpr int kWaves = WI * WJ, kThreads = 64 * kWaves;
     static constexpr int BI = WI * TI * 16, BJ = WJ * TJ * 16;
     using T = _Float16;
-    using A = TileSide<T, BI, kWaves, A_RC, 64>;
-    using B = TileSide<T, BJ, kWaves, false, 64>;
-    static constexpr int kStage = 2 * (A::kBytes + B::kBytes);
+    using A = TileSide<T, A_RC ? 2 * BI : BI, kWaves, A_RC, A_RC ? 64 : 128>;
+    using B = TileSide<T, BJ, kWaves, false, 128>;
+    static constexpr int kStage = A::kBytes + B::kBytes, kLds = STAGES * kStage;
+    static constexpr int kLoads = A::kLoads + B::kLoads;   // a wave and stage
 
-    static __device__ __forceinline__ void run(unsigned char* lds, TileOperand a, int64_t a_plane, TileOperand b,
-                                               int64_t b_plane, int64_t i0, int64_t j0, int64_t k_size,
-                                               f32x4 (&acc)[TI][TJ]) {
+    static __device__ __forceinline__ void run(unsigned char* lds, const TileOperand& a, const TileOperand& b, int64_t i0,
+                                               int64_t j0, int steps, f32x4 (&acc)[TI][TJ]) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wi = wave / WJ, wj = wave % WJ;
-        A sa[2];
-        B sb[2];
-        for (int h = 0; h < 2; ++h) {
-            sa[h].begin({(const T*)a.p + h * a_plane, a.rows, a.cols, a.stride}, i0, 0, wave, lane);
-            sb[h].begin({(const T*)b.p + h * b_plane, b.rows, b.cols, b.stride}, j0, 0, wave, lane);
-        }
+        A sa;
+        B sb;
+        sa.begin(a, A_RC ? 2 * i0 : i0, 0, wave, lane);
+        sb.begin(b, j0, 0, wave, lane);
 #pragma unroll
         for (int u = 0; u < TI; ++u)
 #pragma unroll
             for (int v = 0; v < TJ; ++v) acc[u][v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const auto load = [&](unsigned char* to, int64_t left) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                sa[h].load(to + h * A::kBytes, left, wave, lane);
-                sb[h].load(to + 2 * A::kBytes + h * B::kBytes, left, wave, lane);
-            }
+        int left = steps;
+        unsigned char* fill = lds;
+        const auto load = [&] {
+            sa.load(fill, (int64_t)left * A::kDepth, wave, lane);
+            sb.load(fill + A::kBytes, (int64_t)left * B::kDepth, wave, lane);
+            --left;
+            fill = fill + kStage < lds + kLds ? fill + kStage : lds;
         };
-        const int steps = (int)((k_size + A::kDepth - 1) / A::kDepth);
-        load(lds, k_size);
-        for (int t = 0; t < steps; ++t) {
-            const unsigned char* now = lds + (t & 1) * kStage;
-            wait_all_and_barrier();
-            if (t + 1 < steps) load(lds + ((t + 1) & 1) * kStage, k_size - (int64_t)(t + 1) * A::kDepth);
-            typename Frag<T>::type fa[2][TI], fb[2][TJ];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+        for (int n = 0; n < STAGES; ++n)
+            if (n < steps) load();
+        const unsigned char* from = lds;
+        typename Frag<T>::type fa[2][TI], fb[2][TJ], next[2][TJ];   // hi, lo
+        const auto read_a = [&](int u) {
+            const int r = (wi * TI + u) * 16;
 #pragma unroll
-                for (int v = 0; v < TJ; ++v)
-                    fb[h][v] = B::fragment(now + 2 * A::kBytes + h * B::kBytes, (wj * TJ + v) * 16, 0, lane);
+            for (int h = 0; h < 2; ++h)
+                fa[h][u] = A_RC ? A::fragment(from, (r & ~31) * 2 + 32 * h + (r & 16), 0, lane) : A::fragment(from, r, h, lane);
+        };
+        const auto read_b = [&](auto& to) {
 #pragma unroll
-                for (int u = 0; u < TI; ++u) fa[h][u] = A::fragment(now + h * A::kBytes, (wi * TI + u) * 16, 0, lane);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int v = 0; v < TJ; ++v) to[h][v] = B::fragment(from + A::kBytes, (wj * TJ + v) * 16, h, lane);
+        };
+        const auto multiply_row = [&](int u) {
+#pragma unroll
+            for (int q = 0; q < 3; ++q)   // hi hi, hi lo, lo hi
+#pragma unroll
+                for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[q == 2][u], fb[q == 1][v], acc[u][v]);
+        };
+        wait_for_stage<kLoads>(min(steps - 1, STAGES - 1));
+        read_b(fb);
+#pragma unroll
+        for (int u = 0; u < TI; ++u) read_a(u);
+        for (int t = 0; t + 1 < steps; ++t) {   // as Tile's
+            wait_for_stage<kLoads>(min(steps - 2 - t, STAGES - 2));
+            if (t + STAGES < steps) load();
+            from = from + kStage < lds + kLds ? from + kStage : lds;
+            read_b(next);
+#pragma unroll
+            for (int u = 0; u < TI; ++u) {
+                multiply_row(u);
+                read_a(u);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int q = 0; q < 3; ++q)   // hi hi, hi lo, lo hi: the squares in turn, no sum waits for its last
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int u = 0; u < TI; ++u)
-#pragma unroll
-                    for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[q == 2][u], fb[q == 1][v], acc[u][v]);
+                for (int v = 0; v < TJ; ++v) fb[h][v] = next[h][v];
         }
+#pragma unroll
+        for (int u = 0; u < TI; ++u) multiply_row(u);
     }
 };
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// Gram: G = X X^T. Square: P = b G + c G G. Update: X' = a X + P X. Rows of
-// the stored matrices are 16-byte aligned and zero up to their stride, which
-// the products keep: they run over whole strides.
-template <int PHASE, int WI, int WJ, int TI, int TJ>
-__global__ void __launch_bounds__(64 * WI * WJ) product_kernel(const MuonPart* parts, int count, uint32_t total, int turn) {
+// Gram: G = X X^T. Square: P = b G + c G G. Update: X' = a X + P X. The stored
+// matrices are zero up to a multiple of 32 columns, which the products keep:
+// they run over whole strides.
+template <int PHASE, int WI, int WJ, int TI, int TJ, int STAGES>
+__global__ void __launch_bounds__(64 * WI * WJ) product_kernel(const MuonPart* parts, const uint32_t* firsts, int count,
+                                                               uint32_t total, int turn) {
     constexpr bool kUpdate = PHASE == kMuonUpdate;
-    using P = SplitTile<WI, WJ, TI, TJ, kUpdate>;
-    __shared__ __align__(1024) unsigned char lds[2 * P::kStage];
+    using P = SplitTile<WI, WJ, TI, TJ, STAGES, kUpdate>;
+    __shared__ __align__(1024) unsigned char lds[P::kLds];
     const uint32_t n = xcd_contiguous_index(blockIdx.x, total);
-    const MuonPart& a = parts[part_of(parts, count, kUpdate ? kMuonUpdate : kMuonGram, n)];
+    const MuonPart& a = parts[part_of(firsts, count, n)];
     const uint32_t local = n - a.first[kUpdate ? kMuonUpdate : kMuonGram];
     const _Float16* x = a.x[turn];
     const int64_t out_stride = kUpdate ? a.x_stride : a.g_stride;
-    const uint32_t ni = (uint32_t)((out_stride + P::BI - 1) / P::BI), nj = (uint32_t)((a.side + P::BJ - 1) / P::BJ);
     uint32_t ti, tj;
-    tile_of(local, ni, nj, ti, tj);
+    if constexpr (kUpdate) {
+        tile_of(local, (uint32_t)((out_stride / 2 + P::BI - 1) / P::BI), (uint32_t)((a.side + P::BJ - 1) / P::BJ), ti, tj);
+    } else {   // row ti of the triangle starts at ti (ti + 1) / 2
+        static_assert(P::BI == P::BJ, "the mirrored tile has the same shape");
+        ti = (uint32_t)((sqrtf(8.0f * (float)local + 1.0f) - 1.0f) * 0.5f);
+        while ((uint64_t)ti * (ti + 1) / 2 > local) --ti;
+        while ((uint64_t)(ti + 1) * (ti + 2) / 2 <= local) ++ti;
+        tj = local - (uint32_t)((uint64_t)ti * (ti + 1) / 2);
+    }
     const int64_t i0 = (int64_t)ti * P::BI, j0 = (int64_t)tj * P::BJ;
     f32x4 acc[TI][TJ];
     const TileOperand tx{x, a.side, a.x_stride, a.x_stride};
-    const _Float16* from;   // added to the products, and to where
+    const _Float16* from = nullptr;   // added to the products, and to where
     _Float16* to;
-    int64_t plane;
     if constexpr (PHASE == kMuonGram) {
-        P::run(lds, tx, a.x_plane, tx, a.x_plane, i0, j0, a.x_stride, acc);
-        from = nullptr;
+        P::run(lds, tx, tx, i0, j0, (int)(a.x_stride / 64), acc);
         to = a.gram;
-        plane = a.g_plane;
     } else if constexpr (PHASE == kMuonSquare) {
         const TileOperand tg{a.gram, a.side, a.g_stride, a.g_stride};
-        P::run(lds, tg, a.g_plane, tg, a.g_plane, i0, j0, a.g_stride, acc);
+        P::run(lds, tg, tg, i0, j0, (int)(a.g_stride / 64), acc);
         from = a.gram;
         to = a.poly;
-        plane = a.g_plane;
     } else {
         // k runs over P's columns, X's rows: those past the side are zeros in P and not there in X
         const TileOperand tp{a.poly, a.side, a.g_stride, a.g_stride};
-        P::run(lds, tx, a.x_plane, tp, a.g_plane, i0, j0, a.g_stride, acc);
+        P::run(lds, tx, tp, i0, j0, (int)(a.g_stride / 64), acc);
         from = x;
         to = a.x[turn ^ 1];
-        plane = a.x_plane;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wi = wave / WJ, wj = wave % WJ;
     constexpr float kProducts = (PHASE == kMuonSquare ? kNewtonSchulzC : 1.0f) / kScale;
     constexpr float kAdded = PHASE == kMuonSquare ? kNewtonSchulzB : kNewtonSchulzA;
+    const bool mirrored = !kUpdate && ti != tj;
+    constexpr int kMirrorPitch = P::BJ + 8;   // halves; 16-byte rows, neighbouring ones on other banks
+    static_assert(kUpdate || 2 * P::BI * kMirrorPitch * 2 <= P::kLds, "the stages hold the mirrored tile");
+    _Float16* const mirror = (_Float16*)lds;   // [hi, lo][i][j]
+    if (mirrored) lds_barrier();               // the stages are read
 #pragma unroll
     for (int u = 0; u < TI; u += 2) {
-        const int64_t i = i0 + (wi * TI + u) * 16 + neighbours_at(lane);
+        const int il = (wi * TI + u) * 16 + neighbours_at(lane);
+        const int64_t i = i0 + il;
 #pragma unroll
         for (int t = 0; t < TJ; ++t) {
-            const int64_t j = j0 + (wj * TJ + t) * 16 + (lane & 15);
+            const int jl = (wj * TJ + t) * 16 + (lane & 15);
+            const int64_t j = j0 + jl;
             float v[8];
             neighbours(acc[u][t], acc[u + 1][t], v);
-            if (i >= out_stride || j >= a.side) continue;
-            const int64_t at = j * out_stride + i;
-            f16x8 hi, lo;
-            if (PHASE != kMuonGram) {
+            const bool exists = 2 * i < out_stride && j < a.side;
+            const int64_t at = j * out_stride + column(i);
+            f16x8 hi = {}, lo = {};
+            if (PHASE != kMuonGram && exists) {
                 hi = *(const f16x8*)(from + at);
-                lo = *(const f16x8*)(from + plane + at);
+                lo = *(const f16x8*)(from + at + 32);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -282,9 +333,27 @@ __global__ void __launch_bounds__(64 * WI * WJ) product_kernel(const MuonPart* p
                 hi[e] = h;
                 lo[e] = l;
             }
-            *(f16x8*)(to + at) = hi;
-            *(f16x8*)(to + plane + at) = lo;
+            if (exists) {
+                *(f16x8*)(to + at) = hi;
+                *(f16x8*)(to + at + 32) = lo;
+            }
+            if (mirrored) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    mirror[(il + e) * kMirrorPitch + jl] = hi[e];
+                    mirror[(P::BI + il + e) * kMirrorPitch + jl] = lo[e];
+                }
+            }
         }
+    }
+    if (!mirrored) return;
+    lds_barrier();
+    // rows i of the mirrored tile, 8 of j at a time; j is inside the matrix (tj < ti)
+    for (int q = threadIdx.x; q < 2 * P::BI * (P::BJ / 8); q += 64 * WI * WJ) {
+        const int c = q % (P::BJ / 8), r = q / (P::BJ / 8), il = r % P::BI, h = r / P::BI;
+        if (i0 + il < a.side)
+            *(f16x8*)(to + (i0 + il) * out_stride + column(j0 + 8 * c) + 32 * h) =
+                *(const f16x8*)(mirror + (h * P::BI + il) * kMirrorPitch + 8 * c);
     }
 }
 
@@ -296,14 +365,16 @@ __global__ void __launch_bounds__(256) zero_kernel(Mat m) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tiles of 128 x 128 where they fill the card, else of 64 x 64: a small
-// network's matrices are too few large tiles.
-uint32_t count_tiles(const MuonPart* parts, int count, int edge, int phase, MuonPart* set) {
+// Tiles of 128 x 128 (of the update: 256 x 128) where they occupy half of the
+// card, else of 64 x 64: a small network's matrices are too few large tiles.
+uint32_t count_tiles(const MuonPart* parts, int count, bool large, int phase, MuonPart* set) {
     int64_t n = 0;
+    const int64_t bi = !large ? 64 : phase == kMuonUpdate ? 256 : 128, bj = large ? 128 : 64;
     for (int i = 0; i < count; ++i) {
         const MuonPart& a = parts[i];
         if (set) set[i].first[phase] = (uint32_t)n;
-        n += ceil_div(phase == kMuonUpdate ? a.x_stride : a.g_stride, edge) * ceil_div(a.side, edge);
+        const int64_t down = ceil_div(a.side, bj);
+        n += phase == kMuonUpdate ? ceil_div(a.x_stride / 2, bi) * down : down * (down + 1) / 2;
     }
     return n < 0x7fffffff ? (uint32_t)n : 0x7fffffffu;
 }
@@ -323,24 +394,23 @@ MuonPlan plan_muon(MuonPart* parts, int count) {
         a.tall = a.w.rows > a.w.cols;
         a.side = a.tall ? a.w.cols : a.w.rows;
         a.length = a.tall ? a.w.rows : a.w.cols;
-        a.x_stride = ceil_div(a.length, 8) * 8;
-        a.g_stride = ceil_div(a.side, 8) * 8;
-        a.x_plane = a.side * a.x_stride;
-        a.g_plane = a.side * a.g_stride;
+        a.x_stride = ceil_div(a.length, 32) * 64;
+        a.g_stride = ceil_div(a.side, 32) * 64;
         a.shape = a.tall ? sqrtf((float)a.w.rows / (float)a.w.cols) : 1.0f;
         a.first[kMuonPatches] = (uint32_t)patches;
         patches += ceil_div(a.w.rows, kPatch) * ceil_div(a.w.cols, kPatch);
-        for (int k = 0; k < 2; ++k) a.x[k] = (_Float16*)take(4 * a.x_plane);
-        a.gram = (_Float16*)take(4 * a.g_plane);
-        a.poly = (_Float16*)take(4 * a.g_plane);
+        for (int k = 0; k < 2; ++k) a.x[k] = (_Float16*)take(2 * a.side * a.x_stride);
+        a.gram = (_Float16*)take(2 * a.side * a.g_stride);
+        a.poly = (_Float16*)take(2 * a.side * a.g_stride);
     }
     plan.patches = (uint32_t)patches;
-    plan.large[0] = count_tiles(parts, count, 128, kMuonGram, nullptr) >= 256;
-    plan.large[1] = count_tiles(parts, count, 128, kMuonUpdate, nullptr) >= 256;
-    plan.tiles[0] = count_tiles(parts, count, plan.large[0] ? 128 : 64, kMuonGram, parts);
-    plan.tiles[1] = count_tiles(parts, count, plan.large[1] ? 128 : 64, kMuonUpdate, parts);
+    plan.large[0] = count_tiles(parts, count, true, kMuonGram, nullptr) >= 128;
+    plan.large[1] = count_tiles(parts, count, true, kMuonUpdate, nullptr) >= 128;
+    plan.tiles[0] = count_tiles(parts, count, plan.large[0], kMuonGram, parts);
+    plan.tiles[1] = count_tiles(parts, count, plan.large[1], kMuonUpdate, parts);
     plan.sums_at = take(8 * patches);
     plan.parts_at = take((int64_t)sizeof(MuonPart) * count);
+    plan.firsts_at = take((int64_t)sizeof(uint32_t) * 3 * count);
     plan.bytes = at;
     plan.fits = patches < 0x7fffffff && plan.tiles[0] < 0x7fffffffu && plan.tiles[1] < 0x7fffffffu;
     return plan;
@@ -356,25 +426,34 @@ void place_muon(MuonPart* parts, int count, unsigned char* workspace) {
 }
 
 template <int PHASE>
-static void launch_product(const MuonPlan& plan, const MuonPart* parts, int count, int turn, hipStream_t s) {
+static void launch_product(const MuonPlan& plan, const MuonPart* parts, const uint32_t* firsts, int count, int turn,
+                           hipStream_t s) {
     const int w = PHASE == kMuonUpdate;
-    if (plan.large[w]) product_kernel<PHASE, 2, 2, 4, 4><<<plan.tiles[w], 256, 0, s>>>(parts, count, plan.tiles[w], turn);
-    else product_kernel<PHASE, 2, 2, 2, 2><<<plan.tiles[w], 256, 0, s>>>(parts, count, plan.tiles[w], turn);
+    const uint32_t* f = firsts + (w ? kMuonUpdate : kMuonGram) * count;
+    if (!plan.large[w])
+        product_kernel<PHASE, 2, 2, 2, 2, 4><<<plan.tiles[w], 256, 0, s>>>(parts, f, count, plan.tiles[w], turn);
+    else if constexpr (PHASE == kMuonUpdate)
+        product_kernel<PHASE, 4, 2, 4, 4, 3><<<plan.tiles[w], 512, 0, s>>>(parts, f, count, plan.tiles[w], turn);
+    else
+        product_kernel<PHASE, 2, 4, 4, 2, 4><<<plan.tiles[w], 512, 0, s>>>(parts, f, count, plan.tiles[w], turn);
 }
 
 int launch_muon_step(const MuonPlan& plan, int count, const MuonStep& p, unsigned char* workspace, hipStream_t s) {
     const MuonPart* parts = (const MuonPart*)(workspace + plan.parts_at);
+    const uint32_t* firsts = (const uint32_t*)(workspace + plan.firsts_at);
     double* sums = (double*)(workspace + plan.sums_at);
     by_dtype(p.grad_dtype, [&](auto t) {
-        momentum_kernel<decltype(t)><<<plan.patches, 256, 0, s>>>(parts, count, p, sums);
-        normalise_kernel<decltype(t)><<<plan.patches, 256, 0, s>>>(parts, count, p, sums);
+        momentum_kernel<decltype(t)><<<plan.patches, kPatchThreads, 0, s>>>(parts, firsts, count, p, sums);
+        normalise_kernel<decltype(t)><<<plan.patches, kPatchThreads, 0, s>>>(parts, firsts, count, p, sums);
     });
     for (int k = 0; k < p.iterations; ++k) {
-        launch_product<kMuonGram>(plan, parts, count, k & 1, s);
-        launch_product<kMuonSquare>(plan, parts, count, k & 1, s);
-        launch_product<kMuonUpdate>(plan, parts, count, k & 1, s);
+        launch_product<kMuonGram>(plan, parts, firsts, count, k & 1, s);
+        launch_product<kMuonSquare>(plan, parts, firsts, count, k & 1, s);
+        launch_product<kMuonUpdate>(plan, parts, firsts, count, k & 1, s);
     }
-    by_dtype(p.copy_dtype, [&](auto t) { apply_kernel<decltype(t)><<<plan.patches, 256, 0, s>>>(parts, count, p); });
+    by_dtype(p.copy_dtype, [&](auto t) {
+        apply_kernel<decltype(t)><<<plan.patches, kPatchThreads, 0, s>>>(parts, firsts, count, p);
+    });
     TGS_CHECK_LAUNCH();
     return TGS_OK;
 }

@@ -150,8 +150,8 @@ enum { kMuonPatches = 0, kMuonGram = 1, kMuonUpdate = 2, kMuonSquare = 3 };
 struct MuonPart {
     Mat w, g, m, c;              // weights, gradient, momentum, copy (c.p may be NULL)
     int64_t side, length;        // X is side x length, side <= length
-    int64_t x_stride, x_plane;   // of X's two planes (elements)
-    int64_t g_stride, g_plane;   // of the Gram matrix's and the polynomial's
+    int64_t x_stride;            // of X's rows: hi and lo, in halves
+    int64_t g_stride;            // of the Gram matrix's and the polynomial's
     _Float16 *x[2], *gram, *poly;
     float shape;                 // sqrt(max(1, rows / cols))
     int tall;                    // X is the transpose
@@ -162,7 +162,7 @@ struct MuonPlan {
     uint32_t tiles[2];     // of the products with side x side and side x length outputs
     bool large[2];         // whether those are the large tiles
     bool fits;             // whether the counts fit a launch
-    int64_t sums_at, parts_at, bytes;   // in the workspace
+    int64_t sums_at, parts_at, firsts_at, bytes;   // in the workspace; firsts: the parts' first[0], then [1], [2]
 };
 struct MuonStep {
     float momentum, grad_scale;   // grad_scale = (1 - momentum) scale

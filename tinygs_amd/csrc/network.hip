@@ -16,6 +16,7 @@ struct tgs_network {
 
 struct tgs_muon {
     std::vector<MuonPart> mats;
+    std::vector<uint32_t> firsts;
     bool on_device = false;   // the workspace holds the matrices' table
     MuonPlan plan{};
     int grad_dtype = TGS_DTYPE_FLOAT32;
@@ -293,6 +294,7 @@ int tgs_muon_create(const tgs_matrix* weights, const tgs_matrix* grads, const tg
     if (!m) return fail(TGS_ERR_STATE, "out of host memory");
     try {
         m->mats.resize((size_t)count);
+        m->firsts.resize((size_t)count * 3);
     } catch (...) {
         delete m;
         return fail(TGS_ERR_STATE, "out of host memory");
@@ -376,7 +378,11 @@ int tgs_muon_step(tgs_muon* m, float scale, void* stream) {
         TGS_TRY(ensure(m->workspace, (size_t)plan.bytes, s));
         unsigned char* at = m->workspace.as<unsigned char>();
         place_muon(m->mats.data(), count, at);
+        for (int k = 0; k < 3; ++k)
+            for (int i = 0; i < count; ++i) m->firsts[(size_t)(k * count + i)] = m->mats[(size_t)i].first[k];
         TGS_HIP(hipMemcpyAsync(at + plan.parts_at, m->mats.data(), sizeof(MuonPart) * (size_t)count,
+                               hipMemcpyHostToDevice, s));
+        TGS_HIP(hipMemcpyAsync(at + plan.firsts_at, m->firsts.data(), sizeof(uint32_t) * m->firsts.size(),
                                hipMemcpyHostToDevice, s));
         TGS_HIP(hipStreamSynchronize(s));
         m->plan = plan;
