@@ -43,24 +43,39 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
     }
 }
 
-// Calls f(i, j, n, v) for each run of 8 outputs (i .. i + 7, j) that a lane
-// holds; n of them exist.
-template <class Shape, int TI, int TJ, class F>
+// A lane's outputs are runs of 8 (i .. i + 7, j), n of which exist (0: none, or
+// j is past the end). For every column of TJ runs of one i: before(i, n) and
+// ahead(t, i, j, n) for each t, which start their loads, then
+// f(t, i, j, n, v) with the values.
+template <class Shape, int TI, int TJ, class Before, class Ahead, class F>
 __device__ __forceinline__ void for_outputs(const f32x4 (&acc)[TI][TJ], int64_t i0, int64_t j0, int64_t ni, int64_t nj,
-                                            F f) {
+                                            Before before, Ahead ahead, F f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wi = wave / Shape::kWavesJ, wj = wave % Shape::kWavesJ;
 #pragma unroll
     for (int u = 0; u < TI; u += 2) {
         const int64_t i = i0 + (wi * TI + u) * 16 + neighbours_at(lane);
+        const int n = (int)min(max(ni - i, (int64_t)0), (int64_t)8);
+        before(i, n);
+#pragma unroll
+        for (int t = 0; t < TJ; ++t) {
+            const int64_t j = j0 + (wj * TJ + t) * 16 + (lane & 15);
+            ahead(t, i, j, j < nj ? n : 0);
+        }
 #pragma unroll
         for (int t = 0; t < TJ; ++t) {
             const int64_t j = j0 + (wj * TJ + t) * 16 + (lane & 15);
             float v[8];
             neighbours(acc[u][t], acc[u + 1][t], v);
-            if (i < ni && j < nj) f(i, j, (int)(ni - i < 8 ? ni - i : 8), v);
+            if (n > 0 && j < nj) f(t, i, j, n, v);
         }
     }
+}
+template <class Shape, int TI, int TJ, class F>
+__device__ __forceinline__ void for_outputs(const f32x4 (&acc)[TI][TJ], int64_t i0, int64_t j0, int64_t ni, int64_t nj,
+                                            F f) {
+    for_outputs<Shape>(acc, i0, j0, ni, nj, [](int64_t, int) {}, [](int, int64_t, int64_t, int) {},
+                       [&](int, int64_t i, int64_t j, int n, float(&v)[8]) { f(i, j, n, v); });
 }
 
 // Tile shapes, as waves and squares of 16 a wave on each axis. A ring of two
@@ -94,24 +109,39 @@ void by_shape(int64_t ni, int64_t nj, int64_t splits_most, F f) {
 template <class T, int ACT, class S>
 __device__ __forceinline__ void forward_outputs(const LinearForward& a, const f32x4 (&acc)[S::kSquaresI][S::kSquaresJ],
                                                 int64_t i0, int64_t j0) {
-    for_outputs<S>(acc, i0, j0, a.y.cols, a.y.rows, [&](int64_t i, int64_t j, int n, float (&v)[8]) {
-        if (a.bias) {
-            float b[8];
-            load8(a.bias + i, n, b);
+    // bias and residual are on their way before the first of their runs needs them
+    float bias[8];
+    typename Packed<T>::type residual[S::kSquaresJ];
+    for_outputs<S>(
+        acc, i0, j0, a.y.cols, a.y.rows,
+        [&](int64_t i, int n) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += b[e];
-        }
-        if (a.preact.p) store8((T*)a.preact.p + j * a.preact.stride + i, n, v);
+            for (int e = 0; e < 8; ++e) bias[e] = 0.0f;
+            if (a.bias && n > 0) load8(a.bias + i, n, bias);
+        },
+        [&](int t, int64_t i, int64_t j, int n) {
+            if (a.residual.p && n == 8)
+                residual[t] = *(const typename Packed<T>::type*)((const T*)a.residual.p + j * a.residual.stride + i);
+        },
+        [&](int t, int64_t i, int64_t j, int n, float(&v)[8]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = activate<ACT>(v[e]);
-        if (a.residual.p) {
-            float r[8];
-            load8((const T*)a.residual.p + j * a.residual.stride + i, n, r);
+            for (int e = 0; e < 8; ++e) v[e] += bias[e];
+            if (a.preact.p) store8((T*)a.preact.p + j * a.preact.stride + i, n, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += r[e];
-        }
-        store8((T*)a.y.p + j * a.y.stride + i, n, v);
-    });
+            for (int e = 0; e < 8; ++e) v[e] = activate<ACT>(v[e]);
+            if (a.residual.p) {
+                if (n == 8) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += (float)residual[t][e];
+                } else {
+                    float r[8];
+                    load8((const T*)a.residual.p + j * a.residual.stride + i, n, r);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += r[e];
+                }
+            }
+            store8((T*)a.y.p + j * a.y.stride + i, n, v);
+        });
 }
 
 template <class T, class S>

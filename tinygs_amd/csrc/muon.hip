@@ -27,6 +27,9 @@ namespace {
 constexpr float kScale = 4096.0f;
 constexpr int kPatch = 64;   // edge of the element passes' patches
 
+// Halves between a row's end and the next row: rows of a power of two would all
+// start on the same few channels of the cache.
+constexpr int kRowPad = 64;
 constexpr int kPatchThreads = 1024;
 constexpr int kPatchWaves = kPatchThreads / 64;
 
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(kPatchThreads) normalise_kernel(const MuonPart
             v = (float)((double)update_of(g, ((const float*)a.m.p)[r * a.m.stride + c], p) * inv);
         }
         if (a.tall) t[q][lane] = v;
-        else if (r < a.side && 2 * c < a.x_stride) split(v, x[r * a.x_stride + column(c)], x[r * a.x_stride + column(c) + 32]);
+        else if (r < a.side && 2 * c < a.x_cols) split(v, x[r * a.x_stride + column(c)], x[r * a.x_stride + column(c) + 32]);
     }
     if (!a.tall) return;
     __syncthreads();
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(kPatchThreads) normalise_kernel(const MuonPart
     for (int k = 0; k < kPatch / kPatchWaves; ++k) {
         const int q = wave + k * kPatchWaves;
         const int64_t r = c0 + q, c = r0 + lane;   // of X
-        if (r < a.side && 2 * c < a.x_stride)
+        if (r < a.side && 2 * c < a.x_cols)
             split(t[lane][q], x[r * a.x_stride + column(c)], x[r * a.x_stride + column(c) + 32]);
     }
 }
@@ -267,10 +270,10 @@ __global__ void __launch_bounds__(64 * WI * WJ) product_kernel(const MuonPart* p
     const MuonPart& a = parts[part_of(firsts, count, n)];
     const uint32_t local = n - a.first[kUpdate ? kMuonUpdate : kMuonGram];
     const _Float16* x = a.x[turn];
-    const int64_t out_stride = kUpdate ? a.x_stride : a.g_stride;
+    const int64_t out_stride = kUpdate ? a.x_stride : a.g_stride, out_cols = kUpdate ? a.x_cols : a.g_cols;
     uint32_t ti, tj;
     if constexpr (kUpdate) {
-        tile_of(local, (uint32_t)((out_stride / 2 + P::BI - 1) / P::BI), (uint32_t)((a.side + P::BJ - 1) / P::BJ), ti, tj);
+        tile_of(local, (uint32_t)((out_cols / 2 + P::BI - 1) / P::BI), (uint32_t)((a.side + P::BJ - 1) / P::BJ), ti, tj);
     } else {   // row ti of the triangle starts at ti (ti + 1) / 2
         static_assert(P::BI == P::BJ, "the mirrored tile has the same shape");
         ti = (uint32_t)((sqrtf(8.0f * (float)local + 1.0f) - 1.0f) * 0.5f);
@@ -280,21 +283,21 @@ __global__ void __launch_bounds__(64 * WI * WJ) product_kernel(const MuonPart* p
     }
     const int64_t i0 = (int64_t)ti * P::BI, j0 = (int64_t)tj * P::BJ;
     f32x4 acc[TI][TJ];
-    const TileOperand tx{x, a.side, a.x_stride, a.x_stride};
+    const TileOperand tx{x, a.side, a.x_cols, a.x_stride};
     const _Float16* from = nullptr;   // added to the products, and to where
     _Float16* to;
     if constexpr (PHASE == kMuonGram) {
-        P::run(lds, tx, tx, i0, j0, (int)(a.x_stride / 64), acc);
+        P::run(lds, tx, tx, i0, j0, (int)(a.x_cols / 64), acc);
         to = a.gram;
     } else if constexpr (PHASE == kMuonSquare) {
-        const TileOperand tg{a.gram, a.side, a.g_stride, a.g_stride};
-        P::run(lds, tg, tg, i0, j0, (int)(a.g_stride / 64), acc);
+        const TileOperand tg{a.gram, a.side, a.g_cols, a.g_stride};
+        P::run(lds, tg, tg, i0, j0, (int)(a.g_cols / 64), acc);
         from = a.gram;
         to = a.poly;
     } else {
         // k runs over P's columns, X's rows: those past the side are zeros in P and not there in X
-        const TileOperand tp{a.poly, a.side, a.g_stride, a.g_stride};
-        P::run(lds, tx, tp, i0, j0, (int)(a.g_stride / 64), acc);
+        const TileOperand tp{a.poly, a.side, a.g_cols, a.g_stride};
+        P::run(lds, tx, tp, i0, j0, (int)(a.g_cols / 64), acc);
         from = x;
         to = a.x[turn ^ 1];
     }
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(64 * WI * WJ) product_kernel(const MuonPart* p
             const int64_t j = j0 + jl;
             float v[8];
             neighbours(acc[u][t], acc[u + 1][t], v);
-            const bool exists = 2 * i < out_stride && j < a.side;
+            const bool exists = 2 * i < out_cols && j < a.side;
             const int64_t at = j * out_stride + column(i);
             f16x8 hi = {}, lo = {};
             if (PHASE != kMuonGram && exists) {
@@ -374,7 +377,7 @@ uint32_t count_tiles(const MuonPart* parts, int count, bool large, int phase, Mu
         const MuonPart& a = parts[i];
         if (set) set[i].first[phase] = (uint32_t)n;
         const int64_t down = ceil_div(a.side, bj);
-        n += phase == kMuonUpdate ? ceil_div(a.x_stride / 2, bi) * down : down * (down + 1) / 2;
+        n += phase == kMuonUpdate ? ceil_div(a.x_cols / 2, bi) * down : down * (down + 1) / 2;
     }
     return n < 0x7fffffff ? (uint32_t)n : 0x7fffffffu;
 }
@@ -394,8 +397,10 @@ MuonPlan plan_muon(MuonPart* parts, int count) {
         a.tall = a.w.rows > a.w.cols;
         a.side = a.tall ? a.w.cols : a.w.rows;
         a.length = a.tall ? a.w.rows : a.w.cols;
-        a.x_stride = ceil_div(a.length, 32) * 64;
-        a.g_stride = ceil_div(a.side, 32) * 64;
+        a.x_cols = ceil_div(a.length, 32) * 64;
+        a.g_cols = ceil_div(a.side, 32) * 64;
+        a.x_stride = a.x_cols + kRowPad;
+        a.g_stride = a.g_cols + kRowPad;
         a.shape = a.tall ? sqrtf((float)a.w.rows / (float)a.w.cols) : 1.0f;
         a.first[kMuonPatches] = (uint32_t)patches;
         patches += ceil_div(a.w.rows, kPatch) * ceil_div(a.w.cols, kPatch);

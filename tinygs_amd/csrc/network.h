@@ -150,8 +150,8 @@ enum { kMuonPatches = 0, kMuonGram = 1, kMuonUpdate = 2, kMuonSquare = 3 };
 struct MuonPart {
     Mat w, g, m, c;              // weights, gradient, momentum, copy (c.p may be NULL)
     int64_t side, length;        // X is side x length, side <= length
-    int64_t x_stride;            // of X's rows: hi and lo, in halves
-    int64_t g_stride;            // of the Gram matrix's and the polynomial's
+    int64_t x_cols, x_stride;    // of X's rows: hi and lo, in halves
+    int64_t g_cols, g_stride;    // of the Gram matrix's and the polynomial's
     _Float16 *x[2], *gram, *poly;
     float shape;                 // sqrt(max(1, rows / cols))
     int tall;                    // X is the transpose
