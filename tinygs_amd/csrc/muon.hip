@@ -173,10 +173,11 @@ __global__ void __launch_bounds__(kPatchThreads) apply_kernel(const MuonPart* pa
 
 // ---- the products
 
-// A tile of the three-product sum, in steps of 32 of k. K-contiguous operands
-// are matrices of twice the columns, whose steps of 128 bytes are a row's 32 hi
-// and 32 lo; the R-contiguous X has tiles of twice the rows and steps of 32 k.
-template <int WI, int WJ, int TI, int TJ, int STAGES, bool A_RC>
+// A tile of the three-product sum, in steps of 32 of k, SUBS of them a stage of
+// the ring and a barrier. K-contiguous operands are matrices of twice the
+// columns, whose steps of 128 bytes are a row's 32 hi and 32 lo; the
+// R-contiguous X has tiles of twice the rows and steps of 32 k.
+template <int WI, int WJ, int TI, int TJ, int STAGES, int SUBS, bool A_RC>
 struct SplitTile {
     static constexpr int kWavesI = WI, kWavesJ = WJ;
     static constexpr int kWaves = WI * WJ, kThreads = 64 * kWaves;
@@ -184,8 +185,8 @@ struct SplitTile {
     using T = _Float16;
     using A = TileSide<T, A_RC ? 2 * BI : BI, kWaves, A_RC, A_RC ? 64 : 128>;
     using B = TileSide<T, BJ, kWaves, false, 128>;
-    static constexpr int kStage = A::kBytes + B::kBytes, kLds = STAGES * kStage;
-    static constexpr int kLoads = A::kLoads + B::kLoads;   // a wave and stage
+    static constexpr int kStep = A::kBytes + B::kBytes, kStage = SUBS * kStep, kLds = STAGES * kStage;
+    static constexpr int kLoads = SUBS * (A::kLoads + B::kLoads);   // a wave and stage
 
     static __device__ __forceinline__ void run(unsigned char* lds, const TileOperand& a, const TileOperand& b, int64_t i0,
                                                int64_t j0, int steps, f32x4 (&acc)[TI][TJ]) {
@@ -199,30 +200,36 @@ struct SplitTile {
         for (int u = 0; u < TI; ++u)
 #pragma unroll
             for (int v = 0; v < TJ; ++v) acc[u][v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        int left = steps;
+        const int stages = (steps + SUBS - 1) / SUBS;
+        int left = steps;   // of the steps from the next load on; none: zeros
         unsigned char* fill = lds;
         const auto load = [&] {
-            sa.load(fill, (int64_t)left * A::kDepth, wave, lane);
-            sb.load(fill + A::kBytes, (int64_t)left * B::kDepth, wave, lane);
-            --left;
+#pragma unroll
+            for (int q = 0; q < SUBS; ++q) {
+                sa.load(fill + q * kStep, (int64_t)left * A::kDepth, wave, lane);
+                sb.load(fill + q * kStep + A::kBytes, (int64_t)left * B::kDepth, wave, lane);
+                --left;
+            }
             fill = fill + kStage < lds + kLds ? fill + kStage : lds;
         };
 #pragma unroll
         for (int n = 0; n < STAGES; ++n)
-            if (n < steps) load();
+            if (n < stages) load();
         const unsigned char* from = lds;
         typename Frag<T>::type fa[2][TI], fb[2][TJ], next[2][TJ];   // hi, lo
-        const auto read_a = [&](int u) {
+        const auto read_a = [&](int u, int q) {
             const int r = (wi * TI + u) * 16;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                fa[h][u] = A_RC ? A::fragment(from, (r & ~31) * 2 + 32 * h + (r & 16), 0, lane) : A::fragment(from, r, h, lane);
+                fa[h][u] = A_RC ? A::fragment(from + q * kStep, (r & ~31) * 2 + 32 * h + (r & 16), 0, lane)
+                                : A::fragment(from + q * kStep, r, h, lane);
         };
-        const auto read_b = [&](auto& to) {
+        const auto read_b = [&](auto& to, int q) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int v = 0; v < TJ; ++v) to[h][v] = B::fragment(from + A::kBytes, (wj * TJ + v) * 16, h, lane);
+                for (int v = 0; v < TJ; ++v)
+                    to[h][v] = B::fragment(from + q * kStep + A::kBytes, (wj * TJ + v) * 16, h, lane);
         };
         const auto multiply_row = [&](int u) {
 #pragma unroll
@@ -230,26 +237,33 @@ struct SplitTile {
 #pragma unroll
                 for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[q == 2][u], fb[q == 1][v], acc[u][v]);
         };
-        wait_for_stage<kLoads>(min(steps - 1, STAGES - 1));
-        read_b(fb);
-#pragma unroll
-        for (int u = 0; u < TI; ++u) read_a(u);
-        for (int t = 0; t + 1 < steps; ++t) {   // as Tile's
-            wait_for_stage<kLoads>(min(steps - 2 - t, STAGES - 2));
-            if (t + STAGES < steps) load();
-            from = from + kStage < lds + kLds ? from + kStage : lds;
-            read_b(next);
+        const auto pass = [&](int q) {   // as Tile's
+            read_b(next, q);
 #pragma unroll
             for (int u = 0; u < TI; ++u) {
                 multiply_row(u);
-                read_a(u);
+                read_a(u, q);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int v = 0; v < TJ; ++v) fb[h][v] = next[h][v];
+        };
+        wait_for_stage<kLoads>(min(stages - 1, STAGES - 1));
+        read_b(fb, 0);
+#pragma unroll
+        for (int u = 0; u < TI; ++u) read_a(u, 0);
+        for (int t = 0; t + 1 < stages; ++t) {
+#pragma unroll
+            for (int q = 1; q < SUBS; ++q) pass(q);
+            wait_for_stage<kLoads>(min(stages - 2 - t, STAGES - 2));
+            if (t + STAGES < stages) load();
+            from = from + kStage < lds + kLds ? from + kStage : lds;
+            pass(0);
         }
+#pragma unroll
+        for (int q = 1; q < SUBS; ++q) pass(q);
 #pragma unroll
         for (int u = 0; u < TI; ++u) multiply_row(u);
     }
@@ -260,15 +274,17 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // Gram: G = X X^T. Square: P = b G + c G G. Update: X' = a X + P X. The stored
 // matrices are zero up to a multiple of 32 columns, which the products keep:
 // they run over whole strides.
-template <int PHASE, int WI, int WJ, int TI, int TJ, int STAGES>
+template <int PHASE, int WI, int WJ, int TI, int TJ, int STAGES, int SUBS>
 __global__ void __launch_bounds__(64 * WI * WJ) product_kernel(const MuonPart* parts, const uint32_t* firsts, int count,
                                                                uint32_t total, int turn) {
     constexpr bool kUpdate = PHASE == kMuonUpdate;
-    using P = SplitTile<WI, WJ, TI, TJ, STAGES, kUpdate>;
+    using P = SplitTile<WI, WJ, TI, TJ, STAGES, SUBS, kUpdate>;
     __shared__ __align__(1024) unsigned char lds[P::kLds];
-    const uint32_t n = xcd_contiguous_index(blockIdx.x, total);
-    const MuonPart& a = parts[part_of(firsts, count, n)];
-    const uint32_t local = n - a.first[kUpdate ? kMuonUpdate : kMuonGram];
+    // an XCD's workgroups take neighbouring tiles of each matrix; the larger matrices come first
+    const int part = part_of(firsts, count, blockIdx.x);
+    const MuonPart& a = parts[part];
+    const uint32_t first = firsts[part], tiles = (part + 1 < count ? firsts[part + 1] : total) - first;
+    const uint32_t local = xcd_contiguous_index(blockIdx.x - first, tiles);
     const _Float16* x = a.x[turn];
     const int64_t out_stride = kUpdate ? a.x_stride : a.g_stride, out_cols = kUpdate ? a.x_cols : a.g_cols;
     uint32_t ti, tj;
@@ -368,16 +384,16 @@ __global__ void __launch_bounds__(256) zero_kernel(Mat m) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tiles of 128 x 128 (of the update: 256 x 128) where they occupy half of the
-// card, else of 64 x 64: a small network's matrices are too few large tiles.
+// Tiles of 128 x 128 where they occupy half of the card, else of 64 x 64: a
+// small network's matrices are too few large tiles.
 uint32_t count_tiles(const MuonPart* parts, int count, bool large, int phase, MuonPart* set) {
     int64_t n = 0;
-    const int64_t bi = !large ? 64 : phase == kMuonUpdate ? 256 : 128, bj = large ? 128 : 64;
+    const int64_t edge = large ? 128 : 64;
     for (int i = 0; i < count; ++i) {
         const MuonPart& a = parts[i];
         if (set) set[i].first[phase] = (uint32_t)n;
-        const int64_t down = ceil_div(a.side, bj);
-        n += phase == kMuonUpdate ? ceil_div(a.x_cols / 2, bi) * down : down * (down + 1) / 2;
+        const int64_t down = ceil_div(a.side, edge);
+        n += phase == kMuonUpdate ? ceil_div(a.x_cols / 2, edge) * down : down * (down + 1) / 2;
     }
     return n < 0x7fffffff ? (uint32_t)n : 0x7fffffffu;
 }
@@ -435,12 +451,10 @@ static void launch_product(const MuonPlan& plan, const MuonPart* parts, const ui
                            hipStream_t s) {
     const int w = PHASE == kMuonUpdate;
     const uint32_t* f = firsts + (w ? kMuonUpdate : kMuonGram) * count;
-    if (!plan.large[w])
-        product_kernel<PHASE, 2, 2, 2, 2, 4><<<plan.tiles[w], 256, 0, s>>>(parts, f, count, plan.tiles[w], turn);
-    else if constexpr (PHASE == kMuonUpdate)
-        product_kernel<PHASE, 4, 2, 4, 4, 3><<<plan.tiles[w], 512, 0, s>>>(parts, f, count, plan.tiles[w], turn);
+    if (plan.large[w])
+        product_kernel<PHASE, 2, 4, 4, 2, 2, 2><<<plan.tiles[w], 512, 0, s>>>(parts, f, count, plan.tiles[w], turn);
     else
-        product_kernel<PHASE, 2, 4, 4, 2, 4><<<plan.tiles[w], 512, 0, s>>>(parts, f, count, plan.tiles[w], turn);
+        product_kernel<PHASE, 2, 2, 2, 2, 4, 1><<<plan.tiles[w], 256, 0, s>>>(parts, f, count, plan.tiles[w], turn);
 }
 
 int launch_muon_step(const MuonPlan& plan, int count, const MuonStep& p, unsigned char* workspace, hipStream_t s) {

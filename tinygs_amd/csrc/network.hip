@@ -2,7 +2,9 @@
 // argument checks, workspaces and the optimiser's handle.
 #include <math.h>
 
+#include <algorithm>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "device_buffer.h"
@@ -17,6 +19,7 @@ struct tgs_network {
 struct tgs_muon {
     std::vector<MuonPart> mats;
     std::vector<uint32_t> firsts;
+    std::vector<std::pair<int64_t, int64_t>> shapes;   // in the caller's order
     bool on_device = false;   // the workspace holds the matrices' table
     MuonPlan plan{};
     int grad_dtype = TGS_DTYPE_FLOAT32;
@@ -139,6 +142,10 @@ void bind_muon(tgs_muon* m, const tgs_matrix* weights, const tgs_matrix* grads, 
         a.m = view(&momenta[i]);
         a.c = view(copies ? &copies[i] : nullptr);
     }
+    // a step's launches take the larger matrices first
+    std::sort(m->mats.begin(), m->mats.end(), [](const MuonPart& x, const MuonPart& y) {
+        return x.w.rows * x.w.cols > y.w.rows * y.w.cols;
+    });
     m->plan = plan_muon(m->mats.data(), count);
     m->on_device = false;
     m->grad_dtype = grads[0].dtype;
@@ -295,6 +302,7 @@ int tgs_muon_create(const tgs_matrix* weights, const tgs_matrix* grads, const tg
     try {
         m->mats.resize((size_t)count);
         m->firsts.resize((size_t)count * 3);
+        for (int32_t i = 0; i < count; ++i) m->shapes.emplace_back(weights[i].rows, weights[i].cols);
     } catch (...) {
         delete m;
         return fail(TGS_ERR_STATE, "out of host memory");
@@ -327,7 +335,7 @@ int tgs_muon_set_matrices(tgs_muon* m, const tgs_matrix* weights, const tgs_matr
         (copies && copies[0].dtype != m->copy_dtype))
         return fail(TGS_ERR_INVALID, "the gradients' or copies' dtype is not that of the creation");
     for (int32_t i = 0; i < count; ++i)
-        if (weights[i].rows != m->mats[(size_t)i].w.rows || weights[i].cols != m->mats[(size_t)i].w.cols)
+        if (weights[i].rows != m->shapes[(size_t)i].first || weights[i].cols != m->shapes[(size_t)i].second)
             return fail(TGS_ERR_INVALID, "weights[%d] is not of its shape at creation", i);
     bind_muon(m, weights, grads, momenta, copies, count);
     return TGS_OK;
