@@ -344,42 +344,38 @@ struct Tile {
 #pragma unroll
             for (int n = 0; n < STAGES; ++n)
                 if (n < steps) load();
-            typename Frag<T>::type fa[TI], fb[TJ], next[TJ];
-            const auto multiply_row = [&](int u) {
+            // Two sets of fragments, of a stage's two parts. Each is read while
+            // the other is multiplied, so that the reads are done well before
+            // the barrier that gives their stage up.
+            static_assert(A::kSubs == 2, "");
+            typename Frag<T>::type fa[2][TI], fb[2][TJ];
+            const auto read = [&](int s) {
 #pragma unroll
-                for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[u], fb[v], acc[u][v]);
+                for (int v = 0; v < TJ; ++v) fb[s][v] = B::fragment(from + A::kBytes, (wj * TJ + v) * 16, s, lane);
+#pragma unroll
+                for (int u = 0; u < TI; ++u) fa[s][u] = A::fragment(from, (wi * TI + u) * 16, s, lane);
             };
-            // The products of the fragments held, and the reads of part s of stage `from` in their place.
-            const auto pass = [&](int s) {
+            const auto multiply_all = [&](int s) {
 #pragma unroll
-                for (int v = 0; v < TJ; ++v) next[v] = B::fragment(from + A::kBytes, (wj * TJ + v) * 16, s, lane);
+                for (int u = 0; u < TI; ++u)
 #pragma unroll
-                for (int u = 0; u < TI; ++u) {   // A's fragments are replaced one by one as their products are done
-                    multiply_row(u);
-                    fa[u] = A::fragment(from, (wi * TI + u) * 16, s, lane);
-                    __builtin_amdgcn_sched_barrier(0);   // read earlier, they would take registers of their own
-                }
-#pragma unroll
-                for (int v = 0; v < TJ; ++v) fb[v] = next[v];
+                    for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[s][u], fb[s][v], acc[u][v]);
             };
             wait_for_stage<kLoads>(min(steps - 1, STAGES - 1));
-#pragma unroll
-            for (int v = 0; v < TJ; ++v) fb[v] = B::fragment(from + A::kBytes, (wj * TJ + v) * 16, 0, lane);
-#pragma unroll
-            for (int u = 0; u < TI; ++u) fa[u] = A::fragment(from, (wi * TI + u) * 16, 0, lane);
+            read(0);
             for (int t = 0; t + 1 < steps; ++t) {
-#pragma unroll
-                for (int s = 1; s < A::kSubs; ++s) pass(s);
+                read(1);
+                multiply_all(0);
                 // the next stage is there, and every wave has read this one, which the load fills anew
                 wait_for_stage<kLoads>(min(steps - 2 - t, STAGES - 2));
                 if (t + STAGES < steps) load();
                 from = from + kStage < lds + kLds ? from + kStage : lds;
-                pass(0);
+                read(0);
+                multiply_all(1);
             }
-#pragma unroll
-            for (int s = 1; s < A::kSubs; ++s) pass(s);
-#pragma unroll
-            for (int u = 0; u < TI; ++u) multiply_row(u);
+            read(1);
+            multiply_all(0);
+            multiply_all(1);
         }
     }
 };

@@ -173,11 +173,11 @@ __global__ void __launch_bounds__(kPatchThreads) apply_kernel(const MuonPart* pa
 
 // ---- the products
 
-// A tile of the three-product sum, in steps of 32 of k, SUBS of them a stage of
+// A tile of the three-product sum, in steps of 32 of k, two of them a stage of
 // the ring and a barrier. K-contiguous operands are matrices of twice the
 // columns, whose steps of 128 bytes are a row's 32 hi and 32 lo; the
 // R-contiguous X has tiles of twice the rows and steps of 32 k.
-template <int WI, int WJ, int TI, int TJ, int STAGES, int SUBS, bool A_RC>
+template <int WI, int WJ, int TI, int TJ, int STAGES, bool A_RC>
 struct SplitTile {
     static constexpr int kWavesI = WI, kWavesJ = WJ;
     static constexpr int kWaves = WI * WJ, kThreads = 64 * kWaves;
@@ -185,8 +185,8 @@ struct SplitTile {
     using T = _Float16;
     using A = TileSide<T, A_RC ? 2 * BI : BI, kWaves, A_RC, A_RC ? 64 : 128>;
     using B = TileSide<T, BJ, kWaves, false, 128>;
-    static constexpr int kStep = A::kBytes + B::kBytes, kStage = SUBS * kStep, kLds = STAGES * kStage;
-    static constexpr int kLoads = SUBS * (A::kLoads + B::kLoads);   // a wave and stage
+    static constexpr int kStep = A::kBytes + B::kBytes, kStage = 2 * kStep, kLds = STAGES * kStage;
+    static constexpr int kLoads = 2 * (A::kLoads + B::kLoads);   // a wave and stage
 
     static __device__ __forceinline__ void run(unsigned char* lds, const TileOperand& a, const TileOperand& b, int64_t i0,
                                                int64_t j0, int steps, f32x4 (&acc)[TI][TJ]) {
@@ -200,12 +200,12 @@ struct SplitTile {
         for (int u = 0; u < TI; ++u)
 #pragma unroll
             for (int v = 0; v < TJ; ++v) acc[u][v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const int stages = (steps + SUBS - 1) / SUBS;
+        const int stages = (steps + 1) / 2;
         int left = steps;   // of the steps from the next load on; none: zeros
         unsigned char* fill = lds;
         const auto load = [&] {
 #pragma unroll
-            for (int q = 0; q < SUBS; ++q) {
+            for (int q = 0; q < 2; ++q) {
                 sa.load(fill + q * kStep, (int64_t)left * A::kDepth, wave, lane);
                 sb.load(fill + q * kStep + A::kBytes, (int64_t)left * B::kDepth, wave, lane);
                 --left;
@@ -216,56 +216,44 @@ struct SplitTile {
         for (int n = 0; n < STAGES; ++n)
             if (n < stages) load();
         const unsigned char* from = lds;
-        typename Frag<T>::type fa[2][TI], fb[2][TJ], next[2][TJ];   // hi, lo
-        const auto read_a = [&](int u, int q) {
-            const int r = (wi * TI + u) * 16;
+        typename Frag<T>::type fa[2][2][TI], fb[2][2][TJ];   // of the stage's first and second step; hi, lo
+        const auto read = [&](int q) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                fa[h][u] = A_RC ? A::fragment(from + q * kStep, (r & ~31) * 2 + 32 * h + (r & 16), 0, lane)
-                                : A::fragment(from + q * kStep, r, h, lane);
-        };
-        const auto read_b = [&](auto& to, int q) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int v = 0; v < TJ; ++v)
-                    to[h][v] = B::fragment(from + q * kStep + A::kBytes, (wj * TJ + v) * 16, h, lane);
-        };
-        const auto multiply_row = [&](int u) {
+                    fb[q][h][v] = B::fragment(from + q * kStep + A::kBytes, (wj * TJ + v) * 16, h, lane);
 #pragma unroll
-            for (int q = 0; q < 3; ++q)   // hi hi, hi lo, lo hi
-#pragma unroll
-                for (int v = 0; v < TJ; ++v) acc[u][v] = multiply(fa[q == 2][u], fb[q == 1][v], acc[u][v]);
-        };
-        const auto pass = [&](int q) {   // as Tile's
-            read_b(next, q);
-#pragma unroll
-            for (int u = 0; u < TI; ++u) {
-                multiply_row(u);
-                read_a(u, q);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int u = 0; u < TI; ++u) {
+                    const int r = (wi * TI + u) * 16;
+                    fa[q][h][u] = A_RC ? A::fragment(from + q * kStep, (r & ~31) * 2 + 32 * h + (r & 16), 0, lane)
+                                       : A::fragment(from + q * kStep, r, h, lane);
+                }
             }
+        };
+        const auto multiply_all = [&](int q) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 3; ++h)   // hi hi, hi lo, lo hi: the squares in turn, no sum waits for its last
 #pragma unroll
-                for (int v = 0; v < TJ; ++v) fb[h][v] = next[h][v];
+                for (int u = 0; u < TI; ++u)
+#pragma unroll
+                    for (int v = 0; v < TJ; ++v)
+                        acc[u][v] = multiply(fa[q][h == 2][u], fb[q][h == 1][v], acc[u][v]);
         };
         wait_for_stage<kLoads>(min(stages - 1, STAGES - 1));
-        read_b(fb, 0);
-#pragma unroll
-        for (int u = 0; u < TI; ++u) read_a(u, 0);
-        for (int t = 0; t + 1 < stages; ++t) {
-#pragma unroll
-            for (int q = 1; q < SUBS; ++q) pass(q);
+        read(0);
+        for (int t = 0; t + 1 < stages; ++t) {   // as Tile's
+            read(1);
+            multiply_all(0);
             wait_for_stage<kLoads>(min(stages - 2 - t, STAGES - 2));
             if (t + STAGES < stages) load();
             from = from + kStage < lds + kLds ? from + kStage : lds;
-            pass(0);
+            read(0);
+            multiply_all(1);
         }
-#pragma unroll
-        for (int q = 1; q < SUBS; ++q) pass(q);
-#pragma unroll
-        for (int u = 0; u < TI; ++u) multiply_row(u);
+        read(1);
+        multiply_all(0);
+        multiply_all(1);
     }
 };
 
@@ -274,11 +262,11 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // Gram: G = X X^T. Square: P = b G + c G G. Update: X' = a X + P X. The stored
 // matrices are zero up to a multiple of 32 columns, which the products keep:
 // they run over whole strides.
-template <int PHASE, int WI, int WJ, int TI, int TJ, int STAGES, int SUBS>
+template <int PHASE, int WI, int WJ, int TI, int TJ, int STAGES>
 __global__ void __launch_bounds__(64 * WI * WJ) product_kernel(const MuonPart* parts, const uint32_t* firsts, int count,
                                                                uint32_t total, int turn) {
     constexpr bool kUpdate = PHASE == kMuonUpdate;
-    using P = SplitTile<WI, WJ, TI, TJ, STAGES, SUBS, kUpdate>;
+    using P = SplitTile<WI, WJ, TI, TJ, STAGES, kUpdate>;
     __shared__ __align__(1024) unsigned char lds[P::kLds];
     // an XCD's workgroups take neighbouring tiles of each matrix; the larger matrices come first
     const int part = part_of(firsts, count, blockIdx.x);
@@ -452,9 +440,9 @@ static void launch_product(const MuonPlan& plan, const MuonPart* parts, const ui
     const int w = PHASE == kMuonUpdate;
     const uint32_t* f = firsts + (w ? kMuonUpdate : kMuonGram) * count;
     if (plan.large[w])
-        product_kernel<PHASE, 2, 4, 4, 2, 2, 2><<<plan.tiles[w], 512, 0, s>>>(parts, f, count, plan.tiles[w], turn);
+        product_kernel<PHASE, 2, 4, 4, 2, 2><<<plan.tiles[w], 512, 0, s>>>(parts, f, count, plan.tiles[w], turn);
     else
-        product_kernel<PHASE, 2, 2, 2, 2, 4, 1><<<plan.tiles[w], 256, 0, s>>>(parts, f, count, plan.tiles[w], turn);
+        product_kernel<PHASE, 2, 2, 2, 2, 2><<<plan.tiles[w], 256, 0, s>>>(parts, f, count, plan.tiles[w], turn);
 }
 
 int launch_muon_step(const MuonPlan& plan, int count, const MuonStep& p, unsigned char* workspace, hipStream_t s) {
