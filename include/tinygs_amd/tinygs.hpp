@@ -29,6 +29,8 @@
 //     tgs_*_reorder / tgs_adam_reset_rows entry points.
 //   * GPUGaussian3d can store sh0 / sh_rest as fp16 (sh_dtype), the storage
 //     mode of the 1M-Gaussian 1080p benchmark; gradients stay fp32.
+//   * LayerOps and Muon (the attribute network's operators and the optimiser of
+//     its matrices) have no counterpart in the reference.
 // Every failing call throws std::runtime_error carrying tgs_last_error(), as
 // the reference's CUDA_CHECK_THROW (tinygs/include/tinygs/cuda/common_host.hpp:104-109).
 #pragma once
@@ -1042,5 +1044,103 @@ inline std::shared_ptr<GPUGaussian3d> load_gaussians_ply(const std::string& file
     throw_on(tgs_ply_load_gaussians(filename.c_str(), &c, nullptr), "load_gaussians_ply");
     return g;
 }
+
+// ---------------------------------------------------------------- attribute network
+
+// A matrix of the network's operators: rows of cols elements of dtype
+// (TGS_DTYPE_FLOAT32, _FLOAT16 or _BFLOAT16), `stride` elements apart.
+inline tgs_matrix matrix(void* data, int64_t rows, int64_t cols, int32_t dtype = TGS_DTYPE_FLOAT32, int64_t stride = 0) {
+    return tgs_matrix{data, rows, cols, stride ? stride : cols, dtype};
+}
+
+enum class Activation { None = TGS_ACTIVATION_NONE, Relu = TGS_ACTIVATION_RELU, Silu = TGS_ACTIVATION_SILU,
+                        Gelu = TGS_ACTIVATION_GELU };
+
+// The layer operators on a handle that owns their workspace; its calls run on
+// one stream, or the caller orders them. Optional matrices and vectors are
+// null pointers where they are left out.
+class LayerOps {
+public:
+    LayerOps() { throw_on(tgs_network_create(&m_handle), "LayerOps"); }
+    ~LayerOps() { tgs_network_destroy(m_handle); }
+    LayerOps(const LayerOps&) = delete;
+    LayerOps& operator=(const LayerOps&) = delete;
+
+    // y = act(x w^T + bias) + residual; preact receives x w^T + bias
+    void linear(const tgs_matrix& x, const tgs_matrix& w, const float* bias, Activation activation,
+                const tgs_matrix* residual, const tgs_matrix* preact, const tgs_matrix& y, hipStream_t stream = nullptr) {
+        throw_on(tgs_linear_forward(m_handle, &x, &w, bias, (int32_t)activation, residual, preact, &y, stream),
+                 "LayerOps::linear");
+    }
+    void linear_backward(const tgs_matrix& grad_y, const tgs_matrix& x, const tgs_matrix& w, const tgs_matrix* preact,
+                         Activation activation, const tgs_matrix* grad_x, const tgs_matrix* grad_w, float* grad_bias,
+                         hipStream_t stream = nullptr) {
+        throw_on(tgs_linear_backward(m_handle, &grad_y, &x, &w, preact, (int32_t)activation, grad_x, grad_w, grad_bias,
+                                     stream),
+                 "LayerOps::linear_backward");
+    }
+    void layer_norm(const tgs_matrix& x, const float* gamma, const float* beta, float epsilon, const tgs_matrix& y,
+                    float* mean, float* rstd, hipStream_t stream = nullptr) {
+        throw_on(tgs_layer_norm_forward(m_handle, &x, gamma, beta, epsilon, &y, mean, rstd, stream),
+                 "LayerOps::layer_norm");
+    }
+    void layer_norm_backward(const tgs_matrix& grad_y, const tgs_matrix& x, const float* gamma, const float* mean,
+                             const float* rstd, const tgs_matrix* residual_grad, const tgs_matrix* grad_x,
+                             float* grad_gamma, float* grad_beta, hipStream_t stream = nullptr) {
+        throw_on(tgs_layer_norm_backward(m_handle, &grad_y, &x, gamma, mean, rstd, residual_grad, grad_x, grad_gamma,
+                                         grad_beta, stream),
+                 "LayerOps::layer_norm_backward");
+    }
+
+private:
+    tgs_network* m_handle = nullptr;
+};
+
+// Muon on a network's matrices; copies (may be empty) receive the updated
+// weights in their dtype. The pointers are kept.
+class Muon {
+public:
+    Muon(const std::vector<tgs_matrix>& weights, const std::vector<tgs_matrix>& grads,
+         const std::vector<tgs_matrix>& momenta, const std::vector<tgs_matrix>& copies = {}) {
+        if (grads.size() != weights.size() || momenta.size() != weights.size() ||
+            (!copies.empty() && copies.size() != weights.size()))
+            throw std::runtime_error("Muon: weights, grads, momenta and copies must have the same count");
+        throw_on(tgs_muon_create(weights.data(), grads.data(), momenta.data(), copies.empty() ? nullptr : copies.data(),
+                                 (int32_t)weights.size(), &m_handle),
+                 "Muon");
+    }
+    ~Muon() { tgs_muon_destroy(m_handle); }
+    Muon(const Muon&) = delete;
+    Muon& operator=(const Muon&) = delete;
+
+    void set_lr(float lr) { throw_on(tgs_muon_set_lr(m_handle, lr), "Muon::set_lr"); }
+    float get_lr() const { return tgs_muon_get_lr(m_handle); }
+    // Keys: lr, momentum, weight_decay, epsilon, nesterov (0/1), iterations.
+    void set_params(const ParamMap& p) {
+        tgs_muon_params a{};
+        throw_on(tgs_muon_get_params(m_handle, &a), "Muon::get_params");
+        for (const auto& [k, v] : p) {
+            if (k == "lr") a.lr = (float)v;
+            else if (k == "momentum") a.momentum = (float)v;
+            else if (k == "weight_decay") a.weight_decay = (float)v;
+            else if (k == "epsilon") a.epsilon = (float)v;
+            else if (k == "nesterov") a.nesterov = v != 0.0;
+            else if (k == "iterations") a.iterations = (int32_t)v;
+            else throw std::runtime_error("Muon::set_params: unknown key " + k);
+        }
+        throw_on(tgs_muon_set_params(m_handle, &a), "Muon::set_params");
+    }
+    ParamMap get_params() const {
+        tgs_muon_params a{};
+        throw_on(tgs_muon_get_params(m_handle, &a), "Muon::get_params");
+        return {{"lr", a.lr},           {"momentum", a.momentum}, {"weight_decay", a.weight_decay},
+                {"epsilon", a.epsilon}, {"nesterov", a.nesterov}, {"iterations", a.iterations}};
+    }
+    void step(float scale, hipStream_t stream = nullptr) { throw_on(tgs_muon_step(m_handle, scale, stream), "Muon::step"); }
+    void reset(hipStream_t stream = nullptr) { throw_on(tgs_muon_reset(m_handle, stream), "Muon::reset"); }
+
+private:
+    tgs_muon* m_handle = nullptr;
+};
 
 }  // namespace tinygs_amd

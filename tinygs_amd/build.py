@@ -69,7 +69,7 @@ def build(jobs: int = 8, extra: list[str] | None = None, verbose: bool = True) -
 
 
 ROOT = os.path.dirname(HERE)
-CPP_TESTS = ("train_step", "densify_step")   # tests/cpp/<name>.cpp -> tests/cpp/_build/<name>
+CPP_TESTS = ("train_step", "densify_step", "network_step")   # tests/cpp/<name>.cpp -> tests/cpp/_build/<name>
 CPP_TEST_BIN = os.path.join(ROOT, "tests", "cpp", "_build", "train_step")
 
 

@@ -188,3 +188,118 @@ class LayerOps:
         if rc:
             _lib.check(rc, "layer_norm_backward")
         return grad_x, grad_gamma, grad_beta
+
+
+class AttributeNetwork:
+    """A network over the Gaussians: features [n, inputs] -> attributes [n, outputs].
+
+    h = features w_in^T + b_in; blocks times h = h + act(norm(h) w_1^T + b_1) w_2^T + b_2; attributes =
+    norm(h) w_out^T + b_out. norm is a layer norm with its own gamma and beta. The last matrix starts at zero, so an
+    untrained network changes nothing.
+
+    weights are the float32 matrices that an optimiser updates (create_optimizer("muon", net.weights, net.grads), or
+    net.optimizer()); for a half dtype the products read net.copies, which Muon writes in its step. vectors and
+    vector_grads hold all biases, gammas and betas, and their gradients, as one float32 vector each, for an optimiser
+    of vectors. backward assigns every gradient."""
+
+    def __init__(self, inputs: int, outputs: int, width: int = 256, hidden: int | None = None, blocks: int = 2,
+                 activation: str = "gelu", dtype=None, seed: int = 0, eps: float = 1e-5, device: str = "cuda"):
+        import torch
+        if activation not in ACTIVATIONS:
+            raise RuntimeError(f"AttributeNetwork: unknown activation: {activation}")
+        hidden = width if hidden is None else hidden
+        if min(inputs, outputs, width, hidden) < 1 or blocks < 0:
+            raise RuntimeError("AttributeNetwork: sizes must be positive")
+        self.dtype = torch.float32 if dtype is None else dtype
+        if self.dtype not in _dtypes():
+            raise RuntimeError("AttributeNetwork: only float32, float16 and bfloat16 are supported")
+        self.inputs, self.outputs, self.activation, self.eps = inputs, outputs, activation, float(eps)
+        shapes = [(width, inputs)] + [(hidden, width), (width, hidden)] * blocks + [(outputs, width)]
+        g = torch.Generator().manual_seed(seed)
+        self.weights = [(torch.randn(o, i, generator=g) / math.sqrt(i)).to(device) for o, i in shapes]
+        self.weights[-1].zero_()
+        half = self.dtype != torch.float32
+        self.copies = [w.to(self.dtype) for w in self.weights] if half else None
+        self.grads = [torch.zeros(s, dtype=self.dtype, device=device) for s in shapes]
+        # the vectors: a bias for every matrix, then gamma and beta of the blocks' norms and the last one
+        sizes = [o for o, _ in shapes] + [width, width] * (blocks + 1)
+        self.vectors = torch.zeros(sum(sizes), device=device)
+        self.vector_grads = torch.zeros_like(self.vectors)
+        views, grads = self.vectors.split(sizes), self.vector_grads.split(sizes)
+        m = len(shapes)
+        self.biases, self.bias_grads = views[:m], grads[:m]
+        self.norms = list(zip(views[m::2], views[m + 1::2]))
+        self.norm_grads = list(zip(grads[m::2], grads[m + 1::2]))
+        for gamma, _ in self.norms:
+            gamma.fill_(1.0)
+        self.blocks = blocks
+        self.ops = LayerOps()
+        self._kept = None
+
+    def optimizer(self):
+        """Muon on the matrices, which also writes the half-precision copies."""
+        from .optim import Muon
+        return Muon(self.weights, self.grads, copies=self.copies)
+
+    def matrices(self):
+        """The matrices that the products read."""
+        return self.weights if self.copies is None else self.copies
+
+    def forward(self, features, keep: bool = True, stream=None):
+        """The attributes, in the network's dtype. keep: hold what backward needs (until the next forward)."""
+        ops, w = self.ops, self.matrices()
+        self._kept = None
+        h = ops.linear(features, w[0], self.biases[0], stream=stream)
+        kept = [features]
+        for k in range(self.blocks):
+            n, mean, rstd = ops.layer_norm(h, *self.norms[k], eps=self.eps, stream=stream)
+            up, down = 1 + 2 * k, 2 + 2 * k
+            a = ops.linear(n, w[up], self.biases[up], activation=self.activation, keep_preact=keep, stream=stream)
+            a, z = a if keep else (a, None)
+            if keep:
+                kept.append((h, n, mean, rstd, a, z))
+            # without a backward the block's input is not needed again: its sum takes its place
+            h = ops.linear(a, w[down], self.biases[down], residual=h, out=None if keep else h, stream=stream)
+        n, mean, rstd = ops.layer_norm(h, *self.norms[-1], eps=self.eps, stream=stream)
+        if keep:
+            kept.append((h, n, mean, rstd))
+            self._kept = kept
+        return ops.linear(n, w[-1], self.biases[-1], stream=stream)
+
+    def backward(self, grad_attributes, need_features: bool = False, stream=None):
+        """Fills grads and vector_grads for dL/dattributes (in the network's dtype) of the last forward; returns
+        dL/dfeatures where needed."""
+        if self._kept is None:
+            raise RuntimeError("AttributeNetwork::backward: no forward that kept its values")
+        ops, w, kept = self.ops, self.matrices(), self._kept
+        act = self.activation
+        h, n, mean, rstd = kept[-1]
+        g, _, _ = ops.linear_backward(grad_attributes, n, w[-1], grad_weight=self.grads[-1],
+                                      grad_bias=self.bias_grads[-1], stream=stream)
+        gg, gb = self.norm_grads[-1]
+        g, _, _ = ops.layer_norm_backward(g, h, self.norms[-1][0], mean, rstd, grad_x=g, grad_gamma=gg, grad_beta=gb,
+                                          stream=stream)
+        for k in reversed(range(self.blocks)):
+            h, n, mean, rstd, a, z = kept[1 + k]
+            up, down = 1 + 2 * k, 2 + 2 * k
+            ga, _, _ = ops.linear_backward(g, a, w[down], grad_weight=self.grads[down],
+                                           grad_bias=self.bias_grads[down], stream=stream)
+            gn, _, _ = ops.linear_backward(ga, n, w[up], preact=z, activation=act, grad_weight=self.grads[up],
+                                           grad_bias=self.bias_grads[up], stream=stream)
+            gg, gb = self.norm_grads[k]
+            # the residual path's gradient joins the norm's
+            g, _, _ = ops.layer_norm_backward(gn, h, self.norms[k][0], mean, rstd, residual_grad=g, grad_x=g,
+                                              grad_gamma=gg, grad_beta=gb, stream=stream)
+        gx, _, _ = ops.linear_backward(g, kept[0], w[0], need_x=need_features, grad_weight=self.grads[0],
+                                       grad_bias=self.bias_grads[0], stream=stream)
+        return gx
+
+
+def encode_positions(means, octaves: int = 10, dtype=None):
+    """Positions [n, 3] with the sines and cosines of their multiples by 2^0 .. 2^(octaves - 1): [n, 3 + 6 octaves],
+    the usual input of a network over positions."""
+    import torch
+    scaled = means[:, None, :] * (2.0 ** torch.arange(octaves, device=means.device))[None, :, None]
+    scaled = scaled.reshape(means.shape[0], 3 * octaves)
+    out = torch.cat([means, torch.sin(scaled), torch.cos(scaled)], dim=1)
+    return out if dtype is None else out.to(dtype)
