@@ -375,14 +375,11 @@ __global__ void __launch_bounds__(256) wide_columns_kernel(LayerNormBackward a) 
 }
 
 // Workgroups of a backward with column sums: each writes 8 n bytes of sums, so
-// no more than fill the card four times over, and at least eight rows a group
-// where that leaves one workgroup a compute unit.
+// no more than fill the card four times over, and at least two rows a group
+// (6007 x 323 floats: 10 us with two, 12 with eight).
 int backward_blocks(int64_t rows, int groups) {
-    const int64_t by_rows = (rows + groups - 1) / groups;
-    const int64_t eight = (rows + 8 * groups - 1) / (8 * groups);
-    const int64_t want = eight > 256 ? eight : 256;
-    const int64_t most = want < 1024 ? want : 1024;
-    return (int)(by_rows < most ? by_rows : most);
+    const int64_t want = (rows + 2 * groups - 1) / (2 * groups);
+    return (int)(want < 1024 ? want : 1024);
 }
 
 }  // namespace

@@ -196,29 +196,31 @@ __global__ void __launch_bounds__(S::kThreads) grad_w_kernel(Mat dz, Mat x, Mat 
 }
 
 // The splits' float sums joined in a fixed order: 256 neighbouring ones a
-// workgroup, four a lane; each of its four waves takes every fourth split, with
-// eight loads in flight. A split holds out's elements and, after them, those
-// of `bias` (either may be left out); `width` is the distance between splits.
+// workgroup, four a lane; each of its sixteen waves takes every sixteenth
+// split, with four loads in flight. A split holds out's elements and, after
+// them, those of `bias` (either may be left out); `width` is the distance
+// between splits.
 template <class T>
-__global__ void __launch_bounds__(256) join_kernel(const float* partial, int splits, int64_t width, Mat out, float* bias,
-                                                   int64_t biases) {
-    __shared__ f32x4 s[4][64];
+__global__ void __launch_bounds__(1024) join_kernel(const float* partial, int splits, int64_t width, Mat out, float* bias,
+                                                    int64_t biases) {
+    constexpr int kParts = 16;
+    __shared__ f32x4 s[kParts][64];
     const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
     const int64_t n = out.rows * out.cols, end = n + biases, q = ((int64_t)blockIdx.x * 64 + lane) * 4;
     typedef float loose4 __attribute__((ext_vector_type(4), aligned(4)));
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (q + 4 <= end) {
         int k = part;
-        for (; k + 28 < splits; k += 32) {
-            f32x4 u[8];
+        for (; k + 3 * kParts < splits; k += 4 * kParts) {
+            f32x4 u[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) u[e] = *(const loose4*)(partial + (k + 4 * e) * width + q);
+            for (int e = 0; e < 4; ++e) u[e] = *(const loose4*)(partial + (k + kParts * e) * width + q);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v += u[e];
+            for (int e = 0; e < 4; ++e) v += u[e];
         }
-        for (; k < splits; k += 4) v += *(const loose4*)(partial + k * width + q);
+        for (; k < splits; k += kParts) v += *(const loose4*)(partial + k * width + q);
     } else {
-        for (int k = part; k < splits; k += 4)
+        for (int k = part; k < splits; k += kParts)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (q + e < end) v[e] += partial[k * width + q + e];
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float* partial, int spl
     s[part][lane] = v;
     __syncthreads();
     if (part != 0) return;
-    v = ((v + s[1][lane]) + s[2][lane]) + s[3][lane];
+    for (int k = 1; k < kParts; ++k) v += s[k][lane];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         if (q + e < n) {
@@ -343,10 +345,10 @@ void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) 
         const Mat gw{a.grad_w.p, out, in, a.grad_w.p ? a.grad_w.stride : in};
         const int64_t biases = a.grad_bias ? out : 0;
         if (gw.p)
-            join_kernel<T><<<(unsigned)ceil_div(in * out + biases, 256), 256, 0, s>>>(split, (int)p.splits, in * out + out,
+            join_kernel<T><<<(unsigned)ceil_div(in * out + biases, 256), 1024, 0, s>>>(split, (int)p.splits, in * out + out,
                                                                                       gw, a.grad_bias, biases);
         else if (biases)
-            join_kernel<T><<<(unsigned)ceil_div(out, 256), 256, 0, s>>>(split + in * out, (int)p.splits, in * out + out,
+            join_kernel<T><<<(unsigned)ceil_div(out, 256), 1024, 0, s>>>(split + in * out, (int)p.splits, in * out + out,
                                                                         Mat{nullptr, 0, 1, 1}, a.grad_bias, biases);
         return;
     }
@@ -376,7 +378,7 @@ void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) 
                 dz, a.x, a.grad_w, p.splits > 1 ? partial : nullptr, p.split_rows, ni, nj);
         });
         if (p.splits > 1) {
-            join_kernel<T><<<(unsigned)ceil_div(in * out, 256), 256, 0, s>>>(partial, (int)p.splits, in * out, a.grad_w,
+            join_kernel<T><<<(unsigned)ceil_div(in * out, 256), 1024, 0, s>>>(partial, (int)p.splits, in * out, a.grad_w,
                                                                              nullptr, 0);
         }
     }
@@ -390,6 +392,11 @@ size_t linear_backward_workspace(const LinearBackward& a) {
 }
 
 int launch_linear_forward(const LinearForward& a, hipStream_t s) {
+    if (linear_forward_is_few(a)) {
+        launch_linear_few(a, s);
+        TGS_CHECK_LAUNCH();
+        return TGS_OK;
+    }
     if (linear_forward_by_rows(a)) {
         launch_linear_rows(a, s);
         TGS_CHECK_LAUNCH();

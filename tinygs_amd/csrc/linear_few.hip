@@ -1,0 +1,116 @@
+// y = act(x w^T + bias) + residual for a few rows (a query, a picked set of
+// Gaussians), bound by the bytes of w and by latency.
+//
+// A workgroup makes 16 columns of up to 16 rows. Its eight waves share k: each
+// takes every eighth step of 32, reads the fragments of w and x straight from
+// memory, four steps in flight, and the eight sums are joined through LDS in
+// order. w passes no LDS, and all of k is on its way at once up to 1024.
+#include "narrow_rows.h"
+
+namespace tgs {
+
+namespace {
+
+constexpr int kWaves = 8;
+constexpr int kAhead = 4;
+
+template <class T, int ACT>
+__device__ __forceinline__ void few_outputs(const LinearForward& a, f32x4 v, int64_t row, int64_t column) {
+    const int n = (int)min(a.y.cols - column, (int64_t)4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (e >= n) break;
+        float z = v[e] + (a.bias ? a.bias[column + e] : 0.0f);
+        if (a.preact.p) ((T*)a.preact.p)[row * a.preact.stride + column + e] = (T)z;
+        z = activate<ACT>(z);
+        if (a.residual.p) z += (float)((const T*)a.residual.p)[row * a.residual.stride + column + e];
+        ((T*)a.y.p)[row * a.y.stride + column + e] = (T)z;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(64 * kWaves) few_kernel(LinearForward a) {
+    using C = Chunk<T>;
+    constexpr int V = C::V, kChunks = 8 / V;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int in = (int)a.x.cols, steps = (in + 31) / 32;
+    const int64_t n0 = (int64_t)blockIdx.x * 16, r0 = (int64_t)blockIdx.y * 16;
+    const bool ragged = in % V != 0;   // the last step then has partial chunks
+
+    struct Side {
+        const T* base;
+        __amdgpu_buffer_rsrc_t buffer;
+        uint32_t offset;
+        int64_t stride;
+        bool exists;
+    };
+    const auto side = [&](const Mat& m, int64_t first) {
+        const int64_t held = min(m.rows - first, (int64_t)16), pitch = m.stride * (int64_t)sizeof(T);
+        Side s;
+        s.base = (const T*)m.p + first * m.stride;
+        s.buffer = resource_of(s.base, (held - 1) * pitch + in * (int64_t)sizeof(T));
+        s.offset = (uint32_t)(lane & 15) * (uint32_t)pitch;
+        s.stride = m.stride;
+        s.exists = (lane & 15) < held;
+        return s;
+    };
+    const Side w = side(a.w, n0), x = side(a.x, r0);
+    typedef typename C::type chunk;
+    const auto load = [&](const Side& s, int step, chunk(&to)[kChunks]) {
+#pragma unroll
+        for (int h = 0; h < kChunks; ++h) {
+            const int k = 32 * step + 8 * (lane >> 4) + V * h;
+            if (ragged && step == steps - 1) {
+                const int left = s.exists ? min(max(in - k, 0), V) : 0;
+                to[h] = C::gather(s.base + (left > 0 ? (lane & 15) * s.stride + k : 0), left);
+            } else {
+                to[h] = __builtin_bit_cast(chunk, __builtin_amdgcn_raw_buffer_load_b128(
+                                                      s.buffer, (int)((k < in ? s.offset : kNowhere) + (uint32_t)k * (uint32_t)sizeof(T)), 0, 0));
+            }
+        }
+    };
+    const auto fragment = [&](const chunk(&v)[kChunks]) {
+        if constexpr (sizeof(T) == 4) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = v[e / 4][e % 4];
+            return split3(f);
+        } else {
+            return __builtin_bit_cast(typename Frag<T>::type, v[0]);
+        }
+    };
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = wave; s < steps; s += kWaves * kAhead) {
+        chunk cw[kAhead][kChunks], cx[kAhead][kChunks];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {   // steps past the last are zeros
+            load(w, s + q * kWaves, cw[q]);
+            load(x, s + q * kWaves, cx[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) acc = multiply(fragment(cw[q]), fragment(cx[q]), acc);
+    }
+    __shared__ f32x4 sums[kWaves][64];
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int q = 1; q < kWaves; ++q) acc += sums[q][lane];
+    const int64_t row = r0 + (lane & 15), column = n0 + 4 * (lane >> 4);
+    if (row >= a.y.rows || column >= a.y.cols) return;
+    if (a.activation == kActGelu) few_outputs<T, kActGelu>(a, acc, row, column);
+    else if (a.activation == kActSilu) few_outputs<T, kActSilu>(a, acc, row, column);
+    else if (a.activation == kActRelu) few_outputs<T, kActRelu>(a, acc, row, column);
+    else few_outputs<T, kActNone>(a, acc, row, column);
+}
+
+}  // namespace
+
+bool linear_forward_is_few(const LinearForward& a) { return a.y.rows <= 32; }
+
+void launch_linear_few(const LinearForward& a, hipStream_t s) {
+    const dim3 grid((unsigned)((a.y.cols + 15) / 16), (unsigned)((a.y.rows + 15) / 16));
+    by_dtype(a.dtype, [&](auto t) { few_kernel<decltype(t)><<<grid, 64 * kWaves, 0, s>>>(a); });
+}
+
+}  // namespace tgs

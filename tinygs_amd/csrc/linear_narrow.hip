@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
             for (int v = 0; v < N::TJ; ++v) fz[v] = N::r_fragment(dz, N::kBlockPlane, (wj * N::TJ + v) * 16, 0, near);
 #pragma unroll
             for (int u = 0; u < N::TI; ++u) {
+                if (u >= N::TI / 2 && (wi * N::TI + u) * 16 >= in) break;
                 const auto fx = N::r_fragment(xs, N::kBlockPlane, (wi * N::TI + u) * 16, 0, near);
 #pragma unroll
                 for (int v = 0; v < N::TJ; ++v) acc[u][v] = multiply(fx, fz[v], acc[u][v]);

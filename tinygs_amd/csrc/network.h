@@ -108,6 +108,10 @@ size_t linear_backward_workspace(const LinearBackward& a);
 int launch_linear_forward(const LinearForward& a, hipStream_t s);
 int launch_linear_backward(const LinearBackward& a, void* workspace, hipStream_t s);
 
+// ---- linear_few.hip: a few rows
+bool linear_forward_is_few(const LinearForward& a);
+void launch_linear_few(const LinearForward& a, hipStream_t s);
+
 // ---- linear_rows.hip: many rows of a narrow layer
 bool linear_forward_by_rows(const LinearForward& a);
 void launch_linear_rows(const LinearForward& a, hipStream_t s);
