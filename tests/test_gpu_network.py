@@ -13,7 +13,8 @@ IDS = ["f32", "f16", "bf16"]
 SHAPES = [(1, 1, 1), (1, 256, 256), (1, 1000, 3), (2, 7, 5), (5, 64, 1), (8, 512, 1030), (9, 40, 72), (17, 84, 59),
           (33, 256, 64), (64, 64, 64), (127, 128, 128), (129, 130, 257), (300, 1, 9), (1000, 323, 96),
           (1025, 256, 256), (640, 512, 384), (3, 1024, 2048), (4099, 84, 59), (70001, 72, 40), (20000, 256, 128),
-          (33000, 72, 72), (33000, 520, 72), (70000, 264, 260), (4097, 256, 700), (66000, 24, 260), (70001, 260, 24), (150001, 130, 129)]
+          (33000, 72, 72), (33000, 520, 72), (70000, 264, 260), (4097, 256, 700), (66000, 24, 260), (70001, 260, 24), (150001, 130, 129),
+          (33, 4096, 130), (200, 1300, 77), (70, 600, 2100)]
 
 
 @pytest.fixture(scope="module")

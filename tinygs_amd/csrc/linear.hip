@@ -7,6 +7,8 @@
 // R-contiguous; its long axis (the rows) is split over workgroups whose float
 // sums a second kernel joins in order. An activation's dz is written once, by
 // the pass that also sums its columns, and read by both products.
+#include <algorithm>
+
 #include "mfma_tile.h"
 
 namespace tgs {
@@ -106,6 +108,34 @@ void by_shape(int64_t ni, int64_t nj, int64_t splits_most, F f) {
     else f(Small{});
 }
 
+constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Few tiles and a long k (an ordinary batch of rows through wide layers): k is
+// split over workgroups, in whole stages of 128 bytes and at least four of
+// them, until 256 small tiles are at work, and a second kernel joins the sums.
+// Whole calls, without and with the split: 512 x 4096 -> 512 halves 35.3 and
+// 15.3 us, floats 104 and 33.5; 64 x 4096 -> 256 halves 24.5 and 12.0, floats
+// 102 and 17.8. The join is a launch more, so a short k stays whole: 512 x 512
+// -> 512 halves (8 stages) 7.3 and 9.4 us, 1024 -> 512 (16) 8.7 and 9.7,
+// 2048 x 2048 -> 256 (32) 14.2 and 13.2; floats, whose stage is six products
+// long, 16.2 and 11.4 at 512 x 512 -> 512 (16).
+struct KSplits {
+    int64_t splits = 1, depth = 0;
+};
+KSplits split_k(int64_t ni, int64_t nj, int64_t k, int size) {
+    const int64_t stage = 128 / size, stages = ceil_div(k, stage), tiles = ceil_div(ni, 64) * ceil_div(nj, 64);
+    KSplits s;
+    int64_t want = tiles > 0 ? 256 / tiles : 1;
+    if (want > stages / 4) want = stages / 4;
+    if (want < 2 || stages < (size == 4 ? 16 : 32)) {
+        s.depth = k;
+        return s;
+    }
+    s.depth = ceil_div(stages, want) * stage;
+    s.splits = ceil_div(k, s.depth);
+    return s;
+}
+
 template <class T, int ACT, class S>
 __device__ __forceinline__ void forward_outputs(const LinearForward& a, const f32x4 (&acc)[S::kSquaresI][S::kSquaresJ],
                                                 int64_t i0, int64_t j0) {
@@ -144,32 +174,82 @@ __device__ __forceinline__ void forward_outputs(const LinearForward& a, const f3
         });
 }
 
+// Float sums of a tile to their place in split `split` of rows x cols.
+template <class S, int TI, int TJ>
+__device__ __forceinline__ void store_sums(const f32x4 (&acc)[TI][TJ], int64_t i0, int64_t j0, float* partial, int64_t split,
+                                           int64_t rows, int64_t cols) {
+    float* out = partial + split * rows * cols;
+    for_outputs<S>(acc, i0, j0, cols, rows,
+                   [&](int64_t i, int64_t j, int n, float(&v)[8]) { store8(out + j * cols + i, n, v); });
+}
+
+// With `partial`, the float sums over the k of split blockIdx.y.
 template <class T, class S>
-__global__ void __launch_bounds__(S::kThreads) forward_kernel(LinearForward a, uint32_t ni, uint32_t nj) {
+__global__ void __launch_bounds__(S::kThreads) forward_kernel(LinearForward a, float* partial, int64_t depth, uint32_t ni,
+                                                              uint32_t nj) {
     using P = typename S::template Product<T, false, false>;
     __shared__ __align__(1024) unsigned char lds[P::kLds];
     uint32_t ti, tj;
     tile_of(xcd_contiguous_index(blockIdx.x, ni * nj), ni, nj, ti, tj);
     const int64_t i0 = (int64_t)ti * S::kI, j0 = (int64_t)tj * S::kJ;
+    const int64_t k0 = (int64_t)blockIdx.y * depth, k1 = min(k0 + depth, a.x.cols);
     f32x4 acc[S::kSquaresI][S::kSquaresJ];
-    P::run(lds, {a.w.p, a.w.rows, a.w.cols, a.w.stride}, {a.x.p, a.x.rows, a.x.cols, a.x.stride}, i0, j0, 0, a.x.cols,
-           acc);
-    if (a.activation == kActGelu) forward_outputs<T, kActGelu, S>(a, acc, i0, j0);
+    P::run(lds, {a.w.p, a.w.rows, a.w.cols, a.w.stride}, {a.x.p, a.x.rows, a.x.cols, a.x.stride}, i0, j0, k0, k1, acc);
+    if (partial) store_sums<S>(acc, i0, j0, partial, blockIdx.y, a.y.rows, a.y.cols);
+    else if (a.activation == kActGelu) forward_outputs<T, kActGelu, S>(a, acc, i0, j0);
     else if (a.activation == kActSilu) forward_outputs<T, kActSilu, S>(a, acc, i0, j0);
     else if (a.activation == kActRelu) forward_outputs<T, kActRelu, S>(a, acc, i0, j0);
     else forward_outputs<T, kActNone, S>(a, acc, i0, j0);
 }
 
-// grad_x = dz w
+// The splits' sums joined in order, and the forward's epilogue on them: eight
+// outputs of a row a thread.
+template <class T, int ACT>
+__global__ void __launch_bounds__(256) join_forward_kernel(LinearForward a, const float* partial, int splits) {
+    const int64_t across = (a.y.cols + 7) / 8, q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (q >= across * a.y.rows) return;
+    const int64_t j = q / across, i = q % across * 8, all = a.y.rows * a.y.cols;
+    const int n = (int)min(a.y.cols - i, (int64_t)8);
+    float v[8], u[8];
+    load8(partial + j * a.y.cols + i, n, v);
+#pragma unroll 4
+    for (int k = 1; k < splits; ++k) {
+        load8(partial + k * all + j * a.y.cols + i, n, u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += u[e];
+    }
+    if (a.bias) {
+        load8(a.bias + i, n, u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += u[e];
+    }
+    if (a.preact.p) store8((T*)a.preact.p + j * a.preact.stride + i, n, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = activate<ACT>(v[e]);
+    if (a.residual.p) {
+        load8((const T*)a.residual.p + j * a.residual.stride + i, n, u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += u[e];
+    }
+    store8((T*)a.y.p + j * a.y.stride + i, n, v);
+}
+
+// grad_x = dz w; with `partial`, the float sums over the out of split blockIdx.y.
 template <class T, class S>
-__global__ void __launch_bounds__(S::kThreads) grad_x_kernel(Mat dz, Mat w, Mat gx, uint32_t ni, uint32_t nj) {
+__global__ void __launch_bounds__(S::kThreads) grad_x_kernel(Mat dz, Mat w, Mat gx, float* partial, int64_t depth,
+                                                             uint32_t ni, uint32_t nj) {
     using P = typename S::template Product<T, true, false>;
     __shared__ __align__(1024) unsigned char lds[P::kLds];
     uint32_t ti, tj;
     tile_of(xcd_contiguous_index(blockIdx.x, ni * nj), ni, nj, ti, tj);
     const int64_t i0 = (int64_t)ti * S::kI, j0 = (int64_t)tj * S::kJ;
+    const int64_t k0 = (int64_t)blockIdx.y * depth, k1 = min(k0 + depth, w.rows);
     f32x4 acc[S::kSquaresI][S::kSquaresJ];
-    P::run(lds, {w.p, w.rows, w.cols, w.stride}, {dz.p, dz.rows, dz.cols, dz.stride}, i0, j0, 0, w.rows, acc);
+    P::run(lds, {w.p, w.rows, w.cols, w.stride}, {dz.p, dz.rows, dz.cols, dz.stride}, i0, j0, k0, k1, acc);
+    if (partial) {
+        store_sums<S>(acc, i0, j0, partial, blockIdx.y, gx.rows, gx.cols);
+        return;
+    }
     for_outputs<S>(acc, i0, j0, gx.cols, gx.rows, [&](int64_t i, int64_t j, int n, float (&v)[8]) {
         store8((T*)gx.p + j * gx.stride + i, n, v);
     });
@@ -276,8 +356,6 @@ __global__ void __launch_bounds__(256) slope_kernel(Mat gy, Mat z, Mat dz, float
     }
 }
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // ---- the backward's plan: what it keeps in the workspace
 struct BackwardPlan {
     bool narrow = false;         // one pass over the rows (linear_narrow.hip)
@@ -285,7 +363,8 @@ struct BackwardPlan {
     int64_t dz_stride = 0;
     int across = 1;              // threads on a row of the slope pass
     int64_t slope_x = 0, slope_y = 0;   // its grid; 0: no pass
-    int64_t splits = 1, split_rows = 0;
+    int64_t splits = 1, split_rows = 0;   // of grad_w's rows
+    KSplits gx;                  // of grad_x's out
     size_t dz_bytes = 0, sums_bytes = 0, partial_bytes = 0;
 };
 
@@ -301,6 +380,10 @@ BackwardPlan plan_backward(const LinearBackward& a) {
         return p;
     }
     p.dz = a.activation != kActNone && (a.grad_x.p || a.grad_w.p) && rows > 0;
+    if (a.grad_x.p && rows > 0) {
+        p.gx = split_k(in, rows, out, a.dtype == TGS_DTYPE_FLOAT32 ? 4 : 2);
+        if (p.gx.splits > 1) p.partial_bytes = sizeof(float) * (size_t)(p.gx.splits * rows * in);
+    }
     if (p.dz || a.grad_bias) {
         while (p.across < 256 && p.across * 8 < out) p.across *= 2;
         p.slope_y = ceil_div(out, (int64_t)p.across * 8);
@@ -326,7 +409,8 @@ BackwardPlan plan_backward(const LinearBackward& a) {
         if (p.split_rows < 64) p.split_rows = 64;
         p.splits = ceil_div(rows, p.split_rows);
         if (p.splits < 1) p.splits = 1;
-        if (p.splits > 1) p.partial_bytes = sizeof(float) * (size_t)(p.splits * in * out);
+        // the two products' sums take turns in one place
+        if (p.splits > 1) p.partial_bytes = std::max(p.partial_bytes, sizeof(float) * (size_t)(p.splits * in * out));
     }
     const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
     p.dz_bytes = round(p.dz_bytes);
@@ -367,8 +451,12 @@ void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) 
         by_shape(in, rows, 1, [&](auto shape) {
             using S = decltype(shape);
             const uint32_t ni = (uint32_t)ceil_div(in, S::kI), nj = (uint32_t)ceil_div(rows, S::kJ);
-            grad_x_kernel<T, S><<<ni * nj, S::kThreads, 0, s>>>(dz, a.w, a.grad_x, ni, nj);
+            grad_x_kernel<T, S><<<dim3(ni * nj, (unsigned)p.gx.splits), S::kThreads, 0, s>>>(
+                dz, a.w, a.grad_x, p.gx.splits > 1 ? partial : nullptr, p.gx.depth, ni, nj);
         });
+    if (a.grad_x.p && rows && p.gx.splits > 1)
+        join_kernel<T><<<(unsigned)ceil_div(rows * in, 256), 1024, 0, s>>>(partial, (int)p.gx.splits, rows * in, a.grad_x,
+                                                                           nullptr, 0);
     if (a.grad_w.p) {
         const int64_t most = ceil_div(rows, kSplitRows) > 1 ? ceil_div(rows, kSplitRows) : 1;
         by_shape(in, out, most, [&](auto shape) {
@@ -391,25 +479,34 @@ size_t linear_backward_workspace(const LinearBackward& a) {
     return p.dz_bytes + p.sums_bytes + p.partial_bytes;
 }
 
-int launch_linear_forward(const LinearForward& a, hipStream_t s) {
+size_t linear_forward_workspace(const LinearForward& a) {
+    if (linear_forward_is_few(a) || linear_forward_by_rows(a)) return 0;
+    const KSplits k = split_k(a.y.cols, a.y.rows, a.x.cols, a.dtype == TGS_DTYPE_FLOAT32 ? 4 : 2);
+    return k.splits > 1 ? sizeof(float) * (size_t)(k.splits * a.y.rows * a.y.cols) : 0;
+}
+
+int launch_linear_forward(const LinearForward& a, void* workspace, hipStream_t s) {
     if (linear_forward_is_few(a)) {
         launch_linear_few(a, s);
-        TGS_CHECK_LAUNCH();
-        return TGS_OK;
-    }
-    if (linear_forward_by_rows(a)) {
+    } else if (linear_forward_by_rows(a)) {
         launch_linear_rows(a, s);
-        TGS_CHECK_LAUNCH();
-        return TGS_OK;
-    }
-    by_dtype(a.dtype, [&](auto t) {
-        using T = decltype(t);
-        by_shape(a.y.cols, a.y.rows, 1, [&](auto shape) {
-            using S = decltype(shape);
-            const uint32_t ni = (uint32_t)ceil_div(a.y.cols, S::kI), nj = (uint32_t)ceil_div(a.y.rows, S::kJ);
-            forward_kernel<T, S><<<ni * nj, S::kThreads, 0, s>>>(a, ni, nj);
+    } else {
+        by_dtype(a.dtype, [&](auto t) {
+            using T = decltype(t);
+            const KSplits k = split_k(a.y.cols, a.y.rows, a.x.cols, (int)sizeof(T));
+            float* partial = k.splits > 1 ? (float*)workspace : nullptr;
+            by_shape(a.y.cols, a.y.rows, 1, [&](auto shape) {
+                using S = decltype(shape);
+                const uint32_t ni = (uint32_t)ceil_div(a.y.cols, S::kI), nj = (uint32_t)ceil_div(a.y.rows, S::kJ);
+                forward_kernel<T, S><<<dim3(ni * nj, (unsigned)k.splits), S::kThreads, 0, s>>>(a, partial, k.depth, ni, nj);
+            });
+            if (partial)
+                by_activation(a.activation, [&](auto act) {
+                    join_forward_kernel<T, decltype(act)::value>
+                        <<<(unsigned)ceil_div(ceil_div(a.y.cols, 8) * a.y.rows, 256), 256, 0, s>>>(a, partial, (int)k.splits);
+                });
         });
-    });
+    }
     TGS_CHECK_LAUNCH();
     return TGS_OK;
 }

@@ -105,7 +105,8 @@ struct LinearBackward {
     int dtype;
 };
 size_t linear_backward_workspace(const LinearBackward& a);
-int launch_linear_forward(const LinearForward& a, hipStream_t s);
+size_t linear_forward_workspace(const LinearForward& a);
+int launch_linear_forward(const LinearForward& a, void* workspace, hipStream_t s);
 int launch_linear_backward(const LinearBackward& a, void* workspace, hipStream_t s);
 
 // ---- linear_few.hip: a few rows

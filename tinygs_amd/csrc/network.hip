@@ -194,8 +194,10 @@ int tgs_linear_forward(tgs_network* n, const tgs_matrix* x, const tgs_matrix* w,
     }
     TGS_TRY(check_apart(preact, "preact", y, "y"));
     if (x->rows == 0) return TGS_OK;
-    return launch_linear_forward({view(x), view(w), view(residual), view(preact), view(y), bias, activation, x->dtype},
-                                 (hipStream_t)stream);
+    const LinearForward a{view(x), view(w), view(residual), view(preact), view(y), bias, activation, x->dtype};
+    const size_t bytes = linear_forward_workspace(a);
+    if (bytes) TGS_TRY(ensure(n->workspace, bytes, (hipStream_t)stream));
+    return launch_linear_forward(a, n->workspace.p, (hipStream_t)stream);
 }
 
 int tgs_linear_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_matrix* x, const tgs_matrix* w,
