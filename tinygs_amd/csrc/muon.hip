@@ -30,8 +30,10 @@ constexpr int kPatch = 64;   // edge of the element passes' patches
 // Halves between a row's end and the next row: rows of a power of two would all
 // start on the same few channels of the cache.
 constexpr int kRowPad = 64;
-constexpr int kPatchThreads = 1024;
+// A patch's threads: sixteen on a row, four columns each, over four rows apart by kPatchDown.
+constexpr int kPatchThreads = 256;
 constexpr int kPatchWaves = kPatchThreads / 64;
+constexpr int kPatchDown = kPatchThreads / 16, kPatchTurns = kPatch / kPatchDown;
 
 // The matrix that number `n` of a launch's work belongs to: the last whose
 // first number is not above it. `firsts` are the matrices' first numbers; a
@@ -64,27 +66,80 @@ __device__ __forceinline__ float update_of(float g, float m, const MuonStep& p) 
     return p.nesterov ? fmaf(p.momentum, m, g) : m;
 }
 
+template <class T>
+struct Loose4 {   // four elements of a row, at any element's address
+    typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
+template <class T>
+__device__ __forceinline__ f32x4 load4(const T* p, int n) {
+    if (n >= 4) return __builtin_convertvector(*(const typename Loose4<T>::type*)p, f32x4);
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) v[e] = (float)p[e];
+    return v;
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, int n, f32x4 v) {
+    if (n >= 4) {
+        *(typename Loose4<T>::type*)p = __builtin_convertvector(v, typename Loose4<T>::type);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) p[e] = (T)v[e];
+}
+
+// Where a thread's fours of a patch are: rows r, r + kPatchDown, ..., columns
+// c .. c + 3, of which n exist in a matrix of `cols`.
+struct PatchPlace {
+    int q, l;
+    int64_t r0, c0, r, c;
+    int n;
+    __device__ PatchPlace(uint32_t number, int64_t cols)
+        : q(threadIdx.x >> 4), l(threadIdx.x & 15) {
+        const uint32_t across = (uint32_t)((cols + kPatch - 1) / kPatch);
+        r0 = (int64_t)(number / across) * kPatch;
+        c0 = (int64_t)(number % across) * kPatch;
+        r = r0 + q;
+        c = c0 + 4 * l;
+        n = (int)min(max(cols - c, (int64_t)0), (int64_t)4);
+    }
+};
+
+// The thread's gradients and momenta, all on their way at once.
+template <class G>
+__device__ __forceinline__ void load_patch(const MuonPart& a, const PatchPlace& at, f32x4 (&g)[kPatchTurns],
+                                           f32x4 (&m)[kPatchTurns]) {
+#pragma unroll
+    for (int k = 0; k < kPatchTurns; ++k) {
+        const int64_t r = at.r + k * kPatchDown;
+        const int n = r < a.w.rows ? at.n : 0;
+        g[k] = load4((const G*)a.g.p + r * a.g.stride + at.c, n);
+        m[k] = load4((const float*)a.m.p + r * a.m.stride + at.c, n);
+    }
+}
+
 // M <- mu M + (1 - mu) s G, and the patch's sum of squares of U.
 template <class G>
 __global__ void __launch_bounds__(kPatchThreads) momentum_kernel(const MuonPart* parts, const uint32_t* firsts, int count,
                                                                  MuonStep p, double* sums) {
     const MuonPart& a = parts[part_of(firsts, count, blockIdx.x)];
-    const uint32_t n = blockIdx.x - a.first[kMuonPatches];
-    const int64_t across = (a.w.cols + kPatch - 1) / kPatch;
-    const int64_t r0 = n / across * kPatch, c = n % across * kPatch + (threadIdx.x & 63);
-    const int wave = threadIdx.x >> 6;
+    const PatchPlace at(blockIdx.x - a.first[kMuonPatches], a.w.cols);
+    f32x4 g[kPatchTurns], m[kPatchTurns];
+    load_patch<G>(a, at, g, m);
     double sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < kPatch / kPatchWaves; ++k) {
-        const int64_t r = r0 + wave + k * kPatchWaves;
-        if (r < a.w.rows && c < a.w.cols) {
-            const float g = (float)((const G*)a.g.p)[r * a.g.stride + c] * p.grad_scale;
-            float* at = (float*)a.m.p + r * a.m.stride + c;
-            const float m = fmaf(p.momentum, *at, g);
-            *at = m;
-            const double u = (double)update_of(g, m, p);
-            sum += u * u;
+    for (int k = 0; k < kPatchTurns; ++k) {
+        const int64_t r = at.r + k * kPatchDown;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {   // those that do not exist are zeros
+            const float s = g[k][e] * p.grad_scale;
+            m[k][e] = fmaf(p.momentum, m[k][e], s);
+            const double u = (double)update_of(s, m[k][e], p);
+            if (r < a.w.rows && e < at.n) sum += u * u;
         }
+        store4((float*)a.m.p + r * a.m.stride + at.c, r < a.w.rows ? at.n : 0, m[k]);
     }
     sum = workgroup_sum(sum);
     if (threadIdx.x == 0) sums[blockIdx.x] = sum;
@@ -95,42 +150,62 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
     lo = (_Float16)(v - (float)hi);
 }
 
+// Four columns from c, a multiple of four, of a row of split values.
+__device__ __forceinline__ void store_split(_Float16* row, int64_t c, f32x4 v) {
+    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+    const half4 hi = __builtin_convertvector(v, half4);
+    *(half4*)(row + column(c)) = hi;
+    *(half4*)(row + column(c) + 32) = __builtin_convertvector(v - __builtin_convertvector(hi, f32x4), half4);
+}
+__device__ __forceinline__ f32x4 load_split(const _Float16* row, int64_t c) {
+    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+    return __builtin_convertvector(*(const half4*)(row + column(c)), f32x4) +
+           __builtin_convertvector(*(const half4*)(row + column(c) + 32), f32x4);
+}
+
 // X = U / max(|U|, epsilon), scaled and split; a tall matrix through LDS into
 // its transpose. Columns up to a multiple of 32 are zeros.
 template <class G>
 __global__ void __launch_bounds__(kPatchThreads) normalise_kernel(const MuonPart* parts, const uint32_t* firsts, int count,
                                                                   MuonStep p, const double* sums) {
     const MuonPart& a = parts[part_of(firsts, count, blockIdx.x)];
-    const uint32_t n = blockIdx.x - a.first[kMuonPatches];
-    const int64_t across = (a.w.cols + kPatch - 1) / kPatch, down = (a.w.rows + kPatch - 1) / kPatch;
+    const PatchPlace at(blockIdx.x - a.first[kMuonPatches], a.w.cols);
+    f32x4 g[kPatchTurns], m[kPatchTurns];
+    load_patch<G>(a, at, g, m);
+    const int64_t patches = (a.w.cols + kPatch - 1) / kPatch * ((a.w.rows + kPatch - 1) / kPatch);
     double sum = 0.0;
-    for (int64_t k = threadIdx.x; k < across * down; k += kPatchThreads) sum += sums[a.first[kMuonPatches] + k];
+#pragma unroll 4
+    for (int64_t k = threadIdx.x; k < patches; k += kPatchThreads) sum += sums[a.first[kMuonPatches] + k];
     const double norm = sqrt(workgroup_sum(sum));
     const double inv = (double)kScale / (norm < (double)p.epsilon ? (double)p.epsilon : norm);   // NaN stays
-    const int64_t r0 = n / across * kPatch, c0 = n % across * kPatch;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     _Float16* const x = a.x[0];
     __shared__ float t[kPatch][kPatch + 1];
 #pragma unroll
-    for (int k = 0; k < kPatch / kPatchWaves; ++k) {
-        const int q = wave + k * kPatchWaves;
-        const int64_t r = r0 + q, c = c0 + lane;
-        float v = 0.0f;
-        if (r < a.w.rows && c < a.w.cols) {
-            const float g = (float)((const G*)a.g.p)[r * a.g.stride + c] * p.grad_scale;
-            v = (float)((double)update_of(g, ((const float*)a.m.p)[r * a.m.stride + c], p) * inv);
+    for (int k = 0; k < kPatchTurns; ++k) {
+        const int q = at.q + k * kPatchDown;
+        const int64_t r = at.r0 + q;
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v[e] = r < a.w.rows && e < at.n
+                       ? (float)((double)update_of(g[k][e] * p.grad_scale, m[k][e], p) * inv) : 0.0f;
+        if (a.tall) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[q][4 * at.l + e] = v[e];
+        } else if (r < a.side && 2 * at.c < a.x_cols) {
+            store_split(x + r * a.x_stride, at.c, v);
         }
-        if (a.tall) t[q][lane] = v;
-        else if (r < a.side && 2 * c < a.x_cols) split(v, x[r * a.x_stride + column(c)], x[r * a.x_stride + column(c) + 32]);
     }
     if (!a.tall) return;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kPatch / kPatchWaves; ++k) {
-        const int q = wave + k * kPatchWaves;
-        const int64_t r = c0 + q, c = r0 + lane;   // of X
-        if (r < a.side && 2 * c < a.x_cols)
-            split(t[lane][q], x[r * a.x_stride + column(c)], x[r * a.x_stride + column(c) + 32]);
+    for (int k = 0; k < kPatchTurns; ++k) {
+        const int q = at.q + k * kPatchDown;
+        const int64_t r = at.c0 + q, c = at.r0 + 4 * at.l;   // of X
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = t[4 * at.l + e][q];
+        if (r < a.side && 2 * c < a.x_cols) store_split(x + r * a.x_stride, c, v);
     }
 }
 
@@ -139,35 +214,42 @@ template <class C>
 __global__ void __launch_bounds__(kPatchThreads) apply_kernel(const MuonPart* parts, const uint32_t* firsts, int count,
                                                               MuonStep p) {
     const MuonPart& a = parts[part_of(firsts, count, blockIdx.x)];
-    const uint32_t n = blockIdx.x - a.first[kMuonPatches];
-    const int64_t across = (a.w.cols + kPatch - 1) / kPatch;
-    const int64_t r0 = n / across * kPatch, c0 = n % across * kPatch;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const PatchPlace at(blockIdx.x - a.first[kMuonPatches], a.w.cols);
     const _Float16* const x = a.x[p.iterations & 1];
     const float step = p.lr * a.shape * (1.0f / kScale);
     __shared__ float t[kPatch][kPatch + 1];
-    if (a.tall) {
+    f32x4 w[kPatchTurns], v[kPatchTurns];
 #pragma unroll
-        for (int k = 0; k < kPatch / kPatchWaves; ++k) {
-            const int q = wave + k * kPatchWaves;
-            const int64_t r = c0 + q, c = r0 + lane;
-            if (r < a.side && c < a.length)
-                t[lane][q] = (float)x[r * a.x_stride + column(c)] + (float)x[r * a.x_stride + column(c) + 32];
-        }
-        __syncthreads();
+    for (int k = 0; k < kPatchTurns; ++k) {
+        const int64_t r = at.r + k * kPatchDown;
+        w[k] = load4((const float*)a.w.p + r * a.w.stride + at.c, r < a.w.rows ? at.n : 0);
     }
 #pragma unroll
-    for (int k = 0; k < kPatch / kPatchWaves; ++k) {
-        const int q = wave + k * kPatchWaves;
-        const int64_t r = r0 + q, c = c0 + lane;
-        if (r < a.w.rows && c < a.w.cols) {
-            const float v = a.tall ? t[q][lane]
-                                   : (float)x[r * a.x_stride + column(c)] + (float)x[r * a.x_stride + column(c) + 32];
-            float* w = (float*)a.w.p + r * a.w.stride + c;
-            const float u = fmaf(-step, v, p.keep * *w);
-            *w = u;
-            if (a.c.p) ((C*)a.c.p)[r * a.c.stride + c] = (C)u;
-        }
+    for (int k = 0; k < kPatchTurns; ++k) {   // X's rows are the patch's columns if it is tall
+        const int64_t r = (a.tall ? at.c0 : at.r0) + at.q + k * kPatchDown, c = (a.tall ? at.r0 : at.c0) + 4 * at.l;
+        v[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (r < a.side && 2 * c < a.x_cols) v[k] = load_split(x + r * a.x_stride, c);
+    }
+    if (a.tall) {
+#pragma unroll
+        for (int k = 0; k < kPatchTurns; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[4 * at.l + e][at.q + k * kPatchDown] = v[k][e];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kPatchTurns; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k][e] = t[at.q + k * kPatchDown][4 * at.l + e];
+    }
+#pragma unroll
+    for (int k = 0; k < kPatchTurns; ++k) {
+        const int64_t r = at.r + k * kPatchDown;
+        const int n = r < a.w.rows ? at.n : 0;
+        f32x4 u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = fmaf(-step, v[k][e], p.keep * w[k][e]);
+        store4((float*)a.w.p + r * a.w.stride + at.c, n, u);
+        if (a.c.p) store4((C*)a.c.p + r * a.c.stride + at.c, n, u);
     }
 }
 
