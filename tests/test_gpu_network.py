@@ -14,7 +14,8 @@ SHAPES = [(1, 1, 1), (1, 256, 256), (1, 1000, 3), (2, 7, 5), (5, 64, 1), (8, 512
           (33, 256, 64), (64, 64, 64), (127, 128, 128), (129, 130, 257), (300, 1, 9), (1000, 323, 96),
           (1025, 256, 256), (640, 512, 384), (3, 1024, 2048), (4099, 84, 59), (70001, 72, 40), (20000, 256, 128),
           (33000, 72, 72), (33000, 520, 72), (70000, 264, 260), (4097, 256, 700), (66000, 24, 260), (70001, 260, 24), (150001, 130, 129),
-          (33, 4096, 130), (200, 1300, 77), (70, 600, 2100)]
+          (33, 4096, 130), (200, 1300, 77), (70, 600, 2100),
+          (39, 121, 59), (40, 1, 3), (41, 3, 1), (64, 5, 250), (72, 250, 7), (8193, 59, 123), (70001, 129, 250)]
 
 
 @pytest.fixture(scope="module")
@@ -68,6 +69,37 @@ def test_linear(ops, shape, dtype):
         if r is not None:   # in the residual's place
             buf = r.contiguous().clone()
             assert torch.equal(ops.linear(x, w, b, activation=name, residual=buf, out=buf), y)
+
+
+# enough rows that a call moves more than the caches hold; the first, the last and some of the others are compared
+MANY = [(300001, 130, 200), (260001, 84, 520), (1200001, 59, 61), (700003, 256, 64), (400000, 24, 256), (140000, 128, 700)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", MANY, ids=str)
+def test_linear_many_rows(ops, shape, dtype):
+    rows, i, o = shape
+    g = torch.Generator("cuda").manual_seed(5)
+    at = torch.cat([torch.arange(200), torch.randint(rows, (2000,), generator=torch.Generator().manual_seed(6)),
+                    torch.arange(rows - 200, rows)]).cuda()
+    for k, (name, pad) in enumerate([("none", 0), ("silu", 3), ("gelu", 0)]):
+        print(f"[linear] {shape} {dtype} {name} pad {pad}", flush=True)
+        x = torch.full((rows, i + pad), float("nan"), dtype=dtype, device="cuda")[:, :i]
+        x.copy_(torch.randn(rows, i, generator=g, device="cuda"))
+        w = matrix(11 + k, o, i, dtype, pad, 0, i ** -0.5)
+        b = normal(21 + k, o).cuda()
+        r = torch.randn(rows, o, generator=g, device="cuda").to(dtype) if k else None
+        y, yfull = output(rows, o, dtype, pad)
+        z, zfull = output(rows, o, dtype, pad)
+        ops.linear(x, w, b, activation=name, residual=r, out=y, preact=z)
+        wy, by, wz, bz = R.linear(x[at], w, b, name, None if r is None else r[at], dtype)
+        R.check(y[at], wy, by, "y")
+        R.check(z[at], wz, bz, "z")
+        assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(z).all())
+        untouched(yfull, 0, o)
+        untouched(zfull, 0, o)
+        again = ops.linear(x, w, b, activation=name, residual=r)
+        R.check(again[at], wy, by, "y without the values before the activation")
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)

@@ -27,6 +27,9 @@ struct Plane<float> {
 };
 
 constexpr int kRows = 32;   // of a block
+// Rows after a block's, of two bytes or more each, that hold the 14 bytes which
+// a partial chunk may reach past the block's last row.
+constexpr int kBeyond = 8;
 constexpr int kThreads = 512;
 
 // Matrices in LDS: halves as they are, in rows of 512 bytes; floats as the
@@ -79,9 +82,11 @@ struct Narrow {
 };
 
 // partial + blockIdx.x * (out * in + out): the workgroup's dw and db.
-// RAGGED: in or out is no multiple of a chunk, so that chunks can be partial:
-// rows are gathered element by element. Else buffer loads give zeros where
-// nothing is, and stores there are dropped.
+// Buffer loads give zeros where nothing is, and stores there are dropped.
+// RAGGED: in or out is no multiple of a chunk. A partial chunk is then loaded
+// whole, with what follows in memory, and masked when it is used; the blocks
+// that end the matrix, where nothing need follow, are gathered element by
+// element.
 template <class T, int ACT, bool RAGGED>
 __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, float* partial, int blocks) {
     using N = Narrow<T>;
@@ -97,32 +102,43 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
     const int n_in = min(max(in - chunk * V, 0), V), n_out = min(max(out - chunk * V, 0), V);
 
     // A matrix's 32 rows (from `first` on) as this thread's two chunks.
-    const auto fetch = [&](const Mat& m, int64_t first, int n, typename N::chunk(&to)[2]) {
+    const auto load = [&](const Mat& m, int64_t first, int n, typename N::chunk(&to)[2]) {
         const T* base = (const T*)m.p + first * m.stride;
-        if constexpr (RAGGED) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = r + 16 * h;
-                const bool exists = first + row < m.rows && n > 0;
-                to[h] = N::C::gather(exists ? base + row * m.stride + chunk * V : (const T*)m.p, exists ? n : 0);
-            }
-            return;
-        }
         const int64_t pitch = m.stride * (int64_t)sizeof(T);
-        const auto buffer = resource_of(base, (min(m.rows - first, (int64_t)kRows) - 1) * pitch + m.cols * (int64_t)sizeof(T));
+        // rows beyond the block's lie between it and the buffer's end when a chunk may reach past a row
+        const int64_t held = min(m.rows - first, (int64_t)(RAGGED ? kRows + kBeyond : kRows));
+        const auto buffer = resource_of(base, RAGGED && held < kRows + kBeyond
+                                                  ? 0 : (held - 1) * pitch + m.cols * (int64_t)sizeof(T));
         const uint32_t from = (n > 0 ? 0u : kNowhere) + (uint32_t)chunk * 16u;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             to[h] = __builtin_bit_cast(typename N::chunk, __builtin_amdgcn_raw_buffer_load_b128(
                                                               buffer, (int)(from + (uint32_t)(r + 16 * h) * (uint32_t)pitch), 0, 0));
     };
+    // Ahead of their use, RAGGED: chunks that load left out or loaded more than is there.
+    const auto mend = [&](const Mat& m, int64_t first, int n, typename N::chunk(&v)[2]) {
+        if constexpr (!RAGGED) return;
+        if (m.rows - first < kRows + kBeyond) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = r + 16 * h;
+                const bool exists = first + row < m.rows && n > 0;
+                v[h] = N::C::gather(exists ? (const T*)m.p + (first + row) * m.stride + chunk * V : (const T*)m.p,
+                                    exists ? n : 0);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[h][e] = e < n ? v[h][e] : (T)0.0f;
+    };
 
     typename N::chunk dy[2], z[2], x[2];
     const auto fetch_block = [&](int block) {
         const int64_t first = (int64_t)block * kRows;
-        fetch(a.grad_y, first, n_out, dy);
-        if constexpr (ACT != kActNone) fetch(a.preact, first, n_out, z);
-        if (a.grad_w.p) fetch(a.x, first, n_in, x);
+        load(a.grad_y, first, n_out, dy);
+        if constexpr (ACT != kActNone) load(a.preact, first, n_out, z);
+        if (a.grad_w.p) load(a.x, first, n_in, x);
     };
 
     fetch_block(blockIdx.x);
@@ -132,12 +148,14 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
         const auto place = [&](int n0) {
             typename N::chunk v[kQuarters][2];
 #pragma unroll
-            for (int q = 0; q < kQuarters; ++q) fetch(a.w, n0 + kRows * q, n_in, v[q]);
+            for (int q = 0; q < kQuarters; ++q) load(a.w, n0 + kRows * q, n_in, v[q]);
 #pragma unroll
-            for (int q = 0; q < kQuarters; ++q)
+            for (int q = 0; q < kQuarters; ++q) {
+                mend(a.w, n0 + kRows * q, n_in, v[q]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                     N::place(w, N::kWeightPlane, n0 + kRows * q + r + 16 * h, chunk, v[q][h]);
+            }
         };
         place(0);
         if (deep) place(N::kCols / 2);
@@ -155,6 +173,12 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
 
     for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
         lds_barrier();   // the last block's reads are done
+        if constexpr (RAGGED) {
+            const int64_t first = (int64_t)block * kRows;
+            mend(a.grad_y, first, n_out, dy);
+            if constexpr (ACT != kActNone) mend(a.preact, first, n_out, z);   // no NaN against a zero of dy
+            if (a.grad_w.p) mend(a.x, first, n_in, x);
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if constexpr (ACT != kActNone) {
@@ -225,6 +249,9 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
                     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), buffer,
                                                            (int)((i < in ? 0u : kNowhere) + (uint32_t)row * (uint32_t)pitch + (uint32_t)i * (uint32_t)sizeof(T)),
                                                            0, 0);
+                } else if (first + row < rows && i + V <= in) {
+                    typedef T loose __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+                    *(loose*)(base + row * a.grad_x.stride + i) = __builtin_bit_cast(loose, y);
                 } else if (first + row < rows) {
 #pragma unroll
                     for (int e = 0; e < V; ++e)
@@ -287,8 +314,16 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
 
 }  // namespace
 
+// Against a slope pass and two tile products, with SiLU: 1e6 x 256 -> 256 halves
+// 504 and 778 us, 1e6 x 128 -> 64 284 and 262 (the worst of the halves), 2000 x
+// 72 -> 72 20 and 28; 1e6 x 128 -> 64 floats 401 and 539, 2000 rows 19 and 43.
+// Ragged halves of more than 128 columns take their last rows of w element by
+// element, which fewer rows do not pay back: 250 -> 256, 2000 rows 50 and 28 us,
+// 20000 62 and 41, 200000 178 and 216.
 bool linear_backward_is_narrow(const LinearBackward& a) {
     const int64_t most = 512 / (a.dtype == TGS_DTYPE_FLOAT32 ? 4 : 2);
+    const bool ragged = a.x.cols % 8 || a.grad_y.cols % 8;
+    if (a.dtype != TGS_DTYPE_FLOAT32 && ragged && a.x.cols > 128 && a.grad_y.cols > 128 && a.grad_y.rows < 65536) return false;
     return a.x.cols <= most && a.grad_y.cols <= most && a.grad_y.rows > 0 && a.grad_y.rows < ((int64_t)1 << 35);
 }
 
