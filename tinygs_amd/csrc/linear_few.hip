@@ -106,7 +106,11 @@ __global__ void __launch_bounds__(64 * kWaves) few_kernel(LinearForward a) {
 
 }  // namespace
 
-bool linear_forward_is_few(const LinearForward& a) { return a.y.rows <= 32; }
+// Against tiles with k split, SiLU, whole calls: 1 x 4096 -> 4096 halves 7.9 and
+// 13.3 us, floats 20.0 and 33.2; 16 rows 10.8 and 14.4, 22.9 and 33.3. More rows
+// read w a second time: 32 x 4096 -> 4096 17.9 and 15.1, floats 37.8 and 33.6,
+// but 32 x 1024 -> 1024, all on its way at once, 6.8 and 8.6, floats 7.4 and 10.9.
+bool linear_forward_is_few(const LinearForward& a) { return a.y.rows <= (a.x.cols <= 1024 ? 32 : 16); }
 
 void launch_linear_few(const LinearForward& a, hipStream_t s) {
     const dim3 grid((unsigned)((a.y.cols + 15) / 16), (unsigned)((a.y.rows + 15) / 16));

@@ -7,8 +7,8 @@
 // walks over blocks of 64 rows, so that w is read once a workgroup and not once
 // a tile. x and the residual come to LDS without passing registers, one to three
 // blocks ahead; the wait for a block leaves the loads and stores that were
-// started after it in flight. 1e6 x 256 -> 256 halves with gelu,
-// residual and preact: 2.05 GB.
+// started after it in flight. 1e6 x 256 -> 256 halves with gelu, residual and
+// preact: 2.05 GB in 384 us, 5.3 TB/s.
 #include "narrow_rows.h"
 
 namespace tgs {
@@ -255,9 +255,25 @@ __global__ void __launch_bounds__(kThreads, 2 * resident((int)sizeof(T), PITCH, 
 
 }  // namespace
 
+// Once a call moves more than the card's last cache holds of it, w in registers
+// and few, long waits pay; below, tiles fill the card sooner and their second
+// reads of x are from caches. Here and with tiles, halves: 262144 x 128 -> 256
+// 42 and 52 us, with gelu, preact and residual 97 and 134; 1e6 x 256 -> 256 so
+// 384 and 507; 262144 x 256 -> 128 (201 MB) 44 and 44; 65536 x 128 -> 128 (34 MB)
+// 13 and 9. Half of a workgroup's waves have no columns below 128, so those
+// take more: 262144 x 256 -> 64 (168 MB) 40 and 31, 1e6 x 84 -> 64 (296 MB) 77 and
+// 108. Floats multiply six times as long, w's planes fill the registers, and
+// the products bound narrow outputs: 1e6 x 128 -> 64 197 and 160, 262144 x 84
+// -> 256 (356 MB) 111 and 125, 262144 x 128 -> 256 (402 MB) 142 and 138, with gelu,
+// preact and residual 202 and 232.
 bool linear_forward_by_rows(const LinearForward& a) {
-    const int64_t most = 512 / (a.dtype == TGS_DTYPE_FLOAT32 ? 4 : 2);
-    return a.x.cols <= most && a.y.cols <= 4 * most && a.y.rows >= 4096;
+    const bool floats = a.dtype == TGS_DTYPE_FLOAT32;
+    const int64_t size = floats ? 4 : 2, most = 512 / size;
+    if (a.x.cols > most || a.y.cols > 4 * most) return false;
+    const int64_t arrays = 1 + (a.preact.p ? 1 : 0) + (a.residual.p ? 1 : 0);
+    const int64_t megabytes = (a.y.rows * (a.x.cols + arrays * a.y.cols) * size) >> 20;
+    if (a.y.cols < 128) return !floats && megabytes >= 256;
+    return megabytes >= (floats ? 384 : 130);
 }
 
 void launch_linear_rows(const LinearForward& a, hipStream_t s) {
@@ -278,9 +294,10 @@ void launch_linear_rows(const LinearForward& a, hipStream_t s) {
             else launch(pitch, cw, Constant<0>{});
         };
         const auto by_columns = [&](auto pitch) {
-            if (a.y.cols <= 64) by_residual(pitch, Constant<2>{});
-            else if (sizeof(T) == 4 || a.y.cols <= 128) by_residual(pitch, Constant<4>{});
-            else if constexpr (sizeof(T) == 2) by_residual(pitch, Constant<8>{});
+            if constexpr (sizeof(T) == 4) by_residual(pitch, Constant<4>{});
+            else if (a.y.cols <= 64) by_residual(pitch, Constant<2>{});
+            else if (a.y.cols <= 128) by_residual(pitch, Constant<4>{});
+            else by_residual(pitch, Constant<8>{});
         };
         if (a.x.cols <= kMost / 2) by_columns(Constant<256>{});
         else by_columns(Constant<512>{});
