@@ -4,7 +4,8 @@
 // Each operand is read in one of two forms: K-contiguous (element (r, k) at
 // p + r stride + k) or R-contiguous (p + k stride + r). A workgroup of
 // WI x WJ waves makes a tile of BI x BJ outputs, a wave TI x TJ squares of
-// 16 x 16, in steps of 128 bytes of k (64 halves, 32 floats), or 64.
+// 16 x 16, in steps of 128 bytes of k (64 halves, 32 floats); Muon's R-contiguous side
+// takes 64.
 //
 // Operand tiles go from memory to LDS without passing registers: lane l of a
 // wave's load writes the 16 bytes at its LDS base + 16 l, from any byte
@@ -147,9 +148,10 @@ struct TileSide {
 
     // The chunk that stands in place of chunk c of LDS row r, and back.
     // K-contiguous: lanes 0..15 read rows r .. r + 15 at one chunk, so chunks
-    // are turned by the row (by every fourth where four rows fill the banks). R-contiguous: a read takes 4 (halves: 8) rows at
-    // one run of 16 elements, so the runs are turned by what tells the rows
-    // (8 g + q, floats: 8 g + e at one e) apart; rows of 128 bytes already alternate between the banks' halves.
+    // are turned by the row (by every fourth where four rows fill the banks).
+    // R-contiguous: a read takes 4 (halves: 8) rows at one run of 16 elements,
+    // so the runs are turned by what tells the rows (8 g + q, floats: 8 g + e at
+    // one e) apart; rows of 128 bytes already alternate between the banks' halves.
     static __device__ __forceinline__ int turn(int r) {
         if constexpr (!RC) return STEP == 128 ? r & 7 : (r >> 2) & 3;
         if constexpr (sizeof(T) == 4) return ((r >> 3) & 3) << 2;
@@ -261,14 +263,12 @@ struct TileSide {
     }
 };
 
-// Waits until at most n (0 to 3) groups of L of the wave's loads are in
-// flight and its LDS accesses are done, then for the workgroup.
+// Waits until at most n (0 or 1) groups of L of the wave's loads are in flight
+// and its LDS accesses are done, then for the workgroup.
 template <int L>
 __device__ __forceinline__ void wait_for_stage(int n) {
-    static_assert(3 * L < 64, "what the counter holds");
-    if (n > 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(3 * L) : "memory");
-    else if (n == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * L) : "memory");
-    else if (n == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(L) : "memory");
+    static_assert(L < 64, "what the counter holds");
+    if (n > 0) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(L) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
@@ -298,7 +298,7 @@ struct Tile {
     static constexpr int kStage = A::kBytes + B::kBytes;
     static constexpr int kLds = STAGES * kStage;
     static constexpr int kLoads = A::kLoads + B::kLoads;   // at least these many a wave and stage (gathers add some)
-    static_assert(STAGES >= 2 && STAGES <= 5, "");
+    static_assert(STAGES == 2, "what wait_for_stage waits for");
 
     static __device__ __forceinline__ void run(unsigned char* lds, const TileOperand& a, const TileOperand& b, int64_t i0,
                                                int64_t j0, int64_t k0, int64_t k1, f32x4 (&acc)[TI][TJ]) {
@@ -324,7 +324,7 @@ struct Tile {
         };
         const unsigned char* from = lds;   // the stage of the next read
         if constexpr (sizeof(T) == 4) {
-            static_assert(STAGES == 2 && A::kSubs == 1, "");
+            static_assert(A::kSubs == 1, "");
             load();
             for (int t = 0; t < steps; ++t) {
                 wait_for_stage<kLoads>(0);
