@@ -14,10 +14,10 @@
 // A row holds 32 hi and then their 32 lo in turn, so that a step of 32 of k is
 // one cache line of it.
 //
-// 1024 x 4096 by four: Gram 98 us, square 33, update 131, which is 1.0 to 1.1
-// PFLOP/s of halves where large products reach 1.4, bound by the tiles' turns of
-// LDS reads and matrix instructions and, for Gram's 144 tiles on 256 compute
-// units, by their number. A small network's launches (256 x 256: 7 to 8 us) are
+// Four of 1024 x 4096: Gram 97 us, square 33, update 130, which is 0.61, 0.45 and
+// 0.80 PFLOP/s of halves where large products reach 1.4. Gram's and the square's
+// 144 tiles are on 256 compute units; otherwise the tiles' turns of loads, LDS
+// reads and matrix instructions bound them. A small network's launches (256 x 256: 7 to 8 us) are
 // bound by their chains of waits. The element passes move 12 bytes an element in
 // 39 to 51 us (17 M elements, 4 to 5.2 TB/s).
 //
