@@ -104,14 +104,19 @@ using Small = Shape<2, 2, 2, 2>;    // 64 x 64, 4 waves, 32 KB: few tiles
 // shape taken first: 16384 x 1024 -> 2048 halves 80 us (860 TFLOP/s) in Large, 99
 // in Middle, 134 in Small; 8192 x 1024 -> 1024 (128 large tiles) 27 in Middle, 35
 // in Large, 34 in Small; 2000 x 1024 -> 1024 11.2 in Small and in Middle; floats
-// 345, 393, 518; 96, 150, 132. 100000 x 600 -> 64 floats 63 us in Narrow, 74
-// otherwise; halves 28 both.
+// 345, 393, 518; 96, 150, 132. Of few columns, in Narrow and in Small: floats
+// 100000 x 600 -> 64 62 and 73 us, but 200000 x 84 -> 59 40 and 30; halves 1e6 x
+// 600 -> 64 315 and 341, 200000 x 600 -> 64 61 and 50, 65536 x 84 -> 59 12.3 and
+// 8.7. So Narrow is for `deep` products: of floats with k of 256 and more, where
+// its fewer reads of A are worth its longer tiles, and for the sums over rows.
+template <class T>
+bool is_deep(int64_t k) { return sizeof(T) == 4 && k >= 256; }
 template <class F>
-void by_shape(int64_t ni, int64_t nj, int64_t splits_most, F f) {
+void by_shape(int64_t ni, int64_t nj, int64_t splits_most, bool deep, F f) {
     const auto tiles = [&](int64_t bi, int64_t bj) { return ((ni + bi - 1) / bi) * ((nj + bj - 1) / bj) * splits_most; };
     if (ni > 128 && nj > 128 && tiles(256, 256) >= 256) f(Large{});
     else if (ni > 64 && nj > 64 && tiles(128, 128) >= 256) f(Middle{});
-    else if (ni <= 64 && nj > 64 && tiles(64, 256) >= 256) f(Narrow{});
+    else if (deep && ni <= 64 && nj > 64 && tiles(64, 256) >= 256) f(Narrow{});
     else f(Small{});
 }
 
@@ -425,7 +430,7 @@ BackwardPlan plan_backward(const LinearBackward& a) {
     }
     if (a.grad_w.p) {
         const int64_t most = ceil_div(rows, kSplitRows) > 1 ? ceil_div(rows, kSplitRows) : 1;
-        by_shape(in, out, most, [&](auto shape) {
+        by_shape(in, out, most, true, [&](auto shape) {
             using S = decltype(shape);
             const int64_t tiles = ceil_div(in, S::kI) * ceil_div(out, S::kJ);
             // as many workgroups as fit the card at once (LDS: one to five a compute unit)
@@ -475,7 +480,7 @@ void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) 
     if (a.grad_bias)
         launch_column_sums(sums, (int)p.slope_x, out, out, a.grad_bias, nullptr, s);
     if (a.grad_x.p && rows)
-        by_shape(in, rows, 1, [&](auto shape) {
+        by_shape(in, rows, 1, is_deep<T>(out), [&](auto shape) {
             using S = decltype(shape);
             const uint32_t ni = (uint32_t)ceil_div(in, S::kI), nj = (uint32_t)ceil_div(rows, S::kJ);
             grad_x_kernel<T, S><<<dim3(ni * nj, (unsigned)p.gx.splits), S::kThreads, 0, s>>>(
@@ -485,7 +490,7 @@ void backward(const LinearBackward& a, unsigned char* workspace, hipStream_t s) 
         join<T>(partial, p.gx.splits, a.grad_x, s);
     if (a.grad_w.p) {
         const int64_t most = ceil_div(rows, kSplitRows) > 1 ? ceil_div(rows, kSplitRows) : 1;
-        by_shape(in, out, most, [&](auto shape) {
+        by_shape(in, out, most, true, [&](auto shape) {
             using S = decltype(shape);
             const uint32_t ni = (uint32_t)ceil_div(in, S::kI), nj = (uint32_t)ceil_div(out, S::kJ);
             grad_w_kernel<T, S><<<dim3(ni * nj, (unsigned)p.splits), S::kThreads, 0, s>>>(
@@ -518,7 +523,7 @@ int launch_linear_forward(const LinearForward& a, void* workspace, hipStream_t s
             using T = decltype(t);
             const KSplits k = split_k(a.y.cols, a.y.rows, a.x.cols, (int)sizeof(T));
             float* partial = k.splits > 1 ? (float*)workspace : nullptr;
-            by_shape(a.y.cols, a.y.rows, 1, [&](auto shape) {
+            by_shape(a.y.cols, a.y.rows, 1, is_deep<T>(a.x.cols), [&](auto shape) {
                 using S = decltype(shape);
                 const uint32_t ni = (uint32_t)ceil_div(a.y.cols, S::kI), nj = (uint32_t)ceil_div(a.y.rows, S::kJ);
                 forward_kernel<T, S><<<dim3(ni * nj, (unsigned)k.splits), S::kThreads, 0, s>>>(a, partial, k.depth, ni, nj);
