@@ -261,9 +261,9 @@ __global__ void __launch_bounds__(kThreads, 2 * resident((int)sizeof(T), PITCH, 
 // 42 and 52 us, with gelu, preact and residual 97 and 134; 1e6 x 256 -> 256 so
 // 384 and 507; 262144 x 256 -> 128 (201 MB) 44 and 44; 65536 x 128 -> 128 (34 MB)
 // 13 and 9. Half of a workgroup's waves have no columns below 128, so those
-// take more: 262144 x 256 -> 64 (168 MB) 40 and 31, 1e6 x 84 -> 64 (296 MB) 77 and
-// 108. Floats multiply six times as long, w's planes fill the registers, and
-// the products bound narrow outputs: 1e6 x 128 -> 64 197 and 160, 262144 x 84
+// take more: 262144 x 256 -> 64 (168 MB) 40 and 29, 1e6 x 84 -> 64 (296 MB) 77 and
+// 99. Floats multiply six times as long, w's planes fill the registers, and
+// the products bound narrow outputs: 1e6 x 128 -> 64 197 and 180, 262144 x 84
 // -> 256 (356 MB) 111 and 125, 262144 x 128 -> 256 (402 MB) 142 and 138, with gelu,
 // preact and residual 202 and 232.
 bool linear_forward_by_rows(const LinearForward& a) {
