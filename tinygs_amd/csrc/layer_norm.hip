@@ -440,8 +440,9 @@ int launch_layer_norm_backward(const LayerNormBackward& a, void* workspace, hipS
             launch_column_sums((const float*)workspace, blocks, a.x.cols, 2 * a.x.cols, a.grad_gamma, a.grad_beta, s);
         });
         if (held) return;
-        if (a.grad_x.p && a.x.rows) wide_backward_kernel<T><<<(unsigned)a.x.rows, kWide, 0, s>>>(a);
+        // grad_x may take grad_y's place: its column sums come first
         if (sums) wide_columns_kernel<T><<<(unsigned)a.x.cols, 256, 0, s>>>(a);
+        if (a.grad_x.p && a.x.rows) wide_backward_kernel<T><<<(unsigned)a.x.rows, kWide, 0, s>>>(a);
     });
     TGS_CHECK_LAUNCH();
     return TGS_OK;
