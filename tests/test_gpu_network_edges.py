@@ -45,3 +45,19 @@ def test_layer_norm_backward_in_its_inputs_place(ops, shape, dtype):
     got = ops.layer_norm_backward(gy, x, gamma, mean, rstd, residual_grad=buf, grad_x=buf)
     for t, want, what in zip(got, apart, ("gx", "ggamma", "gbeta")):
         assert torch.equal(t, want), f"{what} over residual_grad"
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("out", [3, 64, 600])
+@pytest.mark.parametrize("name", ["relu", "silu", "gelu"])
+def test_slopes_at_infinity(ops, name, out, dtype):
+    """Values before the activation that left the type's range, as float16's do at 65520: slope 1 above, 0 below."""
+    rows, i = 70, 20
+    z = (2.0 * normal(1, rows, out)).to(dtype)
+    z[3, 0], z[4, 1], z[69, out - 1] = float("inf"), float("-inf"), float("inf")
+    x, w, gy = normal(2, rows, i).to(dtype), normal(3, out, i).to(dtype), normal(4, rows, out).to(dtype)
+    got = ops.linear_backward(gy.cuda(), x.cuda(), w.cuda(), preact=z.cuda(), activation=name)
+    # at +-200 the slopes are 1 and 0 to every bit
+    want = R.linear_backward(gy, x, w, z.double().clamp(-200.0, 200.0), name, dtype)
+    for t, (v, bound), what in zip(got, want, ("gx", "gw", "gb")):
+        R.check(t, v, bound, what)

@@ -75,18 +75,19 @@ __device__ __forceinline__ float activate(float z) {
 
 // act'(z) = p + z p (1 - p) (d/dz of p's argument). The second term is zero in
 // 32 bits well inside the bounds on z and z^2, which keep it from becoming
-// 0 * infinity; p itself keeps a NaN.
+// 0 * infinity at either end (a preact that left its type's range is infinite);
+// p itself keeps a NaN.
 template <int ACT>
 __device__ __forceinline__ float activate_slope(float z) {
     if constexpr (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
     if constexpr (ACT == kActSilu) {
         const float p = logistic2(-kLog2E * z);
-        return fmaf(fmaxf(z, -100.0f) * p, 1.0f - p, p);
+        return fmaf(__builtin_amdgcn_fmed3f(z, -100.0f, 100.0f) * p, 1.0f - p, p);
     }
     if constexpr (ACT == kActGelu) {
         const float q = fminf(z * z, 900.0f);
         const float p = logistic2(z * fmaf(-kLog2E * kGelu3, q, -kLog2E * kGelu1));
-        return fmaf(fmaxf(z, -30.0f) * (p * (1.0f - p)), fmaf(3.0f * kGelu3, q, kGelu1), p);
+        return fmaf(__builtin_amdgcn_fmed3f(z, -30.0f, 30.0f) * (p * (1.0f - p)), fmaf(3.0f * kGelu3, q, kGelu1), p);
     }
     return 1.0f;
 }
