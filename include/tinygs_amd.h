@@ -486,7 +486,8 @@ int tgs_convert(const void* src, int32_t src_dtype, void* dst, int32_t dst_dtype
  * The matrices of one call are of one dtype. Products and sums are held in
  * 32 bits; every stored element is rounded once to its dtype. Products of
  * float32 matrices are of operands held to 24 bits (three bfloat16 each, six
- * products): values of 2^128 (1 - 2^-9) and more count as infinite.
+ * products); what comes out infinite or NaN so is formed again with float32
+ * products, so that infinities, NaN and the largest floats act as in float32.
  * An output may not overlap an input unless its entry says so.
  * A call reads and writes nothing after its last kernel on `stream`; it does
  * not wait for the device, except to grow the handle's workspace. The

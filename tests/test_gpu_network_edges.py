@@ -61,3 +61,78 @@ def test_slopes_at_infinity(ops, name, out, dtype):
     want = R.linear_backward(gy, x, w, z.double().clamp(-200.0, 200.0), name, dtype)
     for t, (v, bound), what in zip(got, want, ("gx", "gw", "gb")):
         R.check(t, v, bound, what)
+
+
+INF, NAN = float("inf"), float("nan")
+HUGE = 3.4e38   # above bfloat16's largest number, below float's
+
+
+def alike(got, want, bound, what):
+    """Equal infinities and NaN, and everything else within its bound. What exceeds float's range is infinite."""
+    got = got.double().cpu()
+    want = torch.where(want.abs() > 3.4028236e38, want.sign() * INF, want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), (what, "NaN")
+    ends = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), ends) and torch.equal(got[ends], want[ends]), (what, "infinities")
+    held = torch.isfinite(want)
+    assert bool(((got - want).abs() <= bound)[held].all()), what
+
+
+def ends(rows, i, o):
+    """x and w whose products meet the ends of float, in some rows of each, the first and the last among them. What
+    HUGE is multiplied with stays below one, so that float sums overflow where exact ones do."""
+    x, w = normal(1, rows, i), 0.3 * i ** -0.5 * normal(2, o, i)
+    k = i // 2
+    x[rows - 1] *= 0.1
+    x[:, k] *= 0.1
+    x[0, k] = INF
+    x[rows // 3, 0], x[rows // 2, i - 1], x[rows - 1, k + 1] = -INF, NAN, HUGE
+    x[rows // 4, k], x[rows // 4, i - 1] = INF, -INF   # NaN where w's signs there agree
+    if o > 4:
+        w[1, k] = 0.0             # times infinity: NaN
+        w[2, k] = 1e-30           # times infinity: infinity
+        w[o - 2, 0] = INF
+    return x, w
+
+
+# few rows; one, several and ragged tiles; k split; many large, middle and narrow tiles; many rows of a narrow layer
+@pytest.mark.parametrize("shape", [(3, 8, 16), (20, 999, 17), (4, 4096, 40), (150, 96, 80), (97, 33, 5), (130, 4096, 64),
+                                   (16384, 130, 1024), (8192, 130, 512), (100000, 300, 40), (800001, 50, 130),
+                                   (700001, 128, 128)], ids=str)
+@pytest.mark.parametrize("name", ["none", "relu"])
+def test_linear_infinities_in_floats(ops, shape, name):
+    """Infinities, NaN and floats past bfloat16's range: what float products and sums give."""
+    rows, i, o = shape
+    x, w = ends(rows, i, o)
+    w[o // 2, i // 2] = HUGE
+    b = normal(3, o)
+    print(f"[linear] {shape} {name}", flush=True)
+    y, z = ops.linear(x.cuda(), w.cuda(), b.cuda(), activation=name, keep_preact=True)
+    at = torch.arange(rows) if rows < 5000 else torch.cat([torch.arange(300), torch.arange(rows // 4 - 40, rows // 4 + 40),
+                                                           torch.arange(rows // 3 - 40, rows // 3 + 40),
+                                                           torch.arange(rows // 2 - 40, rows // 2 + 40),
+                                                           torch.arange(rows - 300, rows)])
+    wz = x[at].double() @ w.double().t() + b.double()
+    bound = torch.nan_to_num(R.product_bound(x[at].double(), w.double().t(), i), nan=INF) + 3 * R.EPS24 * b.double().abs() \
+        + R.EPS24 * torch.nan_to_num(wz.abs(), nan=INF) + R.STEP[torch.float32]
+    alike(z[at], wz, bound, "z")
+    alike(y[at], R.act(wz, name), bound, "y")
+
+
+# narrow layers, whole and ragged chunks; tiles, with their sums over out and over the rows split or not
+@pytest.mark.parametrize("shape", [(3, 8, 16), (70, 72, 40), (5000, 128, 128), (4100, 83, 59), (40, 300, 20),
+                                   (130, 260, 4096), (5000, 260, 300), (20000, 513, 64)], ids=str)
+@pytest.mark.parametrize("name", ["none", "silu"])
+def test_linear_backward_infinities_in_floats(ops, shape, name):
+    rows, i, o = shape
+    x, w = ends(rows, i, o)
+    gy = normal(4, rows, o)
+    gy[rows - 1] *= 0.1
+    gy[rows // 2, o - 1], gy[rows // 2 - 1, 0], gy[1, o // 2], gy[rows - 1, o // 3] = INF, -INF, NAN, HUGE
+    z = normal(5, rows, o) if name != "none" else None
+    if z is not None:
+        z[rows - 1, o // 3] = 0.0   # slope 1/2
+    print(f"[linear_backward] {shape} {name}", flush=True)
+    got = ops.linear_backward(gy.cuda(), x.cuda(), w.cuda(), preact=None if z is None else z.cuda(), activation=name)
+    for t, (v, bound), what in zip(got, R.linear_backward(gy, x, w, z, name, torch.float32), ("gx", "gw", "gb")):
+        alike(t, v, torch.nan_to_num(bound, nan=INF), what)

@@ -92,6 +92,18 @@ __global__ void __launch_bounds__(64 * kWaves) few_kernel(LinearForward a) {
 #pragma unroll
         for (int q = 0; q < kAhead; ++q) acc = multiply(fragment(cw[q]), fragment(cx[q]), acc);
     }
+    if constexpr (sizeof(T) == 4) {   // k as this wave's steps hold it
+        f32x4 one[1][1] = {{acc}};
+        const int own = steps > wave ? (steps - wave - 1) / kWaves + 1 : 0;
+        const auto element = [&](const Side& s, int row, int64_t k) {
+            const int64_t at = 32 * (wave + kWaves * (k >> 5)) + (k & 31);
+            return s.exists && at < in ? s.base[row * s.stride + at] : 0.0f;
+        };
+        form_again(
+            one, 0, 32 * own, [&](int, int row, int64_t k) { return element(w, row, k); },
+            [&](int, int row, int64_t k) { return element(x, row, k); }, [](int, int, int) { return true; });
+        acc = one[0][0];
+    }
     __shared__ f32x4 sums[kWaves][64];
     sums[wave][lane] = acc;
     __syncthreads();

@@ -171,6 +171,12 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
     const int wi = wave >> 2, wj = wave & 3;
     const bool dw_here = a.grad_w.p && wi * N::TI * 16 < in && wj * N::TJ * 16 < out;
     const bool dx_here = a.grad_x.p && wave * N::DI * 16 < in;
+    const auto slope_of = [&](int64_t row, int column) {   // dz as form_again reads it
+        if (row >= rows || column >= out) return 0.0f;
+        const float d = (float)((const T*)a.grad_y.p)[row * a.grad_y.stride + column];
+        if constexpr (ACT == kActNone) return d;
+        else return d * activate_slope<ACT>((float)((const T*)a.preact.p)[row * a.preact.stride + column]);
+    };
 
     for (int block = blockIdx.x; block < blocks; block += gridDim.x) {
         lds_barrier();   // the last block's reads are done
@@ -227,6 +233,15 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
             };
             half(0);
             if (deep) half(N::kSteps / 2);
+            if constexpr (sizeof(T) == 4)
+                form_again(
+                    d, 0, out,
+                    [&](int u, int row, int64_t k) {
+                        const int i = (wave * N::DI + u) * 16 + row;
+                        return i < in ? ((const T*)a.w.p)[k * a.w.stride + i] : 0.0f;
+                    },
+                    [&](int v, int row, int64_t k) { return slope_of((int64_t)block * kRows + 16 * v + row, (int)k); },
+                    [](int, int, int) { return true; });
             const int64_t first = (int64_t)block * kRows, pitch = a.grad_x.stride * (int64_t)sizeof(T);
             T* const base = (T*)a.grad_x.p + first * a.grad_x.stride;
             const auto buffer = resource_of(base, (min(rows - first, (int64_t)kRows) - 1) * pitch + in * (int64_t)sizeof(T));
@@ -275,6 +290,22 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
     }
 
     float* to = partial + (int64_t)blockIdx.x * ((int64_t)out * in + out);
+    if constexpr (sizeof(T) == 4)
+        if (dw_here) {   // k runs over the rows of the workgroup's blocks
+            const int own = (blocks - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;
+            const auto row_of = [&](int64_t k) {
+                return ((int64_t)blockIdx.x + (k / kRows) * gridDim.x) * kRows + k % kRows;
+            };
+            form_again(
+                acc, 0, (int64_t)own * kRows,
+                [&](int u, int row, int64_t k) {
+                    const int64_t r = row_of(k);
+                    const int i = (wi * N::TI + u) * 16 + row;
+                    return r < rows && i < in ? ((const T*)a.x.p)[r * a.x.stride + i] : 0.0f;
+                },
+                [&](int v, int row, int64_t k) { return slope_of(row_of(k), (wj * N::TJ + v) * 16 + row); },
+                [](int, int, int) { return true; });
+        }
     if (dw_here) {
         const auto buffer = resource_of(to, (int64_t)out * in * 4);   // at most 256 KB
         const bool fours = in % 4 == 0;

@@ -206,6 +206,18 @@ __global__ void __launch_bounds__(kThreads, 2 * resident((int)sizeof(T), PITCH, 
         }
 
         const int64_t first = (int64_t)block * kRows;
+        if constexpr (sizeof(T) == 4)
+            form_again(
+                acc, 0, in,
+                [&](int u, int row, int64_t k) {
+                    const int64_t n = column0 + 16 * u + row;
+                    return n < out ? ((const T*)a.w.p)[n * a.w.stride + k] : 0.0f;
+                },
+                [&](int v, int row, int64_t k) {
+                    const int64_t r = first + (wr * K::kRowSquares + v) * 16 + row;
+                    return r < rows ? ((const T*)a.x.p)[r * a.x.stride + k] : 0.0f;
+                },
+                [](int, int, int) { return true; });
         const int64_t held = min(rows - first, (int64_t)kRows) - 1;
         const int64_t y_pitch = a.y.stride * (int64_t)sizeof(T), z_pitch = a.preact.stride * (int64_t)sizeof(T);
         T* const y0 = (T*)a.y.p + first * a.y.stride + at;

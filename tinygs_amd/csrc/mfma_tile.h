@@ -39,8 +39,9 @@ struct Frag<__bf16> {
     typedef __bf16 type __attribute__((ext_vector_type(8)));
 };
 // A float is held as three bfloat16, high + middle + low: 24 bits in all, each
-// the nearest to what the ones before leave. Floats of 2^128 (1 - 2^-9) and
-// more count as infinite.
+// the nearest to what the ones before leave. For infinities, NaN and floats of
+// 2^128 (1 - 2^-9) and more high is not finite, and so is every sum that they
+// enter, whatever it should be (inf - inf, 0 inf): form_again mends those.
 template <>
 struct Frag<float> {
     typedef __bf16 plane __attribute__((ext_vector_type(8)));
@@ -90,6 +91,52 @@ __device__ __forceinline__ f32x4 multiply(const Frag<float>::type& a, const Frag
     c = multiply(a.middle, b.high, c);
     c = multiply(a.high, b.middle, c);
     return multiply(a.high, b.high, c);
+}
+
+// Float outputs that came out infinite or NaN, formed again from the operands by
+// the matrix cores' float instructions, so that they are what float products
+// and sums give; the others keep their bits. fa(u, a, k) and fb(v, a, k) are
+// rows 16 u + a of A and 16 v + a of B at k, which runs from k0 to below k1;
+// exists(u, v, r) tells the lane whether its register r of a square is an
+// output at all. A wave looks at its own squares, one multiply-add a register
+// (16384 x 1024 -> 2048 floats 345 us without it and 348 with it, 1e6 x 128 ->
+// 128 274 and 281); where it finds something it takes several times the
+// products' time.
+template <int TI, int TJ, class FA, class FB, class Exists>
+__device__ __forceinline__ void form_again(f32x4 (&acc)[TI][TJ], int64_t k0, int64_t k1, FA fa, FB fb, Exists exists) {
+    f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};   // 0 where all are finite
+#pragma unroll
+    for (int u = 0; u < TI; ++u)
+#pragma unroll
+        for (int v = 0; v < TJ; ++v)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) none[r] = fmaf(acc[u][v][r], 0.0f, none[r]);
+    if (ballot((none[0] + none[1]) + (none[2] + none[3]) != 0.0f) == 0) return;
+    const int a = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+#pragma unroll
+    for (int u = 0; u < TI; ++u) {
+        bool ends = false;
+#pragma unroll
+        for (int v = 0; v < TJ; ++v)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ends |= !__builtin_isfinite(acc[u][v][r]) && exists(u, v, r);
+        if (ballot(ends) == 0) continue;
+        f32x4 sum[TJ];
+#pragma unroll
+        for (int v = 0; v < TJ; ++v) sum[v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+        for (int64_t from = k0; from < k1; from += 4) {
+            const int64_t k = from + g;
+            const float x = k < k1 ? fa(u, a, k) : 0.0f;
+#pragma unroll
+            for (int v = 0; v < TJ; ++v)
+                sum[v] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, k < k1 ? fb(v, a, k) : 0.0f, sum[v], 0, 0, 0);
+        }
+#pragma unroll
+        for (int v = 0; v < TJ; ++v)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[u][v][r] = __builtin_isfinite(acc[u][v][r]) ? acc[u][v][r] : sum[v][r];
+    }
 }
 
 // An operand of a launch. K-contiguous: `rows` of `cols` = k elements;
@@ -340,6 +387,20 @@ struct Tile {
                 }
                 from = from + kStage < lds + kLds ? from + kStage : lds;
             }
+            const int64_t ni = A_RC ? a.cols : a.rows, nj = B_RC ? b.cols : b.rows;
+            const int64_t iw = i0 + wi * TI * 16, jw = j0 + wj * TJ * 16;
+            // outputs that do not exist hold what follows a row in memory
+            form_again(
+                acc, k0, k1,
+                [&](int u, int row, int64_t k) {
+                    const int64_t i = iw + 16 * u + row;
+                    return i < ni ? ((const T*)a.p)[A_RC ? k * a.stride + i : i * a.stride + k] : 0.0f;
+                },
+                [&](int v, int row, int64_t k) {
+                    const int64_t j = jw + 16 * v + row;
+                    return j < nj ? ((const T*)b.p)[B_RC ? k * b.stride + j : j * b.stride + k] : 0.0f;
+                },
+                [&](int u, int v, int r) { return iw + 16 * u + 4 * (lane >> 4) + r < ni && jw + 16 * v + (lane & 15) < nj; });
         } else {
 #pragma unroll
             for (int n = 0; n < STAGES; ++n)
