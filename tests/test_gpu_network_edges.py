@@ -136,3 +136,24 @@ def test_linear_backward_infinities_in_floats(ops, shape, name):
     got = ops.linear_backward(gy.cuda(), x.cuda(), w.cuda(), preact=None if z is None else z.cuda(), activation=name)
     for t, (v, bound), what in zip(got, R.linear_backward(gy, x, w, z, name, torch.float32), ("gx", "gw", "gb")):
         alike(t, v, torch.nan_to_num(bound, nan=INF), what)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_optimizer_by_name_trains_the_network(hip, dtype):
+    """A network's optimiser made by its name, as the network's documentation has it, steps as net.optimizer() does,
+    and forward reads what it wrote."""
+    from tinygs_amd.network import AttributeNetwork
+    from tinygs_amd.optim import create_optimizer
+    features, grad = normal(1, 300, 20).to(dtype).cuda(), normal(2, 300, 7).to(dtype).cuda()
+    after = []
+    for by_name in (False, True):
+        net = AttributeNetwork(20, 7, width=48, blocks=1, dtype=dtype, seed=3)
+        opt = create_optimizer("muon", net.weights, net.grads, copies=net.copies) if by_name else net.optimizer()
+        first = net.forward(features)
+        net.backward(grad)
+        opt.step(1.0)
+        after.append(net.forward(features, keep=False))
+        assert not torch.equal(after[-1], first)
+        for w, m in zip(net.weights, net.matrices()):
+            assert torch.equal(w.to(dtype), m)
+    assert torch.equal(after[0], after[1])

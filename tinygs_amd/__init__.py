@@ -12,7 +12,7 @@ mirrors tinygs's plugin interfaces on top of it:
 and adds the operators of a network whose outputs are Gaussian attributes:
 
   LayerOps, AttributeNetwork                        (linear layers, layer norm)
-  create_optimizer("muon", matrices, grads)
+  create_optimizer("muon", matrices, grads, copies)
 
 Importing the package does not load the library; the first rasterizer /
 loss / optimizer call does, and raises if it has not been built.

@@ -197,10 +197,11 @@ class AttributeNetwork:
     norm(h) w_out^T + b_out. norm is a layer norm with its own gamma and beta. The last matrix starts at zero, so an
     untrained network changes nothing.
 
-    weights are the float32 matrices that an optimiser updates (create_optimizer("muon", net.weights, net.grads), or
-    net.optimizer()); for a half dtype the products read net.copies, which Muon writes in its step. vectors and
-    vector_grads hold all biases, gammas and betas, and their gradients, as one float32 vector each, for an optimiser
-    of vectors. backward assigns every gradient."""
+    weights are the float32 matrices that an optimiser updates: net.optimizer(), which is create_optimizer("muon",
+    net.weights, net.grads, copies=net.copies). For a half dtype the products read net.copies, which Muon writes in its
+    step: an optimiser that is not given them changes nothing that forward reads. vectors and vector_grads hold all
+    biases, gammas and betas, and their gradients, as one float32 vector each, for an optimiser of vectors. backward
+    assigns every gradient."""
 
     def __init__(self, inputs: int, outputs: int, width: int = 256, hidden: int | None = None, blocks: int = 2,
                  activation: str = "gelu", dtype=None, seed: int = 0, eps: float = 1e-5, device: str = "cuda"):

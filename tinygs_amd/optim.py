@@ -260,11 +260,14 @@ class Muon:
         _lib.check(self._lib.tgs_muon_set_params(self._h, C.byref(p)), "set_params")
 
 
-def create_optimizer(optimizer_type: str, gaussians, gaussians_grad):
-    """"simple_adam" on Gaussians and their gradients, or "muon" on lists of matrices and of theirs."""
+def create_optimizer(optimizer_type: str, gaussians, gaussians_grad, copies=None):
+    """"simple_adam" on Gaussians and their gradients, or "muon" on lists of matrices and of theirs; copies, for "muon",
+    receive the updated matrices rounded to their dtype, which is what a half-precision network reads."""
     t = optimizer_type.lower()
     if t == "simple_adam":
+        if copies is not None:
+            raise RuntimeError("create_optimizer: simple_adam writes no copies")
         return SimpleAdam(gaussians, gaussians_grad)
     if t == "muon":
-        return Muon(gaussians, gaussians_grad)
+        return Muon(gaussians, gaussians_grad, copies=copies)
     raise RuntimeError(f"Unknown optimizer type: {optimizer_type}")
