@@ -157,3 +157,25 @@ def test_optimizer_by_name_trains_the_network(hip, dtype):
         for w, m in zip(net.weights, net.matrices()):
             assert torch.equal(w.to(dtype), m)
     assert torch.equal(after[0], after[1])
+
+
+# rows of fewer elements than 16 bytes hold, one to a few of them after the last whole block of 64; the second number
+# of columns makes the call one of the many-row kernel, or its residual as narrow as x
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("more", [1, 2, 6])
+@pytest.mark.parametrize("i,o", [(1, 128), (3, 129), (7, 260), (3, 3), (5, 1)])
+def test_linear_many_short_rows(ops, i, o, more, dtype):
+    size = 4 if dtype == torch.float32 else 2
+    if size == 4 and o < 128:
+        i, o = i, 128 + o   # floats of fewer columns take tiles
+    rows = ((400 if size == 4 else 270) << 20) // ((i + 2 * o) * size) // 64 * 64 + more
+    print(f"[linear] {rows} x {i} -> {o} {dtype}", flush=True)
+    g = torch.Generator("cuda").manual_seed(5)
+    x = torch.randn(rows, i, generator=g, device="cuda").to(dtype)
+    r = torch.randn(rows, o, generator=g, device="cuda").to(dtype)
+    w, b = normal(11, o, i).to(dtype).cuda(), normal(21, o).cuda()
+    y = ops.linear(x, w, b, activation="silu", residual=r)
+    at = torch.cat([torch.arange(200), torch.arange(rows // 2, rows // 2 + 200), torch.arange(rows - 200, rows)]).cuda()
+    want, bound = R.linear(x[at], w, b, "silu", r[at], dtype)[:2]
+    R.check(y[at], want, bound, "y")
+    assert bool(torch.isfinite(y).all())

@@ -21,6 +21,22 @@ constexpr int kThreads = 512;
 // Workgroups a compute unit holds: two where w's registers allow it.
 constexpr int resident(int size, int pitch, int cw) { return size == 2 && pitch == 256 && cw <= 4 ? 2 : 1; }
 
+// What a block's loads may read of a matrix from the block's first element on:
+// `bytes`, which never pass the matrix's end. A row's partial last chunk is
+// read whole, with up to 14 bytes of what follows, where the `left` rows from
+// the block's first on hold as much after the block (`whole`: rows of a few
+// elements need several of them), and else gathered.
+struct Reach {
+    bool whole;
+    int bytes;   // below 2^30
+};
+__host__ __device__ inline Reach reach_of(int64_t left, int cols, int stride, int size) {
+    const int near = left < 2 * kRows ? (int)left : 2 * kRows, held = near < kRows ? near : kRows;
+    const int chunk = 16 / size, tail = cols % chunk;
+    const bool whole = tail == 0 || chunk - tail <= (near - held) * stride;
+    return {whole, ((held - 1) * stride + (tail && whole ? cols - tail + chunk : cols)) * size};
+}
+
 // PITCH: bytes of a row of x in LDS. CW waves share the columns (COLS of them
 // a workgroup), 8 / CW the rows.
 template <class T, int PITCH, int CW, bool RESIDUAL>
@@ -41,27 +57,26 @@ struct RowsKernel {
     static constexpr int kLds = kStages * kStage;
     static constexpr int kLoads = kStage / 1024 / 8;              // a wave and block
 
-    // Rows `first` .. + 63 of m from column c0 on, as rows of PITCH2 bytes in
+    // Rows `first` .. + 63 of m from column c0 on, as rows of F's pitch in
     // LDS. Chunks past m's columns are filled from what follows in memory,
-    // which its user masks or ignores; the chunk that crosses the matrix's end
-    // is gathered (`last`: the block holds the last row).
+    // which its user masks or ignores.
     template <class F>
-    static __device__ __forceinline__ void load(const Mat& m, int64_t first, int64_t c0, unsigned char* lds, bool last,
-                                                int wave, int lane) {
+    static __device__ __forceinline__ void load(const Mat& m, int64_t first, int64_t c0, unsigned char* lds, int wave,
+                                                int lane) {
         constexpr int kChunks = F::kCols / V, kLoads = kRows * kChunks / 64 / 8;
         const int64_t pitch = m.stride * (int64_t)sizeof(T);
         const T* base = (const T*)m.p + first * m.stride + c0;
         const int64_t rows = min(m.rows - first, (int64_t)kRows);
         const int cols = (int)min(m.cols - c0, (int64_t)F::kCols);
         const int tail = cols % V;   // elements of a partial chunk
-        // whole chunks beyond the columns are left out; a partial one of an inner row may be read whole
-        const i32x4 buffer = buffer_of(base, (rows - 1) * pitch + (int64_t)(tail && !last ? cols - tail + V : cols) * (int64_t)sizeof(T));
+        const Reach reach = reach_of(m.rows - first, cols, (int)m.stride, (int)sizeof(T));
+        const i32x4 buffer = buffer_of(base, reach.bytes);
         const uint32_t to = lds_address(lds);
 #pragma unroll
         for (int n = 0; n < kLoads; ++n) {
             const int slot = (n * 8 + wave) * 64 + lane, r = slot / kChunks, c = (slot % kChunks) ^ F::turn(r);
             const uint32_t offset = (c * V < cols ? 0u : kNowhere) + (uint32_t)r * (uint32_t)pitch + (uint32_t)c * 16u;
-            if (tail && last && c == cols / V) {
+            if (!reach.whole && c == cols / V) {
                 const T* p = base + (r < rows ? r : 0) * m.stride + c * V;
                 *(typename C::type*)(lds + slot * 16) = C::gather(p, r < rows ? tail : 0);
             } else {
@@ -108,9 +123,8 @@ __global__ void __launch_bounds__(kThreads, 2 * resident((int)sizeof(T), PITCH, 
         const int64_t first = (int64_t)block * kRows;
         unsigned char* stage = lds + filled * K::kStage;
         filled = filled + 1 < K::kStages ? filled + 1 : 0;
-        const bool last = first + kRows >= rows;
-        K::template load<X>(a.x, first, 0, stage, last, wave, lane);
-        if constexpr (RESIDUAL) K::template load<typename K::R>(residual, first, c0, stage + K::kXBytes, last, wave, lane);
+        K::template load<X>(a.x, first, 0, stage, wave, lane);
+        if constexpr (RESIDUAL) K::template load<typename K::R>(residual, first, c0, stage + K::kXBytes, wave, lane);
     };
 #pragma unroll
     for (int n = 0; n < K::kStages - 1; ++n)
@@ -266,6 +280,11 @@ __global__ void __launch_bounds__(kThreads, 2 * resident((int)sizeof(T), PITCH, 
 }
 
 }  // namespace
+
+// For tests: how far the loads of a block read.
+int64_t linear_rows_reach(int64_t left, int64_t cols, int64_t stride, int64_t size) {
+    return reach_of(left, (int)cols, (int)stride, (int)size).bytes;
+}
 
 // Once a call moves more than the card's last cache holds of it, w in registers
 // and few, long waits pay; below, tiles fill the card sooner and their second
