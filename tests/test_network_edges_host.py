@@ -1,6 +1,8 @@
 """The attribute network on the host, where its parts meet: what is passed on and what is refused, without a GPU."""
 import ctypes as C
+import glob
 import os
+import re
 
 import pytest
 
@@ -27,3 +29,16 @@ def test_loads_of_row_blocks_end_with_the_matrix(size):
                 reach = f(left, cols, stride, size)
                 held = min(left, 64)
                 assert ((held - 1) * stride + cols) * size <= reach <= ((left - 1) * stride + cols) * size
+
+
+def test_asm_puts_m0_back():
+    """m0 is reserved: the compiler takes no clobber of it, and keeps what it holds there over asm. A statement that
+    writes it saves it first and restores it last."""
+    found = 0
+    for path in sorted(glob.glob(os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc", "*.h*"))):
+        for text in re.findall(r"\basm\b[^;]*?\((.*?)\);", open(path).read(), re.S):
+            steps = "".join(re.findall(r'"((?:[^"\\]|\\.)*)"', text)).replace("\\n", "\n").replace("\\t", "").split("\n")
+            if any(re.match(r"s_mov_b32 m0\b", s) for s in steps):
+                found += 1
+                assert steps[0] == "s_mov_b32 %0, m0" and re.match(r"s_mov_b32 m0, %0", steps[-1]), (path, steps)
+    assert found >= 1

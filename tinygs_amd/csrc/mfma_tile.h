@@ -152,12 +152,14 @@ typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
 __device__ __forceinline__ uint32_t lds_address(void* p) { return (uint32_t)(uintptr_t)(lds_byte*)p; }
 
-// 16 bytes a lane from buffer + offset to LDS at base + 16 lane.
+// 16 bytes a lane from buffer + offset to LDS at base + 16 lane. The base goes
+// through m0, a register that asm cannot declare as changed: it is put back.
 __device__ __forceinline__ void load_to_lds(uint32_t base, uint32_t offset, i32x4 buffer) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
-                     __builtin_amdgcn_readfirstlane(base)),
-                 "v"(offset),
-                 "s"(buffer)
+    uint32_t held;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(held)
+                 : "s"(__builtin_amdgcn_readfirstlane(base)), "v"(offset), "s"(buffer)
                  : "memory");
 }
 
