@@ -179,3 +179,29 @@ def test_linear_many_short_rows(ops, i, o, more, dtype):
     want, bound = R.linear(x[at], w, b, "silu", r[at], dtype)[:2]
     R.check(y[at], want, bound, "y")
     assert bool(torch.isfinite(y).all())
+
+
+def test_linear_more_rows_than_a_launch_of_tiles(ops):
+    """2^30 rows and some, of one column: 256 threads for 64 rows would be 2^32 threads."""
+    rows = (1 << 30) + 100
+    x = torch.arange(rows, dtype=torch.int32, device="cuda").remainder_(1021).to(torch.float32)[:, None]
+    y = torch.full((rows, 1), -7.0, device="cuda")
+    print("[linear] 2^30 + 100 x 1 -> 1", flush=True)
+    ops.linear(x, torch.full((1, 1), 2.0, device="cuda"), torch.ones(1, device="cuda"), out=y)
+    assert torch.equal(y, x.mul_(2.0).add_(1.0))
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 8193), (torch.bfloat16, 16385)], ids=["f32", "bf16"])
+def test_layer_norm_more_wide_rows_than_workgroups(ops, dtype, n):
+    """Rows above 32 KB, more of them than a launch has workgroups for."""
+    rows = 65536 + 77
+    x = torch.randn(64, n, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).to(dtype).repeat(rows // 64 + 1, 1)[:rows]
+    print(f"[layer_norm] {rows} x {n} {dtype}", flush=True)
+    y, mean, rstd = ops.layer_norm(x)
+    for t, (v, bound), what in zip((y, mean, rstd), R.layer_norm(x[:64], None, None, 1e-5, dtype), ("y", "mean", "rstd")):
+        R.check(t[:64], v, bound, what)
+        assert all(torch.equal(t[at:at + 64], t[:64][:rows - at]) for at in range(64, rows, 64)), what
+    gx, gg, gb = ops.layer_norm_backward(y, x, None, mean, rstd)
+    want, bound = R.layer_norm_backward(y[:64], x[:64], None, mean[:64], rstd[:64], None, dtype)[0]
+    R.check(gx[:64], want, bound, "gx")
+    assert all(torch.equal(gx[at:at + 64], gx[:64][:rows - at]) for at in range(64, rows, 64))

@@ -42,3 +42,32 @@ def test_asm_puts_m0_back():
                 found += 1
                 assert steps[0] == "s_mov_b32 %0, m0" and re.match(r"s_mov_b32 m0, %0", steps[-1]), (path, steps)
     assert found >= 1
+
+
+# threads that a launch holds; with more, what is above is lost without an error
+LAUNCH = 1 << 32
+
+
+def test_wide_layer_norm_launches_hold_their_threads():
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built")
+    f = _lib.load()._ZN3tgs22layer_norm_wide_blocksEl
+    f.argtypes, f.restype = [C.c_int64], C.c_int64
+    for rows in (1, 65535, 65537, 1 << 22, (1 << 31) - 1):
+        assert 1 <= f(rows) <= rows and f(rows) * 1024 < LAUNCH
+
+
+@pytest.mark.parametrize("count,fits", [(511, True), (512, False)])
+def test_muon_refuses_more_than_a_launch_holds(count, fits):
+    """Matrices of one row and 2^21 - 1 columns are 2^15 patches of 256 threads each. Their addresses are never read."""
+    lib, n = _lib.load(), (1 << 21) - 1
+
+    def array(slot):
+        return (_lib.tgs_matrix * count)(*[_lib.tgs_matrix((1 << 40) * (slot + 1) + (1 << 23) * k, 1, n, n,
+                                                           _lib.TGS_DTYPE_FLOAT32) for k in range(count)])
+    h = C.c_void_p()
+    rc = lib.tgs_muon_create(array(0), array(1), array(2), None, count, C.byref(h))
+    if fits:
+        assert rc == 0 and lib.tgs_muon_destroy(h) == 0
+    else:
+        assert rc == _lib.TGS_ERR_INVALID and "too large for one step" in lib.tgs_last_error().decode()

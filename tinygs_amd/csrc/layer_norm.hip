@@ -302,34 +302,38 @@ bool by_width(int64_t n, F f) {
 }
 
 // ---- rows over 32 KB: the row is read again from memory for each pass, one
-// workgroup a row; the column sums run one workgroup a column.
+// workgroup a row; the column sums run one workgroup a column. A launch of 2^32
+// threads or more loses what is above without an error: workgroups take further
+// rows.
 constexpr int kWide = 1024;
 
 template <class T>
 __global__ void __launch_bounds__(kWide) wide_forward_kernel(LayerNormForward a) {
     __shared__ float s[2 * kWide / 64];
     int turn = 0;
-    const int64_t r = blockIdx.x, n = a.x.cols;
-    const T* x = (const T*)a.x.p + r * a.x.stride;
-    T* y = (T*)a.y.p + r * a.y.stride;
-    float v[1] = {0.0f};
-    for (int64_t k = threadIdx.x; k < n; k += kWide) v[0] += (float)x[k];
-    group_sum<kWide>(v, s, turn);
-    const float mean = v[0] / (float)n;
-    v[0] = 0.0f;
-    for (int64_t k = threadIdx.x; k < n; k += kWide) {
-        const float d = (float)x[k] - mean;
-        v[0] = fmaf(d, d, v[0]);
-    }
-    group_sum<kWide>(v, s, turn);
-    const float rstd = 1.0f / sqrtf(v[0] / (float)n + a.eps);
-    for (int64_t k = threadIdx.x; k < n; k += kWide) {
-        const float h = ((float)x[k] - mean) * rstd;
-        y[k] = (T)fmaf(h, a.gamma ? a.gamma[k] : 1.0f, a.beta ? a.beta[k] : 0.0f);
-    }
-    if (threadIdx.x == 0) {
-        if (a.mean) a.mean[r] = mean;
-        if (a.rstd) a.rstd[r] = rstd;
+    const int64_t n = a.x.cols;
+    for (int64_t r = blockIdx.x; r < a.x.rows; r += gridDim.x) {
+        const T* x = (const T*)a.x.p + r * a.x.stride;
+        T* y = (T*)a.y.p + r * a.y.stride;
+        float v[1] = {0.0f};
+        for (int64_t k = threadIdx.x; k < n; k += kWide) v[0] += (float)x[k];
+        group_sum<kWide>(v, s, turn);
+        const float mean = v[0] / (float)n;
+        v[0] = 0.0f;
+        for (int64_t k = threadIdx.x; k < n; k += kWide) {
+            const float d = (float)x[k] - mean;
+            v[0] = fmaf(d, d, v[0]);
+        }
+        group_sum<kWide>(v, s, turn);
+        const float rstd = 1.0f / sqrtf(v[0] / (float)n + a.eps);
+        for (int64_t k = threadIdx.x; k < n; k += kWide) {
+            const float h = ((float)x[k] - mean) * rstd;
+            y[k] = (T)fmaf(h, a.gamma ? a.gamma[k] : 1.0f, a.beta ? a.beta[k] : 0.0f);
+        }
+        if (threadIdx.x == 0) {
+            if (a.mean) a.mean[r] = mean;
+            if (a.rstd) a.rstd[r] = rstd;
+        }
     }
 }
 
@@ -337,24 +341,26 @@ template <class T>
 __global__ void __launch_bounds__(kWide) wide_backward_kernel(LayerNormBackward a) {
     __shared__ float s[4 * kWide / 64];
     int turn = 0;
-    const int64_t r = blockIdx.x, n = a.x.cols;
-    const T* x = (const T*)a.x.p + r * a.x.stride;
-    const T* gy = (const T*)a.grad_y.p + r * a.grad_y.stride;
-    const T* res = a.residual.p ? (const T*)a.residual.p + r * a.residual.stride : nullptr;
-    T* gx = (T*)a.grad_x.p + r * a.grad_x.stride;
-    const float mean = a.mean[r], rstd = a.rstd[r];
-    float v[2] = {0.0f, 0.0f};
-    for (int64_t k = threadIdx.x; k < n; k += kWide) {
-        const float h = ((float)x[k] - mean) * rstd, g = (float)gy[k] * (a.gamma ? a.gamma[k] : 1.0f);
-        v[0] += g;
-        v[1] = fmaf(g, h, v[1]);
-    }
-    group_sum<kWide>(v, s, turn);
-    const float c1 = v[0] / (float)n, c2 = v[1] / (float)n;
-    for (int64_t k = threadIdx.x; k < n; k += kWide) {
-        const float h = ((float)x[k] - mean) * rstd, g = (float)gy[k] * (a.gamma ? a.gamma[k] : 1.0f);
-        const float d = rstd * fmaf(-h, c2, g - c1);
-        gx[k] = (T)(res ? d + (float)res[k] : d);
+    const int64_t n = a.x.cols;
+    for (int64_t r = blockIdx.x; r < a.x.rows; r += gridDim.x) {
+        const T* x = (const T*)a.x.p + r * a.x.stride;
+        const T* gy = (const T*)a.grad_y.p + r * a.grad_y.stride;
+        const T* res = a.residual.p ? (const T*)a.residual.p + r * a.residual.stride : nullptr;
+        T* gx = (T*)a.grad_x.p + r * a.grad_x.stride;
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float v[2] = {0.0f, 0.0f};
+        for (int64_t k = threadIdx.x; k < n; k += kWide) {
+            const float h = ((float)x[k] - mean) * rstd, g = (float)gy[k] * (a.gamma ? a.gamma[k] : 1.0f);
+            v[0] += g;
+            v[1] = fmaf(g, h, v[1]);
+        }
+        group_sum<kWide>(v, s, turn);
+        const float c1 = v[0] / (float)n, c2 = v[1] / (float)n;
+        for (int64_t k = threadIdx.x; k < n; k += kWide) {
+            const float h = ((float)x[k] - mean) * rstd, g = (float)gy[k] * (a.gamma ? a.gamma[k] : 1.0f);
+            const float d = rstd * fmaf(-h, c2, g - c1);
+            gx[k] = (T)(res ? d + (float)res[k] : d);
+        }
     }
 }
 
@@ -392,6 +398,9 @@ void launch_column_sums(const float* partial, int blocks, int64_t n, int64_t wid
     column_sums_kernel<<<(unsigned)((width + 31) / 32), 1024, 0, s>>>(partial, blocks, n, width, first, second);
 }
 
+// Workgroups for rows over 32 KB (also for tests).
+int64_t layer_norm_wide_blocks(int64_t rows) { return rows < 65536 ? rows : 65536; }
+
 size_t layer_norm_backward_workspace(const LayerNormBackward& a) {
     if (!a.grad_gamma && !a.grad_beta) return 0;
     size_t bytes = 0;
@@ -414,7 +423,7 @@ int launch_layer_norm_forward(const LayerNormForward& a, hipStream_t s) {
             const unsigned blocks = (unsigned)(want < 2048 ? want : 2048);
             forward_kernel<T, kLanes, decltype(pieces)::value><<<blocks, kThreads, 0, s>>>(a);
         });
-        if (!held) wide_forward_kernel<T><<<(unsigned)a.x.rows, kWide, 0, s>>>(a);
+        if (!held) wide_forward_kernel<T><<<(unsigned)layer_norm_wide_blocks(a.x.rows), kWide, 0, s>>>(a);
     });
     TGS_CHECK_LAUNCH();
     return TGS_OK;
@@ -442,7 +451,7 @@ int launch_layer_norm_backward(const LayerNormBackward& a, void* workspace, hipS
         if (held) return;
         // grad_x may take grad_y's place: its column sums come first
         if (sums) wide_columns_kernel<T><<<(unsigned)a.x.cols, 256, 0, s>>>(a);
-        if (a.grad_x.p && a.x.rows) wide_backward_kernel<T><<<(unsigned)a.x.rows, kWide, 0, s>>>(a);
+        if (a.grad_x.p && a.x.rows) wide_backward_kernel<T><<<(unsigned)layer_norm_wide_blocks(a.x.rows), kWide, 0, s>>>(a);
     });
     TGS_CHECK_LAUNCH();
     return TGS_OK;

@@ -195,6 +195,21 @@ __device__ __forceinline__ void store_sums(const f32x4 (&acc)[TI][TJ], int64_t i
                    [&](int64_t i, int64_t j, int n, float(&v)[8]) { store8(out + j * cols + i, n, v); });
 }
 
+// Rows of a launch at most. A launch of 2^32 threads or more loses what is above
+// without an error: 256 threads for 64 rows reached that at 2^30 rows.
+constexpr int64_t kLaunchRows = (int64_t)1 << 27;
+
+// The call's rows from `first` on, as many as one launch takes.
+template <class T>
+LinearForward rows_of(LinearForward a, int64_t first) {
+    for (Mat* m : {&a.x, &a.residual, &a.preact, &a.y}) {
+        if (!m->p) continue;
+        m->p = (T*)m->p + first * m->stride;
+        m->rows = std::min(m->rows - first, kLaunchRows);
+    }
+    return a;
+}
+
 // With `partial`, the float sums over the k of split blockIdx.y.
 template <class T, class S>
 __global__ void __launch_bounds__(S::kThreads) forward_kernel(LinearForward a, float* partial, int64_t depth, uint32_t ni,
@@ -525,8 +540,12 @@ int launch_linear_forward(const LinearForward& a, void* workspace, hipStream_t s
             float* partial = k.splits > 1 ? (float*)workspace : nullptr;
             by_shape(a.y.cols, a.y.rows, 1, is_deep<T>(a.x.cols), [&](auto shape) {
                 using S = decltype(shape);
-                const uint32_t ni = (uint32_t)ceil_div(a.y.cols, S::kI), nj = (uint32_t)ceil_div(a.y.rows, S::kJ);
-                forward_kernel<T, S><<<dim3(ni * nj, (unsigned)k.splits), S::kThreads, 0, s>>>(a, partial, k.depth, ni, nj);
+                for (int64_t first = 0; first < a.y.rows; first += kLaunchRows) {
+                    const LinearForward part = rows_of<T>(a, first);
+                    const uint32_t ni = (uint32_t)ceil_div(a.y.cols, S::kI), nj = (uint32_t)ceil_div(part.y.rows, S::kJ);
+                    forward_kernel<T, S>
+                        <<<dim3(ni * nj, (unsigned)k.splits), S::kThreads, 0, s>>>(part, partial, k.depth, ni, nj);
+                }
             });
             if (partial)
                 by_activation(a.activation, [&](auto act) {

@@ -513,7 +513,10 @@ MuonPlan plan_muon(MuonPart* parts, int count) {
     plan.parts_at = take((int64_t)sizeof(MuonPart) * count);
     plan.firsts_at = take((int64_t)sizeof(uint32_t) * 3 * count);
     plan.bytes = at;
-    plan.fits = patches < 0x7fffffff && plan.tiles[0] < 0x7fffffffu && plan.tiles[1] < 0x7fffffffu;
+    // a launch of 2^32 threads or more loses what is above without an error
+    const auto holds = [](int64_t workgroups, int64_t threads) { return workgroups * threads < ((int64_t)1 << 32); };
+    plan.fits = holds(patches, kPatchThreads) && holds(plan.tiles[0], plan.large[0] ? 512 : 256) &&
+                holds(plan.tiles[1], plan.large[1] ? 512 : 256);
     return plan;
 }
 
