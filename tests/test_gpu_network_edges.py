@@ -205,3 +205,60 @@ def test_layer_norm_more_wide_rows_than_workgroups(ops, dtype, n):
     want, bound = R.layer_norm_backward(y[:64], x[:64], None, mean[:64], rstd[:64], None, dtype)[0]
     R.check(gx[:64], want, bound, "gx")
     assert all(torch.equal(gx[at:at + 64], gx[:64][:rows - at]) for at in range(64, rows, 64))
+
+
+def test_relu_gradients_are_the_slopes(ops):
+    """The gradients against differences of the forward, every value far from the kink: the loss is a plane there, so
+    the step may be as wide as 2^-4 and leaves the forward's rounding (35 sums of size 20, 2^-24 each, over 2^-3)."""
+    rows, i, o = 5, 6, 7
+    x, w, c = normal(1, rows, i).cuda(), normal(2, o, i).cuda(), normal(4, rows, o).cuda()
+    b = (12.0 * (1 - 2 * (torch.arange(o) % 2)) + normal(3, o)).cuda()
+
+    def loss():
+        return float((ops.linear(x, w, b, activation="relu").double() * c.double()).sum())
+
+    _, z = ops.linear(x, w, b, activation="relu", keep_preact=True)
+    h = 2.0 ** -4
+    assert float(z.abs().min()) > 2 * h * max(1.0, float(x.abs().max()), float(w.abs().max()))
+    assert bool((z > 0).any()) and bool((z < 0).any())
+    for t, g in zip((x, w, b), ops.linear_backward(c, x, w, preact=z, activation="relu")):
+        for at in range(t.numel()):
+            flat, want = t.view(-1), float(g.reshape(-1)[at])
+            keep = float(flat[at])
+            flat[at] = keep + h
+            up = loss()
+            flat[at] = keep - h
+            down = loss()
+            flat[at] = keep
+            assert abs((up - down) / (2 * h) - want) <= 1e-3 * (1 + abs(want)), (tuple(t.shape), at)
+
+
+@pytest.mark.parametrize("shape", [(64, 64), (128, 300), (200, 129), (257, 255), (520, 520), (40, 1030), (700, 130),
+                                   (1024, 1024), (1100, 2100)], ids=str)
+@pytest.mark.parametrize("low_rank", [False, True])
+def test_muon_is_as_near_as_floats(hip, shape, low_rank):
+    """The update alone (no weights, rate 1) against 64 bits, beside the same formula in float products: operands of 22
+    bits are four times as coarse as those of 24, and sums in another order are allowed twice the float's error. A
+    product without one of its low halves is off some hundred times as much."""
+    from tinygs_amd.optim import Muon
+    r, c = shape
+    g = normal(1, r, c) * (3e-3 if low_rank else 1.0)
+    if low_rank:
+        g = g + 2e-3 * normal(2, r, 1) * normal(3, 1, c)
+    w = torch.zeros(r, c, device="cuda")
+    opt = Muon([w], [g.cuda()])
+    opt.set_params({"lr": 1.0, "momentum": 0.0, "weight_decay": 0.0, "nesterov": 0})
+    opt.step(1.0)
+    got = -w.double().cpu() / max(1.0, r / c) ** 0.5
+
+    def update(dtype):
+        x = (g.double() / g.double().norm()).to(dtype)
+        x = x.t() if r > c else x
+        for _ in range(5):
+            a = x @ x.t()
+            x = 3.4445 * x + (-4.7750 * a + 2.0315 * (a @ a)) @ x
+        return (x.t() if r > c else x).double()
+
+    want = update(torch.float64)
+    plain, off = float((update(torch.float32) - want).norm()), float((got - want).norm())
+    assert off <= 8 * plain, (off / float(want.norm()), plain / float(want.norm()))
