@@ -181,6 +181,26 @@ def test_linear_many_short_rows(ops, i, o, more, dtype):
     assert bool(torch.isfinite(y).all())
 
 
+# a narrow layer with many more outputs than inputs: several workgroups share the rows
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(33001, 84, 2001), (20003, 128, 4096), (70003, 30, 1030)], ids=str)
+def test_linear_many_rows_and_columns(ops, shape, dtype):
+    rows, i, o = shape
+    if dtype == torch.float32:
+        o = o // 2
+    print(f"[linear] {rows} x {i} -> {o} {dtype}", flush=True)
+    g = torch.Generator("cuda").manual_seed(5)
+    x = torch.randn(rows, i, generator=g, device="cuda").to(dtype)
+    r = torch.randn(rows, o, generator=g, device="cuda").to(dtype)
+    w, b = (normal(11, o, i) * i ** -0.5).to(dtype).cuda(), normal(21, o).cuda()
+    y, z = ops.linear(x, w, b, activation="gelu", residual=r, keep_preact=True)
+    at = torch.cat([torch.arange(100), torch.arange(rows // 2, rows // 2 + 100), torch.arange(rows - 100, rows)]).cuda()
+    wy, by, wz, bz = R.linear(x[at], w, b, "gelu", r[at], dtype)
+    R.check(y[at], wy, by, "y")
+    R.check(z[at], wz, bz, "z")
+    assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(z).all())
+
+
 def test_linear_more_rows_than_a_launch_of_tiles(ops):
     """2^30 rows and some, of one column: 256 threads for 64 rows would be 2^32 threads."""
     rows = (1 << 30) + 100

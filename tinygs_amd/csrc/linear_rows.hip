@@ -288,23 +288,29 @@ int64_t linear_rows_reach(int64_t left, int64_t cols, int64_t stride, int64_t si
 
 // Once a call moves more than the card's last cache holds of it, w in registers
 // and few, long waits pay; below, tiles fill the card sooner and their second
-// reads of x are from caches. Here and with tiles, halves: 262144 x 128 -> 256
-// 42 and 52 us, with gelu, preact and residual 97 and 134; 1e6 x 256 -> 256 so
+// reads of x are from caches. Here and with tiles, us, halves: 262144 x 128 -> 256
+// 42 and 52, with gelu, preact and residual 97 and 134; 1e6 x 256 -> 256 so
 // 384 and 507; 262144 x 256 -> 128 (201 MB) 44 and 44; 65536 x 128 -> 128 (34 MB)
-// 13 and 9. Half of a workgroup's waves have no columns below 128, so those
-// take more: 262144 x 256 -> 64 (168 MB) 40 and 29, 1e6 x 84 -> 64 (296 MB) 77 and
-// 99. Floats multiply six times as long, w's planes fill the registers, and
-// the products bound narrow outputs: 1e6 x 128 -> 64 197 and 180, 262144 x 84
-// -> 256 (356 MB) 111 and 125, 262144 x 128 -> 256 (402 MB) 142 and 138, with gelu,
-// preact and residual 202 and 232.
+// 13 and 9. Floats: 182044 x 32 -> 256 (200 MB) 51 and 49, 154202 x 84 -> 256 70
+// and 83, with gelu, preact and residual 79996 x 84 -> 256 (260 MB) 60 and 95,
+// 76068 x 128 -> 256 67 and 98; the worst, a few in a hundred: 425984 x 32 -> 128
+// (260 MB) 63 and 64 but 557056 (340 MB) 90 and 83, 460800 x 128 -> 128 132 and 128.
+// Further columns are further workgroups over the same rows: halves 200000 x 128
+// -> 1280 179 and 214, -> 4096 413 and 622, 65536 x 256 -> 1280 71 and 71; floats
+// 100000 x 128 -> 1024 198 and 206. Past sixteen rows' bytes of them nothing was
+// measured, and tiles take it.
+// Half of a workgroup's waves have no columns below 128, so those take more:
+// halves 262144 x 256 -> 64 (168 MB) 40 and 29, 1e6 x 84 -> 64 (296 MB) 77 and
+// 99. Floats multiply six times as long, and the products bound narrow outputs:
+// 1e6 x 128 -> 64 197 and 180.
 bool linear_forward_by_rows(const LinearForward& a) {
     const bool floats = a.dtype == TGS_DTYPE_FLOAT32;
     const int64_t size = floats ? 4 : 2, most = 512 / size;
-    if (a.x.cols > most || a.y.cols > 4 * most) return false;
+    if (a.x.cols > most || a.y.cols > 16 * most) return false;
     const int64_t arrays = 1 + (a.preact.p ? 1 : 0) + (a.residual.p ? 1 : 0);
     const int64_t megabytes = (a.y.rows * (a.x.cols + arrays * a.y.cols) * size) >> 20;
     if (a.y.cols < 128) return !floats && megabytes >= 256;
-    return megabytes >= (floats ? 384 : 130);
+    return megabytes >= 130;
 }
 
 void launch_linear_rows(const LinearForward& a, hipStream_t s) {
