@@ -552,8 +552,9 @@ int tgs_layer_norm_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_
  *   iterations times: A = X X^T, X <- a X + (b A + c A^2) X
  *   W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) X
  * with a, b, c = 3.4445, -4.7750, 2.0315, which bring the singular values of X
- * near one. The products are of matrices held to 22 bits (two halves each), with
- * float sums; the sum of squares is held in 64 bits.
+ * near one. The products are of matrices held to 22 bits (two halves each, 2^-37
+ * absolutely for elements below 2^-14), with float sums; the sum of squares is
+ * held in 64 bits.
  * lr is params.lr times the learning rate of tgs_muon_set_lr (1 at creation). */
 typedef struct tgs_muon_params {
     float lr;             /* 0.02 at creation */

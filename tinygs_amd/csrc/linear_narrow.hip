@@ -10,8 +10,8 @@
 // (128 x 64 a wave for halves); a block's dz and x take 16 KB each. The next
 // block's dy, z and x are on their way into registers while a block is
 // multiplied. The workgroups' sums are joined by a second kernel in a fixed
-// order. 1e6 x 256 -> 256 halves with gelu: 2.05 GB in 500 us (4.1 TB/s) and the
-// join of 256 sums 15 us; 50021 x 84 -> 128 floats 31 and 6 us.
+// order. 1e6 x 256 -> 256 halves with gelu: 2.05 GB in 505 us (4.1 TB/s) and the
+// join of 256 sums 17 us; 50021 x 84 -> 128 floats 31 and 6 us.
 #include "narrow_rows.h"
 
 namespace tgs {
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
                 for (int e = 0; e < V; ++e) {
                     const float d = (float)dy[h][e] * activate_slope<ACT>((float)z[h][e]);
                     sum[e] += d;
-                    dy[h][e] = (T)d;
+                    dy[h][e] = (T)d;   // halves: one operand of the products, and all that LDS has room for beside w
                 }
             } else {
 #pragma unroll

@@ -1,25 +1,29 @@
-// Muon's update of a network's matrices: momentum, the Newton-Schulz steps on
-// the normalised update, the weights. Every phase is one launch over all
-// matrices.
+// Muon's update of a network's matrices (K. Jordan and others, "Muon: an
+// optimizer for hidden layers in neural networks", 2024: the coefficients and
+// the factor for tall matrices; the momentum is averaged here): momentum, the
+// Newton-Schulz steps on the normalised update, the weights. Every phase is one
+// launch over all matrices.
 //
 // X is kept with its shorter side as rows (the transpose of a tall matrix), so
 // that X X^T is the smaller of the two Gram matrices. X, the Gram matrix G and
 // the polynomial P = b G + c G^2 are held as two halves each, hi + lo with
 // lo = half(v - hi), of the value times 2^12: 22 bits of every element down to
-// 2^-25 of one, in the range of halves (|X|, |G| < 2, |P| < 3: the singular
-// values of X stay below 1.3). A product is then three of halves, hi hi + hi lo
-// + lo hi with float sums (lo lo is 2^-22 of it), at the matrix cores' half
-// rate. Halves alone (11 bits) would leave the update's small singular
-// directions, which the steps lift up to 485 times, wrong by several percent.
+// 2^-14 of one and 2^-37 absolutely below, where lo is subnormal, in the range of
+// halves (|X|, |G| < 2, |P| < 3: the singular values of X stay below 1.3). A
+// product is then three of halves, hi hi + hi lo + lo hi with float sums (lo lo
+// is 2^-22 of it), at the matrix cores' half rate: the update is off by 1e-6 to
+// 2e-6 of itself, as the same formula in float products is. Halves alone (11
+// bits) would leave the update's small singular directions, which the steps lift
+// up to 485 times, wrong by several percent.
 // A row holds 32 hi and then their 32 lo in turn, so that a step of 32 of k is
 // one cache line of it.
 //
 // Four of 1024 x 4096: Gram 97 us, square 33, update 130, which is 0.61, 0.45 and
 // 0.80 PFLOP/s of halves where large products reach 1.4. Gram's and the square's
 // 144 tiles are on 256 compute units; otherwise the tiles' turns of loads, LDS
-// reads and matrix instructions bound them. A small network's launches (256 x 256: 7 to 8 us) are
-// bound by their chains of waits. The element passes move 12 bytes an element in
-// 39 to 51 us (17 M elements, 4 to 5.2 TB/s).
+// reads and matrix instructions bound them. A small network's launches (256 x
+// 256: 7 to 9 us) are bound by their chains of waits. The element passes move 12
+// bytes an element in 39 to 51 us (17 M elements, 4 to 5.2 TB/s).
 //
 // G and P are symmetric: only the tiles on and below the diagonal are made, and
 // each is stored a second time transposed, through LDS.
