@@ -282,3 +282,23 @@ def test_muon_is_as_near_as_floats(hip, shape, low_rank):
     want = update(torch.float64)
     plain, off = float((update(torch.float32) - want).norm()), float((got - want).norm())
     assert off <= 8 * plain, (off / float(want.norm()), plain / float(want.norm()))
+
+
+def test_a_failed_allocation_fails_its_own_call_only(ops):
+    """Muon's workspace for matrices that no card holds (their addresses are never read): that step fails, and the next
+    call of another operator does not."""
+    import ctypes as C
+    from tinygs_amd import _lib
+    lib, n, count = _lib.load(), 1 << 14, 200
+
+    def array(slot):
+        return (_lib.tgs_matrix * count)(*[_lib.tgs_matrix((1 << 44) * (slot + 1) + (4 * n * n) * k, n, n, n,
+                                                           _lib.TGS_DTYPE_FLOAT32) for k in range(count)])
+    h = C.c_void_p()
+    assert lib.tgs_muon_create(array(0), array(1), array(2), None, count, C.byref(h)) == 0
+    print("[muon] a workspace of a terabyte", flush=True)
+    assert lib.tgs_muon_step(h, 1.0, None) == _lib.TGS_ERR_HIP
+    x, w = normal(1, 40, 30), normal(2, 20, 30)
+    y = ops.linear(x.cuda(), w.cuda())
+    R.check(y, *R.linear(x, w, None, "none", None, torch.float32)[:2], "y")
+    assert lib.tgs_muon_destroy(h) == 0

@@ -14,12 +14,17 @@ int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 
 }  // namespace tgs
 
+// The error is the caller's by its return: it does not stay behind as the
+// runtime's last error, which the next launch, here or elsewhere in the program,
+// would take for its own.
 #define TGS_HIP(call)                                                                                        \
     do {                                                                                                     \
         hipError_t e_ = (call);                                                                              \
-        if (e_ != hipSuccess)                                                                                \
+        if (e_ != hipSuccess) {                                                                              \
+            (void)hipGetLastError();                                                                         \
             return ::tgs::fail(TGS_ERR_HIP, "%s failed at %s:%d: %s", #call, __FILE__, __LINE__,            \
                                hipGetErrorString(e_));                                                       \
+        }                                                                                                    \
     } while (0)
 
 #define TGS_CHECK_LAUNCH()                                                                                   \
