@@ -302,3 +302,16 @@ def test_a_failed_allocation_fails_its_own_call_only(ops):
     y = ops.linear(x.cuda(), w.cuda())
     R.check(y, *R.linear(x, w, None, "none", None, torch.float32)[:2], "y")
     assert lib.tgs_muon_destroy(h) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_linear_to_a_single_row_between_columns(ops, dtype):
+    """One row of a buffer's right half from the matrix in its left half: they share no element."""
+    buf = normal(1, 12, 48).to(dtype).cuda()
+    w, x = buf[:, :24], normal(2, 1, 24).to(dtype).cuda()
+    y = buf[5:6, 30:42]
+    keep = buf.clone()
+    ops.linear(x, w, out=y)
+    R.check(y, *R.linear(x, keep[:, :24], None, "none", None, dtype)[:2], "y")
+    buf[5:6, 30:42] = keep[5:6, 30:42]
+    assert torch.equal(buf, keep)

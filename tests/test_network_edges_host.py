@@ -71,3 +71,43 @@ def test_muon_refuses_more_than_a_launch_holds(count, fits):
         assert rc == 0 and lib.tgs_muon_destroy(h) == 0
     else:
         assert rc == _lib.TGS_ERR_INVALID and "too large for one step" in lib.tgs_last_error().decode()
+
+
+BASE = 1 << 20   # addresses that nothing reads: every call below is refused
+
+
+def refusal(x, w, y, residual=None):
+    """What a linear forward is refused for whose preact is y's own matrix: that, where nothing before it is."""
+    lib, h = _lib.load(), C.c_void_p()
+    assert lib.tgs_network_create(C.byref(h)) == 0
+    try:
+        assert lib.tgs_linear_forward(h, x, w, None, 0, residual, y, y, None) == _lib.TGS_ERR_INVALID
+        return lib.tgs_last_error().decode()
+    finally:
+        lib.tgs_network_destroy(h)
+
+
+def test_a_single_row_between_anothers_columns():
+    """One row of a buffer's column range beside the rows of another range of it (16 floats a row): a single row's own
+    stride says nothing, as callers that hold one row pass its length."""
+    def mat(row, col, rows, cols, stride=16):
+        return _lib.tgs_matrix(BASE + 4 * (16 * row + col), rows, cols, stride, _lib.TGS_DTYPE_FLOAT32)
+    x = _lib.tgs_matrix(BASE * 4, 1, 8, 8, _lib.TGS_DTYPE_FLOAT32)
+    for stride in (6, 7, 16):
+        for row in (0, 3, 5):
+            w = mat(0, 0, 6, 8)
+            assert refusal(x, w, mat(row, 8, 1, 6, stride)) == "preact overlaps y"
+            assert refusal(x, w, mat(row, 10, 1, 6, stride)) == "preact overlaps y"
+            assert refusal(x, w, mat(row, 7, 1, 6, stride)) == "y overlaps w"
+            assert refusal(x, mat(0, 8, 6, 8), mat(row, 2, 1, 6, stride)) == "preact overlaps y"
+            assert refusal(x, mat(0, 8, 6, 8), mat(row, 3, 1, 6, stride)) == ("y overlaps w" if row < 6 else "preact overlaps y")
+    # past the last row, and a row longer than the distance between rows
+    assert refusal(x, mat(0, 0, 6, 8), mat(6, 0, 1, 6, 6)) == "preact overlaps y"
+    long = _lib.tgs_matrix(BASE + 4 * 8, 1, 20, 20, _lib.TGS_DTYPE_FLOAT32)
+    wide = _lib.tgs_matrix(BASE, 20, 8, 16, _lib.TGS_DTYPE_FLOAT32)
+    assert refusal(x, wide, long) == "y overlaps w"
+    # over the residual: its own matrix, whatever the two strides of the single row say
+    apart = _lib.tgs_matrix(BASE * 8, 6, 8, 8, _lib.TGS_DTYPE_FLOAT32)
+    y = mat(3, 8, 1, 6, 6)
+    assert refusal(x, apart, y, mat(3, 8, 1, 6, 16)) == "preact overlaps residual"
+    assert refusal(x, apart, y, mat(3, 9, 1, 6, 16)) == "y overlaps residual"

@@ -61,7 +61,8 @@ int check_shape(const tgs_matrix* m, const char* name, int64_t rows, int64_t col
 }
 
 // Whether two matrices share elements. Column ranges of one buffer (of the
-// same stride and element size) interleave without sharing any.
+// same stride in bytes) interleave without sharing any; a single row, whose own
+// stride says nothing, lies in the other's.
 bool overlap(const tgs_matrix& a, const tgs_matrix& b) {
     if (!a.rows || !b.rows) return false;
     const int64_t sa = element_size(a.dtype), sb = element_size(b.dtype);
@@ -69,15 +70,16 @@ bool overlap(const tgs_matrix& a, const tgs_matrix& b) {
     const uintptr_t a1 = a0 + (uintptr_t)(((a.rows - 1) * a.stride + a.cols) * sa);
     const uintptr_t b1 = b0 + (uintptr_t)(((b.rows - 1) * b.stride + b.cols) * sb);
     if (a1 <= b0 || b1 <= a0) return false;
-    if (a.stride * sa != b.stride * sb) return true;
-    const int64_t pitch = a.stride * sa;
+    if (a.rows == 1 && b.rows == 1) return true;
+    const int64_t pitch = a.rows == 1 ? b.stride * sb : a.stride * sa;
+    if (a.rows > 1 && b.rows > 1 && pitch != b.stride * sb) return true;
     const int64_t d = (int64_t)((b0 >= a0 ? b0 - a0 : a0 - b0) % (uintptr_t)pitch);
     const int64_t from = b0 >= a0 ? d : (pitch - d) % pitch;   // b's first column after a's, modulo a row
     return from < a.cols * sa || from + b.cols * sb > pitch;
 }
 
 bool same_place(const tgs_matrix& a, const tgs_matrix& b) {
-    return a.data == b.data && a.stride == b.stride && a.dtype == b.dtype;
+    return a.data == b.data && (a.stride == b.stride || a.rows <= 1) && a.dtype == b.dtype;
 }
 
 int check_apart(const tgs_matrix* out, const char* out_name, const tgs_matrix* in, const char* in_name) {
