@@ -201,6 +201,36 @@ def test_linear_many_rows_and_columns(ops, shape, dtype):
     assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(z).all())
 
 
+# many rows of few columns, in and out together at most 256 bytes (floats: half the columns named here)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(300007, 32, 32), (300001, 64, 64), (400000, 3, 64), (300003, 59, 3), (350001, 1, 1),
+                                   (300008, 100, 27)], ids=str)
+@pytest.mark.parametrize("name,pad", [("none", 0), ("gelu", 3)])
+def test_linear_backward_many_rows_of_few_columns(ops, shape, name, pad, dtype):
+    rows, i, o = shape
+    if dtype == torch.float32:
+        i, o = (i + 1) // 2, (o + 1) // 2
+    print(f"[linear_backward] {rows} x {i} -> {o} {dtype} {name} pad {pad}", flush=True)
+
+    def padded(seed, cols, scale):
+        full = torch.full((rows, cols + pad), NAN, dtype=dtype, device="cuda")
+        full[:, :cols] = (scale * torch.randn(rows, cols, generator=torch.Generator("cuda").manual_seed(seed), device="cuda"))
+        return full[:, :cols]
+
+    x, gy, z = padded(1, i, 1.0), padded(2, o, 0.1), padded(3, o, 2.0) if name != "none" else None
+    w = (normal(4, o, i) * i ** -0.5).to(dtype).cuda()
+    full = torch.full((rows, i + pad), -7.0, dtype=dtype, device="cuda")
+    got = ops.linear_backward(gy, x, w, preact=z, activation=name, grad_x=full[:, :i])
+    for t, (want, bound), what in zip(got, R.linear_backward(gy, x, w, z, name, dtype), ("gx", "gw", "gb")):
+        R.check(t, want, bound, what)
+    assert bool((full[:, i:] == -7.0).all())
+    again = ops.linear_backward(gy, x, w, preact=z, activation=name)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    for n in range(3):
+        part = ops.linear_backward(gy, x, w, preact=z, activation=name, need_x=n == 0, need_weight=n == 1, need_bias=n == 2)
+        assert torch.equal(part[n], got[n])
+
+
 def test_linear_more_rows_than_a_launch_of_tiles(ops):
     """2^30 rows and some, of one column: 256 threads for 64 rows would be 2^32 threads."""
     rows = (1 << 30) + 100

@@ -346,17 +346,28 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(LinearBackward a, fl
 
 }  // namespace
 
-// Against a slope pass and two tile products, with SiLU: 1e6 x 256 -> 256 halves
-// 504 and 778 us, 1e6 x 128 -> 64 284 and 262 (the worst of the halves), 2000 x
-// 72 -> 72 20 and 28; 1e6 x 128 -> 64 floats 401 and 539, 2000 rows 19 and 43.
+// Against a slope pass and two tile products, us, with SiLU: 1e6 x 256 -> 256
+// halves 510 and 779, 1e6 x 128 -> 128 289 and 366, 100000 rows 44 and 55, 2000 x
+// 72 -> 72 16 and 22, 1e6 x 128 -> 64 283 and 260; floats 1e6 x 128 -> 64 400 and
+// 550, 2000 rows 18 and 43.
+// A block of 32 rows takes its 2 us however few columns it has, so that many
+// rows of few (in and out together up to 256 bytes) are tiles' sooner: halves
+// 1e6 x 32 -> 32 249 and 113, 64 -> 64 254 and 189, 3 -> 64 373 and 163, 59 -> 3
+// 343 and 148; 200000 rows 59 and 42, 62 and 51, 89 and 51, 84 and 51, without an
+// activation at worst 61 and 67 (63 -> 59); 100000 rows 36 and 32, 37 and 37, 54
+// and 35, 53 and 40, at worst 36 and 43 (16 -> 112). Floats, whose tiles are six
+// products: 1e6 x 32 -> 32 265 and 206, 2 -> 32 333 and 207, 8 -> 56 265 and 282;
+// 400000 rows 113 and 99, 141 and 102, 113 and 129; 200000 rows 63 and 69, 78 and
+// 69, 63 and 84.
 // Ragged halves of more than 128 columns take their last rows of w element by
 // element, which fewer rows do not pay back: 250 -> 256, 2000 rows 50 and 28 us,
 // 20000 62 and 41, 200000 178 and 216.
 bool linear_backward_is_narrow(const LinearBackward& a) {
-    const int64_t most = 512 / (a.dtype == TGS_DTYPE_FLOAT32 ? 4 : 2);
-    const bool ragged = a.x.cols % 8 || a.grad_y.cols % 8;
-    if (a.dtype != TGS_DTYPE_FLOAT32 && ragged && a.x.cols > 128 && a.grad_y.cols > 128 && a.grad_y.rows < 65536) return false;
-    return a.x.cols <= most && a.grad_y.cols <= most && a.grad_y.rows > 0 && a.grad_y.rows < ((int64_t)1 << 35);
+    const bool floats = a.dtype == TGS_DTYPE_FLOAT32;
+    const int64_t size = floats ? 4 : 2, most = 512 / size, in = a.x.cols, out = a.grad_y.cols, rows = a.grad_y.rows;
+    if (!floats && (in % 8 || out % 8) && in > 128 && out > 128 && rows < 65536) return false;
+    if ((in + out) * size <= 256 && rows >= (floats ? 300000 : 200000)) return false;
+    return in <= most && out <= most && rows > 0;
 }
 
 int narrow_backward_splits(const LinearBackward& a) {
