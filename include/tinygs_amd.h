@@ -545,6 +545,86 @@ int tgs_layer_norm_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_
                             const float* mean, const float* rstd, const tgs_matrix* residual_grad,
                             const tgs_matrix* grad_x, float* grad_gamma, float* grad_beta, void* stream);
 
+/* ---- attention of the network's rows to an encoder's states (tokens of an
+ * image, a text, a scene), whose number is their own, and the norms of its
+ * queries and keys.
+ * A row holds its heads one after the other: head h is columns h d .. h d + d - 1
+ * (d: the width of a head). The rows of a batch's elements follow each other,
+ * as many for each. */
+typedef struct tgs_attention {
+    int64_t batch;         /* elements: q has batch x queries rows, k and v batch x states */
+    int32_t heads;         /* of the queries; d = q's columns / heads, 1 to 128 */
+    int32_t kv_heads;      /* of the states; heads is a multiple: head h reads h / (heads / kv_heads) */
+    float scale;           /* of the scores, not negative; 1 / sqrt(d) as a rule */
+    const uint8_t* mask;   /* [batch, states], 0: the state does not exist; NULL: all exist */
+    int64_t mask_stride;   /* bytes from an element's mask to the next one's; 0: one for all */
+} tgs_attention;
+/* For each row and head: s = scale q k^T over the states that exist,
+ * lse = log sum exp s, out = sum exp(s - lse) v. Where no state exists, and
+ * where every score is -infinity, out is 0 and lse -infinity. States that do not
+ * exist may hold anything. q [batch x queries, heads d], k and v
+ * [batch x states, kv_heads d], out like q; lse may be NULL: that of row r and
+ * head h is at lse[r lse_row_step + h lse_head_step], in rows of heads (steps of
+ * at least heads lse_head_step and 1 or more) or heads of rows. Weights of 16-bit matrices are rounded to their dtype ahead of the
+ * product with v; their sum is not. No output may overlap an input. */
+int tgs_attention_forward(tgs_network* n, const tgs_matrix* q, const tgs_matrix* k, const tgs_matrix* v,
+                          const tgs_attention* a, const tgs_matrix* out, float* lse, int64_t lse_row_step,
+                          int64_t lse_head_step, void* stream);
+/* The gradients of tgs_attention_forward from its out and lse: with
+ * p = exp(s - lse) and delta = the sum of grad_out out over a head,
+ * grad_v = p^T grad_out, ds = p (grad_out v^T - delta), grad_q = scale ds k,
+ * grad_k = scale ds^T q; grad_k and grad_v are summed over the heads that share
+ * them. Assigned, or left out when NULL; zeros for states that do not exist. Sums in
+ * an order that depends on the sizes alone. */
+int tgs_attention_backward(tgs_network* n, const tgs_matrix* grad_out, const tgs_matrix* q, const tgs_matrix* k,
+                           const tgs_matrix* v, const tgs_matrix* out, const float* lse, int64_t lse_row_step,
+                           int64_t lse_head_step, const tgs_attention* a, const tgs_matrix* grad_q,
+                           const tgs_matrix* grad_k, const tgs_matrix* grad_v, void* stream);
+/* The turning of a head norm: pair (2 i, 2 i + 1) of every head is turned by
+ * the angle sum over axes of positions[row, axis] frequencies[i, axis], formed
+ * in 64 bits. Both are float32; frequencies has at most d / 2 rows: the columns
+ * past its pairs are not turned. */
+typedef struct tgs_turn {
+    tgs_matrix positions;     /* [rows, axes], axes 1 to 4 */
+    tgs_matrix frequencies;   /* [pairs, axes] */
+} tgs_turn;
+/* For each row and head (of d columns, 1 to 256): h = x / sqrt(mean(x^2) +
+ * epsilon), u = h gamma (gamma [d], shared by the heads, may be NULL: one),
+ * y = u turned (turn may be NULL: y = u). y may be x's own matrix. */
+int tgs_head_norm_forward(tgs_network* n, const tgs_matrix* x, int32_t heads, const float* gamma, const tgs_turn* turn,
+                          float epsilon, const tgs_matrix* y, void* stream);
+/* Its gradients from x: with g = grad_y turned back and r = 1 / sqrt(mean(x^2)
+ * + epsilon), grad_gamma = the sum of g h over rows and heads, grad_x =
+ * r (g gamma - h mean(g gamma h)). Assigned, or left out when NULL. grad_x may
+ * be grad_y's own matrix. Sums in a fixed order. */
+int tgs_head_norm_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_matrix* x, int32_t heads,
+                           const float* gamma, const tgs_turn* turn, float epsilon, const tgs_matrix* grad_x,
+                           float* grad_gamma, void* stream);
+
+/* ---- the norm of many gradients together, and clipping:
+ *   norm = scale sqrt(sum of squares of all elements)
+ *   g <- g f, f = scale min(1, max_norm / (norm + epsilon))
+ * The squares and their sum are held in 64 bits, f in 32. scale undoes a scaled
+ * loss. Where max_norm is infinite f is scale. A norm that is NaN makes every
+ * gradient NaN, an infinite one makes them 0 or NaN, as the formula does: check
+ * the norm. */
+typedef struct tgs_gradient_clip tgs_gradient_clip;
+/* grads: count matrices, each of its own dtype and shape (a packed tensor of n
+ * elements is n rows of one), no two of them overlapping; empty ones are
+ * allowed. clipped: NULL (the gradients themselves are clipped), or matrices of
+ * the same shapes that receive the clipped gradients rounded to their own
+ * dtypes while grads stay as they are. The pointers are kept. */
+int tgs_gradient_clip_create(const tgs_matrix* grads, const tgs_matrix* clipped, int32_t count,
+                             tgs_gradient_clip** out);
+int tgs_gradient_clip_destroy(tgs_gradient_clip* c);
+/* Other matrices; any count, shapes and dtypes. */
+int tgs_gradient_clip_set_matrices(tgs_gradient_clip* c, const tgs_matrix* grads, const tgs_matrix* clipped,
+                                   int32_t count);
+/* norm: a device float, or NULL. Where f is 1, gradients clipped in place are
+ * not written. The first run, and the first after other matrices, place the
+ * matrices' table on the device and wait for it: capture only later ones. */
+int tgs_gradient_clip_run(tgs_gradient_clip* c, float max_norm, float scale, float epsilon, float* norm, void* stream);
+
 /* ---- Muon: the optimiser of the network's matrices. A step, for each matrix
  * W [rows, cols] with momentum M and gradient G (s = scale):
  *   M <- mu M + (1 - mu) s G;  U = (1 - mu) s G + mu M (nesterov), or M

@@ -11,7 +11,9 @@ mirrors tinygs's plugin interfaces on top of it:
 
 and adds the operators of a network whose outputs are Gaussian attributes:
 
-  LayerOps, AttributeNetwork                        (linear layers, layer norm)
+  LayerOps, AttributeNetwork                        (linear layers, layer norm,
+                                                     attention, head norms)
+  GradientClip                                      (norm of all gradients)
   create_optimizer("muon", matrices, grads, copies)
 
 Importing the package does not load the library; the first rasterizer /
@@ -37,7 +39,7 @@ def __getattr__(name):
     if name in ("LayerOps", "AttributeNetwork"):
         from . import network
         return getattr(network, name)
-    if name in ("SimpleAdam", "Muon", "OptimizerBase", "create_optimizer"):
+    if name in ("SimpleAdam", "Muon", "GradientClip", "OptimizerBase", "create_optimizer"):
         from . import optim
         return getattr(optim, name)
     if name in ("GPUGaussian3d", "Image", "GPUBatchInput", "GPUBatchOutput", "RasterizeContext", "LossContext",

@@ -96,6 +96,15 @@ class tgs_muon_params(C.Structure):
                 ("nesterov", C.c_int32), ("iterations", C.c_int32)]
 
 
+class tgs_attention(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("scale", C.c_float),
+                ("mask", C.c_void_p), ("mask_stride", C.c_int64)]
+
+
+class tgs_turn(C.Structure):
+    _fields_ = [("positions", tgs_matrix), ("frequencies", tgs_matrix)]
+
+
 P = C.c_void_p
 PP = C.POINTER(C.c_void_p)
 MP = C.POINTER(tgs_matrix)
@@ -167,6 +176,15 @@ SIGNATURES = {
     "tgs_linear_backward": ([P, MP, MP, MP, MP, C.c_int32, MP, MP, P, P], C.c_int),
     "tgs_layer_norm_forward": ([P, MP, P, P, C.c_float, MP, P, P, P], C.c_int),
     "tgs_layer_norm_backward": ([P, MP, MP, P, P, P, MP, MP, P, P, P], C.c_int),
+    "tgs_attention_forward": ([P, MP, MP, MP, C.POINTER(tgs_attention), MP, P, C.c_int64, C.c_int64, P], C.c_int),
+    "tgs_attention_backward": ([P, MP, MP, MP, MP, MP, P, C.c_int64, C.c_int64, C.POINTER(tgs_attention), MP, MP, MP,
+                                P], C.c_int),
+    "tgs_head_norm_forward": ([P, MP, C.c_int32, P, C.POINTER(tgs_turn), C.c_float, MP, P], C.c_int),
+    "tgs_head_norm_backward": ([P, MP, MP, C.c_int32, P, C.POINTER(tgs_turn), C.c_float, MP, P, P], C.c_int),
+    "tgs_gradient_clip_create": ([MP, MP, C.c_int32, PP], C.c_int),
+    "tgs_gradient_clip_destroy": ([P], C.c_int),
+    "tgs_gradient_clip_set_matrices": ([P, MP, MP, C.c_int32], C.c_int),
+    "tgs_gradient_clip_run": ([P, C.c_float, C.c_float, C.c_float, P, P], C.c_int),
     "tgs_muon_create": ([MP, MP, MP, MP, C.c_int32, PP], C.c_int),
     "tgs_muon_destroy": ([P], C.c_int),
     "tgs_muon_set_matrices": ([P, MP, MP, MP, MP, C.c_int32], C.c_int),

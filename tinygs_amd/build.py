@@ -19,7 +19,9 @@ OUT_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libtinygs_amd.so")
 SOURCES = ["preprocess.hip", "binning.hip", "blend_forward.hip", "blend_backward.hip", "fgs16.hip",
            "preprocess_backward.hip", "loss.hip", "adam.hip", "strategy.hip", "morton.hip", "formats.hip",
-           "linear.hip", "linear_few.hip", "linear_rows.hip", "linear_narrow.hip", "layer_norm.hip", "muon.hip", "network.hip", "selftest.hip", "capi.hip"]
+           "linear.hip", "linear_few.hip", "linear_rows.hip", "linear_narrow.hip", "layer_norm.hip", "muon.hip",
+           "attention.hip", "attention_backward.hip", "head_norm.hip", "gradient_clip.hip", "network.hip", "selftest.hip",
+           "capi.hip"]
 ARCH = os.environ.get("TGS_OFFLOAD_ARCH", "gfx950")
 
 COMMON_FLAGS = [

@@ -1,5 +1,5 @@
 // What the attribute network's operators share: element types, activations,
-// matrix views and the launchers of linear.hip, layer_norm.hip and muon.hip.
+// matrix views and the operators' launchers.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -146,6 +146,64 @@ void launch_column_sums(const float* partial, int blocks, int64_t n, int64_t wid
                         hipStream_t s);
 int launch_layer_norm_forward(const LayerNormForward& a, hipStream_t s);
 int launch_layer_norm_backward(const LayerNormBackward& a, void* workspace, hipStream_t s);
+
+// ---- attention.hip, attention_backward.hip: matrices of batch x queries and
+// batch x states rows
+struct Attention {
+    Mat q, k, v, out;
+    float* lse;            // may be NULL; of row r and head h at r row_step + h head_step
+    int64_t lse_row_step, lse_head_step;
+    const uint8_t* mask;   // may be NULL
+    int64_t mask_stride;
+    int64_t batch, queries, states;
+    int heads, kv_heads, head;   // head: the width of one
+    float scale;
+    int dtype;
+};
+struct AttentionBackward {
+    Attention a;                           // out is read; lse is not NULL
+    Mat grad_out, grad_q, grad_k, grad_v;  // grad_q.p .. grad_v.p may be NULL
+};
+size_t attention_workspace(const Attention& a);
+int launch_attention(const Attention& a, void* workspace, hipStream_t s);
+size_t attention_backward_workspace(const AttentionBackward& a);
+int launch_attention_backward(const AttentionBackward& a, void* workspace, hipStream_t s);
+
+// ---- head_norm.hip
+struct HeadNorm {
+    Mat x, y;                    // y: the output, or backward grad_x (y.p may be NULL there)
+    Mat grad_y;                  // backward
+    Mat positions, frequencies;  // positions.p may be NULL: nothing is turned
+    const float* gamma;          // may be NULL
+    float* grad_gamma;           // backward; may be NULL
+    int heads, head;
+    float eps;
+    int dtype;
+};
+int launch_head_norm(const HeadNorm& a, hipStream_t s);
+size_t head_norm_backward_workspace(const HeadNorm& a);
+int launch_head_norm_backward(const HeadNorm& a, void* workspace, hipStream_t s);
+
+// ---- gradient_clip.hip
+struct ClipPart {
+    const void* g;
+    void* c;                      // where it goes: g itself, or another matrix
+    int64_t count, cols;          // elements in all, and of a row
+    int64_t stride, c_stride;
+    int dtype, c_dtype;
+};
+struct ClipPlan {
+    uint32_t chunks;       // of work, in the parts' order
+    uint32_t workgroups;
+    int64_t sums_at, parts_at, firsts_at, bytes;   // in the workspace; firsts: each part's first chunk
+};
+ClipPlan plan_clip(const ClipPart* parts, int count, uint32_t* firsts);
+struct ClipRun {
+    double max_norm, scale, epsilon;
+    float* norm;   // may be NULL
+    int apart;     // the outputs are other matrices
+};
+int launch_clip(const ClipPlan& plan, int count, const ClipRun& p, unsigned char* workspace, hipStream_t s);
 
 // ---- muon.hip
 constexpr float kNewtonSchulzA = 3.4445f, kNewtonSchulzB = -4.7750f, kNewtonSchulzC = 2.0315f;

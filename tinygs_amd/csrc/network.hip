@@ -29,6 +29,15 @@ struct tgs_muon {
     DevBuf workspace;
 };
 
+struct tgs_gradient_clip {
+    std::vector<ClipPart> parts;
+    std::vector<uint32_t> firsts;
+    bool apart = false;
+    bool on_device = false;   // the workspace holds the table
+    ClipPlan plan{};
+    DevBuf workspace;
+};
+
 namespace {
 
 constexpr int64_t kMaxStride = (int64_t)1 << 21;
@@ -152,6 +161,131 @@ void bind_muon(tgs_muon* m, const tgs_matrix* weights, const tgs_matrix* grads, 
     m->on_device = false;
     m->grad_dtype = grads[0].dtype;
     m->copy_dtype = copies ? copies[0].dtype : TGS_DTYPE_FLOAT32;
+}
+
+// out does not lie on the mask's bytes.
+int check_mask(const tgs_matrix* out, const char* name, const tgs_attention& a, int64_t states) {
+    if (!out || !a.mask || !out->rows) return TGS_OK;
+    const uintptr_t m0 = (uintptr_t)a.mask, m1 = m0 + (uintptr_t)((a.batch - 1) * a.mask_stride + states);
+    const uintptr_t o0 = (uintptr_t)out->data;
+    const uintptr_t o1 = o0 + (uintptr_t)(((out->rows - 1) * out->stride + out->cols) * element_size(out->dtype));
+    if (o0 < m1 && m0 < o1) return fail(TGS_ERR_INVALID, "%s overlaps the mask", name);
+    return TGS_OK;
+}
+
+constexpr int kMaxAttentionHead = 128, kMaxNormHead = 256, kMaxHeads = 4096;
+
+int check_attention(const tgs_matrix* q, const tgs_matrix* k, const tgs_matrix* v, const tgs_attention* a, Attention& to) {
+    TGS_TRY(check_matrix(q, "q"));
+    TGS_TRY(check_matrix(k, "k"));
+    if (!a) return fail(TGS_ERR_INVALID, "attention is NULL");
+    if (a->heads < 1 || a->heads > kMaxHeads || q->cols % a->heads)
+        return fail(TGS_ERR_INVALID, "%d heads of %lld columns", a->heads, (long long)q->cols);
+    const int64_t head = q->cols / a->heads;
+    if (head > kMaxAttentionHead) return fail(TGS_ERR_UNSUPPORTED, "heads of %lld columns", (long long)head);
+    if (a->kv_heads < 1 || a->heads % a->kv_heads)
+        return fail(TGS_ERR_INVALID, "%d heads do not share %d", a->heads, a->kv_heads);
+    if (a->batch < 1 || q->rows % a->batch || k->rows % a->batch)
+        return fail(TGS_ERR_INVALID, "a batch of %lld, %lld queries, %lld states", (long long)a->batch,
+                    (long long)q->rows, (long long)k->rows);
+    if (!(a->scale >= 0.0f) || !isfinite(a->scale)) return fail(TGS_ERR_INVALID, "scale %g", a->scale);
+    TGS_TRY(check_shape(k, "k", k->rows, head * a->kv_heads, q->dtype));
+    TGS_TRY(check_shape(v, "v", k->rows, head * a->kv_heads, q->dtype));
+    const int64_t states = k->rows / a->batch;
+    if (a->mask && (a->mask_stride < 0 || a->mask_stride > ((int64_t)1 << 40)))
+        return fail(TGS_ERR_INVALID, "a mask's stride of %lld", (long long)a->mask_stride);
+    to = Attention{view(q), view(k), view(v), Mat{}, nullptr, 0, 0, a->mask, a->mask_stride, a->batch, q->rows / a->batch, states,
+                   a->heads, a->kv_heads, (int)head, a->scale, q->dtype};
+    return TGS_OK;
+}
+
+// The places of rows x heads floats, in rows of heads or heads of rows, as one vector that holds them.
+int check_lse(const float* lse, int64_t row_step, int64_t head_step, int64_t rows, int64_t heads, tgs_matrix& span) {
+    span = vector_of(nullptr, 1);
+    if (!lse) return TGS_OK;
+    TGS_TRY(check_vector(lse, "lse"));
+    const int64_t most = (int64_t)1 << 40;
+    if (row_step < 1 || head_step < 1 || row_step > most || head_step > most ||
+        (rows > 1 && heads > 1 && row_step < heads * head_step && head_step < rows * row_step))
+        return fail(TGS_ERR_INVALID, "lse's steps %lld and %lld", (long long)row_step, (long long)head_step);
+    if (rows > 0) span = vector_of(lse, (rows - 1) * row_step + (heads - 1) * head_step + 1);
+    return TGS_OK;
+}
+
+int check_head_norm(const tgs_matrix* x, int32_t heads, const float* gamma, const tgs_turn* turn, float epsilon,
+                    HeadNorm& to) {
+    TGS_TRY(check_matrix(x, "x"));
+    if (heads < 1 || heads > kMaxHeads || x->cols % heads)
+        return fail(TGS_ERR_INVALID, "%d heads of %lld columns", heads, (long long)x->cols);
+    const int64_t head = x->cols / heads;
+    if (head > kMaxNormHead) return fail(TGS_ERR_UNSUPPORTED, "heads of %lld columns", (long long)head);
+    TGS_TRY(check_vector(gamma, "gamma"));
+    if (!(epsilon >= 0.0f) || !isfinite(epsilon)) return fail(TGS_ERR_INVALID, "epsilon %g", epsilon);
+    to = HeadNorm{view(x), Mat{}, Mat{}, Mat{}, Mat{}, gamma, nullptr, heads, (int)head, epsilon, x->dtype};
+    if (!turn) return TGS_OK;
+    TGS_TRY(check_matrix(&turn->positions, "positions"));
+    TGS_TRY(check_matrix(&turn->frequencies, "frequencies"));
+    const int64_t axes = turn->positions.cols;
+    if (axes > 4) return fail(TGS_ERR_UNSUPPORTED, "positions of %lld axes", (long long)axes);
+    TGS_TRY(check_shape(&turn->positions, "positions", x->rows, axes, TGS_DTYPE_FLOAT32));
+    TGS_TRY(check_shape(&turn->frequencies, "frequencies", turn->frequencies.rows, axes, TGS_DTYPE_FLOAT32));
+    if (turn->frequencies.rows < 1 || turn->frequencies.rows > head / 2)
+        return fail(TGS_ERR_INVALID, "%lld pairs in heads of %lld columns", (long long)turn->frequencies.rows,
+                    (long long)head);
+    to.positions = view(&turn->positions);
+    to.frequencies = view(&turn->frequencies);
+    return TGS_OK;
+}
+
+int check_clip(const tgs_matrix* grads, const tgs_matrix* clipped, int32_t count) {
+    if (!grads) return fail(TGS_ERR_INVALID, "grads is NULL");
+    if (count < 1 || count > 4096) return fail(TGS_ERR_INVALID, "%d matrices", count);
+    const auto name = [](char (&to)[32], bool out, int32_t i) {
+        snprintf(to, sizeof(to), out ? "clipped[%d]" : "grads[%d]", i);
+        return to;
+    };
+    char x[32], y[32];
+    for (int32_t i = 0; i < count; ++i) {
+        TGS_TRY(check_matrix(&grads[i], name(x, false, i)));
+        if (clipped) {
+            TGS_TRY(check_matrix(&clipped[i], name(x, true, i)));
+            TGS_TRY(check_shape(&clipped[i], name(x, true, i), grads[i].rows, grads[i].cols, clipped[i].dtype));
+        }
+    }
+    // no element counts twice, and what is written shares nothing with the rest
+    for (int32_t i = 0; i < count; ++i)
+        for (int32_t j = 0; j < count; ++j) {
+            if (j > i) TGS_TRY(check_apart(&grads[j], name(x, false, j), &grads[i], name(y, false, i)));
+            if (j > i && clipped) TGS_TRY(check_apart(&clipped[j], name(x, true, j), &clipped[i], name(y, true, i)));
+            if (clipped) TGS_TRY(check_apart(&clipped[j], name(x, true, j), &grads[i], name(y, false, i)));
+        }
+    return TGS_OK;
+}
+
+int bind_clip(tgs_gradient_clip* c, const tgs_matrix* grads, const tgs_matrix* clipped, int32_t count) {
+    std::vector<ClipPart> parts;
+    std::vector<uint32_t> firsts;
+    try {
+        parts.resize((size_t)count);
+        firsts.resize((size_t)count);
+    } catch (...) {
+        return fail(TGS_ERR_STATE, "out of host memory");
+    }
+    for (int32_t i = 0; i < count; ++i) {
+        const tgs_matrix& g = grads[i];
+        const tgs_matrix& to = clipped ? clipped[i] : g;
+        // a single row's stride says nothing
+        parts[(size_t)i] = ClipPart{g.data, to.data, g.rows * g.cols, g.cols, g.rows > 1 ? g.stride : g.cols,
+                                    g.rows > 1 ? to.stride : g.cols, g.dtype, to.dtype};
+    }
+    const ClipPlan plan = plan_clip(parts.data(), count, firsts.data());
+    if (plan.chunks == 0x7fffffffu) return fail(TGS_ERR_INVALID, "too many elements for one norm");
+    c->parts.swap(parts);
+    c->firsts.swap(firsts);
+    c->plan = plan;
+    c->apart = clipped != nullptr;
+    c->on_device = false;
+    return TGS_OK;
 }
 
 }  // namespace
@@ -292,6 +426,181 @@ int tgs_layer_norm_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_
                               grad_gamma, grad_beta, x->dtype};
     TGS_TRY(ensure(n->workspace, layer_norm_backward_workspace(a), (hipStream_t)stream));
     return launch_layer_norm_backward(a, n->workspace.p, (hipStream_t)stream);
+}
+
+// ------------------------------------------------------------------ attention
+
+int tgs_attention_forward(tgs_network* n, const tgs_matrix* q, const tgs_matrix* k, const tgs_matrix* v,
+                          const tgs_attention* a, const tgs_matrix* out, float* lse, int64_t lse_row_step,
+                          int64_t lse_head_step, void* stream) {
+    if (!n) return fail(TGS_ERR_INVALID, "network is NULL");
+    Attention to;
+    TGS_TRY(check_attention(q, k, v, a, to));
+    TGS_TRY(check_shape(out, "out", q->rows, q->cols, q->dtype));
+    tgs_matrix l;
+    TGS_TRY(check_lse(lse, lse_row_step, lse_head_step, q->rows, a->heads, l));
+    const tgs_matrix* outs[2] = {out, &l};
+    const char* names[2] = {"out", "lse"};
+    for (int i = 0; i < 2; ++i) {
+        TGS_TRY(check_apart(outs[i], names[i], q, "q"));
+        TGS_TRY(check_apart(outs[i], names[i], k, "k"));
+        TGS_TRY(check_apart(outs[i], names[i], v, "v"));
+        TGS_TRY(check_mask(outs[i], names[i], *a, to.states));
+    }
+    TGS_TRY(check_apart(&l, "lse", out, "out"));
+    if (q->rows == 0) return TGS_OK;
+    to.out = view(out);
+    to.lse = lse;
+    to.lse_row_step = lse_row_step;
+    to.lse_head_step = lse_head_step;
+    const size_t bytes = attention_workspace(to);
+    if (bytes) TGS_TRY(ensure(n->workspace, bytes, (hipStream_t)stream));
+    return launch_attention(to, n->workspace.p, (hipStream_t)stream);
+}
+
+int tgs_attention_backward(tgs_network* n, const tgs_matrix* grad_out, const tgs_matrix* q, const tgs_matrix* k,
+                           const tgs_matrix* v, const tgs_matrix* out, const float* lse, int64_t lse_row_step,
+                           int64_t lse_head_step, const tgs_attention* a, const tgs_matrix* grad_q,
+                           const tgs_matrix* grad_k, const tgs_matrix* grad_v, void* stream) {
+    if (!n) return fail(TGS_ERR_INVALID, "network is NULL");
+    AttentionBackward to{};
+    TGS_TRY(check_attention(q, k, v, a, to.a));
+    TGS_TRY(check_shape(grad_out, "grad_out", q->rows, q->cols, q->dtype));
+    TGS_TRY(check_shape(out, "out", q->rows, q->cols, q->dtype));
+    if (q->rows > 0 && !lse) return fail(TGS_ERR_INVALID, "lse is NULL");
+    tgs_matrix l;
+    TGS_TRY(check_lse(lse, lse_row_step, lse_head_step, q->rows, a->heads, l));
+    if (grad_q) TGS_TRY(check_shape(grad_q, "grad_q", q->rows, q->cols, q->dtype));
+    if (grad_k) TGS_TRY(check_shape(grad_k, "grad_k", k->rows, k->cols, q->dtype));
+    if (grad_v) TGS_TRY(check_shape(grad_v, "grad_v", k->rows, k->cols, q->dtype));
+    const tgs_matrix* outs[3] = {grad_q, grad_k, grad_v};
+    const char* names[3] = {"grad_q", "grad_k", "grad_v"};
+    const tgs_matrix* ins[6] = {grad_out, q, k, v, out, &l};
+    const char* in_names[6] = {"grad_out", "q", "k", "v", "out", "lse"};
+    for (int i = 0; i < 3; ++i) {
+        for (int j = 0; j < 6; ++j) TGS_TRY(check_apart(outs[i], names[i], ins[j], in_names[j]));
+        for (int j = 0; j < i; ++j) TGS_TRY(check_apart(outs[i], names[i], outs[j], names[j]));
+        TGS_TRY(check_mask(outs[i], names[i], *a, to.a.states));
+    }
+    to.a.out = view(out);
+    to.a.lse = const_cast<float*>(lse);
+    to.a.lse_row_step = lse_row_step;
+    to.a.lse_head_step = lse_head_step;
+    to.grad_out = view(grad_out);
+    to.grad_q = view(grad_q);
+    to.grad_k = view(grad_k);
+    to.grad_v = view(grad_v);
+    const size_t bytes = attention_backward_workspace(to);
+    if (bytes) TGS_TRY(ensure(n->workspace, bytes, (hipStream_t)stream));
+    return launch_attention_backward(to, n->workspace.p, (hipStream_t)stream);
+}
+
+int tgs_head_norm_forward(tgs_network* n, const tgs_matrix* x, int32_t heads, const float* gamma, const tgs_turn* turn,
+                          float epsilon, const tgs_matrix* y, void* stream) {
+    if (!n) return fail(TGS_ERR_INVALID, "network is NULL");
+    HeadNorm to;
+    TGS_TRY(check_head_norm(x, heads, gamma, turn, epsilon, to));
+    TGS_TRY(check_shape(y, "y", x->rows, x->cols, x->dtype));
+    const tgs_matrix g = vector_of(gamma, to.head);
+    TGS_TRY(check_apart(y, "y", &g, "gamma"));
+    if (turn) {
+        TGS_TRY(check_apart(y, "y", &turn->positions, "positions"));
+        TGS_TRY(check_apart(y, "y", &turn->frequencies, "frequencies"));
+    }
+    if (!same_place(*x, *y)) TGS_TRY(check_apart(y, "y", x, "x"));
+    if (x->rows == 0) return TGS_OK;
+    to.y = view(y);
+    return launch_head_norm(to, (hipStream_t)stream);
+}
+
+int tgs_head_norm_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_matrix* x, int32_t heads,
+                           const float* gamma, const tgs_turn* turn, float epsilon, const tgs_matrix* grad_x,
+                           float* grad_gamma, void* stream) {
+    if (!n) return fail(TGS_ERR_INVALID, "network is NULL");
+    HeadNorm to;
+    TGS_TRY(check_head_norm(x, heads, gamma, turn, epsilon, to));
+    TGS_TRY(check_shape(grad_y, "grad_y", x->rows, x->cols, x->dtype));
+    if (grad_x) TGS_TRY(check_shape(grad_x, "grad_x", x->rows, x->cols, x->dtype));
+    TGS_TRY(check_vector(grad_gamma, "grad_gamma"));
+    const tgs_matrix g = vector_of(gamma, to.head), gg = vector_of(grad_gamma, to.head);
+    const tgs_matrix* outs[2] = {grad_x, &gg};
+    const char* names[2] = {"grad_x", "grad_gamma"};
+    for (int i = 0; i < 2; ++i) {
+        TGS_TRY(check_apart(outs[i], names[i], x, "x"));
+        TGS_TRY(check_apart(outs[i], names[i], &g, "gamma"));
+        if (!turn) continue;
+        TGS_TRY(check_apart(outs[i], names[i], &turn->positions, "positions"));
+        TGS_TRY(check_apart(outs[i], names[i], &turn->frequencies, "frequencies"));
+    }
+    TGS_TRY(check_apart(&gg, "grad_gamma", grad_y, "grad_y"));
+    TGS_TRY(check_apart(&gg, "grad_gamma", grad_x, "grad_x"));
+    if (grad_x && !same_place(*grad_x, *grad_y)) TGS_TRY(check_apart(grad_x, "grad_x", grad_y, "grad_y"));
+    to.grad_y = view(grad_y);
+    to.y = view(grad_x);
+    to.grad_gamma = grad_gamma;
+    const size_t bytes = head_norm_backward_workspace(to);
+    if (bytes) TGS_TRY(ensure(n->workspace, bytes, (hipStream_t)stream));
+    return launch_head_norm_backward(to, n->workspace.p, (hipStream_t)stream);
+}
+
+// ------------------------------------------------------------------ clipping
+
+int tgs_gradient_clip_create(const tgs_matrix* grads, const tgs_matrix* clipped, int32_t count,
+                             tgs_gradient_clip** out) {
+    if (!out) return fail(TGS_ERR_INVALID, "out is NULL");
+    *out = nullptr;
+    TGS_TRY(check_clip(grads, clipped, count));
+    tgs_gradient_clip* c = new (std::nothrow) tgs_gradient_clip();
+    if (!c) return fail(TGS_ERR_STATE, "out of host memory");
+    const int rc = bind_clip(c, grads, clipped, count);
+    if (rc != TGS_OK) {
+        delete c;
+        return rc;
+    }
+    *out = c;
+    return TGS_OK;
+}
+
+int tgs_gradient_clip_destroy(tgs_gradient_clip* c) {
+    if (!c) return TGS_OK;
+    release(c->workspace);
+    delete c;
+    return TGS_OK;
+}
+
+int tgs_gradient_clip_set_matrices(tgs_gradient_clip* c, const tgs_matrix* grads, const tgs_matrix* clipped,
+                                   int32_t count) {
+    if (!c) return fail(TGS_ERR_INVALID, "gradient clip is NULL");
+    TGS_TRY(check_clip(grads, clipped, count));
+    return bind_clip(c, grads, clipped, count);
+}
+
+int tgs_gradient_clip_run(tgs_gradient_clip* c, float max_norm, float scale, float epsilon, float* norm, void* stream) {
+    if (!c) return fail(TGS_ERR_INVALID, "gradient clip is NULL");
+    if (!(max_norm >= 0.0f)) return fail(TGS_ERR_INVALID, "max_norm %g", max_norm);
+    if (!(scale > 0.0f) || !isfinite(scale)) return fail(TGS_ERR_INVALID, "scale %g", scale);
+    if (!(epsilon >= 0.0f) || !isfinite(epsilon)) return fail(TGS_ERR_INVALID, "epsilon %g", epsilon);
+    TGS_TRY(check_vector(norm, "norm"));
+    const tgs_matrix v = vector_of(norm, 1);
+    for (const ClipPart& a : c->parts) {
+        const tgs_matrix g{const_cast<void*>(a.g), a.count / a.cols, a.cols, a.stride, a.dtype};
+        const tgs_matrix to{a.c, g.rows, a.cols, a.c_stride, a.c_dtype};
+        TGS_TRY(check_apart(&v, "norm", &g, "a gradient"));
+        TGS_TRY(check_apart(&v, "norm", &to, "a clipped gradient"));
+    }
+    hipStream_t s = (hipStream_t)stream;
+    const int count = (int)c->parts.size();
+    if (!c->on_device) {   // the first run, or the first after a rebinding
+        TGS_TRY(ensure(c->workspace, (size_t)c->plan.bytes, s));
+        unsigned char* at = c->workspace.as<unsigned char>();
+        TGS_HIP(hipMemcpyAsync(at + c->plan.parts_at, c->parts.data(), sizeof(ClipPart) * (size_t)count,
+                               hipMemcpyHostToDevice, s));
+        TGS_HIP(hipMemcpyAsync(at + c->plan.firsts_at, c->firsts.data(), sizeof(uint32_t) * (size_t)count,
+                               hipMemcpyHostToDevice, s));
+        TGS_HIP(hipStreamSynchronize(s));
+        c->on_device = true;
+    }
+    return launch_clip(c->plan, count, {max_norm, scale, epsilon, norm, c->apart}, c->workspace.as<unsigned char>(), s);
 }
 
 // ------------------------------------------------------------------ Muon

@@ -189,6 +189,130 @@ class LayerOps:
             _lib.check(rc, "layer_norm_backward")
         return grad_x, grad_gamma, grad_beta
 
+    def attention(self, q, k, v, heads: int, kv_heads: int | None = None, batch: int = 1, mask=None,
+                  scale: float | None = None, keep_lse: bool = False, out=None, lse=None, stream=None):
+        """softmax(scale q k^T) v for each head over the states that exist; with keep_lse (or lse given) also the
+        logarithms of the weights' sums [rows, heads], which attention_backward takes.
+
+        q [batch x queries, heads d]; k and v [batch x states, kv_heads d], d up to 128; heads share those of the
+        states in equal groups. mask [batch, states] (bool or uint8): False where a state does not exist; it may hold
+        anything then. Rows without a state are 0, their lse -inf. scale: 1 / sqrt(d) unless given."""
+        rows = q.shape[0]
+        if out is None:
+            out = self._empty(stream, q, q.shape)
+        if lse is None and keep_lse:
+            # heads of rows: neighbouring rows' are written together
+            lse = self._empty(stream, q, (heads, rows), _float32()).t()
+        tensors = (matrix(q, "q"), matrix(k, "k"), matrix(v, "v"))
+        a = self._attention(q, k, heads, kv_heads, batch, mask, scale)
+        _on_one_device(q=q, k=k, v=v, mask=mask, out=out, lse=lse)
+        rc = self._lib.tgs_attention_forward(self._h, *tensors, a, matrix(out, "out"), *_lse(lse, rows, heads),
+                                             self._stream(stream, q))
+        if rc:
+            _lib.check(rc, "attention")
+        return out if lse is None else (out, lse)
+
+    def attention_backward(self, grad_out, q, k, v, out, lse, heads: int, kv_heads: int | None = None, batch: int = 1,
+                           mask=None, scale: float | None = None, need_q: bool = True, need_k: bool = True,
+                           need_v: bool = True, grad_q=None, grad_k=None, grad_v=None, stream=None):
+        """(grad_q, grad_k, grad_v) of attention for grad_out, from its out and lse; None where not needed. Gradients
+        are assigned, zeros for states that do not exist."""
+        if need_q and grad_q is None:
+            grad_q = self._empty(stream, q, q.shape)
+        if need_k and grad_k is None:
+            grad_k = self._empty(stream, k, k.shape)
+        if need_v and grad_v is None:
+            grad_v = self._empty(stream, v, v.shape)
+        tensors = (matrix(grad_out, "grad_out"), matrix(q, "q"), matrix(k, "k"), matrix(v, "v"), matrix(out, "out"))
+        a = self._attention(q, k, heads, kv_heads, batch, mask, scale)
+        _on_one_device(grad_out=grad_out, q=q, k=k, v=v, out=out, lse=lse, mask=mask, grad_q=grad_q, grad_k=grad_k,
+                       grad_v=grad_v)
+        rc = self._lib.tgs_attention_backward(
+            self._h, *tensors, *_lse(lse, q.shape[0], heads), a, None if grad_q is None else matrix(grad_q, "grad_q"),
+            None if grad_k is None else matrix(grad_k, "grad_k"), None if grad_v is None else matrix(grad_v, "grad_v"),
+            self._stream(stream, q))
+        if rc:
+            _lib.check(rc, "attention_backward")
+        return grad_q, grad_k, grad_v
+
+    @staticmethod
+    def _attention(q, k, heads, kv_heads, batch, mask, scale):
+        kv_heads = heads if kv_heads is None else kv_heads
+        if scale is None:
+            scale = math.sqrt(heads / max(q.shape[1], 1)) if heads > 0 else 0.0
+        at, step = None, 0
+        if mask is not None:
+            if mask.dim() != 2 or mask.shape[0] != batch or mask.shape[0] * mask.shape[1] != k.shape[0]:
+                raise RuntimeError(f"mask: [batch, states] is needed, not {list(mask.shape)}")
+            if mask.element_size() != 1 or mask.is_floating_point() or (mask.shape[1] > 1 and mask.stride(1) != 1):
+                raise RuntimeError("mask: packed rows of bool or uint8 are needed")
+            at, step = mask.data_ptr(), mask.stride(0)
+        return _lib.tgs_attention(batch, heads, kv_heads, scale, at, step)
+
+    def head_norm(self, x, heads: int, gamma=None, positions=None, frequencies=None, eps: float = 1e-6, out=None,
+                  stream=None):
+        """x / sqrt(mean(x^2) + eps) gamma over each head of d = columns / heads (up to 256) columns; with positions
+        [rows, axes] and frequencies [pairs, axes] (float32, up to 4 axes, up to d / 2 pairs) the pairs (2 i, 2 i + 1)
+        of every head are then turned by the angle positions . frequencies[i]. gamma [d] is shared by the heads.
+        out may be x itself."""
+        if out is None:
+            out = self._empty(stream, x, x.shape)
+        at = matrix(x, "x")
+        turn = _turn(positions, frequencies)
+        _on_one_device(x=x, gamma=gamma, positions=positions, frequencies=frequencies, out=out)
+        rc = self._lib.tgs_head_norm_forward(self._h, at, heads, _vector(gamma, x.shape[1] // max(heads, 1), "gamma"),
+                                             turn, eps, matrix(out, "out"), self._stream(stream, x))
+        if rc:
+            _lib.check(rc, "head_norm")
+        return out
+
+    def head_norm_backward(self, grad_y, x, heads: int, gamma=None, positions=None, frequencies=None,
+                           eps: float = 1e-6, need_x: bool = True, grad_x=None, grad_gamma=None, stream=None):
+        """(grad_x, grad_gamma) of head_norm for grad_y; grad_gamma is None where there is no gamma. Positions and
+        frequencies get no gradient. grad_x may be grad_y itself."""
+        if need_x and grad_x is None:
+            grad_x = self._empty(stream, x, x.shape)
+        d = x.shape[1] // max(heads, 1)
+        if gamma is not None and grad_gamma is None:
+            grad_gamma = self._empty(stream, x, (d,), _float32())
+        at = (matrix(grad_y, "grad_y"), matrix(x, "x"))
+        turn = _turn(positions, frequencies)
+        _on_one_device(grad_y=grad_y, x=x, gamma=gamma, positions=positions, frequencies=frequencies, grad_x=grad_x,
+                       grad_gamma=grad_gamma)
+        rc = self._lib.tgs_head_norm_backward(self._h, *at, heads, _vector(gamma, d, "gamma"), turn, eps,
+                                              None if grad_x is None else matrix(grad_x, "grad_x"),
+                                              _vector(grad_gamma, d, "grad_gamma"), self._stream(stream, x))
+        if rc:
+            _lib.check(rc, "head_norm_backward")
+        return grad_x, grad_gamma
+
+
+def _on_one_device(**tensors):
+    """All on the current device, whose streams and workspaces a handle uses."""
+    import torch
+    current = torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != current:
+            raise RuntimeError(f"{name}: not on the current device")
+
+
+def _lse(t, rows: int, heads: int):
+    """Address and steps of a float32 [rows, heads] tensor, in rows of heads or heads of rows."""
+    if t is None:
+        return None, 1, 1
+    if t.shape != (rows, heads) or t.dtype is not _float32() or not t.is_cuda:
+        raise RuntimeError(f"lse: float32 [{rows}, {heads}] on the device is needed")
+    # the step of a single row or head says nothing
+    return t.data_ptr(), t.stride(0) if rows > 1 else 1, t.stride(1) if heads > 1 else 1
+
+
+def _turn(positions, frequencies):
+    if positions is None and frequencies is None:
+        return None
+    if positions is None or frequencies is None:
+        raise RuntimeError("head_norm: positions and frequencies come together")
+    return _lib.tgs_turn(matrix(positions, "positions"), matrix(frequencies, "frequencies"))
+
 
 class AttributeNetwork:
     """A network over the Gaussians: features [n, inputs] -> attributes [n, outputs].

@@ -1,4 +1,4 @@
-"""SimpleAdam, and Muon for an attribute network's matrices, over the C ABI.
+"""SimpleAdam, Muon for an attribute network's matrices, and the clipping of gradients, over the C ABI.
 
 Mirrors tinygs's OptimizerBase / SimpleAdam / create_optimizer
 (tinygs/include/tinygs/optim/optim.hpp:39-106,
@@ -6,6 +6,7 @@ tinygs/include/tinygs/optim/simple_adam.hpp:30-87, tinygs/src/optim/optim.cu:86-
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 from . import _lib
@@ -258,6 +259,85 @@ class Muon:
                 raise RuntimeError(f"Muon: unknown parameter {k}")
             setattr(p, k, int(v) if k in ("nesterov", "iterations") else float(v))
         _lib.check(self._lib.tgs_muon_set_params(self._h, C.byref(p)), "set_params")
+
+
+class GradientClip:
+    """The norm of many gradients together, and clipping: norm = scale sqrt(sum of squares),
+    g <- g scale min(1, max_norm / (norm + epsilon)). grads are tensors of any shapes and of float32, float16 or
+    bfloat16 each, packed or 2-D with rows further apart; with clipped (tensors of the same shapes) these receive the
+    result in their own dtypes and grads stay as they are. The tensors are kept: a run reads what they hold then. Runs
+    are on one stream, or the caller orders them."""
+
+    def __init__(self, grads, clipped=None):
+        self._lib = _lib.load()
+        self._h = None
+        self._norm = None
+        self._bind(grads, clipped)
+        h = C.c_void_p()
+        _lib.check(self._lib.tgs_gradient_clip_create(*self._arrays(), C.byref(h)), "GradientClip")
+        self._h = h
+
+    def _bind(self, grads, clipped):
+        self.m_grads = list(grads)
+        self.m_clipped = None if clipped is None else list(clipped)
+        if not self.m_grads or (clipped is not None and len(self.m_clipped) != len(self.m_grads)):
+            raise RuntimeError("GradientClip: grads, and as many clipped tensors, are needed")
+        for name, tensors in (("grads", self.m_grads), ("clipped", self.m_clipped or ())):
+            for i, t in enumerate(tensors):
+                if t.get_device() != self.m_grads[0].get_device():
+                    raise RuntimeError(f"GradientClip: {name}[{i}] is on another device")
+                if name == "clipped" and t.shape != self.m_grads[i].shape:
+                    raise RuntimeError(f"GradientClip: clipped[{i}] is not of its gradient's shape")
+
+    def _arrays(self):
+        from .network import matrix
+        outs = self.m_clipped or [None] * len(self.m_grads)
+        views, out_views = [], []
+        for i, (g, c) in enumerate(zip(self.m_grads, outs)):
+            # a packed tensor is a column of its elements, whatever its shape
+            if g.is_contiguous() and (c is None or c.is_contiguous()):
+                g, c = g.reshape(-1, 1), None if c is None else c.reshape(-1, 1)
+            views.append(matrix(g, f"grads[{i}]"))
+            if c is not None:
+                out_views.append(matrix(c, f"clipped[{i}]"))
+        n = len(views)
+        return ((_lib.tgs_matrix * n)(*views), (_lib.tgs_matrix * n)(*out_views) if out_views else None, n)
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            try:
+                self._lib.tgs_gradient_clip_destroy(h)
+            except Exception:
+                pass
+            self._h = None
+
+    def set_grads(self, grads, clipped=None):
+        """Other tensors, of any number and shapes."""
+        kept = self.m_grads, self.m_clipped
+        try:
+            self._bind(grads, clipped)
+            if self.m_grads[0].get_device() != kept[0][0].get_device():
+                raise RuntimeError("GradientClip::set_grads: on another device")
+            _lib.check(self._lib.tgs_gradient_clip_set_matrices(self._h, *self._arrays()), "GradientClip::set_grads")
+        except Exception:
+            self.m_grads, self.m_clipped = kept
+            raise
+
+    def clip(self, max_norm: float, scale: float = 1.0, epsilon: float = 1e-6, stream=None):
+        """One run. Returns the norm (scale included, before clipping), a float32 scalar on the device that the next
+        run overwrites. max_norm infinite: the norm alone, and scale where it is not 1."""
+        import torch
+        first = self.m_grads[0]
+        if first.get_device() != torch.cuda.current_device():
+            raise RuntimeError("GradientClip: the gradients are not on the current device")
+        if self._norm is None:
+            with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
+                self._norm = torch.empty((), dtype=torch.float32, device=first.device)
+        _lib.check(self._lib.tgs_gradient_clip_run(self._h, float(max_norm), float(scale), float(epsilon),
+                                                   C.c_void_p(self._norm.data_ptr()), stream_ptr(stream)),
+                   "GradientClip::clip")
+        return self._norm
 
 
 def create_optimizer(optimizer_type: str, gaussians, gaussians_grad, copies=None):
