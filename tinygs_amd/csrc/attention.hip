@@ -1,71 +1,351 @@
 // Attention of a network's rows to an encoder's states: for each row and head
 // s = scale q k^T over the states that exist, out = softmax(s) v, lse = log sum exp s.
+//
+// One pass over the states with a running maximum m and sum l: a wave holds 32
+// or 64 rows' queries, and their sums out^T = v^T p^T, in registers; tiles of
+// states go through LDS, loaded one ahead. The scores are formed as
+// s^T = k q^T: a lane then has one row's scores, so that maxima and sums need one
+// exchange between the halves of the wave, and the weights p^T are the second
+// product's operand as they stand. The maximum is replaced only where a score
+// passes it by 2^8: the weights stay below that, and the sums are seldom scaled.
+//
+// Heads that share the states' are rows side by side, so that a tile is loaded
+// once for all of them. Where there are few rows, workgroups take parts of the
+// states and their sums are joined by a second kernel.
 #include <math.h>
 
-#include "network.h"
+#include "attention.h"
 
 namespace tgs {
 
 namespace {
 
-constexpr int kMaxHead = 128;
+constexpr float kLazy = 8.0f;   // in powers of two
 
-// One wave a row and head: a lane takes a state of 64 for the scores, then a column or two for the sums.
-template <class T>
-__global__ void __launch_bounds__(64) attention_kernel(Attention a) {
-    __shared__ float q[kMaxHead], p[64];
-    const int lane = threadIdx.x, d = a.head, h = blockIdx.y, g = h / (a.heads / a.kv_heads);
-    for (int64_t r = blockIdx.x; r < a.q.rows; r += gridDim.x) {
-        const int64_t b = r / a.queries;
-        const uint8_t* mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
-        for (int c = lane; c < d; c += 64) q[c] = (float)((const T*)a.q.p)[r * a.q.stride + h * d + c];
-        __syncthreads();
-        float top = -INFINITY, sum = 0.0f, o[2] = {0.0f, 0.0f};
-        for (int64_t j0 = 0; j0 < a.states; j0 += 64) {
-            const int64_t j = j0 + lane;
-            float s = -INFINITY;
-            if (j < a.states && (!mask || mask[j])) {
-                const T* k = (const T*)a.k.p + (b * a.states + j) * a.k.stride + g * d;
-                s = 0.0f;
-                for (int c = 0; c < d; ++c) s = fmaf(q[c], (float)k[c], s);
-                s *= a.scale;
-            }
-            float m = s;
-            for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
-            m = fmaxf(m, top);
-            const float from = m == -INFINITY ? 0.0f : m;
-            const float e = expf(s - from), keep = expf(top - from);
-            top = m;
-            float t = e;
-            for (int k = 32; k > 0; k >>= 1) t += __shfl_xor(t, k, 64);
-            sum = fmaf(sum, keep, t);
-            p[lane] = e;
-            __syncthreads();
-            for (int n = 0; n < 2; ++n) {
-                const int c = lane + 64 * n;
-                o[n] *= keep;
-                if (c < d)
-                    for (int k = 0; k < 64 && j0 + k < a.states; ++k)
-                        if (!mask || mask[j0 + k])
-                            o[n] = fmaf(p[k], (float)((const T*)a.v.p)[(b * a.states + j0 + k) * a.v.stride + g * d + c], o[n]);
-            }
-            __syncthreads();
-        }
-        for (int n = 0; n < 2; ++n)
-            if (lane + 64 * n < d)
-                ((T*)a.out.p)[r * a.out.stride + h * d + lane + 64 * n] = (T)(sum == 0.0f ? 0.0f : o[n] / sum);
-        if (a.lse && lane == 0) a.lse[r * a.lse_row_step + h * a.lse_head_step] = sum == 0.0f ? -INFINITY : top + logf(sum);
+struct Grid {
+    int64_t first;       // number of the launch's first workgroup
+    int64_t blocks;      // of rows, for each batch element and head of the states
+    int64_t rows;        // queries x shared heads
+    int shared;
+    int splits;          // of the states
+    int tiles;           // of a split
+    float c;             // scale log2(e)
+    float* sums;         // of a split's parts: [splits][all rows][D], then m and l
+    float* tops;
+};
+
+// s scale log2(e), or no difference between states for a scale of 0; positive, so
+// that -infinity stays -infinity.
+float exponent_of(float scale) { return scale > 0.0f ? fmaxf(scale * kLog2E, 0x1p-149f) : 0x1p-149f; }
+
+template <class T, int D, int QB, int WAVES, int KT, bool SPLIT>
+__global__ void __launch_bounds__(64 * WAVES, D <= 64 ? 2 : 1) attention_kernel(Attention a, Grid g) {
+    using S = Square<T>;
+    using Tile = RowTile<T, D, KT, WAVES>;
+    constexpr int kSteps = D / S::kDepth;   // of the scores' product
+    constexpr int kParts = 32 / S::kDepth;  // of a square's rows as an operand
+    constexpr int kSubs = KT / 32, kCols = D / 32;
+    constexpr int kAtOnce = D <= 32 ? kSubs : 1;
+    constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
+    __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t number = g.first + xcd_contiguous_index(blockIdx.x, gridDim.x);
+    const int split = SPLIT ? (int)(number % g.splits) : 0;
+    const int64_t block = (SPLIT ? number / g.splits : number) % g.blocks;
+    const int64_t pair = (SPLIT ? number / g.splits : number) / g.blocks;
+    const int64_t b = pair / a.kv_heads;
+    const int kv = (int)(pair % a.kv_heads), d = a.head;
+
+    // the lane's rows
+    int64_t row[QB];
+    int head[QB];
+    bool exists[QB];
+    typename S::Frag q[QB][kSteps];
+#pragma unroll
+    for (int n = 0; n < QB; ++n) {
+        const int64_t i = ((block * WAVES + wave) * QB + n) * 32 + (lane & 31);
+        exists[n] = i < g.rows;
+        const int64_t r = g.shared == 1 ? i : i / g.shared;
+        head[n] = kv * g.shared + (g.shared == 1 ? 0 : (int)(i - r * g.shared));
+        row[n] = b * a.queries + r;
+        const T* p = (const T*)a.q.p + row[n] * a.q.stride + (int64_t)head[n] * d;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) q[n][s] = row_chunk<T>(p, 2 * s + (lane >> 5), d, exists[n]);
     }
+
+    Tile tk, tv;
+    const int64_t k_pitch = a.k.stride * (int64_t)sizeof(T), v_pitch = a.v.stride * (int64_t)sizeof(T);
+    tk.begin(k_pitch, d, wave, lane);
+    tv.begin(v_pitch, d, wave, lane);
+    // bytes of each that belong to this element's head, from its first row on
+    const unsigned char* k0 = (const unsigned char*)a.k.p + b * a.states * k_pitch + (int64_t)kv * d * sizeof(T);
+    const unsigned char* v0 = (const unsigned char*)a.v.p + b * a.states * v_pitch + (int64_t)kv * d * sizeof(T);
+    const int64_t k_end = (a.states - 1) * k_pitch + d * (int64_t)sizeof(T);
+    const int64_t v_end = (a.states - 1) * v_pitch + d * (int64_t)sizeof(T);
+    const uint8_t* mask = a.mask ? a.mask + b * a.mask_stride : nullptr;
+    const int64_t t1 = min((int64_t)(split + 1) * g.tiles, (a.states + KT - 1) / KT);
+    int64_t t = (int64_t)split * g.tiles - 1;   // the last tile whose loads were started
+    const auto state_exists = [&](int64_t tile) {
+        const int64_t j = tile * KT + lane;
+        return lane < KT && j < a.states && (!mask || mask[j]);
+    };
+    bool next = state_exists(t + 1);
+    uint64_t exist = 0;   // of that tile's states
+    const auto load = [&](int buffer) {   // the next tile that has states; false: none
+        do {
+            if (++t >= t1) return false;
+            exist = ballot(next);
+            next = state_exists(t + 1);
+        } while (exist == 0);
+        tk.load(lds[buffer][0], k0 + t * KT * k_pitch, k_end - t * KT * k_pitch, exist, d, wave, lane);
+        tv.load(lds[buffer][1], v0 + t * KT * v_pitch, v_end - t * KT * v_pitch, exist, d, wave, lane);
+        return true;
+    };
+
+    f32x16 out[QB][kCols];
+    float top[QB], sum[QB];
+#pragma unroll
+    for (int n = 0; n < QB; ++n) {
+        top[n] = -INFINITY;
+        sum[n] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) out[n][c][r] = 0.0f;
+    }
+    int buffer = 0;
+    bool more = load(0);
+    while (more) {
+        const uint64_t bits = exist;
+        wait_for_stage<1>(0);   // the tile is there, and every wave is done with the other buffer
+        more = load(buffer ^ 1);
+        const unsigned char *lk = lds[buffer][0], *lv = lds[buffer][1];
+        buffer ^= 1;
+        // kAtOnce squares of states at a time: as many scores as the registers hold beside the sums
+#pragma unroll 1
+        for (int u0 = 0; u0 < kSubs; u0 += kAtOnce) {
+            f32x16 s[QB][kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+#pragma unroll
+                for (int n = 0; n < QB; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[n][u][r] = 0.0f;
+#pragma unroll
+                for (int p = 0; p < kSteps; ++p) {
+                    const auto f = Tile::along(lk, 32 * (u0 + u), p, lane);
+#pragma unroll
+                    for (int n = 0; n < QB; ++n) S::multiply(f, q[n][p], s[n][u]);
+                }
+            }
+            if (bits != kAll) {
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const uint32_t w = (uint32_t)(bits >> (32 * (u0 + u))) >> (4 * (lane >> 5));
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+#pragma unroll
+                        for (int n = 0; n < QB; ++n)
+                            s[n][u][r] = w & (1u << ((r & 3) + 8 * (r >> 2))) ? s[n][u][r] : -INFINITY;
+                }
+            }
+            float new_top[QB];
+            bool passed = false;
+#pragma unroll
+            for (int n = 0; n < QB; ++n) {
+                float m = s[n][0][0];
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) m = fmaxf(m, s[n][u][r]);
+                float other = m;
+                swap32(m, other);
+                new_top[n] = fmaxf(fmaxf(m, other), top[n]);   // a NaN goes into the weights instead
+                passed |= (new_top[n] - top[n]) * g.c > kLazy;
+            }
+            if (ballot(passed)) {
+#pragma unroll
+                for (int n = 0; n < QB; ++n) {
+                    const float to = new_top[n] == -INFINITY ? 0.0f : new_top[n];
+                    const float keep = __builtin_amdgcn_exp2f(fmaf(top[n], g.c, -to * g.c));
+                    top[n] = new_top[n];
+                    sum[n] *= keep;
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) out[n][c][r] *= keep;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < QB; ++n) {
+                const float less = -(top[n] == -INFINITY ? 0.0f : top[n]) * g.c;
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        s[n][u][r] = __builtin_amdgcn_exp2f(fmaf(s[n][u][r], g.c, less));
+                        sum[n] += s[n][u][r];
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    typename S::Frag w[QB];
+#pragma unroll
+                    for (int n = 0; n < QB; ++n) w[n] = S::rounded(s[n][u], p);
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c) {
+                        const auto f = Tile::across(lv, 32 * (u0 + u) + p * S::kDepth, 32 * c, lane);
+#pragma unroll
+                        for (int n = 0; n < QB; ++n) S::multiply(f, w[n], out[n][c]);
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < QB; ++n) {
+        float other = sum[n];
+        swap32(sum[n], other);
+        sum[n] += other;
+        if (!exists[n]) continue;
+        const int64_t place = row[n] * a.heads + head[n];
+        if constexpr (SPLIT) {
+            const int64_t at = (int64_t)split * a.q.rows * a.heads + place;
+            if (lane < 32) {
+                g.tops[2 * at] = top[n];
+                g.tops[2 * at + 1] = sum[n];
+            }
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float v[8];
+                    square_rows(out[n][c], p, v);
+                    store_eight<float>(g.sums + at * D, 32 * c + 16 * p + 8 * (lane >> 5), D, v);
+                }
+        } else {
+            const float inv = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
+            T* to = (T*)a.out.p + row[n] * a.out.stride + (int64_t)head[n] * d;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float v[8];
+                    square_rows(out[n][c], p, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= inv;
+                    store_eight<T>(to, 32 * c + 16 * p + 8 * (lane >> 5), d, v);
+                }
+            if (a.lse && lane < 32)
+                a.lse[row[n] * a.lse_row_step + head[n] * a.lse_head_step] =
+                    sum[n] == 0.0f ? -INFINITY : fmaf(top[n], a.scale, logf(sum[n]));
+        }
+    }
+}
+
+// Joins the splits' sums: a wave for each row and head.
+template <class T, int D>
+__global__ void __launch_bounds__(256) join_kernel(Attention a, Grid g) {
+    const int lane = threadIdx.x & 63;
+    const int64_t n = a.q.rows * a.heads;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
+        float top = -INFINITY;
+        for (int k = 0; k < g.splits; ++k) top = fmaxf(top, g.tops[2 * (k * n + i)]);
+        const float less = -(top == -INFINITY ? 0.0f : top) * g.c;
+        float sum = 0.0f, v[(D + 63) / 64] = {};
+        for (int k = 0; k < g.splits; ++k) {
+            const int64_t at = k * n + i;
+            const float w = __builtin_amdgcn_exp2f(fmaf(g.tops[2 * at], g.c, less));
+            sum = fmaf(w, g.tops[2 * at + 1], sum);
+#pragma unroll
+            for (int c = 0; c < (D + 63) / 64; ++c)
+                if (64 * c + lane < D) v[c] = fmaf(w, g.sums[at * D + 64 * c + lane], v[c]);
+        }
+        const int64_t r = i / a.heads;
+        const int h = (int)(i % a.heads);
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        T* to = (T*)a.out.p + r * a.out.stride + (int64_t)h * a.head;
+#pragma unroll
+        for (int c = 0; c < (D + 63) / 64; ++c)
+            if (64 * c + lane < a.head) to[64 * c + lane] = (T)(v[c] * inv);
+        if (a.lse && lane == 0)
+            a.lse[r * a.lse_row_step + h * a.lse_head_step] =
+                sum == 0.0f ? -INFINITY : fmaf(top, a.scale, logf(sum));
+    }
+}
+
+struct Plan {
+    int qb, kt;
+    Grid grid;
+    int64_t workgroups;
+    size_t bytes;
+};
+
+constexpr int kWaves = 4;
+
+Plan plan_of(const Attention& a) {
+    Plan p{};
+    const bool wide = a.dtype != TGS_DTYPE_FLOAT32;
+    p.grid.shared = a.heads / a.kv_heads;
+    p.grid.rows = a.queries * p.grid.shared;
+    p.kt = wide ? 64 : 32;
+    p.qb = wide && p.grid.rows > 32 * kWaves ? 2 : 1;
+    p.grid.blocks = (p.grid.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
+    p.grid.c = exponent_of(a.scale);
+    const int64_t whole = a.batch * a.kv_heads * p.grid.blocks, tiles = (a.states + p.kt - 1) / p.kt;
+    int64_t splits = 1;
+    if (whole < 256 && tiles > 1) {
+        splits = 512 / whole < tiles ? 512 / whole : tiles;
+        p.grid.tiles = (int)((tiles + splits - 1) / splits);
+        splits = (tiles + p.grid.tiles - 1) / p.grid.tiles;
+    }
+    if (splits == 1) p.grid.tiles = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
+    p.grid.splits = (int)splits;
+    p.workgroups = whole * splits;
+    const int64_t width = (a.head + 31) / 32 * 32;
+    if (splits > 1) p.bytes = sizeof(float) * (size_t)(splits * a.q.rows * a.heads * (width + 2));
+    return p;
 }
 
 }  // namespace
 
-size_t attention_workspace(const Attention&) { return 0; }
+size_t attention_workspace(const Attention& a) { return plan_of(a).bytes; }
 
-int launch_attention(const Attention& a, void*, hipStream_t s) {
-    const int64_t most = (1 << 20) / a.heads;   // a launch of 2^32 threads or more loses what is above
-    const dim3 grid((unsigned)(a.q.rows < most ? a.q.rows : most), (unsigned)a.heads);
-    by_dtype(a.dtype, [&](auto t) { attention_kernel<decltype(t)><<<grid, 64, 0, s>>>(a); });
+int launch_attention(const Attention& a, void* workspace, hipStream_t s) {
+    Plan p = plan_of(a);
+    by_dtype(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        by_head_width(a.head, [&](auto width) {
+            constexpr int D = decltype(width)::value, KT = sizeof(T) == 2 ? 64 : 32;
+            p.grid.sums = (float*)workspace;
+            p.grid.tops = p.grid.sums + (p.grid.splits > 1 ? p.grid.splits * a.q.rows * a.heads * D : 0);
+            // a launch of 2^32 threads or more loses what is above
+            constexpr int64_t kMost = ((int64_t)1 << 32) / (64 * kWaves) / 2;
+            for (p.grid.first = 0; p.grid.first < p.workgroups; p.grid.first += kMost) {
+                const int64_t left = p.workgroups - p.grid.first;
+                const unsigned n = (unsigned)(left < kMost ? left : kMost);
+                const auto launch = [&](auto qb, auto split) {
+                    attention_kernel<T, D, decltype(qb)::value, kWaves, KT, decltype(split)::value != 0>
+                        <<<n, 64 * kWaves, 0, s>>>(a, p.grid);
+                };
+                const auto by_split = [&](auto qb) {
+                    if (p.grid.splits > 1) launch(qb, Constant<1>{});
+                    else launch(qb, Constant<0>{});
+                };
+                if constexpr (sizeof(T) == 2) {
+                    if (p.qb == 2) by_split(Constant<2>{});
+                    else by_split(Constant<1>{});
+                } else {
+                    by_split(Constant<1>{});
+                }
+            }
+            if (p.grid.splits > 1) {
+                const int64_t n = (a.q.rows * a.heads + 3) / 4;
+                join_kernel<T, D><<<(unsigned)(n < 65536 ? n : 65536), 256, 0, s>>>(a, p.grid);
+            }
+        });
+    });
     TGS_CHECK_LAUNCH();
     return TGS_OK;
 }
