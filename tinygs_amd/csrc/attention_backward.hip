@@ -1,22 +1,100 @@
 // The gradients of attention.hip from its out and lse: p = exp(s - lse),
 // delta = sum of do o over a head, dv = p^T do, ds = p (do v^T - delta),
 // dq = scale ds k, dk = scale ds^T q.
+//
+// Two kernels, each with what it sums in registers and the other side in tiles
+// through LDS: dq has rows in the lanes, s^T = k q^T and dp^T = v do^T, and adds
+// k^T ds^T; dk and dv have states in the lanes, s = q k^T and dp = do v^T, and
+// add do^T p and q^T ds. Weights and their gradients are operands as they stand
+// in both. The scores are formed twice (seven products in place of five); in
+// one kernel, either sum would have to leave it in as many parts as there are
+// blocks of the other side.
+//
+// Halves: p is held times 2^10, and ds times a power of two that each lane
+// chooses by the largest it met, so that small ones keep their bits; sums are
+// scaled where it changes.
 #include <math.h>
 
-#include "network.h"
+#include <algorithm>
+
+#include "attention.h"
 
 namespace tgs {
 
 namespace {
 
-constexpr int kMaxHead = 128;
+constexpr int kWaves = 4;
 
 template <class T>
-__device__ __forceinline__ const T* at(const Mat& m, int64_t r, int c) {
-    return (const T*)m.p + r * m.stride + c;
+constexpr float kBoost = 0.0f;   // of p, in powers of two
+template <>
+constexpr float kBoost<_Float16> = 10.0f;
+
+struct Grid {
+    int64_t first;    // number of the launch's first workgroup
+    int64_t blocks;   // of rows (of states), for each batch element and head of the states
+    int64_t rows;     // queries x shared heads
+    int64_t units;    // dk, dv: tiles of rows, of all shared heads
+    int shared;
+    int splits;
+    int64_t part;     // tiles of a split
+    float c;          // scale log2(e)
+    float* delta;     // [row][head]
+    float* sums;      // the splits' parts
+};
+
+// A power of two for each lane by which small gradients of weights are lifted into a half's range.
+struct Lift {
+    float by = 0x1p100f;   // nothing met yet
+
+    // largest: of the lane's column, the same in both halves. Whether the sums have to be multiplied by *change.
+    __device__ __forceinline__ bool meet(float largest, float* change) {
+        const bool passed = !(largest * by <= 0x1p14f);   // NaN and infinity: any power keeps them
+        *change = 1.0f;
+        if (passed) {
+            const float to = __builtin_ldexpf(1.0f, 7 - __builtin_amdgcn_frexp_expf(largest));
+            *change = to / by;
+            by = to;
+        }
+        return ballot(passed) != 0;
+    }
+};
+
+// ds in place of dp's square, from p's; halves: lifted, the sums with it.
+template <class T, int N>
+__device__ __forceinline__ void lift_weights(f32x16& ds, Lift& lift, f32x16 (&sums)[N]) {
+    if constexpr (sizeof(T) == 2 && kBoost<T> != 0.0f) {
+        float largest = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) largest = fmaxf(largest, fabsf(ds[r]));
+        float other = largest;
+        swap32(largest, other);
+        largest = fmaxf(largest, other);
+        float change;
+        if (lift.meet(largest, &change)) {
+#pragma unroll
+            for (int c = 0; c < N; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sums[c][r] *= change;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] *= lift.by;
+    }
 }
 
-// delta[row, head]
+// What undoes the lift and p's boost in a sum of lifted gradients.
+template <class T>
+__device__ __forceinline__ float lowered(const Lift& lift) {
+    return kBoost<T> != 0.0f ? 0x1p-10f / lift.by : 1.0f;
+}
+
+// lse in the exponent's unit; +infinity where there is no state: all weights are 0.
+template <class T>
+__device__ __forceinline__ float lse_exponent(float lse) {
+    return lse == -INFINITY ? INFINITY : lse * kLog2E - kBoost<T>;
+}
+
+// delta, where dq is not asked for; in the order that the two halves of a wave sum it there
 template <class T>
 __global__ void __launch_bounds__(256) delta_kernel(AttentionBackward b, float* delta) {
     const Attention& a = b.a;
@@ -24,124 +102,439 @@ __global__ void __launch_bounds__(256) delta_kernel(AttentionBackward b, float* 
     for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
         const int64_t r = k / a.heads;
         const int h = (int)(k % a.heads);
-        const T *x = at<T>(b.grad_out, r, h * a.head), *y = at<T>(a.out, r, h * a.head);
+        const T* x = (const T*)b.grad_out.p + r * b.grad_out.stride + (int64_t)h * a.head;
+        const T* y = (const T*)a.out.p + r * a.out.stride + (int64_t)h * a.head;
+        float v[2] = {0.0f, 0.0f};
+        for (int c = 0; c < a.head; ++c) {
+            const int half = c / (16 / (int)sizeof(T)) & 1;
+            v[half] = fmaf((float)x[c], (float)y[c], v[half]);
+        }
+        delta[k] = v[0] + v[1];
+    }
+}
+
+template <class T, int D, int QB, int KT, bool SPLIT>
+__global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(AttentionBackward b, Grid g) {
+    using S = Square<T>;
+    using Tile = RowTile<T, D, KT, kWaves>;
+    constexpr int kSteps = D / S::kDepth, kParts = 32 / S::kDepth, kSubs = KT / 32, kCols = D / 32;
+    constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
+    __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes];
+    const Attention& a = b.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t number = g.first + xcd_contiguous_index(blockIdx.x, gridDim.x);
+    const int split = SPLIT ? (int)(number % g.splits) : 0;
+    const int64_t block = (SPLIT ? number / g.splits : number) % g.blocks;
+    const int64_t pair = (SPLIT ? number / g.splits : number) / g.blocks;
+    const int64_t e = pair / a.kv_heads;
+    const int kv = (int)(pair % a.kv_heads), d = a.head;
+
+    int64_t row[QB];
+    int head[QB];
+    bool exists[QB];
+    typename S::Frag q[QB][kSteps], go[QB][kSteps];
+    float lse[QB], delta[QB];
+#pragma unroll
+    for (int n = 0; n < QB; ++n) {
+        const int64_t i = ((block * kWaves + wave) * QB + n) * 32 + (lane & 31);
+        exists[n] = i < g.rows;
+        const int64_t r = g.shared == 1 ? i : i / g.shared;
+        head[n] = kv * g.shared + (g.shared == 1 ? 0 : (int)(i - r * g.shared));
+        row[n] = e * a.queries + r;
+        const T* p = (const T*)a.q.p + row[n] * a.q.stride + (int64_t)head[n] * d;
+        const T* x = (const T*)b.grad_out.p + row[n] * b.grad_out.stride + (int64_t)head[n] * d;
+        const T* y = (const T*)a.out.p + row[n] * a.out.stride + (int64_t)head[n] * d;
+        float dot = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int c = 2 * s + (lane >> 5);
+            q[n][s] = row_chunk<T>(p, c, d, exists[n]);
+            go[n][s] = row_chunk<T>(x, c, d, exists[n]);
+            const auto o = row_chunk<T>(y, c, d, exists[n]);
+#pragma unroll
+            for (int k = 0; k < 16 / (int)sizeof(T); ++k) dot = fmaf((float)go[n][s][k], (float)o[k], dot);
+        }
+        float other = dot;
+        swap32(dot, other);
+        delta[n] = dot + other;
+        lse[n] = INFINITY;
+        if (exists[n]) {
+            lse[n] = lse_exponent<T>(a.lse[row[n] * a.lse_row_step + head[n] * a.lse_head_step]);
+            if (lane < 32 && split == 0) g.delta[row[n] * a.heads + head[n]] = delta[n];
+        }
+    }
+
+    Tile tk, tv;
+    const int64_t k_pitch = a.k.stride * (int64_t)sizeof(T), v_pitch = a.v.stride * (int64_t)sizeof(T);
+    tk.begin(k_pitch, d, wave, lane);
+    tv.begin(v_pitch, d, wave, lane);
+    const unsigned char* k0 = (const unsigned char*)a.k.p + e * a.states * k_pitch + (int64_t)kv * d * sizeof(T);
+    const unsigned char* v0 = (const unsigned char*)a.v.p + e * a.states * v_pitch + (int64_t)kv * d * sizeof(T);
+    const int64_t k_end = (a.states - 1) * k_pitch + d * (int64_t)sizeof(T);
+    const int64_t v_end = (a.states - 1) * v_pitch + d * (int64_t)sizeof(T);
+    const uint8_t* mask = a.mask ? a.mask + e * a.mask_stride : nullptr;
+    const int64_t t1 = min((split + 1) * g.part, (a.states + KT - 1) / KT);
+    int64_t t = split * g.part - 1;
+    const auto state_exists = [&](int64_t tile) {
+        const int64_t j = tile * KT + lane;
+        return lane < KT && j < a.states && (!mask || mask[j]);
+    };
+    bool next = state_exists(t + 1);
+    uint64_t exist = 0;
+    const auto load = [&](int buffer) {   // as the forward's
+        do {
+            if (++t >= t1) return false;
+            exist = ballot(next);
+            next = state_exists(t + 1);
+        } while (exist == 0);
+        tk.load(lds[buffer][0], k0 + t * KT * k_pitch, k_end - t * KT * k_pitch, exist, d, wave, lane);
+        tv.load(lds[buffer][1], v0 + t * KT * v_pitch, v_end - t * KT * v_pitch, exist, d, wave, lane);
+        return true;
+    };
+
+    f32x16 sums[QB][kCols];
+    Lift lift[QB];
+#pragma unroll
+    for (int n = 0; n < QB; ++n)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sums[n][c][r] = 0.0f;
+    int buffer = 0;
+    bool more = load(0);
+    while (more) {
+        const uint64_t bits = exist;
+        wait_for_stage<1>(0);
+        more = load(buffer ^ 1);
+        const unsigned char *lk = lds[buffer][0], *lv = lds[buffer][1];
+        buffer ^= 1;
+#pragma unroll 1
+        for (int u = 0; u < kSubs; ++u) {
+            f32x16 s[QB], dp[QB];
+#pragma unroll
+            for (int n = 0; n < QB; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[n][r] = dp[n][r] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < kSteps; ++p) {
+                const auto f = Tile::along(lk, 32 * u, p, lane);
+#pragma unroll
+                for (int n = 0; n < QB; ++n) S::multiply(f, q[n][p], s[n]);
+                const auto w = Tile::along(lv, 32 * u, p, lane);
+#pragma unroll
+                for (int n = 0; n < QB; ++n) S::multiply(w, go[n][p], dp[n]);
+            }
+            if (bits != kAll) {
+                const uint32_t w = (uint32_t)(bits >> (32 * u)) >> (4 * (lane >> 5));
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+#pragma unroll
+                    for (int n = 0; n < QB; ++n)
+                        s[n][r] = w & (1u << ((r & 3) + 8 * (r >> 2))) ? s[n][r] : -INFINITY;
+            }
+#pragma unroll
+            for (int n = 0; n < QB; ++n) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    dp[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], g.c, -lse[n])) * (dp[n][r] - delta[n]);
+                lift_weights<T>(dp[n], lift[n], sums[n]);
+            }
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+                typename S::Frag w[QB];
+#pragma unroll
+                for (int n = 0; n < QB; ++n) w[n] = S::rounded(dp[n], p);
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    const auto f = Tile::across(lk, 32 * u + p * S::kDepth, 32 * c, lane);
+#pragma unroll
+                    for (int n = 0; n < QB; ++n) S::multiply(f, w[n], sums[n][c]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < QB; ++n) {
+        if (!exists[n]) continue;
+        const float by = a.scale * lowered<T>(lift[n]);
+        const int64_t at = ((int64_t)split * a.q.rows + row[n]) * a.heads + head[n];
+        T* to = SPLIT ? nullptr : (T*)b.grad_q.p + row[n] * b.grad_q.stride + (int64_t)head[n] * d;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                float v[8];
+                square_rows(sums[n][c], p, v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] *= by;
+                const int c0 = 32 * c + 16 * p + 8 * (lane >> 5);
+                if constexpr (SPLIT) store_eight<float>(g.sums + at * D, c0, D, v);
+                else store_eight<T>(to, c0, d, v);
+            }
+    }
+}
+
+// Tiles of QT rows of one of the shared heads at a time; a wave has 32 states.
+template <class T, int D, int QT, bool SPLIT>
+__global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(AttentionBackward b, Grid g) {
+    using S = Square<T>;
+    using Tile = RowTile<T, D, QT, kWaves>;
+    constexpr int kSteps = D / S::kDepth, kParts = 32 / S::kDepth, kSubs = QT / 32, kCols = D / 32;
+    __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes];
+    __shared__ __align__(16) float row_lse[2][QT], row_delta[2][QT];
+    const Attention& a = b.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t number = g.first + xcd_contiguous_index(blockIdx.x, gridDim.x);
+    // blocks of states that read the same rows are neighbours
+    const int64_t block = number % g.blocks, split = number / g.blocks % g.splits, pair = number / g.blocks / g.splits;
+    const int64_t e = pair / a.kv_heads;
+    const int kv = (int)(pair % a.kv_heads), d = a.head;
+
+    const int64_t j = (block * kWaves + wave) * 32 + (lane & 31);   // the lane's state
+    const bool inside = j < a.states;
+    const bool exists = inside && (!a.mask || a.mask[e * a.mask_stride + j]);
+    const int64_t state = e * a.states + j;
+    typename S::Frag k[kSteps], v[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int c = 2 * s + (lane >> 5);
+        k[s] = row_chunk<T>((const T*)a.k.p + state * a.k.stride + (int64_t)kv * d, c, d, exists);
+        v[s] = row_chunk<T>((const T*)a.v.p + state * a.v.stride + (int64_t)kv * d, c, d, exists);
+    }
+
+    Tile tq, to;
+    const int64_t q_pitch = a.q.stride * (int64_t)sizeof(T), o_pitch = b.grad_out.stride * (int64_t)sizeof(T);
+    tq.begin(q_pitch, d, wave, lane);
+    to.begin(o_pitch, d, wave, lane);
+    const unsigned char* q0 = (const unsigned char*)a.q.p + e * a.queries * q_pitch + (int64_t)kv * g.shared * d * sizeof(T);
+    const unsigned char* o0 =
+        (const unsigned char*)b.grad_out.p + e * a.queries * o_pitch + (int64_t)kv * g.shared * d * sizeof(T);
+    const int64_t per_head = g.units / g.shared;
+    const int64_t t1 = min((split + 1) * g.part, g.units);
+    int64_t t = split * g.part - 1;
+    int h = (int)((t + 1) / per_head);         // of the next tile, among the shared heads
+    int64_t in = (t + 1) - h * per_head - 1;   // the tile's number in its head
+    float value = 0.0f;                        // of the thread's row: lse, or delta, on its way to LDS
+    const int of = threadIdx.x % QT;
+    const auto load = [&](int buffer) {
+        if (++t >= t1) return false;
+        if (++in == per_head) {
+            in = 0;
+            ++h;
+        }
+        const int64_t r0 = in * QT, left = a.queries - r0;
+        const uint64_t exist = left >= 64 ? ~0ull : (1ull << left) - 1;
+        const uint64_t bits = QT == 64 ? exist : exist & ((1ull << (QT & 63)) - 1);
+        const int64_t at = (int64_t)h * d * (int64_t)sizeof(T);
+        const int64_t width = d * (int64_t)sizeof(T);
+        tq.load(lds[buffer][0], q0 + at + r0 * q_pitch, (left - 1) * q_pitch + width, bits, d, wave, lane);
+        to.load(lds[buffer][1], o0 + at + r0 * o_pitch, (left - 1) * o_pitch + width, bits, d, wave, lane);
+        const int64_t row = e * a.queries + r0 + of;
+        const int head = kv * g.shared + h;
+        if (threadIdx.x < QT)
+            value = of < left ? lse_exponent<T>(a.lse[row * a.lse_row_step + head * a.lse_head_step]) : INFINITY;
+        else if (threadIdx.x < 2 * QT)
+            value = of < left ? g.delta[row * a.heads + head] : 0.0f;
+        return true;
+    };
+
+    f32x16 gk[kCols], gv[kCols];
+    Lift lift;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) gk[c][r] = gv[c][r] = 0.0f;
+    int buffer = 0;
+    bool more = load(0);
+    while (more) {
+        if (threadIdx.x < QT) row_lse[buffer][of] = value;
+        else if (threadIdx.x < 2 * QT) row_delta[buffer][of] = value;
+        wait_for_stage<1>(0);
+        more = load(buffer ^ 1);
+        const unsigned char *lq = lds[buffer][0], *lo = lds[buffer][1];
+        const float *le = row_lse[buffer], *de = row_delta[buffer];
+        buffer ^= 1;
+#pragma unroll 1
+        for (int u = 0; u < kSubs; ++u) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < kSteps; ++p) {
+                S::multiply(Tile::along(lq, 32 * u, p, lane), k[p], s);
+                S::multiply(Tile::along(lo, 32 * u, p, lane), v[p], dp);
+            }
+#pragma unroll
+            for (int r0 = 0; r0 < 16; r0 += 4) {
+                const int at = 32 * u + square_row(r0, lane);
+                const f32x4 l4 = *(const f32x4*)(le + at), d4 = *(const f32x4*)(de + at);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[r0 + r] = __builtin_amdgcn_exp2f(fmaf(s[r0 + r], g.c, -l4[r]));
+                    dp[r0 + r] = s[r0 + r] * (dp[r0 + r] - d4[r]);
+                }
+            }
+            lift_weights<T>(dp, lift, gk);
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+                const auto w = S::rounded(s, p), x = S::rounded(dp, p);
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    S::multiply(Tile::across(lo, 32 * u + p * S::kDepth, 32 * c, lane), w, gv[c]);
+                    S::multiply(Tile::across(lq, 32 * u + p * S::kDepth, 32 * c, lane), x, gk[c]);
+                }
+            }
+        }
+    }
+    if (!inside) return;
+    // a state that does not exist gets zeros, whatever the rows hold
+    const float by_k = a.scale * lowered<T>(lift), by_v = kBoost<T> != 0.0f ? 0x1p-10f : 1.0f;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            float x[8], y[8];
+            square_rows(gk[c], p, x);
+            square_rows(gv[c], p, y);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                x[n] = exists ? x[n] * by_k : 0.0f;
+                y[n] = exists ? y[n] * by_v : 0.0f;
+            }
+            const int c0 = 32 * c + 16 * p + 8 * (lane >> 5);
+            if constexpr (SPLIT) {
+                const int64_t n = a.k.rows * a.kv_heads, at = state * a.kv_heads + kv;
+                store_eight<float>(g.sums + ((2 * split) * n + at) * D, c0, D, x);
+                store_eight<float>(g.sums + ((2 * split + 1) * n + at) * D, c0, D, y);
+            } else {
+                if (b.grad_k.p) store_eight<T>((T*)b.grad_k.p + state * b.grad_k.stride + (int64_t)kv * d, c0, d, x);
+                if (b.grad_v.p) store_eight<T>((T*)b.grad_v.p + state * b.grad_v.stride + (int64_t)kv * d, c0, d, y);
+            }
+        }
+}
+
+// Sums of the splits' parts, in their order: set `n` x D floats, `step` sets apart.
+template <class T, int D>
+__global__ void __launch_bounds__(256) join_kernel(const float* sums, int splits, int64_t step, Mat to, int heads, int d) {
+    const int64_t n = to.rows * heads * d;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t at = i / d, row = at / heads;
+        const int c = (int)(i - at * d), h = (int)(at - row * heads);
         float v = 0.0f;
-        for (int c = 0; c < a.head; ++c) v = fmaf((float)x[c], (float)y[c], v);
-        delta[k] = v;
+#pragma unroll 8
+        for (int k = 0; k < splits; ++k) v += sums[(k * step + at) * D + c];
+        ((T*)to.p)[row * to.stride + (int64_t)h * d + c] = (T)v;
     }
 }
 
-// One wave a row and head, as the forward's.
-template <class T>
-__global__ void __launch_bounds__(64) grad_q_kernel(AttentionBackward b, const float* delta) {
-    __shared__ float q[kMaxHead], go[kMaxHead], ds[64];
-    const Attention& a = b.a;
-    const int lane = threadIdx.x, d = a.head, h = blockIdx.y, g = h / (a.heads / a.kv_heads);
-    for (int64_t r = blockIdx.x; r < a.q.rows; r += gridDim.x) {
-        const int64_t e = r / a.queries;
-        const uint8_t* mask = a.mask ? a.mask + e * a.mask_stride : nullptr;
-        for (int c = lane; c < d; c += 64) {
-            q[c] = (float)*at<T>(a.q, r, h * d + c);
-            go[c] = (float)*at<T>(b.grad_out, r, h * d + c);
-        }
-        __syncthreads();
-        const float lse = a.lse[r * a.lse_row_step + h * a.lse_head_step], del = delta[r * a.heads + h];
-        float o[2] = {0.0f, 0.0f};
-        for (int64_t j0 = 0; j0 < a.states; j0 += 64) {
-            const int64_t j = j0 + lane;
-            float v = 0.0f;
-            if (j < a.states && (!mask || mask[j]) && lse != -INFINITY) {
-                const T *k = at<T>(a.k, e * a.states + j, g * d), *w = at<T>(a.v, e * a.states + j, g * d);
-                float s = 0.0f, dp = 0.0f;
-                for (int c = 0; c < d; ++c) {
-                    s = fmaf(q[c], (float)k[c], s);
-                    dp = fmaf(go[c], (float)w[c], dp);
-                }
-                v = expf(s * a.scale - lse) * (dp - del) * a.scale;
-            }
-            ds[lane] = v;
-            __syncthreads();
-            for (int n = 0; n < 2; ++n) {
-                const int c = lane + 64 * n;
-                if (c < d)
-                    for (int k = 0; k < 64 && j0 + k < a.states; ++k)
-                        if (!mask || mask[j0 + k]) o[n] = fmaf(ds[k], (float)*at<T>(a.k, e * a.states + j0 + k, g * d + c), o[n]);
-            }
-            __syncthreads();
-        }
-        for (int n = 0; n < 2; ++n)
-            if (lane + 64 * n < d) ((T*)b.grad_q.p)[r * b.grad_q.stride + h * d + lane + 64 * n] = (T)o[n];
-    }
+float exponent_of(float scale) { return scale > 0.0f ? fmaxf(scale * kLog2E, 0x1p-149f) : 0x1p-149f; }
+
+// The splits of `tiles` for about 512 workgroups, and a split's tiles.
+void split_tiles(int64_t whole, int64_t tiles, int& splits, int64_t& part) {
+    int64_t n = 1;
+    if (whole > 0 && whole < 256 && tiles > 1) n = 512 / whole < tiles ? 512 / whole : tiles;
+    part = tiles > 0 ? (tiles + n - 1) / n : 1;
+    splits = tiles > 0 ? (int)((tiles + part - 1) / part) : 1;
 }
 
-// One wave a state and head of the states: a lane takes a row of 64, then a column or two.
-template <class T>
-__global__ void __launch_bounds__(64) grad_kv_kernel(AttentionBackward b, const float* delta) {
-    __shared__ float k[kMaxHead], v[kMaxHead], ps[64], ds[64];
+struct Plan {
+    int qb, tile;
+    Grid q, kv;
+    int64_t q_workgroups, kv_workgroups;
+    size_t delta_bytes, bytes;
+};
+
+Plan plan_of(const AttentionBackward& b) {
     const Attention& a = b.a;
-    const int lane = threadIdx.x, d = a.head, g = blockIdx.y, shared = a.heads / a.kv_heads;
-    for (int64_t j = blockIdx.x; j < a.k.rows; j += gridDim.x) {
-        const int64_t e = j / a.states;
-        const bool exists = !a.mask || a.mask[e * a.mask_stride + j % a.states];
-        for (int c = lane; c < d; c += 64) {
-            k[c] = (float)*at<T>(a.k, j, g * d + c);
-            v[c] = (float)*at<T>(a.v, j, g * d + c);
-        }
-        __syncthreads();
-        float gk[2] = {0.0f, 0.0f}, gv[2] = {0.0f, 0.0f};
-        for (int h = g * shared; exists && h < (g + 1) * shared; ++h)
-            for (int64_t r0 = e * a.queries; r0 < (e + 1) * a.queries; r0 += 64) {
-                const int64_t r = r0 + lane;
-                float p = 0.0f, x = 0.0f;
-                if (r < (e + 1) * a.queries && a.lse[r * a.lse_row_step + h * a.lse_head_step] != -INFINITY) {
-                    const T *q = at<T>(a.q, r, h * d), *go = at<T>(b.grad_out, r, h * d);
-                    float s = 0.0f, dp = 0.0f;
-                    for (int c = 0; c < d; ++c) {
-                        s = fmaf(k[c], (float)q[c], s);
-                        dp = fmaf(v[c], (float)go[c], dp);
-                    }
-                    p = expf(s * a.scale - a.lse[r * a.lse_row_step + h * a.lse_head_step]);
-                    x = p * (dp - delta[r * a.heads + h]) * a.scale;
-                }
-                ps[lane] = p;
-                ds[lane] = x;
-                __syncthreads();
-                for (int n = 0; n < 2; ++n) {
-                    const int c = lane + 64 * n;
-                    if (c < d)
-                        for (int i = 0; i < 64 && r0 + i < (e + 1) * a.queries; ++i) {
-                            gv[n] = fmaf(ps[i], (float)*at<T>(b.grad_out, r0 + i, h * d + c), gv[n]);
-                            gk[n] = fmaf(ds[i], (float)*at<T>(a.q, r0 + i, h * d + c), gk[n]);
-                        }
-                }
-                __syncthreads();
-            }
-        for (int n = 0; n < 2; ++n)
-            if (lane + 64 * n < d) {
-                const int c = g * d + lane + 64 * n;
-                if (b.grad_k.p) ((T*)b.grad_k.p)[j * b.grad_k.stride + c] = (T)gk[n];
-                if (b.grad_v.p) ((T*)b.grad_v.p)[j * b.grad_v.stride + c] = (T)gv[n];
-            }
-        __syncthreads();
-    }
+    Plan p{};
+    const bool halves = a.dtype != TGS_DTYPE_FLOAT32;
+    const int64_t width = (a.head + 31) / 32 * 32;
+    p.tile = halves ? 64 : 32;
+    p.q.shared = p.kv.shared = a.heads / a.kv_heads;
+    p.q.rows = p.kv.rows = a.queries * p.q.shared;
+    p.q.c = p.kv.c = exponent_of(a.scale);
+    p.qb = halves && p.q.rows > 32 * kWaves ? 2 : 1;
+    p.q.blocks = (p.q.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
+    int64_t whole = a.batch * a.kv_heads * p.q.blocks;
+    split_tiles(whole, (a.states + p.tile - 1) / p.tile, p.q.splits, p.q.part);
+    p.q_workgroups = whole * p.q.splits;
+    p.kv.blocks = (a.states + 32 * kWaves - 1) / (32 * kWaves);
+    p.kv.units = (a.queries + p.tile - 1) / p.tile * p.kv.shared;
+    whole = a.batch * a.kv_heads * p.kv.blocks;
+    split_tiles(whole, p.kv.units, p.kv.splits, p.kv.part);
+    p.kv_workgroups = whole * p.kv.splits;
+    p.delta_bytes = (sizeof(float) * (size_t)(a.q.rows * a.heads) + 255) / 256 * 256;
+    size_t sums = 0;
+    if (b.grad_q.p && p.q.splits > 1) sums = sizeof(float) * (size_t)(p.q.splits * a.q.rows * a.heads * width);
+    if ((b.grad_k.p || b.grad_v.p) && p.kv.splits > 1)
+        sums = std::max(sums, sizeof(float) * 2 * (size_t)(p.kv.splits * a.k.rows * a.kv_heads * width));
+    p.bytes = p.delta_bytes + sums;
+    return p;
+}
+
+// f(workgroups) for launches below 2^32 threads; grid.first says where each starts.
+template <class F>
+void in_launches(Grid& grid, int64_t workgroups, F f) {
+    constexpr int64_t kMost = ((int64_t)1 << 32) / (64 * kWaves) / 2;
+    for (grid.first = 0; grid.first < workgroups; grid.first += kMost)
+        f((unsigned)(workgroups - grid.first < kMost ? workgroups - grid.first : kMost));
+}
+
+unsigned join_blocks(int64_t elements) {
+    const int64_t n = (elements + 255) / 256;
+    return (unsigned)(n < 8192 ? n : 8192);
 }
 
 }  // namespace
 
-size_t attention_backward_workspace(const AttentionBackward& b) { return sizeof(float) * (size_t)(b.a.q.rows * b.a.heads); }
+size_t attention_backward_workspace(const AttentionBackward& b) { return plan_of(b).bytes; }
 
 int launch_attention_backward(const AttentionBackward& b, void* workspace, hipStream_t s) {
     const Attention& a = b.a;
-    float* delta = (float*)workspace;
-    const auto grid = [](int64_t n, int64_t most) { return (unsigned)(n < most ? n : most); };
+    Plan p = plan_of(b);
+    p.q.delta = p.kv.delta = (float*)workspace;
+    p.q.sums = p.kv.sums = (float*)((unsigned char*)workspace + p.delta_bytes);
+    const bool states = (b.grad_k.p || b.grad_v.p) && a.k.rows > 0;
     by_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
-        if (a.q.rows) {
-            delta_kernel<T><<<grid((a.q.rows * a.heads + 255) / 256, 4096), 256, 0, s>>>(b, delta);
-            if (b.grad_q.p) grad_q_kernel<T><<<dim3(grid(a.q.rows, (1 << 20) / a.heads), (unsigned)a.heads), 64, 0, s>>>(b, delta);
-        }
-        if (a.k.rows && (b.grad_k.p || b.grad_v.p))
-            grad_kv_kernel<T><<<dim3(grid(a.k.rows, (1 << 20) / a.kv_heads), (unsigned)a.kv_heads), 64, 0, s>>>(b, delta);
+        by_head_width(a.head, [&](auto width) {
+            constexpr int D = decltype(width)::value, kTile = sizeof(T) == 2 ? 64 : 32;
+            if (b.grad_q.p && a.q.rows) {
+                const auto launch = [&](auto qb) {
+                    constexpr int QB = decltype(qb)::value;
+                    in_launches(p.q, p.q_workgroups, [&](unsigned n) {
+                        if (p.q.splits > 1) grad_q_kernel<T, D, QB, kTile, true><<<n, 64 * kWaves, 0, s>>>(b, p.q);
+                        else grad_q_kernel<T, D, QB, kTile, false><<<n, 64 * kWaves, 0, s>>>(b, p.q);
+                    });
+                };
+                if constexpr (sizeof(T) == 2) {
+                    if (p.qb == 2) launch(Constant<2>{});
+                    else launch(Constant<1>{});
+                } else {
+                    launch(Constant<1>{});
+                }
+                if (p.q.splits > 1)
+                    join_kernel<T, D><<<join_blocks(a.q.rows * a.heads * a.head), 256, 0, s>>>(
+                        p.q.sums, p.q.splits, a.q.rows * a.heads, b.grad_q, a.heads, a.head);
+            } else if (a.q.rows && states) {
+                const int64_t n = (a.q.rows * a.heads + 255) / 256;
+                delta_kernel<T><<<(unsigned)(n < 4096 ? n : 4096), 256, 0, s>>>(b, p.q.delta);
+            }
+            if (!states) return;
+            in_launches(p.kv, p.kv_workgroups, [&](unsigned n) {
+                if (p.kv.splits > 1) grad_kv_kernel<T, D, kTile, true><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
+                else grad_kv_kernel<T, D, kTile, false><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
+            });
+            if (p.kv.splits > 1) {
+                const int64_t n = a.k.rows * a.kv_heads;
+                const unsigned blocks = join_blocks(n * a.head);
+                if (b.grad_k.p)
+                    join_kernel<T, D><<<blocks, 256, 0, s>>>(p.kv.sums, p.kv.splits, 2 * n, b.grad_k, a.kv_heads, a.head);
+                if (b.grad_v.p)
+                    join_kernel<T, D><<<blocks, 256, 0, s>>>(p.kv.sums + n * D, p.kv.splits, 2 * n, b.grad_v, a.kv_heads,
+                                                             a.head);
+            }
+        });
     });
     TGS_CHECK_LAUNCH();
     return TGS_OK;
