@@ -307,3 +307,70 @@ def test_many_rows(ops):
     for got, want, terms in ((gv, gvw, p.t() @ go.double().abs()), (gk, gkw, ds.abs().t() @ q.double().abs() / 4.0)):
         bound = (2 ** -8 + 2 ** -12) * terms + 2 ** -8 * want.abs()
         assert bool(((got.double() - want).abs() <= bound).all())
+
+
+# batch, queries, states, heads, kv_heads, d, share of the states (None: no mask)
+LARGE = [(1, 70_003, 256, 4, 4, 64, None), (1, 70_003, 197, 4, 1, 64, 0.7), (2, 70_001, 130, 2, 2, 32, 0.5),
+         (3, 50_001, 65, 2, 1, 96, None), (1, 140_007, 256, 1, 1, 128, 0.9), (1, 60_001, 500, 3, 3, 24, None),
+         (1, 140_001, 1, 1, 1, 64, None), (2, 33_333, 320, 4, 2, 80, 0.8), (1, 9_001, 90, 16, 16, 64, None)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", LARGE, ids=lambda s: "x".join(map(str, s)))
+def test_many_rows_of_many_heads(ops, dtype, shape):
+    """The card full of rows: a sample of them checked in each element of the batch, the states' gradients against
+    float64 on the device. One element's states do not exist where there are several."""
+    batch, rows, states, heads, kv_heads, d, share = shape
+    q, k, v, go = case(rows + states, dtype, batch, rows, states, heads, kv_heads, d, 3)
+    m = None
+    if share is not None:
+        m = mask_of(states, batch, states, share, empty=(1,) if batch > 1 else ())
+        forget(k, m, float("nan"))
+        forget(v, m, float("nan"))
+    args = dict(kv_heads=kv_heads, batch=batch, mask=m)
+    print(f"[attention] large {shape} {dtype}", flush=True)
+    out, lse = ops.attention(q, k, v, heads, keep_lse=True, **args)
+    gq, gk, gv = ops.attention_backward(go, q, k, v, out, lse, heads, **args)
+    within = torch.cat([torch.arange(0, rows, 2777), torch.tensor([rows - 1])])
+    pick = (within[None, :] + rows * torch.arange(batch)[:, None]).reshape(-1).cuda()
+    qs, gs, os, ls = (x[pick].contiguous() for x in (q, go, out, lse))
+    (o, ob), (l, lb) = A.attention(qs, k, v, heads, kv_heads, batch, m)
+    A.check(os, o, ob, "out")
+    dead = l == -math.inf
+    assert torch.equal(ls.cpu() == -math.inf, dead)
+    A.check(torch.where(dead, torch.zeros_like(l), ls.cpu().double()), l.masked_fill(dead, 0.0), lb.masked_fill(dead, 0.0),
+            "lse")
+    x, b = A.attention_backward(gs, qs, k, v, os, ls, heads, kv_heads, batch, m)[0]
+    A.check(gq[pick], x, b, "grad_q")
+    unit = A.UNIT[dtype]
+    for e in range(batch):
+        at, of = slice(e * rows, (e + 1) * rows), slice(e * states, (e + 1) * states)
+        there = torch.ones(states, dtype=torch.bool, device="cuda") if m is None else m[e]
+        for g in range(kv_heads):
+            cols = slice(g * d, (g + 1) * d)
+            ke, ve = (t[of, cols].double()[there] for t in (k, v))
+            sums = [torch.zeros_like(ke) for _ in range(4)]
+            own = torch.zeros_like(ke)
+            for h in range(g * heads // kv_heads, (g + 1) * heads // kv_heads):
+                hc = slice(h * d, (h + 1) * d)
+                qe, oe, ye = (t[at, hc].double() for t in (q, go, out))
+                p = torch.exp(qe @ ke.t() / math.sqrt(d) - lse[at, h].double()[:, None])
+                ds = p * (oe @ ve.t() - (oe * ye).sum(1, keepdim=True))
+                sums[0] += p.t() @ oe
+                sums[1] += p.t() @ oe.abs()
+                sums[2] += ds.t() @ qe / math.sqrt(d)
+                sums[3] += ds.abs().t() @ qe.abs() / math.sqrt(d)
+                # dp and delta are sums of d products each: off by (d + 17) 2^-24 of their terms' sizes, whatever
+                # is left of them in the difference (nothing, for a single state)
+                size = oe.abs() @ ve.abs().t() + (oe * ye).abs().sum(1, keepdim=True)
+                own += (d + 20) * A.EPS24 * (p * size).t() @ qe.abs() / math.sqrt(d)
+            # weights are rounded once: by a unit each at most, with the scores' error (d + 17 roundings of terms of
+            # a few units' size, 2^-15 at the most here) and the sums' over as many rows, each far below a unit of
+            # 16-bit types; floats: 2^-14 of the terms
+            rel = max(unit + 2.0 ** -14, 2.0 ** -14)
+            step = 2.0 ** -24 * 70 if dtype == torch.float16 else 0.0   # products' and results' smallest steps
+            for got, want, terms, more in ((gv, sums[0], sums[1], 0.0), (gk, sums[2], sums[3], own)):
+                y = got[of, cols].double()
+                assert not y[~there].any()
+                bound = rel * terms + 1.01 * more + unit * want.abs() + step
+                assert bool(((y[there] - want).abs() <= bound).all()), (shape, e, g)

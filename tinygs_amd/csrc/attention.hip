@@ -29,6 +29,7 @@ struct Grid {
     int shared;
     int splits;          // of the states
     int tiles;           // of a split
+    int64_t part;        // held states: blocks of a wave's rows for each workgroup
     float c;             // scale log2(e)
     float* sums;         // of a split's parts: [splits][all rows][D], then m and l
     float* tops;
@@ -38,15 +39,184 @@ struct Grid {
 // that -infinity stays -infinity.
 float exponent_of(float scale) { return scale > 0.0f ? fmaxf(scale * kLog2E, 0x1p-149f) : 0x1p-149f; }
 
+// A wave's 32 or 64 rows on their way over the states.
+template <class T, int D, int QB>
+struct WaveRows {
+    using S = Square<T>;
+    static constexpr int kSteps = D / S::kDepth;    // of the scores' product
+    static constexpr int kParts = 32 / S::kDepth;   // of a square's rows as an operand
+    static constexpr int kCols = D / 32;
+    int64_t row[QB];
+    int head[QB];
+    bool exists[QB];
+    typename S::Frag q[QB][kSteps];
+    f32x16 out[QB][kCols];   // sums of weights times v
+    float top[QB], sum[QB];
+
+    // Rows from number i0 on of batch element b and head kv of the states.
+    __device__ __forceinline__ void begin(const Attention& a, const Grid& g, int64_t b, int kv, int64_t i0, int lane) {
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            const int64_t i = i0 + 32 * n + (lane & 31);
+            exists[n] = i < g.rows;
+            const int64_t r = g.shared == 1 ? i : i / g.shared;
+            head[n] = kv * g.shared + (g.shared == 1 ? 0 : (int)(i - r * g.shared));
+            row[n] = b * a.queries + r;
+            const T* p = (const T*)a.q.p + row[n] * a.q.stride + (int64_t)head[n] * a.head;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) q[n][s] = row_chunk<T>(p, 2 * s + (lane >> 5), a.head, exists[n]);
+            top[n] = -INFINITY;
+            sum[n] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) out[n][c][r] = 0.0f;
+        }
+    }
+
+    // N squares of states at a time, from row r0 of the tiles on; `bits`: which of them exist.
+    template <class Tile, int N>
+    __device__ __forceinline__ void add(const unsigned char* lk, const unsigned char* lv, int r0, uint64_t bits, float c,
+                                        int lane) {
+        f32x16 s[QB][N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+#pragma unroll
+            for (int n = 0; n < QB; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[n][u][r] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < kSteps; ++p) {
+                const auto f = Tile::along(lk, r0 + 32 * u, p, lane);
+#pragma unroll
+                for (int n = 0; n < QB; ++n) S::multiply(f, q[n][p], s[n][u]);
+            }
+        }
+        constexpr uint64_t kAll = N == 2 ? ~0ull : 0xffffffffull;
+        if ((bits & kAll) != kAll) {
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const uint32_t w = (uint32_t)(bits >> (32 * u)) >> (4 * (lane >> 5));
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+#pragma unroll
+                    for (int n = 0; n < QB; ++n)
+                        s[n][u][r] = w & (1u << ((r & 3) + 8 * (r >> 2))) ? s[n][u][r] : -INFINITY;
+            }
+        }
+        float new_top[QB];
+        bool passed = false;
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            float m = s[n][0][0];
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) m = fmaxf(m, s[n][u][r]);
+            float other = m;
+            swap32(m, other);
+            new_top[n] = fmaxf(fmaxf(m, other), top[n]);   // a NaN goes into the weights instead
+            passed |= (new_top[n] - top[n]) * c > kLazy;
+        }
+        if (ballot(passed)) {
+#pragma unroll
+            for (int n = 0; n < QB; ++n) {
+                const float to = new_top[n] == -INFINITY ? 0.0f : new_top[n];
+                const float keep = __builtin_amdgcn_exp2f(fmaf(top[n], c, -to * c));
+                top[n] = new_top[n];
+                sum[n] *= keep;
+#pragma unroll
+                for (int k = 0; k < kCols; ++k)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) out[n][k][r] *= keep;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            const float less = -(top[n] == -INFINITY ? 0.0f : top[n]) * c;
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[n][u][r] = __builtin_amdgcn_exp2f(fmaf(s[n][u][r], c, less));
+                    sum[n] += s[n][u][r];
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+                typename S::Frag w[QB];
+#pragma unroll
+                for (int n = 0; n < QB; ++n) w[n] = S::rounded(s[n][u], p);
+#pragma unroll
+                for (int k = 0; k < kCols; ++k) {
+                    const auto f = Tile::across(lv, r0 + 32 * u + p * S::kDepth, 32 * k, lane);
+#pragma unroll
+                    for (int n = 0; n < QB; ++n) S::multiply(f, w[n], out[n][k]);
+                }
+            }
+    }
+
+    // The sums of the lane's half of the states become those of all.
+    __device__ __forceinline__ void join() {
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            float other = sum[n];
+            swap32(sum[n], other);
+            sum[n] += other;
+        }
+    }
+
+    __device__ __forceinline__ void store(const Attention& a, int lane) {
+        join();
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            if (!exists[n]) continue;
+            const float inv = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
+            T* to = (T*)a.out.p + row[n] * a.out.stride + (int64_t)head[n] * a.head;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float v[8];
+                    square_rows(out[n][c], p, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= inv;
+                    store_eight<T>(to, 32 * c + 16 * p + 8 * (lane >> 5), a.head, v);
+                }
+            if (a.lse && lane < 32)
+                a.lse[row[n] * a.lse_row_step + head[n] * a.lse_head_step] =
+                    sum[n] == 0.0f ? -INFINITY : fmaf(top[n], a.scale, logf(sum[n]));
+        }
+    }
+
+    __device__ __forceinline__ void store_part(const Attention& a, const Grid& g, int split, int lane) {
+        join();
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            if (!exists[n]) continue;
+            const int64_t at = ((int64_t)split * a.q.rows + row[n]) * a.heads + head[n];
+            if (lane < 32) {
+                g.tops[2 * at] = top[n];
+                g.tops[2 * at + 1] = sum[n];
+            }
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float v[8];
+                    square_rows(out[n][c], p, v);
+                    store_eight<float>(g.sums + at * D, 32 * c + 16 * p + 8 * (lane >> 5), D, v);
+                }
+        }
+    }
+};
+
 template <class T, int D, int QB, int WAVES, int KT, bool SPLIT>
 __global__ void __launch_bounds__(64 * WAVES, D <= 64 ? 2 : 1) attention_kernel(Attention a, Grid g) {
-    using S = Square<T>;
     using Tile = RowTile<T, D, KT, WAVES>;
-    constexpr int kSteps = D / S::kDepth;   // of the scores' product
-    constexpr int kParts = 32 / S::kDepth;  // of a square's rows as an operand
-    constexpr int kSubs = KT / 32, kCols = D / 32;
-    constexpr int kAtOnce = D <= 32 ? kSubs : 1;
-    constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
+    constexpr int kAtOnce = D <= 32 ? KT / 32 : 1;   // squares: as many scores as the registers hold beside the sums
     __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t number = g.first + xcd_contiguous_index(blockIdx.x, gridDim.x);
@@ -55,23 +225,6 @@ __global__ void __launch_bounds__(64 * WAVES, D <= 64 ? 2 : 1) attention_kernel(
     const int64_t pair = (SPLIT ? number / g.splits : number) / g.blocks;
     const int64_t b = pair / a.kv_heads;
     const int kv = (int)(pair % a.kv_heads), d = a.head;
-
-    // the lane's rows
-    int64_t row[QB];
-    int head[QB];
-    bool exists[QB];
-    typename S::Frag q[QB][kSteps];
-#pragma unroll
-    for (int n = 0; n < QB; ++n) {
-        const int64_t i = ((block * WAVES + wave) * QB + n) * 32 + (lane & 31);
-        exists[n] = i < g.rows;
-        const int64_t r = g.shared == 1 ? i : i / g.shared;
-        head[n] = kv * g.shared + (g.shared == 1 ? 0 : (int)(i - r * g.shared));
-        row[n] = b * a.queries + r;
-        const T* p = (const T*)a.q.p + row[n] * a.q.stride + (int64_t)head[n] * d;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) q[n][s] = row_chunk<T>(p, 2 * s + (lane >> 5), d, exists[n]);
-    }
 
     Tile tk, tv;
     const int64_t k_pitch = a.k.stride * (int64_t)sizeof(T), v_pitch = a.v.stride * (int64_t)sizeof(T);
@@ -101,146 +254,76 @@ __global__ void __launch_bounds__(64 * WAVES, D <= 64 ? 2 : 1) attention_kernel(
         tv.load(lds[buffer][1], v0 + t * KT * v_pitch, v_end - t * KT * v_pitch, exist, d, wave, lane);
         return true;
     };
-
-    f32x16 out[QB][kCols];
-    float top[QB], sum[QB];
-#pragma unroll
-    for (int n = 0; n < QB; ++n) {
-        top[n] = -INFINITY;
-        sum[n] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) out[n][c][r] = 0.0f;
-    }
     int buffer = 0;
     bool more = load(0);
+    WaveRows<T, D, QB> rows;
+    rows.begin(a, g, b, kv, (block * WAVES + wave) * QB * 32, lane);
     while (more) {
         const uint64_t bits = exist;
         wait_for_stage<1>(0);   // the tile is there, and every wave is done with the other buffer
         more = load(buffer ^ 1);
-        const unsigned char *lk = lds[buffer][0], *lv = lds[buffer][1];
-        buffer ^= 1;
-        // kAtOnce squares of states at a time: as many scores as the registers hold beside the sums
 #pragma unroll 1
-        for (int u0 = 0; u0 < kSubs; u0 += kAtOnce) {
-            f32x16 s[QB][kAtOnce];
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u) {
-#pragma unroll
-                for (int n = 0; n < QB; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[n][u][r] = 0.0f;
-#pragma unroll
-                for (int p = 0; p < kSteps; ++p) {
-                    const auto f = Tile::along(lk, 32 * (u0 + u), p, lane);
-#pragma unroll
-                    for (int n = 0; n < QB; ++n) S::multiply(f, q[n][p], s[n][u]);
-                }
-            }
-            if (bits != kAll) {
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u) {
-                    const uint32_t w = (uint32_t)(bits >> (32 * (u0 + u))) >> (4 * (lane >> 5));
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-#pragma unroll
-                        for (int n = 0; n < QB; ++n)
-                            s[n][u][r] = w & (1u << ((r & 3) + 8 * (r >> 2))) ? s[n][u][r] : -INFINITY;
-                }
-            }
-            float new_top[QB];
-            bool passed = false;
-#pragma unroll
-            for (int n = 0; n < QB; ++n) {
-                float m = s[n][0][0];
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) m = fmaxf(m, s[n][u][r]);
-                float other = m;
-                swap32(m, other);
-                new_top[n] = fmaxf(fmaxf(m, other), top[n]);   // a NaN goes into the weights instead
-                passed |= (new_top[n] - top[n]) * g.c > kLazy;
-            }
-            if (ballot(passed)) {
-#pragma unroll
-                for (int n = 0; n < QB; ++n) {
-                    const float to = new_top[n] == -INFINITY ? 0.0f : new_top[n];
-                    const float keep = __builtin_amdgcn_exp2f(fmaf(top[n], g.c, -to * g.c));
-                    top[n] = new_top[n];
-                    sum[n] *= keep;
-#pragma unroll
-                    for (int c = 0; c < kCols; ++c)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) out[n][c][r] *= keep;
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < QB; ++n) {
-                const float less = -(top[n] == -INFINITY ? 0.0f : top[n]) * g.c;
-#pragma unroll
-                for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        s[n][u][r] = __builtin_amdgcn_exp2f(fmaf(s[n][u][r], g.c, less));
-                        sum[n] += s[n][u][r];
-                    }
-            }
-#pragma unroll
-            for (int u = 0; u < kAtOnce; ++u)
-#pragma unroll
-                for (int p = 0; p < kParts; ++p) {
-                    typename S::Frag w[QB];
-#pragma unroll
-                    for (int n = 0; n < QB; ++n) w[n] = S::rounded(s[n][u], p);
-#pragma unroll
-                    for (int c = 0; c < kCols; ++c) {
-                        const auto f = Tile::across(lv, 32 * (u0 + u) + p * S::kDepth, 32 * c, lane);
-#pragma unroll
-                        for (int n = 0; n < QB; ++n) S::multiply(f, w[n], out[n][c]);
-                    }
-                }
-        }
+        for (int u = 0; u < KT / 32; u += kAtOnce)
+            if (kAtOnce > 1 || (uint32_t)(bits >> (32 * u)) != 0)
+                rows.template add<Tile, kAtOnce>(lds[buffer][0], lds[buffer][1], 32 * u, bits >> (32 * u), g.c, lane);
+        buffer ^= 1;
     }
-#pragma unroll
-    for (int n = 0; n < QB; ++n) {
-        float other = sum[n];
-        swap32(sum[n], other);
-        sum[n] += other;
-        if (!exists[n]) continue;
-        const int64_t place = row[n] * a.heads + head[n];
-        if constexpr (SPLIT) {
-            const int64_t at = (int64_t)split * a.q.rows * a.heads + place;
-            if (lane < 32) {
-                g.tops[2 * at] = top[n];
-                g.tops[2 * at + 1] = sum[n];
-            }
-#pragma unroll
-            for (int c = 0; c < kCols; ++c)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    float v[8];
-                    square_rows(out[n][c], p, v);
-                    store_eight<float>(g.sums + at * D, 32 * c + 16 * p + 8 * (lane >> 5), D, v);
-                }
-        } else {
-            const float inv = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
-            T* to = (T*)a.out.p + row[n] * a.out.stride + (int64_t)head[n] * d;
-#pragma unroll
-            for (int c = 0; c < kCols; ++c)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    float v[8];
-                    square_rows(out[n][c], p, v);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] *= inv;
-                    store_eight<T>(to, 32 * c + 16 * p + 8 * (lane >> 5), d, v);
-                }
-            if (a.lse && lane < 32)
-                a.lse[row[n] * a.lse_row_step + head[n] * a.lse_head_step] =
-                    sum[n] == 0.0f ? -INFINITY : fmaf(top[n], a.scale, logf(sum[n]));
+    if constexpr (SPLIT) rows.store_part(a, g, split, lane);
+    else rows.store(a, lane);
+}
+
+// All states of a head in LDS, loaded once; the waves go over rows by
+// themselves, without a barrier, while another wave of the SIMD computes.
+constexpr int kHeldWaves = 8, kHeldBytes = 64 * 1024;   // of the keys, and as many of the values
+template <class T, int D, int QB>
+__global__ void __launch_bounds__(64 * kHeldWaves, 2) held_kernel(Attention a, Grid g) {
+    constexpr int kLoaders = D * (int)sizeof(T) * 64 / 1024 % kHeldWaves == 0 ? kHeldWaves : kHeldWaves / 2;
+    using Tile = RowTile<T, D, 64, kLoaders>;
+    constexpr int kAtOnce = D <= 32 ? 2 : 1, kTiles = kHeldBytes / Tile::kBytes;
+    __shared__ __align__(1024) unsigned char lk[kHeldBytes], lv[kHeldBytes];
+    __shared__ uint64_t exist[kTiles];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t number = xcd_contiguous_index(blockIdx.x, gridDim.x);
+    const int64_t part = number % g.blocks, pair = number / g.blocks;
+    const int64_t b = pair / a.kv_heads;
+    const int kv = (int)(pair % a.kv_heads), d = a.head;
+    const int tiles = (int)((a.states + 63) / 64);
+    {
+        Tile tk, tv;
+        const int64_t k_pitch = a.k.stride * (int64_t)sizeof(T), v_pitch = a.v.stride * (int64_t)sizeof(T);
+        tk.begin(k_pitch, d, wave, lane);
+        tv.begin(v_pitch, d, wave, lane);
+        const unsigned char* k0 = (const unsigned char*)a.k.p + b * a.states * k_pitch + (int64_t)kv * d * sizeof(T);
+        const unsigned char* v0 = (const unsigned char*)a.v.p + b * a.states * v_pitch + (int64_t)kv * d * sizeof(T);
+        const int64_t k_end = (a.states - 1) * k_pitch + d * (int64_t)sizeof(T);
+        const int64_t v_end = (a.states - 1) * v_pitch + d * (int64_t)sizeof(T);
+        for (int t = 0; t < tiles; ++t) {
+            const int j = t * 64 + lane;
+            const uint64_t bits = ballot(j < a.states && (!a.mask || a.mask[b * a.mask_stride + j]));
+            if (threadIdx.x == 0) exist[t] = bits;
+            if (wave >= kLoaders) continue;
+            tk.load(lk + t * Tile::kBytes, k0 + t * 64 * k_pitch, k_end - t * 64 * k_pitch, bits, d, wave, lane);
+            tv.load(lv + t * Tile::kBytes, v0 + t * 64 * v_pitch, v_end - t * 64 * v_pitch, bits, d, wave, lane);
         }
+        wait_for_stage<1>(0);
+    }
+    const int64_t wave_blocks = (g.rows + QB * 32 - 1) / (QB * 32);
+    const int64_t last = min((part + 1) * g.part, wave_blocks);
+    for (int64_t i = part * g.part + wave; i < last; i += kHeldWaves) {
+        WaveRows<T, D, QB> rows;
+        rows.begin(a, g, b, kv, i * QB * 32, lane);
+        for (int t = 0; t < tiles; ++t) {
+            const uint64_t held = exist[t];
+            const uint64_t bits = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(held >> 32)) << 32 |
+                                  (uint32_t)__builtin_amdgcn_readfirstlane((int)held);
+            if (bits == 0) continue;
+#pragma unroll 1
+            for (int u = 0; u < 2; u += kAtOnce)
+                if (kAtOnce > 1 || (uint32_t)(bits >> (32 * u)) != 0)
+                    rows.template add<Tile, kAtOnce>(lk + t * Tile::kBytes, lv + t * Tile::kBytes, 32 * u, bits >> (32 * u),
+                                                 g.c, lane);
+        }
+        rows.store(a, lane);
     }
 }
 
@@ -276,7 +359,8 @@ __global__ void __launch_bounds__(256) join_kernel(Attention a, Grid g) {
 }
 
 struct Plan {
-    int qb, kt;
+    int qb;
+    bool held;
     Grid grid;
     int64_t workgroups;
     size_t bytes;
@@ -284,16 +368,33 @@ struct Plan {
 
 constexpr int kWaves = 4;
 
+// The rows' squares of a wave: two where the registers hold them.
+template <class T, int D>
+constexpr int kHeldSquares = sizeof(T) == 2 && D <= 64 ? 2 : 1;
+
 Plan plan_of(const Attention& a) {
     Plan p{};
-    const bool wide = a.dtype != TGS_DTYPE_FLOAT32;
+    const bool halves = a.dtype != TGS_DTYPE_FLOAT32;
+    const int64_t width = (a.head + 31) / 32 * 32, pairs = a.batch * a.kv_heads;
     p.grid.shared = a.heads / a.kv_heads;
     p.grid.rows = a.queries * p.grid.shared;
-    p.kt = wide ? 64 : 32;
-    p.qb = wide && p.grid.rows > 32 * kWaves ? 2 : 1;
-    p.grid.blocks = (p.grid.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
     p.grid.c = exponent_of(a.scale);
-    const int64_t whole = a.batch * a.kv_heads * p.grid.blocks, tiles = (a.states + p.kt - 1) / p.kt;
+    p.grid.splits = 1;
+    const int64_t held_rows = 32 * (halves && width <= 64 ? 2 : 1);
+    const int64_t wave_blocks = (p.grid.rows + held_rows - 1) / held_rows;
+    p.held = a.states > 0 && (a.states + 63) / 64 * 64 * width * (halves ? 2 : 4) <= kHeldBytes && (halves || width <= 64) &&
+             wave_blocks * pairs >= 256 * kHeldWaves && pairs <= 65536;
+    if (p.held) {
+        const int64_t parts = pairs < 256 ? 256 / pairs : 1;
+        p.grid.part = (wave_blocks + parts - 1) / parts;
+        p.grid.blocks = (wave_blocks + p.grid.part - 1) / p.grid.part;
+        p.workgroups = p.grid.blocks * pairs;
+        return p;
+    }
+    const int kt = halves ? 64 : 32;
+    p.qb = halves && p.grid.rows > 32 * kWaves ? 2 : 1;
+    p.grid.blocks = (p.grid.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
+    const int64_t whole = pairs * p.grid.blocks, tiles = (a.states + kt - 1) / kt;
     int64_t splits = 1;
     if (whole < 256 && tiles > 1) {
         splits = 512 / whole < tiles ? 512 / whole : tiles;
@@ -303,7 +404,6 @@ Plan plan_of(const Attention& a) {
     if (splits == 1) p.grid.tiles = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
     p.grid.splits = (int)splits;
     p.workgroups = whole * splits;
-    const int64_t width = (a.head + 31) / 32 * 32;
     if (splits > 1) p.bytes = sizeof(float) * (size_t)(splits * a.q.rows * a.heads * (width + 2));
     return p;
 }
@@ -318,6 +418,12 @@ int launch_attention(const Attention& a, void* workspace, hipStream_t s) {
         using T = decltype(t);
         by_head_width(a.head, [&](auto width) {
             constexpr int D = decltype(width)::value, KT = sizeof(T) == 2 ? 64 : 32;
+            if (p.held) {
+                if constexpr (sizeof(T) == 2 || D <= 64)
+                    held_kernel<T, D, kHeldSquares<T, D>>
+                        <<<(unsigned)p.workgroups, 64 * kHeldWaves, 0, s>>>(a, p.grid);
+                return;
+            }
             p.grid.sums = (float*)workspace;
             p.grid.tops = p.grid.sums + (p.grid.splits > 1 ? p.grid.splits * a.q.rows * a.heads * D : 0);
             // a launch of 2^32 threads or more loses what is above
