@@ -24,6 +24,7 @@ struct Square {   // halves: 16 of k a step
     static constexpr int kDepth = 16;
     using Frag = typename tgs::Frag<T>::type;
     static __device__ __forceinline__ void multiply(const Frag& a, const Frag& b, f32x16& c);
+    static __device__ __forceinline__ f32x16 product(const Frag& a, const Frag& b);   // on its own
     // Registers 8 u .. 8 u + 7 of a square, rounded.
     static __device__ __forceinline__ Frag rounded(const f32x16& s, int u) {
         typedef float f32x8 __attribute__((ext_vector_type(8)));
@@ -38,6 +39,14 @@ __device__ __forceinline__ void Square<_Float16>::multiply(const Frag& a, const 
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 template <>
+__device__ __forceinline__ f32x16 Square<_Float16>::product(const Frag& a, const Frag& b) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, f32x16{}, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x16 Square<__bf16>::product(const Frag& a, const Frag& b) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, f32x16{}, 0, 0, 0);
+}
+template <>
 __device__ __forceinline__ void Square<__bf16>::multiply(const Frag& a, const Frag& b, f32x16& c) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
@@ -48,6 +57,12 @@ struct Square<float> {
     static __device__ __forceinline__ void multiply(const Frag& a, const Frag& b, f32x16& c) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 product(const Frag& a, const Frag& b) {
+        f32x16 c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[0], b[0], f32x16{}, 0, 0, 0);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
     }
     static __device__ __forceinline__ Frag rounded(const f32x16& s, int u) {
         return Frag{s[4 * u], s[4 * u + 1], s[4 * u + 2], s[4 * u + 3]};
@@ -119,14 +134,14 @@ struct RowTile {
         }
     }
 
-    // Operand of rows r0 .. r0 + 31 (a multiple of 32) along step s of their columns.
-    static __device__ __forceinline__ typename S::Frag along(const unsigned char* lds, int r0, int s, int lane) {
-        const int r = r0 + (lane & 31);
+    // Operand of 32 rows along step s of their columns. lds: the first row, a multiple of 32.
+    static __device__ __forceinline__ typename S::Frag along(const unsigned char* lds, int s, int lane) {
+        const int r = lane & 31;
         return *(const typename S::Frag*)(lds + r * kRowBytes + (((2 * s + (lane >> 5)) ^ turn(r)) << 4));
     }
 
     // Operand of columns c0 .. c0 + 31 (a multiple of 32) across the rows
-    // r0 .. r0 + kDepth - 1, in the order of a square's registers.
+    // r0 .. r0 + kDepth - 1 of the 32 from lds on, in the order of a square's registers.
     static __device__ __forceinline__ typename S::Frag across(const unsigned char* lds, int r0, int c0, int lane) {
         if constexpr (sizeof(T) == 4) {
             typename S::Frag f;
@@ -158,27 +173,67 @@ struct RowTile {
     }
 };
 
-// The queries' rows of a batch's element that read one head of the states:
-// index i is row i / shared, head first + i % shared.
-struct Rows {
-    int64_t count;
-    int shared;
-};
+// The rows that 32 QB lanes of a wave take, of those that read one head of the
+// states in one element of a batch: number i is row i / shared of the element, head
+// first + i % shared, so that heads that share lie side by side.
+template <int QB>
+struct LaneRows {
+    int64_t base;      // the first lane's row
+    int down[QB];      // the lane's, from there
+    int head[QB];
+    bool exists[QB];
 
-// Chunk c of a row's head of d columns, zeros past it; `exists`: whether there is a row.
-template <class T>
-__device__ __forceinline__ typename Square<T>::Frag row_chunk(const T* row, int c, int d, bool exists) {
-    using F = typename Square<T>::Frag;
-    constexpr int V = 16 / (int)sizeof(T);
-    typedef F Loose __attribute__((aligned(sizeof(T))));
-    F f = {};
-    if (!exists) return f;
-    if ((c + 1) * V <= d) return *(const Loose*)(row + c * V);
+    __device__ __forceinline__ void begin(int64_t element_row, int64_t i0, int64_t count, int first, int shared, int lane) {
+        const int64_t r0 = shared == 1 ? i0 : i0 / shared;
+        const uint32_t left = (uint32_t)(i0 - r0 * shared);
+        base = element_row + r0;
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-        if (c * V + e < d) f[e] = row[c * V + e];
-    return f;
-}
+        for (int n = 0; n < QB; ++n) {
+            const uint32_t i = 32 * n + (lane & 31);
+            exists[n] = i0 + i < count;
+            const uint32_t at = left + i;   // below shared + 64
+            down[n] = (int)(shared == 1 ? at : at / (uint32_t)shared);
+            head[n] = first + (int)(shared == 1 ? 0 : at - (uint32_t)down[n] * (uint32_t)shared);
+        }
+    }
+    __device__ __forceinline__ int64_t row(int n) const { return base + down[n]; }
+
+    // The lanes' chunks of matrix m: chunk 2 s + lane / 32 in f[n][s]. Columns past
+    // the head and rows that do not exist are zeros.
+    template <class T, int STEPS>
+    __device__ __forceinline__ void load(const Mat& m, int d, int lane, typename Square<T>::Frag (&f)[QB][STEPS]) const {
+        using F = typename Square<T>::Frag;
+        constexpr int V = 16 / (int)sizeof(T);
+        const int64_t pitch = m.stride * (int64_t)sizeof(T);
+        const unsigned char* from = (const unsigned char*)m.p + base * pitch;
+        if (d % V == 0) {   // all loads on their way at once, without branches
+            const auto buffer = resource_of(from, (m.rows - 1 - base) * pitch + m.cols * (int64_t)sizeof(T));
+#pragma unroll
+            for (int n = 0; n < QB; ++n)
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    const int c = 2 * s + (lane >> 5);
+                    const uint32_t at = (uint32_t)(down[n] * pitch + (head[n] * d + c * V) * (int)sizeof(T));
+                    f[n][s] = __builtin_bit_cast(
+                        F, __builtin_amdgcn_raw_buffer_load_b128(buffer, exists[n] && c * V < d ? (int)at : (int)kPastEnd, 0, 0));
+                }
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            const T* p = (const T*)(from + down[n] * pitch) + (int64_t)head[n] * d;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const int c = 2 * s + (lane >> 5);
+                F v = {};
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (exists[n] && c * V + e < d) v[e] = p[c * V + e];
+                f[n][s] = v;
+            }
+        }
+    }
+};
 
 // Eight columns from c0 on of a row's head of d columns.
 template <class T>

@@ -1,13 +1,16 @@
 // Attention of a network's rows to an encoder's states: for each row and head
 // s = scale q k^T over the states that exist, out = softmax(s) v, lse = log sum exp s.
 //
-// One pass over the states with a running maximum m and sum l: a wave holds 32
-// or 64 rows' queries, and their sums out^T = v^T p^T, in registers; tiles of
+// One pass over the states: a wave holds 32 or 64 rows' queries, and their sums out^T = v^T p^T, in registers; tiles of
 // states go through LDS, loaded one ahead. The scores are formed as
 // s^T = k q^T: a lane then has one row's scores, so that maxima and sums need one
 // exchange between the halves of the wave, and the weights p^T are the second
-// product's operand as they stand. The maximum is replaced only where a score
-// passes it by 2^8: the weights stay below that, and the sums are seldom scaled.
+// product's operand as they stand. The maximum m is that of a row's first 32
+// states: later scores may pass it by what the weights' type holds, and the sum of
+// the weights tells if they did. Then the wave looks for the maxima of all states and
+// adds them once more. A running maximum takes a tenth more of the vector
+// instructions, and a scaling of the sums on the way, even one that is never reached,
+// made the compiler copy them all at every step.
 //
 // Heads that share the states' are rows side by side, so that a tile is loaded
 // once for all of them. Where there are few rows, workgroups take parts of the
@@ -20,7 +23,12 @@ namespace tgs {
 
 namespace {
 
-constexpr float kLazy = 8.0f;   // in powers of two
+// The sum of a lane's weights up to which none of them can have left its type's
+// range (2^16 for halves), nor their products with values that of floats.
+template <class T>
+constexpr float kMostSum = 0x1p40f;
+template <>
+constexpr float kMostSum<_Float16> = 0x1p15f;
 
 struct Grid {
     int64_t first;       // number of the launch's first workgroup
@@ -46,26 +54,24 @@ struct WaveRows {
     static constexpr int kSteps = D / S::kDepth;    // of the scores' product
     static constexpr int kParts = 32 / S::kDepth;   // of a square's rows as an operand
     static constexpr int kCols = D / 32;
-    int64_t row[QB];
-    int head[QB];
-    bool exists[QB];
+    LaneRows<QB> at;
     typename S::Frag q[QB][kSteps];
     f32x16 out[QB][kCols];   // sums of weights times v
-    float top[QB], sum[QB];
+    float top[QB], sum[QB];  // the maximum that the weights are relative to; of the weights
+    bool low[QB];            // the maximum is to be raised
 
     // Rows from number i0 on of batch element b and head kv of the states.
     __device__ __forceinline__ void begin(const Attention& a, const Grid& g, int64_t b, int kv, int64_t i0, int lane) {
+        at.begin(b * a.queries, i0, g.rows, kv * g.shared, g.shared, lane);
+        at.template load<T, kSteps>(a.q, a.head, lane, q);
+#pragma unroll
+        for (int n = 0; n < QB; ++n) top[n] = -INFINITY;
+    }
+
+    // Before a pass over the states.
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
-            const int64_t i = i0 + 32 * n + (lane & 31);
-            exists[n] = i < g.rows;
-            const int64_t r = g.shared == 1 ? i : i / g.shared;
-            head[n] = kv * g.shared + (g.shared == 1 ? 0 : (int)(i - r * g.shared));
-            row[n] = b * a.queries + r;
-            const T* p = (const T*)a.q.p + row[n] * a.q.stride + (int64_t)head[n] * a.head;
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) q[n][s] = row_chunk<T>(p, 2 * s + (lane >> 5), a.head, exists[n]);
-            top[n] = -INFINITY;
             sum[n] = 0.0f;
 #pragma unroll
             for (int c = 0; c < kCols; ++c)
@@ -74,88 +80,87 @@ struct WaveRows {
         }
     }
 
-    // N squares of states at a time, from row r0 of the tiles on; `bits`: which of them exist.
-    template <class Tile, int N>
-    __device__ __forceinline__ void add(const unsigned char* lk, const unsigned char* lv, int r0, uint64_t bits, float c,
-                                        int lane) {
-        f32x16 s[QB][N];
+    // Scores of the 32 states whose keys start at lk; `bits`: which of them exist.
+    template <class Tile>
+    __device__ __forceinline__ void score(const unsigned char* lk, uint32_t bits, f32x16 (&s)[QB], int lane) {
+        typename S::Frag k[kSteps];
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
+        for (int p = 0; p < kSteps; ++p) k[p] = Tile::along(lk, p, lane);
 #pragma unroll
-            for (int n = 0; n < QB; ++n)
+        for (int n = 0; n < QB; ++n) s[n] = S::product(k[0], q[n][0]);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[n][u][r] = 0.0f;
+        for (int p = 1; p < kSteps; ++p)
 #pragma unroll
-            for (int p = 0; p < kSteps; ++p) {
-                const auto f = Tile::along(lk, r0 + 32 * u, p, lane);
+            for (int n = 0; n < QB; ++n) S::multiply(k[p], q[n][p], s[n]);
+        if (__builtin_expect(bits != ~0u, 0)) {
+            const uint32_t w = bits >> (4 * (lane >> 5));
 #pragma unroll
-                for (int n = 0; n < QB; ++n) S::multiply(f, q[n][p], s[n][u]);
-            }
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+                for (int n = 0; n < QB; ++n) s[n][r] = w & (1u << ((r & 3) + 8 * (r >> 2))) ? s[n][r] : -INFINITY;
         }
-        constexpr uint64_t kAll = N == 2 ? ~0ull : 0xffffffffull;
-        if ((bits & kAll) != kAll) {
-#pragma unroll
-            for (int u = 0; u < N; ++u) {
-                const uint32_t w = (uint32_t)(bits >> (32 * u)) >> (4 * (lane >> 5));
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-#pragma unroll
-                    for (int n = 0; n < QB; ++n)
-                        s[n][u][r] = w & (1u << ((r & 3) + 8 * (r >> 2))) ? s[n][u][r] : -INFINITY;
-            }
-        }
-        float new_top[QB];
-        bool passed = false;
+    }
+
+    // Raises the maxima, or only those that do not do, to those of the scores. A NaN
+    // goes into the weights instead.
+    template <bool ALL>
+    __device__ __forceinline__ void raise(const f32x16 (&s)[QB]) {
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
-            float m = s[n][0][0];
+            float m = s[n][0];
 #pragma unroll
-            for (int u = 0; u < N; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) m = fmaxf(m, s[n][u][r]);
+            for (int r = 1; r < 16; ++r) m = fmaxf(m, s[n][r]);
             float other = m;
             swap32(m, other);
-            new_top[n] = fmaxf(fmaxf(m, other), top[n]);   // a NaN goes into the weights instead
-            passed |= (new_top[n] - top[n]) * c > kLazy;
+            if (ALL || low[n]) top[n] = fmaxf(fmaxf(m, other), top[n]);
         }
-        if (ballot(passed)) {
+    }
+
+    // Adds 32 states, whose rows start at lk and lv. `first`: the maxima are theirs.
+    template <class Tile>
+    __device__ __forceinline__ void add(const unsigned char* lk, const unsigned char* lv, uint32_t bits, bool first, float c,
+                                        int lane) {
+        f32x16 s[QB];
+        typename S::Frag v[kParts][kCols];
+        score<Tile>(lk, bits, s, lane);
+        // the second product's operands are read while the weights are formed
 #pragma unroll
-            for (int n = 0; n < QB; ++n) {
-                const float to = new_top[n] == -INFINITY ? 0.0f : new_top[n];
-                const float keep = __builtin_amdgcn_exp2f(fmaf(top[n], c, -to * c));
-                top[n] = new_top[n];
-                sum[n] *= keep;
+        for (int p = 0; p < kParts; ++p)
 #pragma unroll
-                for (int k = 0; k < kCols; ++k)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) out[n][k][r] *= keep;
-            }
-        }
+            for (int k = 0; k < kCols; ++k) v[p][k] = Tile::across(lv, p * S::kDepth, 32 * k, lane);
+        if (first) raise<true>(s);
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
             const float less = -(top[n] == -INFINITY ? 0.0f : top[n]) * c;
 #pragma unroll
-            for (int u = 0; u < N; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[n][u][r] = __builtin_amdgcn_exp2f(fmaf(s[n][u][r], c, less));
-                    sum[n] += s[n][u][r];
-                }
+            for (int r = 0; r < 16; ++r) {
+                s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, less));
+                sum[n] += s[n][r];
+            }
         }
 #pragma unroll
-        for (int u = 0; u < N; ++u)
+        for (int p = 0; p < kParts; ++p)
 #pragma unroll
-            for (int p = 0; p < kParts; ++p) {
-                typename S::Frag w[QB];
+            for (int n = 0; n < QB; ++n) {
+                const auto w = S::rounded(s[n], p);
 #pragma unroll
-                for (int n = 0; n < QB; ++n) w[n] = S::rounded(s[n][u], p);
-#pragma unroll
-                for (int k = 0; k < kCols; ++k) {
-                    const auto f = Tile::across(lv, r0 + 32 * u + p * S::kDepth, 32 * k, lane);
-#pragma unroll
-                    for (int n = 0; n < QB; ++n) S::multiply(f, w[n], out[n][k]);
-                }
+                for (int k = 0; k < kCols; ++k) S::multiply(v[p][k], w, out[n][k]);
             }
+    }
+
+    // Whether the maxima of the first states do not do for some row: scores passed it
+    // by more than the weights' range, or its first scores were all -infinity. The other rows keep theirs,
+    // and so their results do not depend on it.
+    __device__ __forceinline__ bool passed() {
+        bool any = false;
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            float a = sum[n], b = sum[n];
+            swap32(a, b);
+            low[n] = a > kMostSum<T> || b > kMostSum<T> || top[n] == -INFINITY;
+            any |= low[n];
+        }
+        return ballot(any) != 0;
     }
 
     // The sums of the lane's half of the states become those of all.
@@ -172,9 +177,9 @@ struct WaveRows {
         join();
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
-            if (!exists[n]) continue;
+            if (!at.exists[n]) continue;
             const float inv = sum[n] == 0.0f ? 0.0f : 1.0f / sum[n];
-            T* to = (T*)a.out.p + row[n] * a.out.stride + (int64_t)head[n] * a.head;
+            T* to = (T*)a.out.p + at.row(n) * a.out.stride + (int64_t)at.head[n] * a.head;
 #pragma unroll
             for (int c = 0; c < kCols; ++c)
 #pragma unroll
@@ -186,7 +191,7 @@ struct WaveRows {
                     store_eight<T>(to, 32 * c + 16 * p + 8 * (lane >> 5), a.head, v);
                 }
             if (a.lse && lane < 32)
-                a.lse[row[n] * a.lse_row_step + head[n] * a.lse_head_step] =
+                a.lse[at.row(n) * a.lse_row_step + at.head[n] * a.lse_head_step] =
                     sum[n] == 0.0f ? -INFINITY : fmaf(top[n], a.scale, logf(sum[n]));
         }
     }
@@ -195,11 +200,11 @@ struct WaveRows {
         join();
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
-            if (!exists[n]) continue;
-            const int64_t at = ((int64_t)split * a.q.rows + row[n]) * a.heads + head[n];
+            if (!at.exists[n]) continue;
+            const int64_t place = ((int64_t)split * a.q.rows + at.row(n)) * a.heads + at.head[n];
             if (lane < 32) {
-                g.tops[2 * at] = top[n];
-                g.tops[2 * at + 1] = sum[n];
+                g.tops[2 * place] = top[n];
+                g.tops[2 * place + 1] = sum[n];
             }
 #pragma unroll
             for (int c = 0; c < kCols; ++c)
@@ -207,7 +212,7 @@ struct WaveRows {
                 for (int p = 0; p < 2; ++p) {
                     float v[8];
                     square_rows(out[n][c], p, v);
-                    store_eight<float>(g.sums + at * D, 32 * c + 16 * p + 8 * (lane >> 5), D, v);
+                    store_eight<float>(g.sums + place * D, 32 * c + 16 * p + 8 * (lane >> 5), D, v);
                 }
         }
     }
@@ -216,7 +221,6 @@ struct WaveRows {
 template <class T, int D, int QB, int WAVES, int KT, bool SPLIT>
 __global__ void __launch_bounds__(64 * WAVES, D <= 64 ? 2 : 1) attention_kernel(Attention a, Grid g) {
     using Tile = RowTile<T, D, KT, WAVES>;
-    constexpr int kAtOnce = D <= 32 ? KT / 32 : 1;   // squares: as many scores as the registers hold beside the sums
     __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t number = g.first + xcd_contiguous_index(blockIdx.x, gridDim.x);
@@ -254,19 +258,46 @@ __global__ void __launch_bounds__(64 * WAVES, D <= 64 ? 2 : 1) attention_kernel(
         tv.load(lds[buffer][1], v0 + t * KT * v_pitch, v_end - t * KT * v_pitch, exist, d, wave, lane);
         return true;
     };
-    int buffer = 0;
-    bool more = load(0);
     WaveRows<T, D, QB> rows;
+    bool more = load(0);
     rows.begin(a, g, b, kv, (block * WAVES + wave) * QB * 32, lane);
-    while (more) {
-        const uint64_t bits = exist;
-        wait_for_stage<1>(0);   // the tile is there, and every wave is done with the other buffer
-        more = load(buffer ^ 1);
+    const auto each = [&](auto f) {   // f(keys, values, which exist) of 32 states at a time
+        int buffer = 0;
+        while (more) {
+            const uint64_t bits = exist;
+            wait_for_stage<1>(0);   // the tile is there, and every wave is done with the other buffer
+            more = load(buffer ^ 1);
+            const unsigned char *lk = lds[buffer][0], *lv = lds[buffer][1];
+            buffer ^= 1;
 #pragma unroll 1
-        for (int u = 0; u < KT / 32; u += kAtOnce)
-            if (kAtOnce > 1 || (uint32_t)(bits >> (32 * u)) != 0)
-                rows.template add<Tile, kAtOnce>(lds[buffer][0], lds[buffer][1], 32 * u, bits >> (32 * u), g.c, lane);
-        buffer ^= 1;
+            for (int u = 0; u < KT; u += 32) f(lk + u * Tile::kRowBytes, lv + u * Tile::kRowBytes, (uint32_t)(bits >> u));
+        }
+    };
+    const auto restart = [&] {
+        t = (int64_t)split * g.tiles - 1;
+        next = state_exists(t + 1);
+        more = load(0);
+    };
+    bool first = true;
+    const auto add = [&](const unsigned char* lk, const unsigned char* lv, uint32_t bits) {
+        rows.template add<Tile>(lk, lv, bits, first && bits != 0, g.c, lane);
+        first = first && bits == 0;
+    };
+    rows.clear();
+    each(add);
+    // the tiles are loaded for all waves: any of them takes the others along
+    if (__builtin_expect(__syncthreads_or(rows.passed()), 0)) {
+        restart();
+        each([&](const unsigned char* lk, const unsigned char*, uint32_t bits) {
+            f32x16 s[QB];
+            rows.template score<Tile>(lk, bits, s, lane);
+            rows.template raise<false>(s);
+        });
+        __syncthreads();
+        restart();
+        rows.clear();
+        first = false;
+        each(add);
     }
     if constexpr (SPLIT) rows.store_part(a, g, split, lane);
     else rows.store(a, lane);
@@ -274,14 +305,21 @@ __global__ void __launch_bounds__(64 * WAVES, D <= 64 ? 2 : 1) attention_kernel(
 
 // All states of a head in LDS, loaded once; the waves go over rows by
 // themselves, without a barrier, while another wave of the SIMD computes.
-constexpr int kHeldWaves = 8, kHeldBytes = 64 * 1024;   // of the keys, and as many of the values
+constexpr int held_waves(int size, int width) { return width <= (size == 2 ? 64 : 32) ? 16 : 8; }
+template <class T, int D>
+constexpr int kHeldWaves = held_waves((int)sizeof(T), D);
+// Bytes of the keys, and as many of the values: narrow heads' kernels need so few
+// registers that two workgroups fit on a compute unit.
+constexpr int held_bytes(int width) { return 64 * 1024; }
+
 template <class T, int D, int QB>
-__global__ void __launch_bounds__(64 * kHeldWaves, 2) held_kernel(Attention a, Grid g) {
-    constexpr int kLoaders = D * (int)sizeof(T) * 64 / 1024 % kHeldWaves == 0 ? kHeldWaves : kHeldWaves / 2;
+__global__ void __launch_bounds__((64 * kHeldWaves<T, D>)) held_kernel(Attention a, Grid g) {
+    constexpr int kTileLoads = D * (int)sizeof(T) * 64 / 1024;
+    constexpr int kLoaders = kTileLoads % kHeldWaves<T, D> == 0 ? kHeldWaves<T, D> : kTileLoads % 8 == 0 ? 8 : 4;
     using Tile = RowTile<T, D, 64, kLoaders>;
-    constexpr int kAtOnce = D <= 32 ? 2 : 1, kTiles = kHeldBytes / Tile::kBytes;
-    __shared__ __align__(1024) unsigned char lk[kHeldBytes], lv[kHeldBytes];
-    __shared__ uint64_t exist[kTiles];
+    constexpr int kTiles = held_bytes(D) / Tile::kBytes;
+    __shared__ __align__(1024) unsigned char lk[held_bytes(D)], lv[held_bytes(D)];
+    __shared__ uint32_t exist[2 * kTiles];   // of each 32 states
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t number = xcd_contiguous_index(blockIdx.x, gridDim.x);
     const int64_t part = number % g.blocks, pair = number / g.blocks;
@@ -300,28 +338,39 @@ __global__ void __launch_bounds__(64 * kHeldWaves, 2) held_kernel(Attention a, G
         for (int t = 0; t < tiles; ++t) {
             const int j = t * 64 + lane;
             const uint64_t bits = ballot(j < a.states && (!a.mask || a.mask[b * a.mask_stride + j]));
-            if (threadIdx.x == 0) exist[t] = bits;
+            if (threadIdx.x < 2) exist[2 * t + threadIdx.x] = (uint32_t)(bits >> (32 * threadIdx.x));
             if (wave >= kLoaders) continue;
             tk.load(lk + t * Tile::kBytes, k0 + t * 64 * k_pitch, k_end - t * 64 * k_pitch, bits, d, wave, lane);
             tv.load(lv + t * Tile::kBytes, v0 + t * 64 * v_pitch, v_end - t * 64 * v_pitch, bits, d, wave, lane);
         }
         wait_for_stage<1>(0);
     }
+    const int squares = (int)((a.states + 31) / 32);
+    const auto next = [&](int u, uint32_t& bits) {   // the next 32 states after the u-th of which any exists
+        do {
+            if (++u == squares) break;
+            bits = (uint32_t)__builtin_amdgcn_readfirstlane((int)exist[u]);
+        } while (bits == 0);
+        return u;
+    };
     const int64_t wave_blocks = (g.rows + QB * 32 - 1) / (QB * 32);
     const int64_t last = min((part + 1) * g.part, wave_blocks);
-    for (int64_t i = part * g.part + wave; i < last; i += kHeldWaves) {
+    for (int64_t i = part * g.part + wave; i < last; i += kHeldWaves<T, D>) {
         WaveRows<T, D, QB> rows;
         rows.begin(a, g, b, kv, i * QB * 32, lane);
-        for (int t = 0; t < tiles; ++t) {
-            const uint64_t held = exist[t];
-            const uint64_t bits = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(held >> 32)) << 32 |
-                                  (uint32_t)__builtin_amdgcn_readfirstlane((int)held);
-            if (bits == 0) continue;
-#pragma unroll 1
-            for (int u = 0; u < 2; u += kAtOnce)
-                if (kAtOnce > 1 || (uint32_t)(bits >> (32 * u)) != 0)
-                    rows.template add<Tile, kAtOnce>(lk + t * Tile::kBytes, lv + t * Tile::kBytes, 32 * u, bits >> (32 * u),
-                                                 g.c, lane);
+        for (bool again = false;; again = true) {
+            rows.clear();
+            uint32_t bits = 0;
+            const int u0 = next(-1, bits);
+            for (int u = u0; u < squares; u = next(u, bits))
+                rows.template add<Tile>(lk + u * 32 * Tile::kRowBytes, lv + u * 32 * Tile::kRowBytes, bits,
+                                        u == u0 && !again, g.c, lane);
+            if (__builtin_expect(again || !rows.passed(), 1)) break;
+            for (int u = next(-1, bits); u < squares; u = next(u, bits)) {
+                f32x16 s[QB];
+                rows.template score<Tile>(lk + u * 32 * Tile::kRowBytes, bits, s, lane);
+                rows.template raise<false>(s);
+            }
         }
         rows.store(a, lane);
     }
@@ -370,7 +419,7 @@ constexpr int kWaves = 4;
 
 // The rows' squares of a wave: two where the registers hold them.
 template <class T, int D>
-constexpr int kHeldSquares = sizeof(T) == 2 && D <= 64 ? 2 : 1;
+constexpr int kHeldSquares = 1;
 
 Plan plan_of(const Attention& a) {
     Plan p{};
@@ -380,10 +429,10 @@ Plan plan_of(const Attention& a) {
     p.grid.rows = a.queries * p.grid.shared;
     p.grid.c = exponent_of(a.scale);
     p.grid.splits = 1;
-    const int64_t held_rows = 32 * (halves && width <= 64 ? 2 : 1);
+    const int64_t held_rows = 32;
     const int64_t wave_blocks = (p.grid.rows + held_rows - 1) / held_rows;
-    p.held = a.states > 0 && (a.states + 63) / 64 * 64 * width * (halves ? 2 : 4) <= kHeldBytes && (halves || width <= 64) &&
-             wave_blocks * pairs >= 256 * kHeldWaves && pairs <= 65536;
+    p.held = a.states > 0 && (a.states + 63) / 64 * 64 * width * (halves ? 2 : 4) <= held_bytes((int)width) && (halves || width <= 64) &&
+             wave_blocks * pairs >= 256 * held_waves(halves ? 2 : 4, (int)width) && pairs <= 65536;
     if (p.held) {
         const int64_t parts = pairs < 256 ? 256 / pairs : 1;
         p.grid.part = (wave_blocks + parts - 1) / parts;
@@ -421,7 +470,7 @@ int launch_attention(const Attention& a, void* workspace, hipStream_t s) {
             if (p.held) {
                 if constexpr (sizeof(T) == 2 || D <= 64)
                     held_kernel<T, D, kHeldSquares<T, D>>
-                        <<<(unsigned)p.workgroups, 64 * kHeldWaves, 0, s>>>(a, p.grid);
+                        <<<(unsigned)p.workgroups, 64 * kHeldWaves<T, D>, 0, s>>>(a, p.grid);
                 return;
             }
             p.grid.sums = (float*)workspace;

@@ -129,38 +129,30 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
     const int64_t e = pair / a.kv_heads;
     const int kv = (int)(pair % a.kv_heads), d = a.head;
 
-    int64_t row[QB];
-    int head[QB];
-    bool exists[QB];
+    LaneRows<QB> rows;
     typename S::Frag q[QB][kSteps], go[QB][kSteps];
     float lse[QB], delta[QB];
+    rows.begin(e * a.queries, (block * kWaves + wave) * QB * 32, g.rows, kv * g.shared, g.shared, lane);
+    {
+        typename S::Frag o[QB][kSteps];
+        rows.template load<T, kSteps>(b.grad_out, d, lane, go);
+        rows.template load<T, kSteps>(a.out, d, lane, o);
+        rows.template load<T, kSteps>(a.q, d, lane, q);
 #pragma unroll
-    for (int n = 0; n < QB; ++n) {
-        const int64_t i = ((block * kWaves + wave) * QB + n) * 32 + (lane & 31);
-        exists[n] = i < g.rows;
-        const int64_t r = g.shared == 1 ? i : i / g.shared;
-        head[n] = kv * g.shared + (g.shared == 1 ? 0 : (int)(i - r * g.shared));
-        row[n] = e * a.queries + r;
-        const T* p = (const T*)a.q.p + row[n] * a.q.stride + (int64_t)head[n] * d;
-        const T* x = (const T*)b.grad_out.p + row[n] * b.grad_out.stride + (int64_t)head[n] * d;
-        const T* y = (const T*)a.out.p + row[n] * a.out.stride + (int64_t)head[n] * d;
-        float dot = 0.0f;
+        for (int n = 0; n < QB; ++n) {
+            float dot = 0.0f;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int c = 2 * s + (lane >> 5);
-            q[n][s] = row_chunk<T>(p, c, d, exists[n]);
-            go[n][s] = row_chunk<T>(x, c, d, exists[n]);
-            const auto o = row_chunk<T>(y, c, d, exists[n]);
+            for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-            for (int k = 0; k < 16 / (int)sizeof(T); ++k) dot = fmaf((float)go[n][s][k], (float)o[k], dot);
-        }
-        float other = dot;
-        swap32(dot, other);
-        delta[n] = dot + other;
-        lse[n] = INFINITY;
-        if (exists[n]) {
-            lse[n] = lse_exponent<T>(a.lse[row[n] * a.lse_row_step + head[n] * a.lse_head_step]);
-            if (lane < 32 && split == 0) g.delta[row[n] * a.heads + head[n]] = delta[n];
+                for (int k = 0; k < 16 / (int)sizeof(T); ++k) dot = fmaf((float)go[n][s][k], (float)o[n][s][k], dot);
+            float other = dot;
+            swap32(dot, other);
+            delta[n] = dot + other;
+            lse[n] = INFINITY;
+            if (rows.exists[n]) {
+                lse[n] = lse_exponent<T>(a.lse[rows.row(n) * a.lse_row_step + rows.head[n] * a.lse_head_step]);
+                if (lane < 32 && split == 0) g.delta[rows.row(n) * a.heads + rows.head[n]] = delta[n];
+            }
         }
     }
 
@@ -206,10 +198,11 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
         const uint64_t bits = exist;
         wait_for_stage<1>(0);
         more = load(buffer ^ 1);
-        const unsigned char *lk = lds[buffer][0], *lv = lds[buffer][1];
+        const unsigned char* const at = lds[buffer][0];
         buffer ^= 1;
 #pragma unroll 1
         for (int u = 0; u < kSubs; ++u) {
+            const unsigned char *lk = at + 32 * u * Tile::kRowBytes, *lv = lk + Tile::kBytes;
             f32x16 s[QB], dp[QB];
 #pragma unroll
             for (int n = 0; n < QB; ++n)
@@ -217,10 +210,10 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
                 for (int r = 0; r < 16; ++r) s[n][r] = dp[n][r] = 0.0f;
 #pragma unroll
             for (int p = 0; p < kSteps; ++p) {
-                const auto f = Tile::along(lk, 32 * u, p, lane);
+                const auto f = Tile::along(lk, p, lane);
 #pragma unroll
                 for (int n = 0; n < QB; ++n) S::multiply(f, q[n][p], s[n]);
-                const auto w = Tile::along(lv, 32 * u, p, lane);
+                const auto w = Tile::along(lv, p, lane);
 #pragma unroll
                 for (int n = 0; n < QB; ++n) S::multiply(w, go[n][p], dp[n]);
             }
@@ -246,7 +239,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
                 for (int n = 0; n < QB; ++n) w[n] = S::rounded(dp[n], p);
 #pragma unroll
                 for (int c = 0; c < kCols; ++c) {
-                    const auto f = Tile::across(lk, 32 * u + p * S::kDepth, 32 * c, lane);
+                    const auto f = Tile::across(lk, p * S::kDepth, 32 * c, lane);
 #pragma unroll
                     for (int n = 0; n < QB; ++n) S::multiply(f, w[n], sums[n][c]);
                 }
@@ -255,10 +248,10 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
     }
 #pragma unroll
     for (int n = 0; n < QB; ++n) {
-        if (!exists[n]) continue;
+        if (!rows.exists[n]) continue;
         const float by = a.scale * lowered<T>(lift[n]);
-        const int64_t at = ((int64_t)split * a.q.rows + row[n]) * a.heads + head[n];
-        T* to = SPLIT ? nullptr : (T*)b.grad_q.p + row[n] * b.grad_q.stride + (int64_t)head[n] * d;
+        const int64_t at = ((int64_t)split * a.q.rows + rows.row(n)) * a.heads + rows.head[n];
+        T* to = SPLIT ? nullptr : (T*)b.grad_q.p + rows.row(n) * b.grad_q.stride + (int64_t)rows.head[n] * d;
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
 #pragma unroll
@@ -294,13 +287,12 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(A
     const bool inside = j < a.states;
     const bool exists = inside && (!a.mask || a.mask[e * a.mask_stride + j]);
     const int64_t state = e * a.states + j;
-    typename S::Frag k[kSteps], v[kSteps];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        const int c = 2 * s + (lane >> 5);
-        k[s] = row_chunk<T>((const T*)a.k.p + state * a.k.stride + (int64_t)kv * d, c, d, exists);
-        v[s] = row_chunk<T>((const T*)a.v.p + state * a.v.stride + (int64_t)kv * d, c, d, exists);
-    }
+    typename S::Frag k[1][kSteps], v[1][kSteps];
+    LaneRows<1> states;
+    states.begin(e * a.states, (block * kWaves + wave) * 32, a.states, kv, 1, lane);
+    states.exists[0] = exists;
+    states.template load<T, kSteps>(a.k, d, lane, k);
+    states.template load<T, kSteps>(a.v, d, lane, v);
 
     Tile tq, to;
     const int64_t q_pitch = a.q.stride * (int64_t)sizeof(T), o_pitch = b.grad_out.stride * (int64_t)sizeof(T);
@@ -351,18 +343,19 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(A
         else if (threadIdx.x < 2 * QT) row_delta[buffer][of] = value;
         wait_for_stage<1>(0);
         more = load(buffer ^ 1);
-        const unsigned char *lq = lds[buffer][0], *lo = lds[buffer][1];
+        const unsigned char* const from = lds[buffer][0];
         const float *le = row_lse[buffer], *de = row_delta[buffer];
         buffer ^= 1;
 #pragma unroll 1
         for (int u = 0; u < kSubs; ++u) {
+            const unsigned char *lq = from + 32 * u * Tile::kRowBytes, *lo = lq + Tile::kBytes;
             f32x16 s, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
 #pragma unroll
             for (int p = 0; p < kSteps; ++p) {
-                S::multiply(Tile::along(lq, 32 * u, p, lane), k[p], s);
-                S::multiply(Tile::along(lo, 32 * u, p, lane), v[p], dp);
+                S::multiply(Tile::along(lq, p, lane), k[0][p], s);
+                S::multiply(Tile::along(lo, p, lane), v[0][p], dp);
             }
 #pragma unroll
             for (int r0 = 0; r0 < 16; r0 += 4) {
@@ -380,8 +373,8 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(A
                 const auto w = S::rounded(s, p), x = S::rounded(dp, p);
 #pragma unroll
                 for (int c = 0; c < kCols; ++c) {
-                    S::multiply(Tile::across(lo, 32 * u + p * S::kDepth, 32 * c, lane), w, gv[c]);
-                    S::multiply(Tile::across(lq, 32 * u + p * S::kDepth, 32 * c, lane), x, gk[c]);
+                    S::multiply(Tile::across(lo, p * S::kDepth, 32 * c, lane), w, gv[c]);
+                    S::multiply(Tile::across(lq, p * S::kDepth, 32 * c, lane), x, gk[c]);
                 }
             }
         }
