@@ -171,6 +171,26 @@ struct RowTile {
             return u.whole;
         }
     }
+
+    // Of a 16 x 16 square's product over 32 rows from r0 on: columns c0 .. c0 + 15, and the
+    // rows in the order 4 (lane / 16) + (e & 3) + 16 (e >> 2).
+    static __device__ __forceinline__ typename S::Frag across16(const unsigned char* lds, int r0, int c0, int lane) {
+        static_assert(sizeof(T) == 2, "");
+        const int a = lane & 15;
+        typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+        union {
+            i16x4 part[2];
+            typename S::Frag whole;
+        } u;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int r = r0 + 16 * p + 4 * (lane >> 4) + (a >> 2);
+            const int c = c0 / 8 + ((a & 3) >> 1);
+            u.part[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_i16x4*)(lds_byte*)(lds + r * kRowBytes + ((c ^ turn(r)) << 4) + (a & 1) * 8));
+        }
+        return u.whole;
+    }
 };
 
 // The rows that 32 QB lanes of a wave take, of those that read one head of the

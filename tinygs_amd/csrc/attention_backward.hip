@@ -16,8 +16,10 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.h"
+#include "row_chunks.h"
 
 namespace tgs {
 
@@ -406,6 +408,214 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(A
         }
 }
 
+// ---- up to 256 states of heads up to 64: all three gradients in one pass over
+// the rows. A workgroup's waves hold 32 states each, with the sums of dk and dv;
+// tiles of 64 rows go by. What a tile's ds is to dq needs all states: it goes to LDS
+// as [state][row], and in the next step, behind that tile's barrier, the waves share the
+// product k^T ds^T among them, 16 columns by 16 rows at a time, with k^T in registers.
+constexpr int kOnceWaves = 8, kOnceStates = 32 * kOnceWaves, kOnceRows = 64;
+
+template <class T, int D>
+__global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackward b, Grid g) {
+    using S = Square<T>;
+    constexpr int kTileLoads = kOnceRows * D * (int)sizeof(T) / 1024;
+    constexpr int kLoaders = kTileLoads < kOnceWaves ? kTileLoads : kOnceWaves;
+    using Tile = RowTile<T, D, kOnceRows, kLoaders>;
+    using Weights = RowTile<T, kOnceRows, kOnceStates, kOnceWaves>;   // ds: a row a state
+    constexpr int kSteps = D / 16, kCols = D / 32;
+    constexpr int kAcross = D / 16, kDown = 4 * kAcross / kOnceWaves;   // 16 x 16 squares of dq across; a wave's
+    constexpr int kChunks = D / 8;                                      // of a row's head
+    __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes], weights[2][Weights::kBytes];
+    __shared__ __align__(16) float row_lse[2][kOnceRows], row_delta[2][kOnceRows];
+    const Attention& a = b.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t number = xcd_contiguous_index(blockIdx.x, gridDim.x);
+    const int64_t split = number % g.splits, pair = number / g.splits;
+    const int64_t e = pair / a.kv_heads;
+    const int kv = (int)(pair % a.kv_heads), d = a.head;
+
+    const int64_t j = wave * 32 + (lane & 31);   // the lane's state
+    const bool inside = j < a.states;
+    const bool exists = inside && (!a.mask || a.mask[e * a.mask_stride + j]);
+    const int64_t state = e * a.states + j;
+    typename S::Frag k[1][kSteps], v[1][kSteps];
+    LaneRows<1> states;
+    states.begin(e * a.states, wave * 32, a.states, kv, 1, lane);
+    states.exists[0] = exists;
+    states.template load<T, kSteps>(a.k, d, lane, k);
+    states.template load<T, kSteps>(a.v, d, lane, v);
+
+    // k^T of the wave's 16 columns, all states, through LDS
+    const int across = wave % kAcross, down = wave / kAcross * kDown;
+    typename S::Frag kt[kOnceStates / 32];
+    {
+        using Keys = RowTile<T, D, kOnceStates, kOnceWaves>;
+        static_assert(Keys::kBytes <= 2 * Weights::kBytes, "");
+        unsigned char* const at = weights[0];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {   // the lane's row, as it would be loaded
+            const int r = (int)j, c = (2 * s + (lane >> 5)) ^ Keys::turn(r);
+            *(typename S::Frag*)(at + r * Keys::kRowBytes + (c << 4)) = k[0][s];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < kOnceStates / 32; ++s) kt[s] = Keys::across16(at, 32 * s, 16 * across, lane);
+        __syncthreads();
+    }
+
+    Tile tq, to;
+    const int64_t q_pitch = a.q.stride * (int64_t)sizeof(T), o_pitch = b.grad_out.stride * (int64_t)sizeof(T);
+    tq.begin(q_pitch, d, wave, lane);
+    to.begin(o_pitch, d, wave, lane);
+    const int64_t first_row = e * a.queries;
+    const int64_t per_head = g.units / g.shared;
+    const int64_t t0 = split * g.part, t1 = min(t0 + g.part, g.units);
+    int64_t t = t0 - 1;
+    int h = (int)(t0 / per_head);         // of the next tile, among the shared heads
+    int64_t in = t0 - h * per_head - 1;   // the tile's number in its head
+    float lse = 0.0f;                     // of the thread's row, on its way to LDS
+    bool lse_there = false;
+    typename S::Frag o = {}, go = {};     // the thread's chunks of a row, for delta
+    const int of = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks;
+    const auto load = [&](int buffer) {
+        if (++t >= t1) return false;
+        if (++in == per_head) {
+            in = 0;
+            ++h;
+        }
+        const int64_t r0 = in * kOnceRows, left = a.queries - r0;
+        const uint64_t bits = left >= 64 ? ~0ull : (1ull << left) - 1;
+        const int head = kv * g.shared + h;
+        const int64_t at = (int64_t)head * d * (int64_t)sizeof(T), width = d * (int64_t)sizeof(T);
+        if (wave < kLoaders) {
+            tq.load(lds[buffer][0], (const unsigned char*)a.q.p + at + (first_row + r0) * q_pitch,
+                    (left - 1) * q_pitch + width, bits, d, wave, lane);
+            to.load(lds[buffer][1], (const unsigned char*)b.grad_out.p + at + (first_row + r0) * o_pitch,
+                    (left - 1) * o_pitch + width, bits, d, wave, lane);
+        }
+        // without branches, which would wait for the loads where they meet
+        const int64_t x_pitch = a.out.stride * (int64_t)sizeof(T);
+        const auto outs = resource_of((const unsigned char*)a.out.p + at + (first_row + r0) * x_pitch,
+                                      (left - 1) * x_pitch + width);
+        const auto grads = resource_of((const unsigned char*)b.grad_out.p + at + (first_row + r0) * o_pitch,
+                                       (left - 1) * o_pitch + width);
+        const bool there = of < kOnceRows && of < left && chunk * 8 < d;
+        o = __builtin_bit_cast(typename S::Frag, __builtin_amdgcn_raw_buffer_load_b128(
+            outs, there ? (int)(uint32_t)(of * x_pitch + chunk * 16) : (int)kPastEnd, 0, 0));
+        go = __builtin_bit_cast(typename S::Frag, __builtin_amdgcn_raw_buffer_load_b128(
+            grads, there ? (int)(uint32_t)(of * o_pitch + chunk * 16) : (int)kPastEnd, 0, 0));
+        const int64_t row = threadIdx.x % kOnceRows;
+        lse = a.lse[(first_row + r0 + min(row, left - 1)) * a.lse_row_step + head * a.lse_head_step];
+        lse_there = row < left;
+        return true;
+    };
+    // dq of the tile whose ds stands in `from`: rows r0 .. of the head
+    const auto add_rows = [&](const unsigned char* from, int head, int64_t r0) {
+        const int64_t left = a.queries - r0;
+#pragma unroll
+        for (int n = 0; n < kDown; ++n) {
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < kOnceStates / 32; ++s)
+                x = multiply(kt[s], Weights::across16(from, 32 * s, 16 * (down + n), lane), x);
+            const int row = 16 * (down + n) + (lane & 15), c0 = 16 * across + 4 * (lane >> 4);
+            if (row < left && c0 < d) {   // d is a multiple of 8
+                typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+                Four y;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) y[c] = (T)(x[c] * a.scale);
+                *(Four*)((T*)b.grad_q.p + (first_row + r0 + row) * b.grad_q.stride + (int64_t)head * d + c0) = y;
+            }
+        }
+    };
+
+    f32x16 gk[kCols], gv[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) gk[c][r] = gv[c][r] = 0.0f;
+    const uint32_t keep = exists ? ~0u : 0u;
+    int buffer = 0, last_head = 0;
+    int64_t last_row = 0;
+    bool more = load(0), begun = false;
+    while (more) {
+        float delta = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) delta = fmaf((float)go[c], (float)o[c], delta);
+        float parts[1] = {delta};
+        int none = 0;
+        group_sum<kChunks>(parts, nullptr, none);
+        if (of < kOnceRows && chunk == 0) row_delta[buffer][of] = parts[0];
+        if (threadIdx.x < kOnceRows) row_lse[buffer][threadIdx.x] = lse_there ? lse_exponent<T>(lse) : INFINITY;
+        const int head = kv * g.shared + h;
+        const int64_t r0 = in * kOnceRows;
+        wait_for_stage<1>(0);   // the tile is there, and the last one's ds; their buffers are free
+        more = load(buffer ^ 1);
+        if (begun && b.grad_q.p) add_rows(weights[buffer ^ 1], last_head, last_row);
+        begun = true;
+        last_head = head;
+        last_row = r0;
+        unsigned char* const to_weights = weights[buffer] + (int)j * Weights::kRowBytes;
+#pragma unroll 1
+        for (int u = 0; u < kOnceRows / 32; ++u) {
+            const unsigned char *lq = lds[buffer][0] + 32 * u * Tile::kRowBytes, *lo = lq + Tile::kBytes;
+            f32x16 s = S::product(Tile::along(lq, 0, lane), k[0][0]), dp = S::product(Tile::along(lo, 0, lane), v[0][0]);
+#pragma unroll
+            for (int p = 1; p < kSteps; ++p) {
+                S::multiply(Tile::along(lq, p, lane), k[0][p], s);
+                S::multiply(Tile::along(lo, p, lane), v[0][p], dp);
+            }
+#pragma unroll
+            for (int r0 = 0; r0 < 16; r0 += 4) {
+                const int at = 32 * u + square_row(r0, lane);
+                const f32x4 l4 = *(const f32x4*)(row_lse[buffer] + at), d4 = *(const f32x4*)(row_delta[buffer] + at);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[r0 + r] = __builtin_amdgcn_exp2f(fmaf(s[r0 + r], g.c, -l4[r]));
+                    dp[r0 + r] = s[r0 + r] * (dp[r0 + r] - d4[r]);
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const auto w = S::rounded(s, p), x = S::rounded(dp, p);
+                typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                const u32x4 bits = __builtin_bit_cast(u32x4, x) & keep;   // zeros for a state that does not exist
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {   // rows 32 u + 16 p + 8 n + 4 (lane / 32) .. + 3
+                    const int c = (4 * u + 2 * p + n) ^ Weights::turn((int)j);
+                    *(u32x2*)(to_weights + (c << 4) + 8 * (lane >> 5)) = u32x2{bits[2 * n], bits[2 * n + 1]};
+                }
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    S::multiply(Tile::across(lo, p * 16, 32 * c, lane), w, gv[c]);
+                    S::multiply(Tile::across(lq, p * 16, 32 * c, lane), x, gk[c]);
+                }
+            }
+        }
+        buffer ^= 1;
+    }
+    __syncthreads();
+    if (begun && b.grad_q.p) add_rows(weights[buffer ^ 1], last_head, last_row);
+    if (!inside) return;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            float x[8], y[8];
+            square_rows(gk[c], p, x);
+            square_rows(gv[c], p, y);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                x[n] = exists ? x[n] * a.scale : 0.0f;
+                y[n] = exists ? y[n] : 0.0f;
+            }
+            const int c0 = 32 * c + 16 * p + 8 * (lane >> 5);
+            const int64_t n = a.k.rows * a.kv_heads, at = state * a.kv_heads + kv;
+            store_eight<float>(g.sums + ((2 * split) * n + at) * D, c0, D, x);
+            store_eight<float>(g.sums + ((2 * split + 1) * n + at) * D, c0, D, y);
+        }
+}
+
 // Sums of the splits' parts, in their order: set `n` x D floats, `step` sets apart.
 template <class T, int D>
 __global__ void __launch_bounds__(256) join_kernel(const float* sums, int splits, int64_t step, Mat to, int heads, int d) {
@@ -430,7 +640,17 @@ void split_tiles(int64_t whole, int64_t tiles, int& splits, int64_t& part) {
     splits = tiles > 0 ? (int)((tiles + part - 1) / part) : 1;
 }
 
+// Whether the one-pass kernel takes it: states and heads that it holds, and as many
+// rows as pay for its start and its sums' join.
+bool at_once(const AttentionBackward& b) {
+    const Attention& a = b.a;
+    return a.dtype == TGS_DTYPE_BFLOAT16 && b.grad_q.p && (b.grad_k.p || b.grad_v.p) && a.head <= 64 && a.head % 8 == 0 &&
+           a.states >= 1 && a.states <= kOnceStates && a.batch * a.kv_heads <= 65536 &&
+           (a.queries + kOnceRows - 1) / kOnceRows * (a.heads / a.kv_heads) * a.batch * a.kv_heads >= 1024;
+}
+
 struct Plan {
+    bool once;
     int qb, tile;
     Grid q, kv;
     int64_t q_workgroups, kv_workgroups;
@@ -446,6 +666,17 @@ Plan plan_of(const AttentionBackward& b) {
     p.q.shared = p.kv.shared = a.heads / a.kv_heads;
     p.q.rows = p.kv.rows = a.queries * p.q.shared;
     p.q.c = p.kv.c = exponent_of(a.scale);
+    p.once = at_once(b);
+    if (p.once) {
+        const int64_t pairs = a.batch * a.kv_heads;
+        p.kv.units = (a.queries + kOnceRows - 1) / kOnceRows * p.kv.shared;
+        const int64_t splits = pairs < 256 ? 256 / pairs : 1;
+        p.kv.part = (p.kv.units + splits - 1) / splits;
+        p.kv.splits = (int)((p.kv.units + p.kv.part - 1) / p.kv.part);
+        p.kv_workgroups = pairs * p.kv.splits;
+        p.bytes = sizeof(float) * 2 * (size_t)(p.kv.splits * a.k.rows * a.kv_heads * width);
+        return p;
+    }
     p.qb = halves && p.q.rows > 32 * kWaves ? 2 : 1;
     p.q.blocks = (p.q.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
     int64_t whole = a.batch * a.kv_heads * p.q.blocks;
@@ -492,6 +723,22 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
         using T = decltype(t);
         by_head_width(a.head, [&](auto width) {
             constexpr int D = decltype(width)::value, kTile = sizeof(T) == 2 ? 64 : 32;
+            const auto join = [&] {
+                const int64_t n = a.k.rows * a.kv_heads;
+                const unsigned blocks = join_blocks(n * a.head);
+                if (b.grad_k.p)
+                    join_kernel<T, D><<<blocks, 256, 0, s>>>(p.kv.sums, p.kv.splits, 2 * n, b.grad_k, a.kv_heads, a.head);
+                if (b.grad_v.p)
+                    join_kernel<T, D><<<blocks, 256, 0, s>>>(p.kv.sums + n * D, p.kv.splits, 2 * n, b.grad_v, a.kv_heads,
+                                                             a.head);
+            };
+            if (p.once) {
+                if constexpr (D <= 64 && std::is_same_v<T, __bf16>) {
+                    once_kernel<T, D><<<(unsigned)p.kv_workgroups, 64 * kOnceWaves, 0, s>>>(b, p.kv);
+                    join();
+                }
+                return;
+            }
             if (b.grad_q.p && a.q.rows) {
                 const auto launch = [&](auto qb) {
                     constexpr int QB = decltype(qb)::value;
@@ -518,15 +765,7 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
                 if (p.kv.splits > 1) grad_kv_kernel<T, D, kTile, true><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
                 else grad_kv_kernel<T, D, kTile, false><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
             });
-            if (p.kv.splits > 1) {
-                const int64_t n = a.k.rows * a.kv_heads;
-                const unsigned blocks = join_blocks(n * a.head);
-                if (b.grad_k.p)
-                    join_kernel<T, D><<<blocks, 256, 0, s>>>(p.kv.sums, p.kv.splits, 2 * n, b.grad_k, a.kv_heads, a.head);
-                if (b.grad_v.p)
-                    join_kernel<T, D><<<blocks, 256, 0, s>>>(p.kv.sums + n * D, p.kv.splits, 2 * n, b.grad_v, a.kv_heads,
-                                                             a.head);
-            }
+            if (p.kv.splits > 1) join();
         });
     });
     TGS_CHECK_LAUNCH();
