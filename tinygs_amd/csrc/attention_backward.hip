@@ -10,9 +10,9 @@
 // one kernel, either sum would have to leave it in as many parts as there are
 // blocks of the other side.
 //
-// Halves: p is held times 2^10, and ds times a power of two that each lane
-// chooses by the largest it met, so that small ones keep their bits; sums are
-// scaled where it changes.
+// Halves: p is held times 2^10, and ds times a power of two that brings the
+// largest it can be, |do| |v| + |delta|, to 2^14: of a row's and all states' in
+// dq, of a state's and all rows' in dk, so that small ones keep their bits.
 #include <math.h>
 
 #include <algorithm>
@@ -42,85 +42,109 @@ struct Grid {
     int64_t part;     // tiles of a split
     float c;          // scale log2(e)
     float* delta;     // [row][head]
+    float* norms;     // halves: of each 64 states' values; then the pairs of the workgroups' largest |do| and |delta|
+    int64_t lifts;    // how many of the latter
+    float* largest;
     float* sums;      // the splits' parts
 };
 
-// A power of two for each lane by which small gradients of weights are lifted into a half's range.
-struct Lift {
-    float by = 0x1p100f;   // nothing met yet
+// The exponent of the power of two that lifts gradients of weights up to `largest` to 2^14; 0 where that says nothing.
+template <class T>
+__device__ __forceinline__ int lift_of(float largest) {
+    if constexpr (kBoost<T> == 0.0f) return 0;
+    return largest > 0.0f && largest < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(largest) : 0;
+}
 
-    // largest: of the lane's column, the same in both halves. Whether the sums have to be multiplied by *change.
-    __device__ __forceinline__ bool meet(float largest, float* change) {
-        const bool passed = !(largest * by <= 0x1p14f);   // NaN and infinity: any power keeps them
-        *change = 1.0f;
-        if (passed) {
-            const float to = __builtin_ldexpf(1.0f, 7 - __builtin_amdgcn_frexp_expf(largest));
-            *change = to / by;
-            by = to;
-        }
-        return ballot(passed) != 0;
-    }
-};
+// The largest of n numbers, for all lanes of the workgroup's waves.
+__device__ __forceinline__ float largest_of(const float* p, int64_t n, int64_t step) {
+    float v = 0.0f;
+    for (int64_t k = threadIdx.x & 63; k < n; k += 64) v = fmaxf(v, p[k * step]);
+    for (int k = 32; k > 0; k >>= 1) v = fmaxf(v, __shfl_xor(v, k, 64));
+    return v;
+}
 
-// ds in place of dp's square, from p's; halves: lifted, the sums with it.
-template <class T, int N>
-__device__ __forceinline__ void lift_weights(f32x16& ds, Lift& lift, f32x16 (&sums)[N]) {
-    if constexpr (sizeof(T) == 2 && kBoost<T> != 0.0f) {
-        float largest = 0.0f;
+// Halves: of each 64 states' values, the largest norm of a row.
+template <class T>
+__global__ void __launch_bounds__(256) norms_kernel(Attention a, float* norms) {
+    static_assert(kChunk<T> == 8, "");
+    const int64_t blocks = (a.states + 63) / 64, n = a.batch * a.kv_heads * blocks;
+    const int lane = threadIdx.x & 63;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
+        const int64_t pair = i / blocks, j = (i - pair * blocks) * 64 + lane, e = pair / a.kv_heads;
+        const int kv = (int)(pair - e * a.kv_heads);
+        float v = 0.0f;
+        if (j < a.states && (!a.mask || a.mask[e * a.mask_stride + j])) {
+            const T* p = (const T*)a.v.p + (e * a.states + j) * a.v.stride + (int64_t)kv * a.head;
+#pragma unroll 8
+            for (int c = 0; c < (a.head + 7) / 8; ++c) {
+                float x[8];
+                load_chunk<T>(p, c, a.head, x);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) largest = fmaxf(largest, fabsf(ds[r]));
-        float other = largest;
-        swap32(largest, other);
-        largest = fmaxf(largest, other);
-        float change;
-        if (lift.meet(largest, &change)) {
-#pragma unroll
-            for (int c = 0; c < N; ++c)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) sums[c][r] *= change;
+                for (int k = 0; k < 8; ++k) v = fmaf(x[k], x[k], v);
+            }
         }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ds[r] *= lift.by;
+        for (int k = 32; k > 0; k >>= 1) v = fmaxf(v, __shfl_xor(v, k, 64));
+        if (lane == 0) norms[i] = sqrtf(v);
     }
 }
 
-// What undoes the lift and p's boost in a sum of lifted gradients.
-template <class T>
-__device__ __forceinline__ float lowered(const Lift& lift) {
-    return kBoost<T> != 0.0f ? 0x1p-10f / lift.by : 1.0f;
+// The workgroup's largest |do|^2 and |delta| to its place, as |do| and |delta|.
+__device__ __forceinline__ void leave_largest(const Grid& g, float most, float most_delta) {
+    __shared__ float s[2][4];
+    for (int k = 32; k > 0; k >>= 1) {
+        most = fmaxf(most, __shfl_xor(most, k, 64));
+        most_delta = fmaxf(most_delta, __shfl_xor(most_delta, k, 64));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        s[0][threadIdx.x >> 6] = most;
+        s[1][threadIdx.x >> 6] = most_delta;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 4; ++k) {
+            most = fmaxf(most, s[0][k]);
+            most_delta = fmaxf(most_delta, s[1][k]);
+        }
+        g.largest[2 * (g.first + blockIdx.x)] = sqrtf(most);
+        g.largest[2 * (g.first + blockIdx.x) + 1] = most_delta;
+    }
 }
 
 // lse in the exponent's unit; +infinity where there is no state: all weights are 0.
 template <class T>
 __device__ __forceinline__ float lse_exponent(float lse) {
-    return lse == -INFINITY ? INFINITY : lse * kLog2E - kBoost<T>;
+    return lse == -INFINITY ? INFINITY : lse * kLog2E;
 }
 
 // delta, where dq is not asked for; in the order that the two halves of a wave sum it there
 template <class T>
-__global__ void __launch_bounds__(256) delta_kernel(AttentionBackward b, float* delta) {
+__global__ void __launch_bounds__(256) delta_kernel(AttentionBackward b, Grid g) {
     const Attention& a = b.a;
     const int64_t n = a.q.rows * a.heads;
+    float most = 0.0f, most_delta = 0.0f;
     for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
         const int64_t r = k / a.heads;
         const int h = (int)(k % a.heads);
         const T* x = (const T*)b.grad_out.p + r * b.grad_out.stride + (int64_t)h * a.head;
         const T* y = (const T*)a.out.p + r * a.out.stride + (int64_t)h * a.head;
-        float v[2] = {0.0f, 0.0f};
+        float v[2] = {0.0f, 0.0f}, w[2] = {0.0f, 0.0f};
         for (int c = 0; c < a.head; ++c) {
             const int half = c / (16 / (int)sizeof(T)) & 1;
             v[half] = fmaf((float)x[c], (float)y[c], v[half]);
+            w[half] = fmaf((float)x[c], (float)x[c], w[half]);
         }
-        delta[k] = v[0] + v[1];
+        g.delta[k] = v[0] + v[1];
+        most = fmaxf(most, w[0] + w[1]);
+        most_delta = fmaxf(most_delta, fabsf(v[0] + v[1]));
     }
+    if constexpr (kBoost<T> != 0.0f) leave_largest(g, most, most_delta);
 }
 
 template <class T, int D, int QB, int KT, bool SPLIT>
-__global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(AttentionBackward b, Grid g) {
+__global__ void __launch_bounds__(64 * kWaves, D <= 64 || sizeof(T) == 2 ? 2 : 1) grad_q_kernel(AttentionBackward b, Grid g) {
     using S = Square<T>;
     using Tile = RowTile<T, D, KT, kWaves>;
     constexpr int kSteps = D / S::kDepth, kParts = 32 / S::kDepth, kSubs = KT / 32, kCols = D / 32;
-    constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
     __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes];
     const Attention& a = b.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -133,29 +157,45 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
 
     LaneRows<QB> rows;
     typename S::Frag q[QB][kSteps], go[QB][kSteps];
-    float lse[QB], delta[QB];
+    float lse[QB], delta[QB], by[QB];   // by: of the sums
     rows.begin(e * a.queries, (block * kWaves + wave) * QB * 32, g.rows, kv * g.shared, g.shared, lane);
     {
         typename S::Frag o[QB][kSteps];
         rows.template load<T, kSteps>(b.grad_out, d, lane, go);
         rows.template load<T, kSteps>(a.out, d, lane, o);
         rows.template load<T, kSteps>(a.q, d, lane, q);
+        float norm = 0.0f, most = 0.0f, most_delta = 0.0f;
+        if constexpr (kBoost<T> != 0.0f) {
+            const int64_t blocks = (a.states + 63) / 64;
+            norm = largest_of(g.norms + pair * blocks, blocks, 1);
+        }
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
-            float dot = 0.0f;
+            float dot = 0.0f, square = 0.0f;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-                for (int k = 0; k < 16 / (int)sizeof(T); ++k) dot = fmaf((float)go[n][s][k], (float)o[n][s][k], dot);
+                for (int k = 0; k < 16 / (int)sizeof(T); ++k) {
+                    dot = fmaf((float)go[n][s][k], (float)o[n][s][k], dot);
+                    if constexpr (kBoost<T> != 0.0f) square = fmaf((float)go[n][s][k], (float)go[n][s][k], square);
+                }
             float other = dot;
             swap32(dot, other);
             delta[n] = dot + other;
+            other = square;
+            swap32(square, other);
+            square += other;
+            most = fmaxf(most, square);
+            most_delta = fmaxf(most_delta, fabsf(delta[n]));
+            const int lift = lift_of<T>(fmaf(sqrtf(square), norm, fabsf(delta[n])));
+            by[n] = __builtin_ldexpf(a.scale, -lift);
             lse[n] = INFINITY;
             if (rows.exists[n]) {
-                lse[n] = lse_exponent<T>(a.lse[rows.row(n) * a.lse_row_step + rows.head[n] * a.lse_head_step]);
+                lse[n] = lse_exponent<T>(a.lse[rows.row(n) * a.lse_row_step + rows.head[n] * a.lse_head_step]) - (float)lift;
                 if (lane < 32 && split == 0) g.delta[rows.row(n) * a.heads + rows.head[n]] = delta[n];
             }
         }
+        if constexpr (kBoost<T> != 0.0f) leave_largest(g, most, most_delta);
     }
 
     Tile tk, tv;
@@ -187,7 +227,6 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
     };
 
     f32x16 sums[QB][kCols];
-    Lift lift[QB];
 #pragma unroll
     for (int n = 0; n < QB; ++n)
 #pragma unroll
@@ -207,19 +246,20 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
             const unsigned char *lk = at + 32 * u * Tile::kRowBytes, *lv = lk + Tile::kBytes;
             f32x16 s[QB], dp[QB];
 #pragma unroll
-            for (int n = 0; n < QB; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[n][r] = dp[n][r] = 0.0f;
-#pragma unroll
             for (int p = 0; p < kSteps; ++p) {
-                const auto f = Tile::along(lk, p, lane);
+                const auto f = Tile::along(lk, p, lane), w = Tile::along(lv, p, lane);
 #pragma unroll
-                for (int n = 0; n < QB; ++n) S::multiply(f, q[n][p], s[n]);
-                const auto w = Tile::along(lv, p, lane);
-#pragma unroll
-                for (int n = 0; n < QB; ++n) S::multiply(w, go[n][p], dp[n]);
+                for (int n = 0; n < QB; ++n) {
+                    if (p == 0) {
+                        s[n] = S::product(f, q[n][0]);
+                        dp[n] = S::product(w, go[n][0]);
+                    } else {
+                        S::multiply(f, q[n][p], s[n]);
+                        S::multiply(w, go[n][p], dp[n]);
+                    }
+                }
             }
-            if (bits != kAll) {
+            if (__builtin_expect((uint32_t)(bits >> (32 * u)) != ~0u, 0)) {
                 const uint32_t w = (uint32_t)(bits >> (32 * u)) >> (4 * (lane >> 5));
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -228,12 +268,10 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
                         s[n][r] = w & (1u << ((r & 3) + 8 * (r >> 2))) ? s[n][r] : -INFINITY;
             }
 #pragma unroll
-            for (int n = 0; n < QB; ++n) {
+            for (int n = 0; n < QB; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     dp[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], g.c, -lse[n])) * (dp[n][r] - delta[n]);
-                lift_weights<T>(dp[n], lift[n], sums[n]);
-            }
 #pragma unroll
             for (int p = 0; p < kParts; ++p) {
                 typename S::Frag w[QB];
@@ -251,8 +289,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
 #pragma unroll
     for (int n = 0; n < QB; ++n) {
         if (!rows.exists[n]) continue;
-        const float by = a.scale * lowered<T>(lift[n]);
-        const int64_t at = ((int64_t)split * a.q.rows + rows.row(n)) * a.heads + rows.head[n];
+        const int64_t place = ((int64_t)split * a.q.rows + rows.row(n)) * a.heads + rows.head[n];
         T* to = SPLIT ? nullptr : (T*)b.grad_q.p + rows.row(n) * b.grad_q.stride + (int64_t)rows.head[n] * d;
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
@@ -261,17 +298,24 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_q_kernel(At
                 float v[8];
                 square_rows(sums[n][c], p, v);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] *= by;
+                for (int k = 0; k < 8; ++k) v[k] *= by[n];
                 const int c0 = 32 * c + 16 * p + 8 * (lane >> 5);
-                if constexpr (SPLIT) store_eight<float>(g.sums + at * D, c0, D, v);
+                if constexpr (SPLIT) store_eight<float>(g.sums + place * D, c0, D, v);
                 else store_eight<T>(to, c0, d, v);
             }
     }
 }
 
 // Tiles of QT rows of one of the shared heads at a time; a wave has 32 states.
-template <class T, int D, int QT, bool SPLIT>
-__global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(AttentionBackward b, Grid g) {
+// Both sums of wide heads would leave room for one wave a SIMD: they are formed by
+// a launch each, the scores in both (five products in place of four; 128 columns,
+// 2 x 8192 rows x 8 heads at 4096 shared states: 1018 us together).
+enum { kGradK = 1, kGradV = 2 };
+template <class T, int D>
+constexpr bool kApart = sizeof(T) == 2 && D > 64;
+
+template <class T, int D, int QT, bool SPLIT, int WHAT>
+__global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)) grad_kv_kernel(AttentionBackward b, Grid g) {
     using S = Square<T>;
     using Tile = RowTile<T, D, QT, kWaves>;
     constexpr int kSteps = D / S::kDepth, kParts = 32 / S::kDepth, kSubs = QT / 32, kCols = D / 32;
@@ -295,6 +339,19 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(A
     states.exists[0] = exists;
     states.template load<T, kSteps>(a.k, d, lane, k);
     states.template load<T, kSteps>(a.v, d, lane, v);
+    int lift = 0;
+    if constexpr (kBoost<T> != 0.0f) {
+        const float most = largest_of(g.largest, g.lifts, 2), most_delta = largest_of(g.largest + 1, g.lifts, 2);
+        float square = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) square = fmaf((float)v[0][s][c], (float)v[0][s][c], square);
+        float other = square;
+        swap32(square, other);
+        lift = lift_of<T>(fmaf(most, sqrtf(square + other), most_delta));
+    }
+    const float lifted = __builtin_ldexpf(1.0f, lift - (int)kBoost<T>);   // p is held lifted by kBoost
 
     Tile tq, to;
     const int64_t q_pitch = a.q.stride * (int64_t)sizeof(T), o_pitch = b.grad_out.stride * (int64_t)sizeof(T);
@@ -326,14 +383,13 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(A
         const int64_t row = e * a.queries + r0 + of;
         const int head = kv * g.shared + h;
         if (threadIdx.x < QT)
-            value = of < left ? lse_exponent<T>(a.lse[row * a.lse_row_step + head * a.lse_head_step]) : INFINITY;
+            value = of < left ? lse_exponent<T>(a.lse[row * a.lse_row_step + head * a.lse_head_step]) - kBoost<T> : INFINITY;
         else if (threadIdx.x < 2 * QT)
             value = of < left ? g.delta[row * a.heads + head] : 0.0f;
         return true;
     };
 
     f32x16 gk[kCols], gv[kCols];
-    Lift lift;
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
 #pragma unroll
@@ -351,13 +407,12 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(A
 #pragma unroll 1
         for (int u = 0; u < kSubs; ++u) {
             const unsigned char *lq = from + 32 * u * Tile::kRowBytes, *lo = lq + Tile::kBytes;
-            f32x16 s, dp;
+            f32x16 s = S::product(Tile::along(lq, 0, lane), k[0][0]), dp;
+            if constexpr (WHAT & kGradK) dp = S::product(Tile::along(lo, 0, lane), v[0][0]);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.0f;
-#pragma unroll
-            for (int p = 0; p < kSteps; ++p) {
+            for (int p = 1; p < kSteps; ++p) {
                 S::multiply(Tile::along(lq, p, lane), k[0][p], s);
-                S::multiply(Tile::along(lo, p, lane), v[0][p], dp);
+                if constexpr (WHAT & kGradK) S::multiply(Tile::along(lo, p, lane), v[0][p], dp);
             }
 #pragma unroll
             for (int r0 = 0; r0 < 16; r0 += 4) {
@@ -366,24 +421,28 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(A
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     s[r0 + r] = __builtin_amdgcn_exp2f(fmaf(s[r0 + r], g.c, -l4[r]));
-                    dp[r0 + r] = s[r0 + r] * (dp[r0 + r] - d4[r]);
+                    if constexpr (WHAT & kGradK) {
+                        const float x = dp[r0 + r] - d4[r];
+                        dp[r0 + r] = s[r0 + r] * (kBoost<T> != 0.0f ? x * lifted : x);
+                    }
                 }
             }
-            lift_weights<T>(dp, lift, gk);
 #pragma unroll
             for (int p = 0; p < kParts; ++p) {
-                const auto w = S::rounded(s, p), x = S::rounded(dp, p);
+                typename S::Frag w, x;
+                if constexpr (WHAT & kGradV) w = S::rounded(s, p);
+                if constexpr (WHAT & kGradK) x = S::rounded(dp, p);
 #pragma unroll
                 for (int c = 0; c < kCols; ++c) {
-                    S::multiply(Tile::across(lo, p * S::kDepth, 32 * c, lane), w, gv[c]);
-                    S::multiply(Tile::across(lq, p * S::kDepth, 32 * c, lane), x, gk[c]);
+                    if constexpr (WHAT & kGradV) S::multiply(Tile::across(lo, p * S::kDepth, 32 * c, lane), w, gv[c]);
+                    if constexpr (WHAT & kGradK) S::multiply(Tile::across(lq, p * S::kDepth, 32 * c, lane), x, gk[c]);
                 }
             }
         }
     }
     if (!inside) return;
     // a state that does not exist gets zeros, whatever the rows hold
-    const float by_k = a.scale * lowered<T>(lift), by_v = kBoost<T> != 0.0f ? 0x1p-10f : 1.0f;
+    const float by_k = __builtin_ldexpf(a.scale, -lift), by_v = __builtin_ldexpf(1.0f, -(int)kBoost<T>);
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
 #pragma unroll
@@ -399,11 +458,13 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 ? 2 : 1) grad_kv_kernel(A
             const int c0 = 32 * c + 16 * p + 8 * (lane >> 5);
             if constexpr (SPLIT) {
                 const int64_t n = a.k.rows * a.kv_heads, at = state * a.kv_heads + kv;
-                store_eight<float>(g.sums + ((2 * split) * n + at) * D, c0, D, x);
-                store_eight<float>(g.sums + ((2 * split + 1) * n + at) * D, c0, D, y);
+                if constexpr (WHAT & kGradK) store_eight<float>(g.sums + ((2 * split) * n + at) * D, c0, D, x);
+                if constexpr (WHAT & kGradV) store_eight<float>(g.sums + ((2 * split + 1) * n + at) * D, c0, D, y);
             } else {
-                if (b.grad_k.p) store_eight<T>((T*)b.grad_k.p + state * b.grad_k.stride + (int64_t)kv * d, c0, d, x);
-                if (b.grad_v.p) store_eight<T>((T*)b.grad_v.p + state * b.grad_v.stride + (int64_t)kv * d, c0, d, y);
+                if ((WHAT & kGradK) && b.grad_k.p)
+                    store_eight<T>((T*)b.grad_k.p + state * b.grad_k.stride + (int64_t)kv * d, c0, d, x);
+                if ((WHAT & kGradV) && b.grad_v.p)
+                    store_eight<T>((T*)b.grad_v.p + state * b.grad_v.stride + (int64_t)kv * d, c0, d, y);
             }
         }
 }
@@ -510,8 +571,8 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
         return true;
     };
     // dq of the tile whose ds stands in `from`: rows r0 .. of the head
-    const auto add_rows = [&](const unsigned char* from, int head, int64_t r0) {
-        const int64_t left = a.queries - r0;
+    const auto add_rows = [&](const unsigned char* from, int head, int64_t r0, bool there) {
+        const int64_t left = there ? a.queries - r0 : 0;
 #pragma unroll
         for (int n = 0; n < kDown; ++n) {
             f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -551,12 +612,10 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
         const int64_t r0 = in * kOnceRows;
         wait_for_stage<1>(0);   // the tile is there, and the last one's ds; their buffers are free
         more = load(buffer ^ 1);
-        if (begun && b.grad_q.p) add_rows(weights[buffer ^ 1], last_head, last_row);
-        begun = true;
-        last_head = head;
-        last_row = r0;
+        // the two waves of a SIMD in opposite order: one's products beside the other's exponentials
+        if (wave < kOnceWaves / 2) add_rows(weights[buffer ^ 1], last_head, last_row, begun);
         unsigned char* const to_weights = weights[buffer] + (int)j * Weights::kRowBytes;
-#pragma unroll 1
+#pragma unroll
         for (int u = 0; u < kOnceRows / 32; ++u) {
             const unsigned char *lq = lds[buffer][0] + 32 * u * Tile::kRowBytes, *lo = lq + Tile::kBytes;
             f32x16 s = S::product(Tile::along(lq, 0, lane), k[0][0]), dp = S::product(Tile::along(lo, 0, lane), v[0][0]);
@@ -592,10 +651,14 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
                 }
             }
         }
+        if (wave >= kOnceWaves / 2) add_rows(weights[buffer ^ 1], last_head, last_row, begun);
+        begun = true;
+        last_head = head;
+        last_row = r0;
         buffer ^= 1;
     }
     __syncthreads();
-    if (begun && b.grad_q.p) add_rows(weights[buffer ^ 1], last_head, last_row);
+    add_rows(weights[buffer ^ 1], last_head, last_row, begun);
     if (!inside) return;
 #pragma unroll
     for (int c = 0; c < kCols; ++c)
@@ -654,7 +717,8 @@ struct Plan {
     int qb, tile;
     Grid q, kv;
     int64_t q_workgroups, kv_workgroups;
-    size_t delta_bytes, bytes;
+    int64_t delta_blocks;      // of its kernel, where dq is not asked for
+    size_t delta_bytes, norms_bytes, largest_bytes, bytes;
 };
 
 Plan plan_of(const AttentionBackward& b) {
@@ -677,7 +741,7 @@ Plan plan_of(const AttentionBackward& b) {
         p.bytes = sizeof(float) * 2 * (size_t)(p.kv.splits * a.k.rows * a.kv_heads * width);
         return p;
     }
-    p.qb = halves && p.q.rows > 32 * kWaves ? 2 : 1;
+    p.qb = halves && width <= 64 && p.q.rows > 32 * kWaves ? 2 : 1;
     p.q.blocks = (p.q.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
     int64_t whole = a.batch * a.kv_heads * p.q.blocks;
     split_tiles(whole, (a.states + p.tile - 1) / p.tile, p.q.splits, p.q.part);
@@ -692,7 +756,13 @@ Plan plan_of(const AttentionBackward& b) {
     if (b.grad_q.p && p.q.splits > 1) sums = sizeof(float) * (size_t)(p.q.splits * a.q.rows * a.heads * width);
     if ((b.grad_k.p || b.grad_v.p) && p.kv.splits > 1)
         sums = std::max(sums, sizeof(float) * 2 * (size_t)(p.kv.splits * a.k.rows * a.kv_heads * width));
-    p.bytes = p.delta_bytes + sums;
+    p.delta_blocks = std::min<int64_t>((a.q.rows * a.heads + 255) / 256, 4096);
+    if (a.dtype == TGS_DTYPE_FLOAT16) {
+        p.kv.lifts = b.grad_q.p ? p.q_workgroups : p.delta_blocks;
+        p.norms_bytes = (sizeof(float) * (size_t)(a.batch * a.kv_heads * ((a.states + 63) / 64)) + 255) / 256 * 256;
+        p.largest_bytes = (sizeof(float) * 2 * (size_t)p.kv.lifts + 255) / 256 * 256;
+    }
+    p.bytes = p.delta_bytes + p.norms_bytes + p.largest_bytes + sums;
     return p;
 }
 
@@ -717,7 +787,10 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
     const Attention& a = b.a;
     Plan p = plan_of(b);
     p.q.delta = p.kv.delta = (float*)workspace;
-    p.q.sums = p.kv.sums = (float*)((unsigned char*)workspace + p.delta_bytes);
+    unsigned char* at = (unsigned char*)workspace + p.delta_bytes;
+    p.q.norms = p.kv.norms = (float*)at;
+    p.q.largest = p.kv.largest = (float*)(at += p.norms_bytes);
+    p.q.sums = p.kv.sums = (float*)(at += p.largest_bytes);
     const bool states = (b.grad_k.p || b.grad_v.p) && a.k.rows > 0;
     by_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
@@ -740,6 +813,10 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
                 return;
             }
             if (b.grad_q.p && a.q.rows) {
+                if (p.norms_bytes) {
+                    const int64_t n = (a.batch * a.kv_heads * ((a.states + 63) / 64) + 3) / 4;
+                    if constexpr (sizeof(T) == 2) norms_kernel<T><<<(unsigned)std::min<int64_t>(n, 4096), 256, 0, s>>>(a, p.q.norms);
+                }
                 const auto launch = [&](auto qb) {
                     constexpr int QB = decltype(qb)::value;
                     in_launches(p.q, p.q_workgroups, [&](unsigned n) {
@@ -747,7 +824,7 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
                         else grad_q_kernel<T, D, QB, kTile, false><<<n, 64 * kWaves, 0, s>>>(b, p.q);
                     });
                 };
-                if constexpr (sizeof(T) == 2) {
+                if constexpr (sizeof(T) == 2 && D <= 64) {
                     if (p.qb == 2) launch(Constant<2>{});
                     else launch(Constant<1>{});
                 } else {
@@ -757,14 +834,23 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
                     join_kernel<T, D><<<join_blocks(a.q.rows * a.heads * a.head), 256, 0, s>>>(
                         p.q.sums, p.q.splits, a.q.rows * a.heads, b.grad_q, a.heads, a.head);
             } else if (a.q.rows && states) {
-                const int64_t n = (a.q.rows * a.heads + 255) / 256;
-                delta_kernel<T><<<(unsigned)(n < 4096 ? n : 4096), 256, 0, s>>>(b, p.q.delta);
+                p.kv.first = 0;
+                delta_kernel<T><<<(unsigned)p.delta_blocks, 256, 0, s>>>(b, p.kv);
             }
             if (!states) return;
-            in_launches(p.kv, p.kv_workgroups, [&](unsigned n) {
-                if (p.kv.splits > 1) grad_kv_kernel<T, D, kTile, true><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
-                else grad_kv_kernel<T, D, kTile, false><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
-            });
+            const auto launch = [&](auto what) {
+                constexpr int W = decltype(what)::value;
+                in_launches(p.kv, p.kv_workgroups, [&](unsigned n) {
+                    if (p.kv.splits > 1) grad_kv_kernel<T, D, kTile, true, W><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
+                    else grad_kv_kernel<T, D, kTile, false, W><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
+                });
+            };
+            if constexpr (kApart<T, D>) {
+                if (b.grad_k.p) launch(Constant<kGradK>{});
+                if (b.grad_v.p) launch(Constant<kGradV>{});
+            } else {
+                launch(Constant<kGradK | kGradV>{});
+            }
             if (p.kv.splits > 1) join();
         });
     });
