@@ -219,7 +219,7 @@ struct WaveRows {
 };
 
 template <class T, int D, int QB, int WAVES, int KT, bool SPLIT>
-__global__ void __launch_bounds__(64 * WAVES, D <= 64 ? 2 : 1) attention_kernel(Attention a, Grid g) {
+__global__ void __launch_bounds__(64 * WAVES, (D <= 64 || sizeof(T) == 2 ? 2 : 1)) attention_kernel(Attention a, Grid g) {
     using Tile = RowTile<T, D, KT, WAVES>;
     __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -441,7 +441,7 @@ Plan plan_of(const Attention& a) {
         return p;
     }
     const int kt = halves ? 64 : 32;
-    p.qb = halves && p.grid.rows > 32 * kWaves ? 2 : 1;
+    p.qb = halves && width <= 64 && p.grid.rows > 32 * kWaves ? 2 : 1;
     p.grid.blocks = (p.grid.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
     const int64_t whole = pairs * p.grid.blocks, tiles = (a.states + kt - 1) / kt;
     int64_t splits = 1;
@@ -488,7 +488,7 @@ int launch_attention(const Attention& a, void* workspace, hipStream_t s) {
                     if (p.grid.splits > 1) launch(qb, Constant<1>{});
                     else launch(qb, Constant<0>{});
                 };
-                if constexpr (sizeof(T) == 2) {
+                if constexpr (sizeof(T) == 2 && D <= 64) {
                     if (p.qb == 2) by_split(Constant<2>{});
                     else by_split(Constant<1>{});
                 } else {

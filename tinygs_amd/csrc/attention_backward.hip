@@ -361,7 +361,8 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
     const unsigned char* o0 =
         (const unsigned char*)b.grad_out.p + e * a.queries * o_pitch + (int64_t)kv * g.shared * d * sizeof(T);
     const int64_t per_head = g.units / g.shared;
-    const int64_t t1 = min((split + 1) * g.part, g.units);
+    // a workgroup whose states all do not exist only writes zeros
+    const int64_t t1 = __syncthreads_or(exists) ? min((split + 1) * g.part, g.units) : 0;
     int64_t t = split * g.part - 1;
     int h = (int)((t + 1) / per_head);         // of the next tile, among the shared heads
     int64_t in = (t + 1) - h * per_head - 1;   // the tile's number in its head
