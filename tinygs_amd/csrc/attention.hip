@@ -18,10 +18,13 @@
 #include <math.h>
 
 #include "attention.h"
+#include "row_chunks.h"
 
 namespace tgs {
 
 namespace {
+
+constexpr float kLn2 = 0.69314718055994531f;
 
 // The sum of a lane's weights up to which none of them can have left its type's
 // range (2^16 for halves), nor their products with values that of floats.
@@ -376,6 +379,114 @@ __global__ void __launch_bounds__((64 * kHeldWaves<T, D>)) held_kernel(Attention
     }
 }
 
+// One to four rows (heads that share the states' included) at a few hundred states:
+// one workgroup for each batch element and head of the states, eight lanes a state,
+// plain multiply-adds, and one launch, where the matrix cores' kernel would have
+// most of its rows empty and its parts joined by a second launch (1 row of 4 heads
+// of 64 at 256 states, the call: 13.3 us so). Keys and values are on their way
+// together; the scores meet in LDS.
+constexpr int kFewThreads = 1024, kFewAtOnce = kFewThreads / 8, kFewTurns = 4, kFewStates = kFewAtOnce * kFewTurns;
+constexpr int kFewRows = 4;
+
+template <class T, int PIECES, int R>
+__global__ void __launch_bounds__(kFewThreads) few_kernel(Attention a, Grid g) {
+    constexpr int V = kChunk<T>, kWavesFew = kFewThreads / 64, kWidth = 8 * PIECES * V;
+    __shared__ float weights[R][kFewStates], parts[kWavesFew][R][kWidth];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = threadIdx.x & 7, d = a.head;
+    const int64_t b = blockIdx.x / a.kv_heads;
+    const int kv = (int)(blockIdx.x % a.kv_heads), states = (int)a.states;
+    float q[R][PIECES][V];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = min(r, (int)g.rows - 1);
+        const T* p = (const T*)a.q.p + (b * a.queries + i / g.shared) * a.q.stride + (int64_t)(kv * g.shared + i % g.shared) * d;
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) load_chunk<T>(p, l + 8 * n, d, q[r][n]);
+    }
+    float v[kFewTurns][PIECES][V];
+#pragma unroll
+    for (int t = 0; t < kFewTurns; ++t) {
+        const int j = t * kFewAtOnce + (int)threadIdx.x / 8;
+        const int64_t at = b * a.states + min(j, states - 1);   // the loads need no branch
+        const bool exists = j < states && (!a.mask || a.mask[b * a.mask_stride + j]);
+        float k[PIECES][V], s[R];
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) {
+            load_chunk<T>((const T*)a.k.p + at * a.k.stride + (int64_t)kv * d, l + 8 * n, d, k[n]);
+            load_chunk<T>((const T*)a.v.p + at * a.v.stride + (int64_t)kv * d, l + 8 * n, d, v[t][n]);
+        }
+        int none = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            s[r] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n)
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[r] = fmaf(q[r][n][e], k[n][e], s[r]);
+        }
+        group_sum<8>(s, nullptr, none);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (l == 0) weights[r][j] = exists ? s[r] * g.c : -INFINITY;
+    }
+    __syncthreads();
+    float top[R], sum[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {   // each wave by itself
+        top[r] = -INFINITY;
+        sum[r] = 0.0f;
+        for (int j = lane; j < kFewStates; j += 64) top[r] = fmaxf(top[r], weights[r][j]);
+        for (int k = 32; k > 0; k >>= 1) top[r] = fmaxf(top[r], __shfl_xor(top[r], k, 64));
+        const float from = top[r] == -INFINITY ? 0.0f : top[r];
+        for (int j = lane; j < kFewStates; j += 64) sum[r] += __builtin_amdgcn_exp2f(weights[r][j] - from);
+        for (int k = 32; k > 0; k >>= 1) sum[r] += __shfl_xor(sum[r], k, 64);
+        float out[PIECES][V] = {};
+#pragma unroll
+        for (int t = 0; t < kFewTurns; ++t) {
+            const float s = weights[r][t * kFewAtOnce + (int)threadIdx.x / 8], w = __builtin_amdgcn_exp2f(s - from);
+            if (s == -INFINITY) continue;   // what does not exist may hold anything
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n)
+#pragma unroll
+                for (int e = 0; e < V; ++e) out[n][e] = fmaf(w, v[t][n][e], out[n][e]);
+        }
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                float x = out[n][e], y;
+                x = dpp_add<0x128>(x);   // eight lanes on
+                y = x;
+                swap16(x, y);
+                y = x += y;
+                swap32(x, y);
+                x += y;
+                if (lane < 8) parts[wave][r][(l + 8 * n) * V + e] = x;
+            }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < (int)g.rows * kWidth; i += kFewThreads) {
+        const int r = i / kWidth, c = i % kWidth;
+        if (c >= d) continue;
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWavesFew; ++w) x += parts[w][r][c];
+        float of = 0.0f, most = 0.0f;
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            of = k == r ? sum[k] : of;
+            most = k == r ? top[k] : most;
+        }
+        const int64_t row = b * a.queries + r / g.shared;
+        const int head = kv * g.shared + r % g.shared;
+        ((T*)a.out.p)[row * a.out.stride + (int64_t)head * d + c] = (T)(of == 0.0f ? 0.0f : x * (1.0f / of));
+        // the maximum is in the exponent's unit, of a scale that is never 0
+        if (a.lse && c == 0)
+            a.lse[row * a.lse_row_step + head * a.lse_head_step] =
+                of == 0.0f ? -INFINITY : fmaf(most, kLn2, logf(of));
+    }
+}
+
 // Joins the splits' sums: a wave for each row and head.
 template <class T, int D>
 __global__ void __launch_bounds__(256) join_kernel(Attention a, Grid g) {
@@ -383,9 +494,11 @@ __global__ void __launch_bounds__(256) join_kernel(Attention a, Grid g) {
     const int64_t n = a.q.rows * a.heads;
     for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
         float top = -INFINITY;
+#pragma unroll 8
         for (int k = 0; k < g.splits; ++k) top = fmaxf(top, g.tops[2 * (k * n + i)]);
         const float less = -(top == -INFINITY ? 0.0f : top) * g.c;
         float sum = 0.0f, v[(D + 63) / 64] = {};
+#pragma unroll 8
         for (int k = 0; k < g.splits; ++k) {
             const int64_t at = k * n + i;
             const float w = __builtin_amdgcn_exp2f(fmaf(g.tops[2 * at], g.c, less));
@@ -409,7 +522,7 @@ __global__ void __launch_bounds__(256) join_kernel(Attention a, Grid g) {
 
 struct Plan {
     int qb;
-    bool held;
+    bool held, few;
     Grid grid;
     int64_t workgroups;
     size_t bytes;
@@ -440,8 +553,18 @@ Plan plan_of(const Attention& a) {
         p.workgroups = p.grid.blocks * pairs;
         return p;
     }
+    // several rows of heads above 128 bytes are no faster so (4 rows of 128 halves at 300 states 17.9 us and 17.0, of
+    // 128 floats at 500 25.3 and 16.4; of 64 halves at 100 13.7 and 16.2)
+    p.few = (p.grid.rows == 1 || (p.grid.rows <= kFewRows && a.head * (halves ? 2 : 4) <= 128)) && a.states >= 1 &&
+            a.states <= kFewStates && pairs <= 65536;
+    if (p.few) {
+        p.workgroups = pairs;
+        return p;
+    }
     const int kt = halves ? 64 : 32;
-    p.qb = halves && width <= 64 && p.grid.rows > 32 * kWaves ? 2 : 1;
+    // two squares of rows a wave where their workgroups still fill the card twice: 2000 rows of 4 heads of 64 at 2000
+    // states 34.2 us with two and 25.9 with one, 16384 of 8 at 4096 193 and 225
+    p.qb = halves && width <= 64 && pairs * ((p.grid.rows + 64 * kWaves - 1) / (64 * kWaves)) >= 512 ? 2 : 1;
     p.grid.blocks = (p.grid.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
     const int64_t whole = pairs * p.grid.blocks, tiles = (a.states + kt - 1) / kt;
     int64_t splits = 1;
@@ -471,6 +594,12 @@ int launch_attention(const Attention& a, void* workspace, hipStream_t s) {
                 if constexpr (sizeof(T) == 2 || D <= 64)
                     held_kernel<T, D, kHeldSquares<T, D>>
                         <<<(unsigned)p.workgroups, 64 * kHeldWaves<T, D>, 0, s>>>(a, p.grid);
+                return;
+            }
+            if (p.few) {
+                constexpr int kPieces = (D + 8 * kChunk<T> - 1) / (8 * kChunk<T>);
+                if (p.grid.rows == 1) few_kernel<T, kPieces, 1><<<(unsigned)p.workgroups, kFewThreads, 0, s>>>(a, p.grid);
+                else few_kernel<T, 1, kFewRows><<<(unsigned)p.workgroups, kFewThreads, 0, s>>>(a, p.grid);
                 return;
             }
             p.grid.sums = (float*)workspace;
