@@ -74,7 +74,27 @@ struct Turn {
     }
 };
 
-template <class T, int LANES>
+// A lane's chunk of a head as it lies in memory; zeros past the head. WHOLE: heads of
+// whole chunks. Their loads have no branch, which would wait for each where its
+// paths meet: lanes without a chunk read another one's.
+template <class T, bool WHOLE>
+__device__ __forceinline__ typename ChunkOf<T>::type load_raw(const T* head, int lane, int d) {
+    constexpr int V = kChunk<T>;
+    using Raw = typename ChunkOf<T>::type;
+    if constexpr (WHOLE) return *(const Raw*)(head + min(lane, d / V - 1) * V);
+    Raw u = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (lane * V + i < d) u[i] = head[lane * V + i];
+    return u;
+}
+template <class T, bool WHOLE>
+__device__ __forceinline__ void unpack(const typename ChunkOf<T>::type& u, int lane, int d, float* v) {
+#pragma unroll
+    for (int i = 0; i < kChunk<T>; ++i) v[i] = !WHOLE || lane * kChunk<T> < d ? (float)u[i] : 0.0f;
+}
+
+template <class T, int LANES, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) forward_kernel(HeadNorm a) {
     constexpr int V = kChunk<T>, kRows = kThreads / LANES;
     const int lane = threadIdx.x % LANES, d = a.head;
@@ -87,31 +107,32 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(HeadNorm a) {
     for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES; r < a.x.rows; r += (int64_t)gridDim.x * kRows) {
         const T* x = (const T*)a.x.p + r * a.x.stride;
         T* y = (T*)a.y.p + r * a.y.stride;
-        turn.row(a, r, lane);
         for (int h0 = 0; h0 < a.heads; h0 += kHeads) {
-            float v[kHeads][V];
+            typename ChunkOf<T>::type raw[kHeads];
 #pragma unroll
             for (int k = 0; k < kHeads; ++k)
-                if (h0 + k < a.heads) load_chunk<T>(x + (int64_t)(h0 + k) * d, lane, d, v[k]);
+                raw[k] = load_raw<T, WHOLE>(x + (int64_t)min(h0 + k, a.heads - 1) * d, lane, d);
+            if (h0 == 0) turn.row(a, r, lane);   // beside the first loads
 #pragma unroll
             for (int k = 0; k < kHeads; ++k) {
                 if (h0 + k >= a.heads) break;
-                float sum[1] = {0.0f};
+                float v[V], sum[1] = {0.0f};
+                unpack<T, WHOLE>(raw[k], lane, d, v);
 #pragma unroll
-                for (int i = 0; i < V; ++i) sum[0] = fmaf(v[k][i], v[k][i], sum[0]);
+                for (int i = 0; i < V; ++i) sum[0] = fmaf(v[i], v[i], sum[0]);
                 group_sum<LANES>(sum, nullptr, none);
                 const float rstd = 1.0f / sqrtf(fmaf(sum[0], inv, a.eps));
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[k][i] = v[k][i] * rstd * gamma[i];
-                turn.template apply<1>(v[k]);
-                store_chunk<T>(y + (int64_t)(h0 + k) * d, lane, d, v[k]);
+                for (int i = 0; i < V; ++i) v[i] = v[i] * rstd * gamma[i];
+                turn.template apply<1>(v);
+                store_chunk<T>(y + (int64_t)(h0 + k) * d, lane, d, v);
             }
         }
     }
 }
 
 // Column sums: a workgroup's, over its rows and all heads, to row blockIdx.x of `partial`.
-template <class T, int LANES, bool SUMS>
+template <class T, int LANES, bool WHOLE, bool SUMS>
 __global__ void __launch_bounds__(kThreads) backward_kernel(HeadNorm a, float* partial) {
     constexpr int V = kChunk<T>, kRows = kThreads / LANES;
     const int lane = threadIdx.x % LANES, d = a.head;
@@ -127,35 +148,37 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(HeadNorm a, float* p
         const T* x = (const T*)a.x.p + r * a.x.stride;
         const T* gy = (const T*)a.grad_y.p + r * a.grad_y.stride;
         T* gx = a.y.p ? (T*)a.y.p + r * a.y.stride : nullptr;
-        turn.row(a, r, lane);
         for (int h0 = 0; h0 < a.heads; h0 += kHeads) {
-            float v[kHeads][V], g[kHeads][V];
+            typename ChunkOf<T>::type rx[kHeads], rg[kHeads];
 #pragma unroll
-            for (int k = 0; k < kHeads; ++k)
-                if (h0 + k < a.heads) {
-                    load_chunk<T>(x + (int64_t)(h0 + k) * d, lane, d, v[k]);
-                    load_chunk<T>(gy + (int64_t)(h0 + k) * d, lane, d, g[k]);
-                }
+            for (int k = 0; k < kHeads; ++k) {
+                const int64_t at = (int64_t)min(h0 + k, a.heads - 1) * d;
+                rx[k] = load_raw<T, WHOLE>(x + at, lane, d);
+                rg[k] = load_raw<T, WHOLE>(gy + at, lane, d);
+            }
+            if (h0 == 0) turn.row(a, r, lane);
 #pragma unroll
             for (int k = 0; k < kHeads; ++k) {
                 if (h0 + k >= a.heads) break;
-                turn.template apply<-1>(g[k]);
-                float sum[2] = {0.0f, 0.0f};
+                float v[V], g[V], sum[2] = {0.0f, 0.0f};
+                unpack<T, WHOLE>(rx[k], lane, d, v);
+                unpack<T, WHOLE>(rg[k], lane, d, g);
+                turn.template apply<-1>(g);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    sum[0] = fmaf(v[k][i], v[k][i], sum[0]);
-                    sum[1] = fmaf(g[k][i] * gamma[i], v[k][i], sum[1]);
+                    sum[0] = fmaf(v[i], v[i], sum[0]);
+                    sum[1] = fmaf(g[i] * gamma[i], v[i], sum[1]);
                 }
                 group_sum<LANES>(sum, nullptr, none);
                 const float rstd = 1.0f / sqrtf(fmaf(sum[0], inv, a.eps));
                 const float c = sum[1] * rstd * inv;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float h = v[k][i] * rstd;
-                    if (SUMS) grad_gamma[i] = fmaf(g[k][i], h, grad_gamma[i]);
-                    v[k][i] = rstd * fmaf(-h, c, g[k][i] * gamma[i]);
+                    const float h = v[i] * rstd;
+                    if (SUMS) grad_gamma[i] = fmaf(g[i], h, grad_gamma[i]);
+                    v[i] = rstd * fmaf(-h, c, g[i] * gamma[i]);
                 }
-                if (gx) store_chunk<T>(gx + (int64_t)(h0 + k) * d, lane, d, v[k]);
+                if (gx) store_chunk<T>(gx + (int64_t)(h0 + k) * d, lane, d, v);
             }
         }
     }
@@ -172,10 +195,14 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(HeadNorm a, float* p
     }
 }
 
-// f<lanes> with the least power of two of lanes whose chunks hold a head.
+// f<lanes, whether heads are whole chunks> with the least power of two of lanes whose chunks hold a head.
 template <class T, class F>
-void by_head(int head, F f) {
+void by_head(int head, F with) {
     constexpr int V = kChunk<T>;
+    const auto f = [&](auto lanes) {
+        if (head % V == 0) with(lanes, Constant<1>{});
+        else with(lanes, Constant<0>{});
+    };
     if (head <= V) f(Constant<1>{});
     else if (head <= 2 * V) f(Constant<2>{});
     else if (head <= 4 * V) f(Constant<4>{});
@@ -201,9 +228,10 @@ size_t head_norm_backward_workspace(const HeadNorm& a) {
 int launch_head_norm(const HeadNorm& a, hipStream_t s) {
     by_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
-        by_head<T>(a.head, [&](auto lanes) {
+        by_head<T>(a.head, [&](auto lanes, auto whole) {
             constexpr int kLanes = decltype(lanes)::value;
-            forward_kernel<T, kLanes><<<blocks_of(a.x.rows, kLanes, 2048), kThreads, 0, s>>>(a);
+            constexpr bool kWhole = decltype(whole)::value != 0;
+            forward_kernel<T, kLanes, kWhole><<<blocks_of(a.x.rows, kLanes, 2048), kThreads, 0, s>>>(a);
         });
     });
     TGS_CHECK_LAUNCH();
@@ -213,15 +241,16 @@ int launch_head_norm(const HeadNorm& a, hipStream_t s) {
 int launch_head_norm_backward(const HeadNorm& a, void* workspace, hipStream_t s) {
     by_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
-        by_head<T>(a.head, [&](auto lanes) {
+        by_head<T>(a.head, [&](auto lanes, auto whole) {
             constexpr int kLanes = decltype(lanes)::value;
+            constexpr bool kWhole = decltype(whole)::value != 0;
             if (!a.grad_gamma) {
                 const unsigned blocks = blocks_of(a.x.rows, kLanes, 2048);
-                if (blocks && a.y.p) backward_kernel<T, kLanes, false><<<blocks, kThreads, 0, s>>>(a, nullptr);
+                if (blocks && a.y.p) backward_kernel<T, kLanes, kWhole, false><<<blocks, kThreads, 0, s>>>(a, nullptr);
                 return;
             }
             const unsigned blocks = blocks_of(a.x.rows, kLanes, kSumBlocks);
-            if (blocks) backward_kernel<T, kLanes, true><<<blocks, kThreads, 0, s>>>(a, (float*)workspace);
+            if (blocks) backward_kernel<T, kLanes, kWhole, true><<<blocks, kThreads, 0, s>>>(a, (float*)workspace);
             launch_column_sums((const float*)workspace, (int)blocks, a.head, a.head, a.grad_gamma, nullptr, s);
         });
     });
