@@ -49,9 +49,24 @@ __device__ __forceinline__ double workgroup_sum(double v) {
 // in chunks of 16 bytes where its rows follow each other without gaps.
 template <class T, class F>
 __device__ __forceinline__ void each(const ClipPart& a, int64_t first, int64_t last, F f) {
-    constexpr int V = kChunk<T>, kAhead = 4;
+    constexpr int V = kChunk<T>, kAhead = 4, kWhole = (int)(kChunkElements / (kThreads * V));
     const T* g = (const T*)a.g;
-    if (a.stride == a.cols && a.c_stride == a.cols) {
+    const bool packed = a.stride == a.cols && a.c_stride == a.cols;
+    if (packed && last - first == kChunkElements) {   // all loads on their way, without branches between them
+        typename ChunkOf<T>::type raw[kWhole];
+        const int64_t k = first + threadIdx.x * V;
+#pragma unroll
+        for (int q = 0; q < kWhole; ++q) raw[q] = *(const typename ChunkOf<T>::type*)(g + k + q * kThreads * V);
+#pragma unroll
+        for (int q = 0; q < kWhole; ++q) {
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = (float)raw[q][i];
+            f(k + q * kThreads * V, Constant<V>{}, v);
+        }
+        return;
+    }
+    if (packed) {
         for (int64_t k = first + threadIdx.x * V; k < last; k += kThreads * V * kAhead) {
             float v[kAhead][V];
 #pragma unroll
