@@ -1,9 +1,12 @@
 """Recolours a scene through an attribute network: the network maps encoded positions to a change of every Gaussian's
 base colour (SH degree 0) and is trained through the rasteriser, with Muon on its matrices and Adam on its vectors.
 
-    python examples/recolour.py [--gaussians N] [--steps K] [--dtype float32|float16|bfloat16]
+    python examples/recolour.py [--gaussians N] [--steps K] [--dtype float32|float16|bfloat16] [--states S]
+                                [--max-grad-norm M]
 
-The target is the same scene with its colours shifted along x; each step renders, evaluates L1 + SSIM and steps."""
+The target is the same scene with its colours shifted along x; each step renders, evaluates L1 + SSIM and steps. With
+--states the Gaussians also attend to that many states: encoded places and target colours of some of them, by their
+positions. --max-grad-norm bounds the norm of the network's gradients."""
 import argparse
 import os
 import sys
@@ -12,7 +15,7 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 
 def recolour(gaussians: int = 20000, steps: int = 60, width: int = 128, blocks: int = 2, dtype: str = "bfloat16",
-             image: int = 256, log=print):
+             image: int = 256, log=print, states: int = 0, max_grad_norm: float | None = None):
     """The losses of the steps (mean of the loss image)."""
     import torch
     from tinygs_amd import scenes
@@ -32,7 +35,13 @@ def recolour(gaussians: int = 20000, steps: int = 60, width: int = 128, blocks: 
 
     t = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.bfloat16}[dtype]
     features = encode_positions(means, octaves=6, dtype=t)
-    net = AttributeNetwork(features.shape[1], 3, width=width, blocks=blocks, dtype=t)
+    context, attend = None, {}
+    if states:   # what an encoder of the target would say: some places, and the colours there
+        at = torch.linspace(0, gaussians - 1, states, device=means.device).long()
+        context = torch.cat([encode_positions(means[at], octaves=6), (base + 0.8 * shift)[at].reshape(states, 3)], 1).to(t)
+        attend = {"context": context, "positions": means, "context_positions": means[at]}
+    net = AttributeNetwork(features.shape[1], 3, width=width, blocks=blocks, dtype=t,
+                           **({"context": context.shape[1], "axes": 3, "extent": float(means.abs().max())} if states else {}))
     muon = net.optimizer()
     muon.set_params({"lr": 0.02, "weight_decay": 0.0})
     net.vectors.grad = net.vector_grads
@@ -41,13 +50,15 @@ def recolour(gaussians: int = 20000, steps: int = 60, width: int = 128, blocks: 
     scale = 4096.0 if t == torch.float16 else 1.0
     losses = []
     for step in range(steps):
-        change = net.forward(features)
+        change = net.forward(features, **attend)
         ts.gaussians.sh_coefficient_0().copy_(base + change.float())
         ts.zero()
         ts.forward()
         ts.losses_and_grad()
         ts.backward()
         net.backward((ts.grads.sh_coefficient_0() * scale).to(t))
+        if max_grad_norm is not None:
+            net.clip(max_grad_norm * scale)
         muon.step(1.0)
         if scale != 1.0:
             net.vector_grads.mul_(1.0 / scale)
@@ -63,5 +74,7 @@ if __name__ == "__main__":
     ap.add_argument("--gaussians", type=int, default=20000)
     ap.add_argument("--steps", type=int, default=60)
     ap.add_argument("--dtype", default="bfloat16", choices=["float32", "float16", "bfloat16"])
+    ap.add_argument("--states", type=int, default=0)
+    ap.add_argument("--max-grad-norm", type=float, default=None)
     a = ap.parse_args()
-    recolour(a.gaussians, a.steps, dtype=a.dtype)
+    recolour(a.gaussians, a.steps, dtype=a.dtype, states=a.states, max_grad_norm=a.max_grad_norm)

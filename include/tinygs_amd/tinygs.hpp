@@ -1092,8 +1092,62 @@ public:
                  "LayerOps::layer_norm_backward");
     }
 
+    // out = softmax(scale q k^T) v for each head over the states that exist; lse [heads][rows] may be null.
+    void attention(const tgs_matrix& q, const tgs_matrix& k, const tgs_matrix& v, const tgs_attention& a,
+                   const tgs_matrix& out, float* lse = nullptr, hipStream_t stream = nullptr) {
+        throw_on(tgs_attention_forward(m_handle, &q, &k, &v, &a, &out, lse, 1, q.rows > 0 ? q.rows : 1, stream),
+                 "LayerOps::attention");
+    }
+    void attention_backward(const tgs_matrix& grad_out, const tgs_matrix& q, const tgs_matrix& k, const tgs_matrix& v,
+                            const tgs_matrix& out, const float* lse, const tgs_attention& a, const tgs_matrix* grad_q,
+                            const tgs_matrix* grad_k, const tgs_matrix* grad_v, hipStream_t stream = nullptr) {
+        throw_on(tgs_attention_backward(m_handle, &grad_out, &q, &k, &v, &out, lse, 1, q.rows > 0 ? q.rows : 1, &a, grad_q,
+                                        grad_k, grad_v, stream),
+                 "LayerOps::attention_backward");
+    }
+    // x / sqrt(mean(x^2) + epsilon) gamma over each head, its pairs turned by `turn` where it is not null.
+    void head_norm(const tgs_matrix& x, int32_t heads, const float* gamma, const tgs_turn* turn, float epsilon,
+                   const tgs_matrix& y, hipStream_t stream = nullptr) {
+        throw_on(tgs_head_norm_forward(m_handle, &x, heads, gamma, turn, epsilon, &y, stream), "LayerOps::head_norm");
+    }
+    void head_norm_backward(const tgs_matrix& grad_y, const tgs_matrix& x, int32_t heads, const float* gamma,
+                            const tgs_turn* turn, float epsilon, const tgs_matrix* grad_x, float* grad_gamma,
+                            hipStream_t stream = nullptr) {
+        throw_on(tgs_head_norm_backward(m_handle, &grad_y, &x, heads, gamma, turn, epsilon, grad_x, grad_gamma, stream),
+                 "LayerOps::head_norm_backward");
+    }
+
 private:
     tgs_network* m_handle = nullptr;
+};
+
+// Attention of `heads` heads, which share the states' kv_heads in equal groups; mask [batch][states] may be null.
+inline tgs_attention attention_of(int64_t batch, int32_t heads, int32_t kv_heads, float scale, const uint8_t* mask = nullptr,
+                                  int64_t mask_stride = 0) {
+    return tgs_attention{batch, heads, kv_heads, scale, mask, mask_stride};
+}
+
+// The norm of many gradients together, and clipping: in place, or into `clipped`. The pointers are kept.
+class GradientClip {
+public:
+    explicit GradientClip(const std::vector<tgs_matrix>& grads, const std::vector<tgs_matrix>& clipped = {}) {
+        if (!clipped.empty() && clipped.size() != grads.size())
+            throw std::runtime_error("GradientClip: grads and clipped must have the same count");
+        throw_on(tgs_gradient_clip_create(grads.data(), clipped.empty() ? nullptr : clipped.data(), (int32_t)grads.size(),
+                                          &m_handle),
+                 "GradientClip");
+    }
+    ~GradientClip() { tgs_gradient_clip_destroy(m_handle); }
+    GradientClip(const GradientClip&) = delete;
+    GradientClip& operator=(const GradientClip&) = delete;
+
+    // g <- g scale min(1, max_norm / (norm + epsilon)); norm: a device float, or null.
+    void clip(float max_norm, float scale = 1.0f, float epsilon = 1e-6f, float* norm = nullptr, hipStream_t stream = nullptr) {
+        throw_on(tgs_gradient_clip_run(m_handle, max_norm, scale, epsilon, norm, stream), "GradientClip::clip");
+    }
+
+private:
+    tgs_gradient_clip* m_handle = nullptr;
 };
 
 // Muon on a network's matrices; copies (may be empty) receive the updated

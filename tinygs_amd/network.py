@@ -1,10 +1,11 @@
 """The attribute network over the C ABI: a small network whose outputs are Gaussian attributes (or changes of them)
 and the operators it is built from. No counterpart in the reference.
 
-  LayerOps          linear layers with bias, activation and residual, layer norm, and their gradients: one call each
-                    on the caller's tensors
-  AttributeNetwork  features -> linear -> [layer norm -> linear, activation -> linear + residual] x blocks ->
-                    layer norm -> linear -> attributes, forward and backward over every Gaussian
+  LayerOps          linear layers with bias, activation and residual, layer norm, attention to an encoder's states,
+                    norms of its heads with turned pairs, and their gradients: one call each on the caller's tensors
+  AttributeNetwork  features -> linear -> [attention to states + residual -> layer norm -> linear, activation ->
+                    linear + residual] x blocks -> layer norm -> linear -> attributes, forward and backward over every
+                    Gaussian; the attention is there where the network has a context
 
 Matrices are 2-D tensors of one dtype (float32, float16 or bfloat16) whose rows' elements lie next to each other;
 rows may lie further apart (a column range of a wider tensor). Vectors are packed float32.
@@ -321,14 +322,22 @@ class AttributeNetwork:
     norm(h) w_out^T + b_out. norm is a layer norm with its own gamma and beta. The last matrix starts at zero, so an
     untrained network changes nothing.
 
+    With context (the columns of an encoder's states) each block first attends to the states: h = h +
+    attention(q, k, v) w_o^T + b_o with q of norm(h), k and v of the states, each a linear layer, and a head norm on q
+    and k. heads divide width (heads of at most 128), kv_heads divide heads. With axes (1 to 4) forward takes positions of
+    the rows and of the states, and the head norms turn queries and keys by them: scores then depend on where a state
+    lies from a row. extent is the positions' usual size: the slowest pairs turn once over it, the fastest 64 times.
+
     weights are the float32 matrices that an optimiser updates: net.optimizer(), which is create_optimizer("muon",
     net.weights, net.grads, copies=net.copies). For a half dtype the products read net.copies, which Muon writes in its
     step: an optimiser that is not given them changes nothing that forward reads. vectors and vector_grads hold all
     biases, gammas and betas, and their gradients, as one float32 vector each, for an optimiser of vectors. backward
-    assigns every gradient."""
+    assigns every gradient; clip bounds their norm together."""
 
     def __init__(self, inputs: int, outputs: int, width: int = 256, hidden: int | None = None, blocks: int = 2,
-                 activation: str = "gelu", dtype=None, seed: int = 0, eps: float = 1e-5, device: str = "cuda"):
+                 activation: str = "gelu", dtype=None, seed: int = 0, eps: float = 1e-5, device: str = "cuda",
+                 context: int | None = None, heads: int = 4, kv_heads: int | None = None, axes: int = 0,
+                 extent: float = 1.0):
         import torch
         if activation not in ACTIVATIONS:
             raise RuntimeError(f"AttributeNetwork: unknown activation: {activation}")
@@ -340,43 +349,145 @@ class AttributeNetwork:
             raise RuntimeError("AttributeNetwork: only float32, float16 and bfloat16 are supported")
         self.inputs, self.outputs, self.activation, self.eps = inputs, outputs, activation, float(eps)
         shapes = [(width, inputs)] + [(hidden, width), (width, hidden)] * blocks + [(outputs, width)]
+        sizes = [o for o, _ in shapes] + [width, width] * (blocks + 1)
+        m, self.last = len(shapes), len(shapes) - 1
+        self.context, self.heads, self.kv_heads, self.axes = context, heads, heads if kv_heads is None else kv_heads, axes
+        if context is not None:
+            head = self._check_context(width, extent)
+            # after the others': the matrices of q, k, v and the output; their biases, the norm, the head norms' gammas
+            kv = self.kv_heads * head
+            attending = [(width, width), (kv, context), (kv, context), (width, width)] * blocks
+            sizes = sizes + [o for o, _ in attending] + [width, width, head, head] * blocks
+            shapes = shapes + attending
         g = torch.Generator().manual_seed(seed)
         self.weights = [(torch.randn(o, i, generator=g) / math.sqrt(i)).to(device) for o, i in shapes]
-        self.weights[-1].zero_()
+        self.weights[self.last].zero_()
         half = self.dtype != torch.float32
         self.copies = [w.to(self.dtype) for w in self.weights] if half else None
         self.grads = [torch.zeros(s, dtype=self.dtype, device=device) for s in shapes]
         # the vectors: a bias for every matrix, then gamma and beta of the blocks' norms and the last one
-        sizes = [o for o, _ in shapes] + [width, width] * (blocks + 1)
         self.vectors = torch.zeros(sum(sizes), device=device)
         self.vector_grads = torch.zeros_like(self.vectors)
         views, grads = self.vectors.split(sizes), self.vector_grads.split(sizes)
-        m = len(shapes)
+        n = m + 2 * (blocks + 1)
         self.biases, self.bias_grads = views[:m], grads[:m]
-        self.norms = list(zip(views[m::2], views[m + 1::2]))
-        self.norm_grads = list(zip(grads[m::2], grads[m + 1::2]))
-        for gamma, _ in self.norms:
+        self.norms = list(zip(views[m:n:2], views[m + 1:n:2]))
+        self.norm_grads = list(zip(grads[m:n:2], grads[m + 1:n:2]))
+        ones = [gamma for gamma, _ in self.norms]
+        if context is not None:
+            self.biases, self.bias_grads = (t[:m] + t[n:n + 4 * blocks] for t in (views, grads))
+            # of each block: gamma, beta, and the gammas of q and k
+            self.attention_norms = [views[n + 4 * (blocks + k):n + 4 * (blocks + k + 1)] for k in range(blocks)]
+            self.attention_norm_grads = [grads[n + 4 * (blocks + k):n + 4 * (blocks + k + 1)] for k in range(blocks)]
+            ones += [v[i] for v in self.attention_norms for i in (0, 2, 3)]
+            if axes:   # pairs from one turn over the extent to 64, in directions all around
+                pairs = head // 2
+                size = 2.0 * math.pi / extent * torch.logspace(0.0, 6.0, pairs, base=2.0)
+                direction = torch.randn(pairs, axes, generator=g)
+                self.frequencies = (size[:, None] * direction / direction.norm(dim=1, keepdim=True)).to(device)
+        for gamma in ones:
             gamma.fill_(1.0)
         self.blocks = blocks
         self.ops = LayerOps()
         self._kept = None
+        self._clip = None
+
+    def _check_context(self, width: int, extent: float) -> int:
+        if self.context < 1 or self.heads < 1 or self.kv_heads < 1 or width % self.heads or self.heads % self.kv_heads:
+            raise RuntimeError("AttributeNetwork: heads must divide the width, and kv_heads the heads")
+        head = width // self.heads
+        if head > 128 or not 0 <= self.axes <= 4 or (self.axes and head < 2) or not extent > 0.0:
+            raise RuntimeError("AttributeNetwork: heads of at most 128 columns, 0 to 4 axes and a positive extent are "
+                               "supported")
+        return head
 
     def optimizer(self):
         """Muon on the matrices, which also writes the half-precision copies."""
         from .optim import Muon
         return Muon(self.weights, self.grads, copies=self.copies)
 
+    def clip(self, max_norm: float, scale: float = 1.0, stream=None):
+        """Bounds the norm of all gradients together, those of the vectors included, in place; returns the norm on the
+        device (GradientClip). scale multiplies the gradients first: 1 / the factor of a scaled loss."""
+        if self._clip is None:
+            from .optim import GradientClip
+            self._clip = GradientClip(self.grads + [self.vector_grads])
+        return self._clip.clip(max_norm, scale=scale, stream=stream)
+
     def matrices(self):
         """The matrices that the products read."""
         return self.weights if self.copies is None else self.copies
 
-    def forward(self, features, keep: bool = True, stream=None):
-        """The attributes, in the network's dtype. keep: hold what backward needs (until the next forward)."""
+    def _turn(self, positions):
+        if not self.axes:
+            return {}
+        if positions is None:
+            raise RuntimeError("AttributeNetwork: positions of the rows and of the states are needed")
+        return {"positions": positions, "frequencies": self.frequencies}
+
+    def _attend(self, k, h, context, turns, mask, batch, keep, stream):
+        """h + the block's attention to the states, and what its backward needs."""
         ops, w = self.ops, self.matrices()
+        wq = self.last + 1 + 4 * k
+        gamma, beta, gamma_q, gamma_k = self.attention_norms[k]
+        n, mean, rstd = ops.layer_norm(h, gamma, beta, eps=self.eps, stream=stream)
+        q = ops.linear(n, w[wq], self.biases[wq], stream=stream)
+        key = ops.linear(context, w[wq + 1], self.biases[wq + 1], stream=stream)
+        v = ops.linear(context, w[wq + 2], self.biases[wq + 2], stream=stream)
+        qn = ops.head_norm(q, self.heads, gamma_q, out=None if keep else q, stream=stream, **turns[0])
+        kn = ops.head_norm(key, self.kv_heads, gamma_k, out=None if keep else key, stream=stream, **turns[1])
+        a = ops.attention(qn, kn, v, self.heads, kv_heads=self.kv_heads, batch=batch, mask=mask, keep_lse=keep,
+                          stream=stream)
+        a, lse = a if keep else (a, None)
+        to = ops.linear(a, w[wq + 3], self.biases[wq + 3], residual=h, out=None if keep else h, stream=stream)
+        return to, (h, n, mean, rstd, q, key, v, qn, kn, a, lse)
+
+    def _attend_backward(self, k, g, kept, context, turns, mask, batch, need_context, stream):
+        """The gradient of the block's input for its output's g, and that of the states by this block."""
+        ops, w = self.ops, self.matrices()
+        wq = self.last + 1 + 4 * k
+        h, n, mean, rstd, q, key, v, qn, kn, a, lse = kept
+        gamma, _, gamma_q, gamma_k = self.attention_norms[k]
+        grad_gamma, grad_beta, grad_gamma_q, grad_gamma_k = self.attention_norm_grads[k]
+
+        def linear(i, gy, x, need=True):
+            return ops.linear_backward(gy, x, w[wq + i], need_x=need, grad_weight=self.grads[wq + i],
+                                       grad_bias=self.bias_grads[wq + i], stream=stream)[0]
+
+        ga = linear(3, g, a)
+        gq, gk, gv = ops.attention_backward(ga, qn, kn, v, a, lse, self.heads, kv_heads=self.kv_heads, batch=batch,
+                                            mask=mask, stream=stream)
+        ops.head_norm_backward(gq, q, self.heads, gamma_q, grad_x=gq, grad_gamma=grad_gamma_q, stream=stream, **turns[0])
+        ops.head_norm_backward(gk, key, self.kv_heads, gamma_k, grad_x=gk, grad_gamma=grad_gamma_k, stream=stream,
+                               **turns[1])
+        gn = linear(0, gq, n)
+        parts = [linear(1, gk, context, need_context), linear(2, gv, context, need_context)]
+        g, _, _ = ops.layer_norm_backward(gn, h, gamma, mean, rstd, residual_grad=g, grad_x=g, grad_gamma=grad_gamma,
+                                          grad_beta=grad_beta, stream=stream)
+        return g, parts
+
+    def forward(self, features, keep: bool = True, stream=None, context=None, mask=None, batch: int = 1, positions=None,
+                context_positions=None):
+        """The attributes, in the network's dtype. keep: hold what backward needs (until the next forward).
+
+        A network with context takes the states [batch x states, context] in its dtype (features are batch x rows then),
+        mask [batch, states] where some do not exist, and with axes the float32 positions [rows, axes] and
+        context_positions [states, axes] of both."""
+        ops, w, last = self.ops, self.matrices(), self.last
         self._kept = None
+        turns = None
+        if (context is None) != (self.context is None):
+            raise RuntimeError("AttributeNetwork::forward: states are for a network with context")
+        if context is not None:
+            turns = self._turn(positions), self._turn(context_positions)
         h = ops.linear(features, w[0], self.biases[0], stream=stream)
         kept = [features]
+        attended = []
         for k in range(self.blocks):
+            if context is not None:
+                h, of = self._attend(k, h, context, turns, mask, batch, keep, stream)
+                if keep:
+                    attended.append(of)
             n, mean, rstd = ops.layer_norm(h, *self.norms[k], eps=self.eps, stream=stream)
             up, down = 1 + 2 * k, 2 + 2 * k
             a = ops.linear(n, w[up], self.biases[up], activation=self.activation, keep_preact=keep, stream=stream)
@@ -388,22 +499,26 @@ class AttributeNetwork:
         n, mean, rstd = ops.layer_norm(h, *self.norms[-1], eps=self.eps, stream=stream)
         if keep:
             kept.append((h, n, mean, rstd))
-            self._kept = kept
-        return ops.linear(n, w[-1], self.biases[-1], stream=stream)
+            self._kept = kept, attended, (context, turns, mask, batch)
+        return ops.linear(n, w[last], self.biases[last], stream=stream)
 
-    def backward(self, grad_attributes, need_features: bool = False, stream=None):
+    def backward(self, grad_attributes, need_features: bool = False, stream=None, need_context: bool = False):
         """Fills grads and vector_grads for dL/dattributes (in the network's dtype) of the last forward; returns
-        dL/dfeatures where needed."""
+        dL/dfeatures where needed, and with need_context a pair of it and dL/dcontext (float32)."""
         if self._kept is None:
             raise RuntimeError("AttributeNetwork::backward: no forward that kept its values")
-        ops, w, kept = self.ops, self.matrices(), self._kept
+        ops, w, last = self.ops, self.matrices(), self.last
+        kept, attended, (context, turns, mask, batch) = self._kept
+        if need_context and context is None:
+            raise RuntimeError("AttributeNetwork::backward: a network without context")
         act = self.activation
         h, n, mean, rstd = kept[-1]
-        g, _, _ = ops.linear_backward(grad_attributes, n, w[-1], grad_weight=self.grads[-1],
-                                      grad_bias=self.bias_grads[-1], stream=stream)
+        g, _, _ = ops.linear_backward(grad_attributes, n, w[last], grad_weight=self.grads[last],
+                                      grad_bias=self.bias_grads[last], stream=stream)
         gg, gb = self.norm_grads[-1]
         g, _, _ = ops.layer_norm_backward(g, h, self.norms[-1][0], mean, rstd, grad_x=g, grad_gamma=gg, grad_beta=gb,
                                           stream=stream)
+        parts = []
         for k in reversed(range(self.blocks)):
             h, n, mean, rstd, a, z = kept[1 + k]
             up, down = 1 + 2 * k, 2 + 2 * k
@@ -415,9 +530,26 @@ class AttributeNetwork:
             # the residual path's gradient joins the norm's
             g, _, _ = ops.layer_norm_backward(gn, h, self.norms[k][0], mean, rstd, residual_grad=g, grad_x=g,
                                               grad_gamma=gg, grad_beta=gb, stream=stream)
+            if context is not None:
+                g, of = self._attend_backward(k, g, attended[k], context, turns, mask, batch, need_context, stream)
+                parts += of
         gx, _, _ = ops.linear_backward(g, kept[0], w[0], need_x=need_features, grad_weight=self.grads[0],
                                        grad_bias=self.bias_grads[0], stream=stream)
-        return gx
+        if not need_context:
+            return gx
+        return gx, self._sum(parts, context, stream)
+
+    @staticmethod
+    def _sum(parts, like, stream):
+        """Of the blocks' gradients, in float32."""
+        import contextlib
+
+        import torch
+        with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
+            total = torch.zeros(like.shape, dtype=torch.float32, device=like.device)
+            for t in parts:
+                total += t
+        return total
 
 
 def encode_positions(means, octaves: int = 10, dtype=None):

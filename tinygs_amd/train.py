@@ -7,6 +7,7 @@ Orchestrator::train_step (tinygs/src/orchestrator.cu:335-439):
      with both on, one fused evaluation that assigns the loss / gradient images
      (the zeroing of :354-355 folded in)
   -> FastGSRasterizer::backward with grad_output = loss gradient (:377-380)
+  -> (max_grad_norm: the gradients' norm bounded; not in the reference)
   -> SimpleAdam::step(1 / (grad_scaler * accumulate_grad_steps)) (:393-404)
 
 The parameter-gradient zeroing of :351-353 is folded into the backward:
@@ -39,14 +40,16 @@ class TrainStep:
                  eps: float = 1e-15, shs_lr: float | None = None, means_lr: float | None = None,
                  max_grad_1: float | None = None, device: str = "cuda", stream=None, sparse_grads: bool = True,
                  no_sync: bool = False, image_dtype: str = DataType.Float32, overlap_adam: bool = False,
-                 check_interval: int = 64):
+                 check_interval: int = 64, max_grad_norm: float | None = None):
         """image_dtype: float32, or float16 for the fp16-image rasterizer
         (fastgs.cu:143-188) with the fp16 losses; the target is rounded to half.
         overlap_adam (needs sparse_grads): Adam updates the rows without
         gradient on a second stream while the loss and the backward run, then
         the others; the parameters equal those of the sequential step. Off by
         default: on one MI355X at 1M Gaussians the concurrent kernels slow each
-        other down more than the overlap hides (1.16 against 0.98 ms per step)."""
+        other down more than the overlap hides (1.16 against 0.98 ms per step).
+        max_grad_norm bounds the norm of all Gaussians' gradients of a step together (unscaled, before Adam;
+        GradientClip); it reads every gradient, so sparse_grads must be off. grad_norm holds the last step's norm."""
         import torch
         self.scene = scene
         self.no_sync = bool(no_sync)
@@ -61,6 +64,11 @@ class TrainStep:
         self.overlap_adam = bool(overlap_adam)
         if self.overlap_adam and not self.sparse_grads:
             raise ValueError("overlap_adam needs sparse_grads")
+        if max_grad_norm is not None and self.sparse_grads:
+            raise ValueError("max_grad_norm needs sparse_grads=False: a sparse backward leaves rows unwritten")
+        self.max_grad_norm = max_grad_norm
+        self._clip = None
+        self.grad_norm = None   # a float32 scalar on the device, of gradients times grad_scaler
         self._side = None   # the second stream and the fork / join events of overlap_adam
         self._fork = self._join = None
         self.stream = stream
@@ -156,6 +164,11 @@ class TrainStep:
 
     def optimize(self):
         mask = self.rasterizer.grad_row_mask() if self.sparse_grads else None
+        if self.max_grad_norm is not None:
+            if self._clip is None:
+                from .optim import GradientClip
+                self._clip = GradientClip([t for t in self.grads.tensors()])
+            self.grad_norm = self._clip.clip(self.max_grad_norm * self.grad_scaler, stream=self.stream)
         # no_sync: the step count on the device too, so a whole step can be captured
         self.optimizer.step(1.0 / self.grad_scaler, self.stream, row_mask=mask, device_step=self.no_sync)
 
