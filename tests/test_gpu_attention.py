@@ -206,6 +206,24 @@ def test_needed_gradients_alone(ops):
             assert (x is None) if not n else torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("d", [5, 32, 64, 98, 128])
+@pytest.mark.parametrize("masked", [False, True])
+def test_one_state_has_no_gradient_of_scores(ops, dtype, d, masked):
+    """Where a row has one state its weight is 1 whatever the score: grad_q and grad_k are 0, not the difference of two
+    sums of the same terms."""
+    states = 70 if masked else 1
+    q, k, v, go = case(d, dtype, 2, 150, states, 4, 2, d)
+    m = None
+    if masked:
+        m = torch.zeros(2, states, dtype=torch.bool, device="cuda")
+        m[0, 40] = m[1, 69] = True
+    out, lse = ops.attention(q, k, v, 4, kv_heads=2, batch=2, mask=m, keep_lse=True)
+    for need_q in (True, False):
+        gq, gk, gv = ops.attention_backward(go, q, k, v, out, lse, 4, kv_heads=2, batch=2, mask=m, need_q=need_q)
+        assert (not need_q or not gq.any()) and not gk.any() and gv.any()
+
+
 def test_gradients_against_differences(ops):
     """In 64 bits around float32 inputs: (f(x + e) - f(x - e)) / 2e of the sum of out with a direction is off by e^2 of
     the third derivative and 2^-24 / e of out; e = 2^-6 leaves less than 1 in 300 of the largest."""

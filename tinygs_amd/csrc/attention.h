@@ -226,31 +226,31 @@ struct LaneRows {
         constexpr int V = 16 / (int)sizeof(T);
         const int64_t pitch = m.stride * (int64_t)sizeof(T);
         const unsigned char* from = (const unsigned char*)m.p + base * pitch;
-        if (d % V == 0) {   // all loads on their way at once, without branches
-            const auto buffer = resource_of(from, (m.rows - 1 - base) * pitch + m.cols * (int64_t)sizeof(T));
+        // whole chunks: all loads on their way at once, without branches
+        const auto buffer = resource_of(from, (m.rows - 1 - base) * pitch + m.cols * (int64_t)sizeof(T));
 #pragma unroll
-            for (int n = 0; n < QB; ++n)
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) {
-                    const int c = 2 * s + (lane >> 5);
-                    const uint32_t at = (uint32_t)(down[n] * pitch + (head[n] * d + c * V) * (int)sizeof(T));
-                    f[n][s] = __builtin_bit_cast(
-                        F, __builtin_amdgcn_raw_buffer_load_b128(buffer, exists[n] && c * V < d ? (int)at : (int)kPastEnd, 0, 0));
-                }
-            return;
-        }
-#pragma unroll
-        for (int n = 0; n < QB; ++n) {
-            const T* p = (const T*)(from + down[n] * pitch) + (int64_t)head[n] * d;
+        for (int n = 0; n < QB; ++n)
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 const int c = 2 * s + (lane >> 5);
-                F v = {};
-#pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (exists[n] && c * V + e < d) v[e] = p[c * V + e];
-                f[n][s] = v;
+                const uint32_t at = (uint32_t)(down[n] * pitch + (head[n] * d + c * V) * (int)sizeof(T));
+                f[n][s] = __builtin_bit_cast(F, __builtin_amdgcn_raw_buffer_load_b128(
+                                                    buffer, exists[n] && (c + 1) * V <= d ? (int)at : (int)kPastEnd, 0, 0));
             }
+        if (d % V == 0) return;
+        const int last = d / V;   // the chunk that the head ends in, element by element
+        if ((lane >> 5) != (last & 1)) return;
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            if (!exists[n]) continue;
+            const T* p = (const T*)(from + down[n] * pitch) + (int64_t)head[n] * d + last * V;
+            F v = {};
+#pragma unroll
+            for (int e = 0; e < V - 1; ++e)
+                if (last * V + e < d) v[e] = p[e];
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+                if (s == last / 2) f[n][s] = v;
         }
     }
 };

@@ -116,26 +116,40 @@ __device__ __forceinline__ float lse_exponent(float lse) {
     return lse == -INFINITY ? INFINITY : lse * kLog2E;
 }
 
-// delta, where dq is not asked for; in the order that the two halves of a wave sum it there
-template <class T>
+// delta where dq is not asked for, with the same bits: a wave for 32 rows of a head.
+template <class T, int D>
 __global__ void __launch_bounds__(256) delta_kernel(AttentionBackward b, Grid g) {
+    using S = Square<T>;
+    constexpr int kSteps = D / S::kDepth;
     const Attention& a = b.a;
-    const int64_t n = a.q.rows * a.heads;
+    const int lane = threadIdx.x & 63;
+    const int64_t blocks = (a.q.rows + 31) / 32, n = blocks * a.heads;
     float most = 0.0f, most_delta = 0.0f;
-    for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
-        const int64_t r = k / a.heads;
-        const int h = (int)(k % a.heads);
-        const T* x = (const T*)b.grad_out.p + r * b.grad_out.stride + (int64_t)h * a.head;
-        const T* y = (const T*)a.out.p + r * a.out.stride + (int64_t)h * a.head;
-        float v[2] = {0.0f, 0.0f}, w[2] = {0.0f, 0.0f};
-        for (int c = 0; c < a.head; ++c) {
-            const int half = c / (16 / (int)sizeof(T)) & 1;
-            v[half] = fmaf((float)x[c], (float)y[c], v[half]);
-            w[half] = fmaf((float)x[c], (float)x[c], w[half]);
-        }
-        g.delta[k] = v[0] + v[1];
-        most = fmaxf(most, w[0] + w[1]);
-        most_delta = fmaxf(most_delta, fabsf(v[0] + v[1]));
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
+        const int h = (int)(i % a.heads);
+        LaneRows<1> rows;
+        rows.begin(0, i / a.heads * 32, a.q.rows, h, 1, lane);
+        typename S::Frag go[1][kSteps], o[1][kSteps];
+        rows.template load<T, kSteps>(b.grad_out, a.head, lane, go);
+        rows.template load<T, kSteps>(a.out, a.head, lane, o);
+        f32x16 dots = S::product(o[0][0], go[0][0]);
+#pragma unroll
+        for (int s = 1; s < kSteps; ++s) S::multiply(o[0][s], go[0][s], dots);
+        float dot = 0.0f, square = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dot = square_row(r, lane) == (lane & 31) ? dots[r] : dot;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int k = 0; k < 16 / (int)sizeof(T); ++k) square = fmaf((float)go[0][s][k], (float)go[0][s][k], square);
+        float other = dot;
+        swap32(dot, other);
+        dot += other;
+        other = square;
+        swap32(square, other);
+        most = fmaxf(most, square + other);
+        most_delta = fmaxf(most_delta, fabsf(dot));
+        if (rows.exists[0] && lane < 32) g.delta[rows.row(0) * a.heads + h] = dot;
     }
     if constexpr (kBoost<T> != 0.0f) leave_largest(g, most, most_delta);
 }
@@ -171,15 +185,20 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 || sizeof(T) == 2 ? 2 : 1
         }
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
+            // by the product that forms dp: where a row has one state, dp - delta is nothing
+            f32x16 dots = S::product(o[n][0], go[n][0]);
+#pragma unroll
+            for (int s = 1; s < kSteps; ++s) S::multiply(o[n][s], go[n][s], dots);
             float dot = 0.0f, square = 0.0f;
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
+            for (int r = 0; r < 16; ++r) dot = square_row(r, lane) == (lane & 31) ? dots[r] : dot;
+            if constexpr (kBoost<T> != 0.0f) {
 #pragma unroll
-                for (int k = 0; k < 16 / (int)sizeof(T); ++k) {
-                    dot = fmaf((float)go[n][s][k], (float)o[n][s][k], dot);
-                    if constexpr (kBoost<T> != 0.0f) square = fmaf((float)go[n][s][k], (float)go[n][s][k], square);
-                }
-            float other = dot;
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int k = 0; k < 16 / (int)sizeof(T); ++k) square = fmaf((float)go[n][s][k], (float)go[n][s][k], square);
+            }
+            float other = dot;   // one of the halves has it, the other 0
             swap32(dot, other);
             delta[n] = dot + other;
             other = square;
@@ -704,12 +723,12 @@ void split_tiles(int64_t whole, int64_t tiles, int& splits, int64_t& part) {
     splits = tiles > 0 ? (int)((tiles + part - 1) / part) : 1;
 }
 
-// Whether the one-pass kernel takes it: states and heads that it holds, and as many
+// Whether the one-pass kernel takes it: states and heads that it holds, more states than one wave's, and as many
 // rows as pay for its start and its sums' join.
 bool at_once(const AttentionBackward& b) {
     const Attention& a = b.a;
     return a.dtype == TGS_DTYPE_BFLOAT16 && b.grad_q.p && (b.grad_k.p || b.grad_v.p) && a.head <= 64 && a.head % 8 == 0 &&
-           a.states >= 1 && a.states <= kOnceStates && a.batch * a.kv_heads <= 65536 &&
+           a.states > 32 && a.states <= kOnceStates && a.batch * a.kv_heads <= 65536 &&
            (a.queries + kOnceRows - 1) / kOnceRows * (a.heads / a.kv_heads) * a.batch * a.kv_heads >= 1024;
 }
 
@@ -757,7 +776,7 @@ Plan plan_of(const AttentionBackward& b) {
     if (b.grad_q.p && p.q.splits > 1) sums = sizeof(float) * (size_t)(p.q.splits * a.q.rows * a.heads * width);
     if ((b.grad_k.p || b.grad_v.p) && p.kv.splits > 1)
         sums = std::max(sums, sizeof(float) * 2 * (size_t)(p.kv.splits * a.k.rows * a.kv_heads * width));
-    p.delta_blocks = std::min<int64_t>((a.q.rows * a.heads + 255) / 256, 4096);
+    p.delta_blocks = std::min<int64_t>(((a.q.rows + 31) / 32 * a.heads + 3) / 4, 4096);
     if (a.dtype == TGS_DTYPE_FLOAT16) {
         p.kv.lifts = b.grad_q.p ? p.q_workgroups : p.delta_blocks;
         p.norms_bytes = (sizeof(float) * (size_t)(a.batch * a.kv_heads * ((a.states + 63) / 64)) + 255) / 256 * 256;
@@ -836,7 +855,7 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
                         p.q.sums, p.q.splits, a.q.rows * a.heads, b.grad_q, a.heads, a.head);
             } else if (a.q.rows && states) {
                 p.kv.first = 0;
-                delta_kernel<T><<<(unsigned)p.delta_blocks, 256, 0, s>>>(b, p.kv);
+                delta_kernel<T, D><<<(unsigned)p.delta_blocks, 256, 0, s>>>(b, p.kv);
             }
             if (!states) return;
             const auto launch = [&](auto what) {
