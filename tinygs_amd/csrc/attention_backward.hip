@@ -715,13 +715,20 @@ __global__ void __launch_bounds__(256) join_kernel(const float* sums, int splits
 
 float exponent_of(float scale) { return scale > 0.0f ? fmaxf(scale * kLog2E, 0x1p-149f) : 0x1p-149f; }
 
-// The splits of `tiles` for about 512 workgroups, and a split's tiles.
-void split_tiles(int64_t whole, int64_t tiles, int& splits, int64_t& part) {
+// The splits of `tiles` for about `target` workgroups where there are half as many
+// or fewer, no shorter than `least` tiles.
+void split_tiles(int64_t whole, int64_t tiles, int64_t target, int64_t least, int& splits, int64_t& part) {
     int64_t n = 1;
-    if (whole > 0 && whole < 256 && tiles > 1) n = 512 / whole < tiles ? 512 / whole : tiles;
+    if (whole > 0 && 2 * whole <= target && tiles >= 2 * least) n = std::min(target / whole, tiles / least);
     part = tiles > 0 ? (tiles + n - 1) / n : 1;
     splits = tiles > 0 ? (int)((tiles + part - 1) / part) : 1;
 }
+// dq, as the forward: 100 rows of 4 heads of 64 at 4096 states, all three gradients,
+// 24 us in 64 parts and 40 in 128, 16000 of one at 272 47 whole and 65 in parts.
+// dk and dv: two workgroups a compute unit (2 x 8192 rows of 8 heads of 128 at 4096
+// states 1255 us, 3060 in half as many), two tiles a part (132 rows of 2 heads of
+// 16 at 448 states 24 us, 30 with one).
+constexpr int64_t kRowTarget = 256, kRowLeast = 4, kStateTarget = 512, kStateLeast = 2;
 
 // Whether the one-pass kernel takes it: states and heads that it holds, more states than one wave's, and as many
 // rows as pay for its start and its sums' join.
@@ -764,12 +771,12 @@ Plan plan_of(const AttentionBackward& b) {
     p.qb = halves && width <= 64 && p.q.rows > 32 * kWaves ? 2 : 1;
     p.q.blocks = (p.q.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
     int64_t whole = a.batch * a.kv_heads * p.q.blocks;
-    split_tiles(whole, (a.states + p.tile - 1) / p.tile, p.q.splits, p.q.part);
+    split_tiles(whole, (a.states + p.tile - 1) / p.tile, kRowTarget, kRowLeast, p.q.splits, p.q.part);
     p.q_workgroups = whole * p.q.splits;
     p.kv.blocks = (a.states + 32 * kWaves - 1) / (32 * kWaves);
     p.kv.units = (a.queries + p.tile - 1) / p.tile * p.kv.shared;
     whole = a.batch * a.kv_heads * p.kv.blocks;
-    split_tiles(whole, p.kv.units, p.kv.splits, p.kv.part);
+    split_tiles(whole, p.kv.units, kStateTarget, kStateLeast, p.kv.splits, p.kv.part);
     p.kv_workgroups = whole * p.kv.splits;
     p.delta_bytes = (sizeof(float) * (size_t)(a.q.rows * a.heads) + 255) / 256 * 256;
     size_t sums = 0;
