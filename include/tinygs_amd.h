@@ -493,7 +493,8 @@ int tgs_convert(const void* src, int32_t src_dtype, void* dst, int32_t dst_dtype
  * not wait for the device, except to grow the handle's workspace. The
  * workspace is shared by the calls on a handle: calls on one handle run on one
  * stream, or the caller orders them. A captured call must not grow it: run one
- * with the same sizes before capturing. */
+ * with the same sizes before capturing. A later call that grows it frees what
+ * the captured ones use: larger calls go to a handle of their own, or come first. */
 typedef struct tgs_matrix {
     void* data;
     int64_t rows;
@@ -622,7 +623,8 @@ int tgs_gradient_clip_set_matrices(tgs_gradient_clip* c, const tgs_matrix* grads
                                    int32_t count);
 /* norm: a device float, or NULL. Where f is 1, gradients clipped in place are
  * not written. The first run, and the first after other matrices, place the
- * matrices' table on the device and wait for it: capture only later ones. */
+ * matrices' table on the device and wait for it: capture only later ones, and
+ * do not rebind while the graph is in use. */
 int tgs_gradient_clip_run(tgs_gradient_clip* c, float max_norm, float scale, float epsilon, float* norm, void* stream);
 
 /* ---- Muon: the optimiser of the network's matrices. A step, for each matrix

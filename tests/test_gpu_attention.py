@@ -206,6 +206,54 @@ def test_needed_gradients_alone(ops):
             assert (x is None) if not n else torch.equal(x, y)
 
 
+def test_tensors_elsewhere_are_refused(ops):
+    """A tensor that is not on the current device, among those that are."""
+    q, k, v, go = case(1, torch.float16, 1, 4, 6, 2, 2, 16)
+    out, lse = ops.attention(q, k, v, 2, keep_lse=True)
+    with pytest.raises(RuntimeError, match="mask: not on the current device"):
+        ops.attention(q, k, v, 2, mask=torch.ones(1, 6, dtype=torch.bool))
+    with pytest.raises(RuntimeError, match="lse"):
+        ops.attention_backward(go, q, k, v, out, lse.cpu(), 2)
+    with pytest.raises(RuntimeError, match="not on the device"):
+        ops.attention(q, k.cpu(), v, 2)
+    with pytest.raises(RuntimeError, match="lse"):
+        ops.attention(q, k, v, 2, lse=torch.empty(4, 3, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_many_small_elements(ops, dtype):
+    """More elements of a batch than a card has room for at once, a row or two of each."""
+    for queries, states, heads, kv_heads, d in ((1, 9, 2, 2, 16), (2, 40, 2, 1, 24), (40, 9, 1, 1, 64)):
+        t = case(queries, dtype, 3000, queries, states, heads, kv_heads, d)
+        m = mask_of(1, 3000, states, 0.6, empty=(5, 2999))
+        run_both(ops, *t, heads, kv_heads, 3000, m, what=(queries, states))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_maxima_far_behind(ops, dtype):
+    """Scores that rise with the states: the largest comes last, by more than a weight's range above the first ones, in
+    some rows; the others' results do not change by a bit."""
+    for rows, states, d in ((200, 300, 32), (40_003, 250, 64), (1, 400, 64), (30, 5000, 128)):
+        heads = 4
+        q, k, v, go = case(rows, dtype, 1, rows, states, heads, heads, d)
+        want, wlse = ops.attention(q, k, v, heads, keep_lse=True)
+        steep = q.clone()
+        pick = torch.arange(0, rows, 7, device="cuda")
+        steep[pick] = 0.0
+        steep[pick, 0] = 24.0            # of head 0
+        rising = k.clone()
+        rising[:, 0] = torch.linspace(-6, 12, states).to(dtype).cuda()
+        out, lse = ops.attention(steep, rising, v, heads, keep_lse=True)
+        sample = torch.arange(0, rows, max(1, rows // 60), device="cuda")
+        (o, ob), (l, lb) = A.attention(steep[sample].contiguous(), rising, v, heads, heads)
+        A.check(out[sample], o, ob, (rows, "out"))
+        A.check(lse[sample], l, lb, (rows, "lse"))
+        # heads other than the first: the same inputs, but for the zeroed rows
+        keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+        keep[pick] = False
+        assert torch.equal(out[keep][:, d:], want[keep][:, d:]) and torch.equal(lse[keep][:, 1:], wlse[keep][:, 1:])
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("d", [5, 32, 64, 98, 128])
 @pytest.mark.parametrize("masked", [False, True])

@@ -13,6 +13,8 @@
 // and the A operand is read from LDS in that order.
 #pragma once
 
+#include <math.h>
+
 #include "mfma_tile.h"
 
 namespace tgs {
@@ -281,6 +283,10 @@ __device__ __forceinline__ void square_rows(const f32x16& s, int p, float (&v)[8
         swap32(v[r], v[4 + r]);
     }
 }
+
+// s scale log2(e), or no difference between states for a scale of 0; positive, so
+// that -infinity stays -infinity.
+inline float exponent_of(float scale) { return scale > 0.0f ? fmaxf(scale * kLog2E, 0x1p-149f) : 0x1p-149f; }
 
 // The least multiple of 32 that the kernels hold heads in.
 template <class F>

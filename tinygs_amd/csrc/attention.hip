@@ -12,6 +12,10 @@
 // instructions, and a scaling of the sums on the way, even one that is never reached,
 // made the compiler copy them all at every step.
 //
+// 2 x 8192 rows of 8 heads of 128 halves, 2 shared, at 4096 states: 252 to 283 us by
+// card, 0.77 PFLOP/s; wide heads with 32 rows a wave, two waves a SIMD (one wave of 64
+// rows 361).
+//
 // Heads that share the states' are rows side by side, so that a tile is loaded
 // once for all of them. Where there are few rows, workgroups take parts of the
 // states and their sums are joined by a second kernel.
@@ -45,10 +49,6 @@ struct Grid {
     float* sums;         // of a split's parts: [splits][all rows][D], then m and l
     float* tops;
 };
-
-// s scale log2(e), or no difference between states for a scale of 0; positive, so
-// that -infinity stays -infinity.
-float exponent_of(float scale) { return scale > 0.0f ? fmaxf(scale * kLog2E, 0x1p-149f) : 0x1p-149f; }
 
 // A wave's 32 or 64 rows on their way over the states.
 template <class T, int D, int QB>
@@ -307,22 +307,24 @@ __global__ void __launch_bounds__(64 * WAVES, (D <= 64 || sizeof(T) == 2 ? 2 : 1
     else rows.store(a, lane);
 }
 
-// All states of a head in LDS, loaded once; the waves go over rows by
-// themselves, without a barrier, while another wave of the SIMD computes.
+// All states of a head in LDS, loaded once; the waves go over rows by themselves,
+// without a barrier, while others of the SIMD compute: four of them where a wave's
+// square of rows needs 128 registers. 1e6 rows of 4 heads of 64 bfloat16 at 256
+// states 386 us (0.68 PFLOP/s; 470 with tiles through LDS): a third of the time the
+// matrix cores are busy, two thirds the vector units, half of whose time are the
+// exponentials.
 constexpr int held_waves(int size, int width) { return width <= (size == 2 ? 64 : 32) ? 16 : 8; }
 template <class T, int D>
 constexpr int kHeldWaves = held_waves((int)sizeof(T), D);
-// Bytes of the keys, and as many of the values: narrow heads' kernels need so few
-// registers that two workgroups fit on a compute unit.
-constexpr int held_bytes(int width) { return 64 * 1024; }
+constexpr int kHeldBytes = 64 * 1024;   // of the keys, and as many of the values
 
-template <class T, int D, int QB>
+template <class T, int D>
 __global__ void __launch_bounds__((64 * kHeldWaves<T, D>)) held_kernel(Attention a, Grid g) {
     constexpr int kTileLoads = D * (int)sizeof(T) * 64 / 1024;
     constexpr int kLoaders = kTileLoads % kHeldWaves<T, D> == 0 ? kHeldWaves<T, D> : kTileLoads % 8 == 0 ? 8 : 4;
     using Tile = RowTile<T, D, 64, kLoaders>;
-    constexpr int kTiles = held_bytes(D) / Tile::kBytes;
-    __shared__ __align__(1024) unsigned char lk[held_bytes(D)], lv[held_bytes(D)];
+    constexpr int kTiles = kHeldBytes / Tile::kBytes;
+    __shared__ __align__(1024) unsigned char lk[kHeldBytes], lv[kHeldBytes];
     __shared__ uint32_t exist[2 * kTiles];   // of each 32 states
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t number = xcd_contiguous_index(blockIdx.x, gridDim.x);
@@ -357,11 +359,11 @@ __global__ void __launch_bounds__((64 * kHeldWaves<T, D>)) held_kernel(Attention
         } while (bits == 0);
         return u;
     };
-    const int64_t wave_blocks = (g.rows + QB * 32 - 1) / (QB * 32);
+    const int64_t wave_blocks = (g.rows + 31) / 32;
     const int64_t last = min((part + 1) * g.part, wave_blocks);
     for (int64_t i = part * g.part + wave; i < last; i += kHeldWaves<T, D>) {
-        WaveRows<T, D, QB> rows;
-        rows.begin(a, g, b, kv, i * QB * 32, lane);
+        WaveRows<T, D, 1> rows;
+        rows.begin(a, g, b, kv, i * 32, lane);
         for (bool again = false;; again = true) {
             rows.clear();
             uint32_t bits = 0;
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__((64 * kHeldWaves<T, D>)) held_kernel(Attention
                                         u == u0 && !again, g.c, lane);
             if (__builtin_expect(again || !rows.passed(), 1)) break;
             for (int u = next(-1, bits); u < squares; u = next(u, bits)) {
-                f32x16 s[QB];
+                f32x16 s[1];
                 rows.template score<Tile>(lk + u * 32 * Tile::kRowBytes, bits, s, lane);
                 rows.template raise<false>(s);
             }
@@ -530,10 +532,7 @@ struct Plan {
 };
 
 constexpr int kWaves = 4;
-
-// The rows' squares of a wave: two where the registers hold them.
-template <class T, int D>
-constexpr int kHeldSquares = 1;
+constexpr int64_t kMostPairs = 1 << 21;   // of 1024 threads: a launch below 2^32
 
 Plan plan_of(const Attention& a) {
     Plan p{};
@@ -543,10 +542,10 @@ Plan plan_of(const Attention& a) {
     p.grid.rows = a.queries * p.grid.shared;
     p.grid.c = exponent_of(a.scale);
     p.grid.splits = 1;
-    const int64_t held_rows = 32;
-    const int64_t wave_blocks = (p.grid.rows + held_rows - 1) / held_rows;
-    p.held = a.states > 0 && (a.states + 63) / 64 * 64 * width * (halves ? 2 : 4) <= held_bytes((int)width) && (halves || width <= 64) &&
-             wave_blocks * pairs >= 256 * held_waves(halves ? 2 : 4, (int)width) && pairs <= 65536;
+    const int64_t wave_blocks = (p.grid.rows + 31) / 32;
+    // where the states fit and every wave has rows; floats of wide heads need too many registers for its eight waves
+    p.held = a.states > 0 && (a.states + 63) / 64 * 64 * width * (halves ? 2 : 4) <= kHeldBytes && (halves || width <= 64) &&
+             wave_blocks * pairs >= 256 * held_waves(halves ? 2 : 4, (int)width) && pairs <= kMostPairs;
     if (p.held) {
         const int64_t parts = pairs < 256 ? 256 / pairs : 1;
         p.grid.part = (wave_blocks + parts - 1) / parts;
@@ -557,7 +556,7 @@ Plan plan_of(const Attention& a) {
     // several rows of heads above 128 bytes are no faster so (4 rows of 128 halves at 300 states 17.9 us and 17.0, of
     // 128 floats at 500 25.3 and 16.4; of 64 halves at 100 13.7 and 16.2)
     p.few = (p.grid.rows == 1 || (p.grid.rows <= kFewRows && a.head * (halves ? 2 : 4) <= 128)) && a.states >= 1 &&
-            a.states <= kFewStates && pairs <= 65536;
+            a.states <= kFewStates && pairs <= kMostPairs;
     if (p.few) {
         p.workgroups = pairs;
         return p;
@@ -595,7 +594,7 @@ int launch_attention(const Attention& a, void* workspace, hipStream_t s) {
             constexpr int D = decltype(width)::value, KT = sizeof(T) == 2 ? 64 : 32;
             if (p.held) {
                 if constexpr (sizeof(T) == 2 || D <= 64)
-                    held_kernel<T, D, kHeldSquares<T, D>>
+                    held_kernel<T, D>
                         <<<(unsigned)p.workgroups, 64 * kHeldWaves<T, D>, 0, s>>>(a, p.grid);
                 return;
             }
