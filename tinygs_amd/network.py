@@ -206,7 +206,7 @@ class LayerOps:
             lse = self._empty(stream, q, (heads, rows), _float32()).t()
         tensors = (matrix(q, "q"), matrix(k, "k"), matrix(v, "v"))
         a = self._attention(q, k, heads, kv_heads, batch, mask, scale)
-        _on_one_device(q=q, k=k, v=v, mask=mask, out=out, lse=lse)
+        _on_one_device("q k v mask out lse", q, k, v, mask, out, lse)
         rc = self._lib.tgs_attention_forward(self._h, *tensors, a, matrix(out, "out"), *_lse(lse, rows, heads),
                                              self._stream(stream, q))
         if rc:
@@ -226,8 +226,8 @@ class LayerOps:
             grad_v = self._empty(stream, v, v.shape)
         tensors = (matrix(grad_out, "grad_out"), matrix(q, "q"), matrix(k, "k"), matrix(v, "v"), matrix(out, "out"))
         a = self._attention(q, k, heads, kv_heads, batch, mask, scale)
-        _on_one_device(grad_out=grad_out, q=q, k=k, v=v, out=out, lse=lse, mask=mask, grad_q=grad_q, grad_k=grad_k,
-                       grad_v=grad_v)
+        _on_one_device("grad_out q k v out lse mask grad_q grad_k grad_v", grad_out, q, k, v, out, lse, mask, grad_q,
+                       grad_k, grad_v)
         rc = self._lib.tgs_attention_backward(
             self._h, *tensors, *_lse(lse, q.shape[0], heads), a, None if grad_q is None else matrix(grad_q, "grad_q"),
             None if grad_k is None else matrix(grad_k, "grad_k"), None if grad_v is None else matrix(grad_v, "grad_v"),
@@ -260,7 +260,7 @@ class LayerOps:
             out = self._empty(stream, x, x.shape)
         at = matrix(x, "x")
         turn = _turn(positions, frequencies)
-        _on_one_device(x=x, gamma=gamma, positions=positions, frequencies=frequencies, out=out)
+        _on_one_device("x gamma positions frequencies out", x, gamma, positions, frequencies, out)
         rc = self._lib.tgs_head_norm_forward(self._h, at, heads, _vector(gamma, x.shape[1] // max(heads, 1), "gamma"),
                                              turn, eps, matrix(out, "out"), self._stream(stream, x))
         if rc:
@@ -278,8 +278,8 @@ class LayerOps:
             grad_gamma = self._empty(stream, x, (d,), _float32())
         at = (matrix(grad_y, "grad_y"), matrix(x, "x"))
         turn = _turn(positions, frequencies)
-        _on_one_device(grad_y=grad_y, x=x, gamma=gamma, positions=positions, frequencies=frequencies, grad_x=grad_x,
-                       grad_gamma=grad_gamma)
+        _on_one_device("grad_y x gamma positions frequencies grad_x grad_gamma", grad_y, x, gamma, positions,
+                       frequencies, grad_x, grad_gamma)
         rc = self._lib.tgs_head_norm_backward(self._h, *at, heads, _vector(gamma, d, "gamma"), turn, eps,
                                               None if grad_x is None else matrix(grad_x, "grad_x"),
                                               _vector(grad_gamma, d, "grad_gamma"), self._stream(stream, x))
@@ -288,13 +288,25 @@ class LayerOps:
         return grad_x, grad_gamma
 
 
-def _on_one_device(**tensors):
+_CURRENT = None
+
+
+def _current_device() -> int:
+    global _CURRENT
+    if _CURRENT is None:
+        import torch
+        torch.cuda.current_device()   # initialises
+        # without the checks around it, which take longer than the question
+        _CURRENT = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    return _CURRENT()
+
+
+def _on_one_device(names: str, *tensors):
     """All on the current device, whose streams and workspaces a handle uses."""
-    import torch
-    current = torch.cuda.current_device()
-    for name, t in tensors.items():
+    current = _current_device()
+    for i, t in enumerate(tensors):
         if t is not None and t.get_device() != current:
-            raise RuntimeError(f"{name}: not on the current device")
+            raise RuntimeError(f"{names.split()[i]}: not on the current device")
 
 
 def _lse(t, rows: int, heads: int):

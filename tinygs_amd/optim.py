@@ -327,16 +327,21 @@ class GradientClip:
     def clip(self, max_norm: float, scale: float = 1.0, epsilon: float = 1e-6, stream=None):
         """One run. Returns the norm (scale included, before clipping), a float32 scalar on the device that the next
         run overwrites. max_norm infinite: the norm alone, and scale where it is not 1."""
-        import torch
-        first = self.m_grads[0]
-        if first.get_device() != torch.cuda.current_device():
+        from .network import _current_device
+        device = self.m_grads[0].get_device()
+        if device != _current_device():
             raise RuntimeError("GradientClip: the gradients are not on the current device")
         if self._norm is None:
+            import torch
             with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
-                self._norm = torch.empty((), dtype=torch.float32, device=first.device)
-        _lib.check(self._lib.tgs_gradient_clip_run(self._h, float(max_norm), float(scale), float(epsilon),
-                                                   C.c_void_p(self._norm.data_ptr()), stream_ptr(stream)),
-                   "GradientClip::clip")
+                self._norm = torch.empty((), dtype=torch.float32, device=self.m_grads[0].device)
+            # the stream's address without the Stream object around it: 0.1 us a call against 2.8
+            self._current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+                lambda index: torch.cuda.current_stream(index).cuda_stream)
+        rc = self._lib.tgs_gradient_clip_run(self._h, max_norm, scale, epsilon, self._norm.data_ptr(),
+                                             self._current(device) if stream is None else stream.cuda_stream)
+        if rc:
+            _lib.check(rc, "GradientClip::clip")
         return self._norm
 
 
