@@ -266,7 +266,8 @@ class GradientClip:
     g <- g scale min(1, max_norm / (norm + epsilon)). grads are tensors of any shapes and of float32, float16 or
     bfloat16 each, packed or 2-D with rows further apart; with clipped (tensors of the same shapes) these receive the
     result in their own dtypes and grads stay as they are. The tensors are kept: a run reads what they hold then. Runs
-    are on one stream, or the caller orders them."""
+    are on one stream, or the caller orders them. The first run, and the first after set_grads, place a table on the
+    device and wait for it: capture only later ones, and do not call set_grads while the graph is in use."""
 
     def __init__(self, grads, clipped=None):
         self._lib = _lib.load()
