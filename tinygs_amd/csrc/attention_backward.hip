@@ -733,9 +733,10 @@ void split_tiles(int64_t whole, int64_t tiles, int64_t target, int64_t least, in
 // dq, as the forward: 100 rows of 4 heads of 64 at 4096 states, all three gradients,
 // 24 us in 64 parts and 40 in 128, 16000 of one at 272 47 whole and 65 in parts.
 // dk and dv: two workgroups a compute unit (2 x 8192 rows of 8 heads of 128 at 4096
-// states 1255 us, 3060 in half as many), two tiles a part (132 rows of 2 heads of
-// 16 at 448 states 24 us, 30 with one).
-constexpr int64_t kRowTarget = 256, kRowLeast = 4, kStateTarget = 512, kStateLeast = 2;
+// states 1255 us, 3060 in half as many), 64 rows a part of floats (3000 rows of 2 heads
+// of 64 at 33 states 41 us, 53 with 128) and 128 of halves (132 rows of 2 heads of 16
+// at 448 states 24 us, 30 with 64).
+constexpr int64_t kRowTarget = 256, kRowLeast = 4, kStateTarget = 512, kStateLeast = 64;
 
 // Whether the one-pass kernel takes it: states and heads that it holds, more states than one wave's, and as many
 // rows as pay for its start and its sums' join.
@@ -746,9 +747,13 @@ bool at_once(const AttentionBackward& b) {
            (a.queries + kOnceRows - 1) / kOnceRows * (a.heads / a.kv_heads) * a.batch * a.kv_heads >= 1024;
 }
 
+// Rows of a tile of dk's and dv's: 64 but for wide floats (2e5 rows of 4 heads of 64 floats at 256 states 1539 us,
+// 1555 with 32; 5e5 of 2 heads of 32 at 33 474 and 509).
+constexpr int row_tile_of(int size, int64_t width) { return size == 2 || width <= 64 ? 64 : 32; }
+
 struct Plan {
     bool once;
-    int qb, tile;
+    int qb;
     Grid q, kv;
     int64_t q_workgroups, kv_workgroups;
     int64_t delta_blocks;      // of its kernel, where dq is not asked for
@@ -760,7 +765,7 @@ Plan plan_of(const AttentionBackward& b) {
     Plan p{};
     const bool halves = a.dtype != TGS_DTYPE_FLOAT32;
     const int64_t width = (a.head + 31) / 32 * 32;
-    p.tile = halves ? 64 : 32;
+    const int size = halves ? 2 : 4, state_tile = halves ? 64 : 32, row_tile = row_tile_of(size, width);
     p.q.shared = p.kv.shared = a.heads / a.kv_heads;
     p.q.rows = p.kv.rows = a.queries * p.q.shared;
     p.q.c = p.kv.c = exponent_of(a.scale);
@@ -778,12 +783,12 @@ Plan plan_of(const AttentionBackward& b) {
     p.qb = halves && width <= 64 && p.q.rows > 32 * kWaves ? 2 : 1;
     p.q.blocks = (p.q.rows + 32 * kWaves * p.qb - 1) / (32 * kWaves * p.qb);
     int64_t whole = a.batch * a.kv_heads * p.q.blocks;
-    split_tiles(whole, (a.states + p.tile - 1) / p.tile, kRowTarget, kRowLeast, p.q.splits, p.q.part);
+    split_tiles(whole, (a.states + state_tile - 1) / state_tile, kRowTarget, kRowLeast, p.q.splits, p.q.part);
     p.q_workgroups = whole * p.q.splits;
     p.kv.blocks = (a.states + 32 * kWaves - 1) / (32 * kWaves);
-    p.kv.units = (a.queries + p.tile - 1) / p.tile * p.kv.shared;
+    p.kv.units = (a.queries + row_tile - 1) / row_tile * p.kv.shared;
     whole = a.batch * a.kv_heads * p.kv.blocks;
-    split_tiles(whole, p.kv.units, kStateTarget, kStateLeast, p.kv.splits, p.kv.part);
+    split_tiles(whole, p.kv.units, kStateTarget, (halves ? 2 : 1) * kStateLeast / row_tile, p.kv.splits, p.kv.part);
     p.kv_workgroups = whole * p.kv.splits;
     p.delta_bytes = (sizeof(float) * (size_t)(a.q.rows * a.heads) + 255) / 256 * 256;
     size_t sums = 0;
@@ -830,6 +835,7 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
         using T = decltype(t);
         by_head_width(a.head, [&](auto width) {
             constexpr int D = decltype(width)::value, kTile = sizeof(T) == 2 ? 64 : 32;
+            constexpr int kRowTile = row_tile_of(sizeof(T), D);
             const auto join = [&] {
                 const int64_t n = a.k.rows * a.kv_heads;
                 const unsigned blocks = join_blocks(n * a.head);
@@ -875,8 +881,8 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
             const auto launch = [&](auto what) {
                 constexpr int W = decltype(what)::value;
                 in_launches(p.kv, p.kv_workgroups, [&](unsigned n) {
-                    if (p.kv.splits > 1) grad_kv_kernel<T, D, kTile, true, W><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
-                    else grad_kv_kernel<T, D, kTile, false, W><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
+                    if (p.kv.splits > 1) grad_kv_kernel<T, D, kRowTile, true, W><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
+                    else grad_kv_kernel<T, D, kRowTile, false, W><<<n, 64 * kWaves, 0, s>>>(b, p.kv);
                 });
             };
             if constexpr (kApart<T, D>) {
