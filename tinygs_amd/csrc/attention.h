@@ -35,6 +35,17 @@ struct Square {   // halves: 16 of k a step
         for (int e = 0; e < 8; ++e) v[e] = s[8 * u + e];
         return __builtin_convertvector(v, Frag);
     }
+    // What they were rounded by, rounded; nothing beside an infinity.
+    static __device__ __forceinline__ Frag rest(const f32x16& s, int u, const Frag& whole) {
+        typedef float f32x8 __attribute__((ext_vector_type(8)));
+        f32x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = s[8 * u + e] - (float)whole[e];
+            v[e] = fabsf(x) < INFINITY ? x : 0.0f;
+        }
+        return __builtin_convertvector(v, Frag);
+    }
 };
 template <>
 __device__ __forceinline__ void Square<_Float16>::multiply(const Frag& a, const Frag& b, f32x16& c) {

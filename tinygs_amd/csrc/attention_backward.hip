@@ -113,6 +113,13 @@ __device__ __forceinline__ void leave_largest(const Grid& g, float most, float m
     }
 }
 
+// Whether weights and their gradients are operands in two parts, the second what the first was rounded by: halves of
+// heads up to 32, whose kernels take 10 to 28% longer so (2 x 2e5 rows of 4 heads of 32 halves at 200 states, 2
+// shared, 586 us and 458). Over few columns the sums cancel more than they average the roundings: in one part, heads
+// of 16 are off by 1.6 times what rounding the gradients themselves leaves, heads of 2 by 2.6 and of 64 by 1.4.
+template <class T, int D>
+constexpr bool kTwoParts = sizeof(T) == 2 && D == 32;
+
 // lse in the exponent's unit; +infinity where there is no state: all weights are 0.
 template <class T>
 __device__ __forceinline__ float lse_exponent(float lse) {
@@ -303,7 +310,10 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 || sizeof(T) == 2 ? 2 : 1
                 for (int c = 0; c < kCols; ++c) {
                     const auto f = Tile::across(lk, p * S::kDepth, 32 * c, lane);
 #pragma unroll
-                    for (int n = 0; n < QB; ++n) S::multiply(f, w[n], sums[n][c]);
+                    for (int n = 0; n < QB; ++n) {
+                        S::multiply(f, w[n], sums[n][c]);
+                        if constexpr (kTwoParts<T, D>) S::multiply(f, S::rest(dp[n], p, w[n]), sums[n][c]);
+                    }
                 }
             }
         }
@@ -459,6 +469,14 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
                 if constexpr (WHAT & kGradK) x = S::rounded(dp, p);
 #pragma unroll
                 for (int c = 0; c < kCols; ++c) {
+                    if constexpr (kTwoParts<T, D>) {
+                        const auto fo = Tile::across(lo, p * S::kDepth, 0, lane), fq = Tile::across(lq, p * S::kDepth, 0, lane);
+                        S::multiply(fo, w, gv[0]);
+                        S::multiply(fq, x, gk[0]);
+                        S::multiply(fo, S::rest(s, p, w), gv[0]);
+                        S::multiply(fq, S::rest(dp, p, x), gk[0]);
+                        continue;
+                    }
                     if constexpr (WHAT & kGradV) S::multiply(Tile::across(lo, p * S::kDepth, 32 * c, lane), w, gv[c]);
                     if constexpr (WHAT & kGradK) S::multiply(Tile::across(lq, p * S::kDepth, 32 * c, lane), x, gk[c]);
                 }
@@ -494,7 +512,7 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
         }
 }
 
-// ---- up to 256 states of heads up to 64: all three gradients in one pass over
+// ---- up to 256 states of heads of 24 to 64: all three gradients in one pass over
 // the rows. A workgroup's waves hold 32 states each, with the sums of dk and dv;
 // tiles of 64 rows go by. What a tile's ds is to dq needs all states: it goes to LDS
 // as [state][row], and in the next step, behind that tile's barrier, the waves share the
@@ -738,12 +756,14 @@ void split_tiles(int64_t whole, int64_t tiles, int64_t target, int64_t least, in
 // at 448 states 24 us, 30 with 64).
 constexpr int64_t kRowTarget = 256, kRowLeast = 4, kStateTarget = 512, kStateLeast = 64;
 
-// Whether the one-pass kernel takes it: states and heads that it holds, more states than one wave's, and as many
+// Whether the one-pass kernel takes it: states and heads that it holds, heads that its one part of the weights does for
+// (kTwoParts; of 32 they are off by 1.45 times what rounding leaves, and 1e6 rows of 4 at 256 states take 727 us, 1466 in
+// two parts and two kernels), more states than one wave's, and as many
 // rows as pay for its start and its sums' join.
 bool at_once(const AttentionBackward& b) {
     const Attention& a = b.a;
-    return a.dtype == TGS_DTYPE_BFLOAT16 && b.grad_q.p && (b.grad_k.p || b.grad_v.p) && a.head <= 64 && a.head % 8 == 0 &&
-           a.states > 32 && a.states <= kOnceStates && a.batch * a.kv_heads <= 1 << 21 &&
+    return a.dtype == TGS_DTYPE_BFLOAT16 && b.grad_q.p && (b.grad_k.p || b.grad_v.p) && a.head > 16 &&
+           a.head <= 64 && a.head % 8 == 0 && a.states > 32 && a.states <= kOnceStates && a.batch * a.kv_heads <= 1 << 21 &&
            (a.queries + kOnceRows - 1) / kOnceRows * (a.heads / a.kv_heads) * a.batch * a.kv_heads >= 1024;
 }
 
