@@ -15,7 +15,8 @@
 //
 // Halves: p is held times 2^10, and ds times a power of two that brings the
 // largest it can be, |do| |v| + |delta|, to 2^14: of a row's and all states' in
-// dq, of a state's and all rows' in dk, so that small ones keep their bits.
+// dq, of a state's and all rows' of its element and head in dk, so that small ones
+// keep their bits, and no element's or head's gradients depend on another's.
 #include <math.h>
 
 #include <algorithm>
@@ -37,17 +38,17 @@ constexpr float kBoost<_Float16> = 10.0f;
 
 struct Grid {
     int64_t first;    // number of the launch's first workgroup
-    int64_t blocks;   // of rows (of states), for each batch element and head of the states
-    int64_t rows;     // queries x shared heads
+    int64_t blocks;   // of rows (of states), for each pair: a batch element and a head of the states
+    int64_t rows;     // of a pair: queries x shared heads
     int64_t units;    // dk, dv: tiles of rows, of all shared heads
     int shared;
     int splits;
     int64_t part;     // tiles of a split
     float c;          // scale log2(e)
     float* delta;     // [row][head]
-    float* norms;     // halves: of each 64 states' values; then the pairs of the workgroups' largest |do| and |delta|
-    int64_t lifts;    // how many of the latter
-    float* largest;
+    float* norms;     // halves: of each 64 states' values
+    float* largest;   // halves: [pair][lifts][2], the largest |do| and |delta| of parts of a pair's rows
+    int64_t lifts;
     float* sums;      // the splits' parts
 };
 
@@ -58,10 +59,11 @@ __device__ __forceinline__ int lift_of(float largest) {
     return largest > 0.0f && largest < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(largest) : 0;
 }
 
-// The largest of n numbers, for all lanes of the workgroup's waves.
-__device__ __forceinline__ float largest_of(const float* p, int64_t n, int64_t step) {
+// The largest of n numbers, for all lanes of a wave.
+__device__ __forceinline__ float largest_of(const float* p, int64_t n) {
     float v = 0.0f;
-    for (int64_t k = threadIdx.x & 63; k < n; k += 64) v = fmaxf(v, p[k * step]);
+#pragma unroll 4
+    for (int64_t k = threadIdx.x & 63; k < n; k += 64) v = fmaxf(v, p[k]);
     for (int k = 32; k > 0; k >>= 1) v = fmaxf(v, __shfl_xor(v, k, 64));
     return v;
 }
@@ -91,26 +93,45 @@ __global__ void __launch_bounds__(256) norms_kernel(Attention a, float* norms) {
     }
 }
 
-// The workgroup's largest |do|^2 and |delta| to its place, as |do| and |delta|.
-__device__ __forceinline__ void leave_largest(const Grid& g, float most, float most_delta) {
-    __shared__ float s[2][4];
+// The largest of each of two numbers over the workgroup's threads.
+__device__ __forceinline__ void workgroup_largest(float& x, float& y) {
+    __shared__ float s[2][kWaves];
     for (int k = 32; k > 0; k >>= 1) {
-        most = fmaxf(most, __shfl_xor(most, k, 64));
-        most_delta = fmaxf(most_delta, __shfl_xor(most_delta, k, 64));
+        x = fmaxf(x, __shfl_xor(x, k, 64));
+        y = fmaxf(y, __shfl_xor(y, k, 64));
     }
     if ((threadIdx.x & 63) == 0) {
-        s[0][threadIdx.x >> 6] = most;
-        s[1][threadIdx.x >> 6] = most_delta;
+        s[0][threadIdx.x >> 6] = x;
+        s[1][threadIdx.x >> 6] = y;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 4; ++k) {
-            most = fmaxf(most, s[0][k]);
-            most_delta = fmaxf(most_delta, s[1][k]);
-        }
-        g.largest[2 * (g.first + blockIdx.x)] = sqrtf(most);
-        g.largest[2 * (g.first + blockIdx.x) + 1] = most_delta;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+        x = fmaxf(x, s[0][k]);
+        y = fmaxf(y, s[1][k]);
     }
+}
+
+// A workgroup's largest |do|^2 and |delta| to place n of its pair, as |do| and |delta|.
+__device__ __forceinline__ void leave_largest(const Grid& g, int64_t pair, int64_t n, float most, float most_delta) {
+    workgroup_largest(most, most_delta);
+    if (threadIdx.x != 0) return;
+    float* const to = g.largest + 2 * (pair * g.lifts + n);
+    to[0] = sqrtf(most);
+    to[1] = most_delta;
+}
+// The largest of those of a pair's rows, for all threads of the workgroup.
+__device__ __forceinline__ void find_largest(const Grid& g, int64_t pair, float& most, float& most_delta) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2* const from = (const f32x2*)(g.largest + 2 * pair * g.lifts);
+    most = most_delta = 0.0f;
+#pragma unroll 4
+    for (int64_t k = threadIdx.x; k < g.lifts; k += 64 * kWaves) {
+        const f32x2 x = from[k];
+        most = fmaxf(most, x[0]);
+        most_delta = fmaxf(most_delta, x[1]);
+    }
+    workgroup_largest(most, most_delta);
 }
 
 // Whether weights and their gradients are operands in two parts, the second what the first was rounded by: halves of
@@ -126,19 +147,21 @@ __device__ __forceinline__ float lse_exponent(float lse) {
     return lse == -INFINITY ? INFINITY : lse * kLog2E;
 }
 
-// delta where dq is not asked for, with the same bits: a wave for 32 rows of a head.
+// delta where dq is not asked for, with the same bits: a workgroup for g.part times 128 rows of a pair.
 template <class T, int D>
-__global__ void __launch_bounds__(256) delta_kernel(AttentionBackward b, Grid g) {
+__global__ void __launch_bounds__(64 * kWaves) delta_kernel(AttentionBackward b, Grid g) {
     using S = Square<T>;
     constexpr int kSteps = D / S::kDepth;
     const Attention& a = b.a;
-    const int lane = threadIdx.x & 63;
-    const int64_t blocks = (a.q.rows + 31) / 32, n = blocks * a.heads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t number = g.first + blockIdx.x, pair = number / g.blocks, block = number % g.blocks;
+    const int64_t e = pair / a.kv_heads;
+    const int kv = (int)(pair % a.kv_heads);
     float most = 0.0f, most_delta = 0.0f;
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
-        const int h = (int)(i % a.heads);
+    const int64_t last = min((block + 1) * g.part * kWaves, (g.rows + 31) / 32);
+    for (int64_t i = block * g.part * kWaves + wave; i < last; i += kWaves) {
         LaneRows<1> rows;
-        rows.begin(0, i / a.heads * 32, a.q.rows, h, 1, lane);
+        rows.begin(e * a.queries, i * 32, g.rows, kv * g.shared, g.shared, lane);
         typename S::Frag go[1][kSteps], o[1][kSteps];
         rows.template load<T, kSteps>(b.grad_out, a.head, lane, go);
         rows.template load<T, kSteps>(a.out, a.head, lane, o);
@@ -159,9 +182,9 @@ __global__ void __launch_bounds__(256) delta_kernel(AttentionBackward b, Grid g)
         swap32(square, other);
         most = fmaxf(most, square + other);
         most_delta = fmaxf(most_delta, fabsf(dot));
-        if (rows.exists[0] && lane < 32) g.delta[rows.row(0) * a.heads + h] = dot;
+        if (rows.exists[0] && lane < 32) g.delta[rows.row(0) * a.heads + rows.head[0]] = dot;
     }
-    if constexpr (kBoost<T> != 0.0f) leave_largest(g, most, most_delta);
+    if constexpr (kBoost<T> != 0.0f) leave_largest(g, pair, block, most, most_delta);
 }
 
 template <class T, int D, int QB, int KT, bool SPLIT>
@@ -191,7 +214,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 || sizeof(T) == 2 ? 2 : 1
         float norm = 0.0f, most = 0.0f, most_delta = 0.0f;
         if constexpr (kBoost<T> != 0.0f) {
             const int64_t blocks = (a.states + 63) / 64;
-            norm = largest_of(g.norms + pair * blocks, blocks, 1);
+            norm = largest_of(g.norms + pair * blocks, blocks);
         }
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
@@ -224,7 +247,8 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 || sizeof(T) == 2 ? 2 : 1
                 if (lane < 32 && split == 0) g.delta[rows.row(n) * a.heads + rows.head[n]] = delta[n];
             }
         }
-        if constexpr (kBoost<T> != 0.0f) leave_largest(g, most, most_delta);
+        if constexpr (kBoost<T> != 0.0f)
+            if (split == 0) leave_largest(g, pair, block, most, most_delta);
     }
 
     Tile tk, tv;
@@ -372,9 +396,9 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
     states.template load<T, kSteps>(a.k, d, lane, k);
     states.template load<T, kSteps>(a.v, d, lane, v);
     int lift = 0;
-    if constexpr (kBoost<T> != 0.0f) {
-        const float most = largest_of(g.largest, g.lifts, 2), most_delta = largest_of(g.largest + 1, g.lifts, 2);
-        float square = 0.0f;
+    if constexpr (kBoost<T> != 0.0f && (WHAT & kGradK)) {
+        float most, most_delta, square = 0.0f;
+        find_largest(g, pair, most, most_delta);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s)
 #pragma unroll
@@ -774,9 +798,8 @@ constexpr int row_tile_of(int size, int64_t width) { return size == 2 || width <
 struct Plan {
     bool once;
     int qb;
-    Grid q, kv;
-    int64_t q_workgroups, kv_workgroups;
-    int64_t delta_blocks;      // of its kernel, where dq is not asked for
+    Grid q, kv, delta;         // delta: its kernel's, where dq is not asked for
+    int64_t q_workgroups, kv_workgroups, delta_workgroups;
     size_t delta_bytes, norms_bytes, largest_bytes, bytes;
 };
 
@@ -786,8 +809,8 @@ Plan plan_of(const AttentionBackward& b) {
     const bool halves = a.dtype != TGS_DTYPE_FLOAT32;
     const int64_t width = (a.head + 31) / 32 * 32;
     const int size = halves ? 2 : 4, state_tile = halves ? 64 : 32, row_tile = row_tile_of(size, width);
-    p.q.shared = p.kv.shared = a.heads / a.kv_heads;
-    p.q.rows = p.kv.rows = a.queries * p.q.shared;
+    p.q.shared = p.kv.shared = p.delta.shared = a.heads / a.kv_heads;
+    p.q.rows = p.kv.rows = p.delta.rows = a.queries * p.q.shared;
     p.q.c = p.kv.c = exponent_of(a.scale);
     p.once = at_once(b);
     if (p.once) {
@@ -815,11 +838,16 @@ Plan plan_of(const AttentionBackward& b) {
     if (b.grad_q.p && p.q.splits > 1) sums = sizeof(float) * (size_t)(p.q.splits * a.q.rows * a.heads * width);
     if ((b.grad_k.p || b.grad_v.p) && p.kv.splits > 1)
         sums = std::max(sums, sizeof(float) * 2 * (size_t)(p.kv.splits * a.k.rows * a.kv_heads * width));
-    p.delta_blocks = std::min<int64_t>(((a.q.rows + 31) / 32 * a.heads + 3) / 4, 4096);
+    // the delta kernel: up to 4096 workgroups, one a pair at least
+    const int64_t pairs = a.batch * a.kv_heads, row_blocks = (p.delta.rows + 32 * kWaves - 1) / (32 * kWaves);
+    const int64_t most = std::max<int64_t>(4096 / pairs, 1);
+    p.delta.part = row_blocks > 0 ? (row_blocks + most - 1) / most : 1;
+    p.delta.blocks = (row_blocks + p.delta.part - 1) / p.delta.part;
+    p.delta_workgroups = pairs * p.delta.blocks;
     if (a.dtype == TGS_DTYPE_FLOAT16) {
-        p.kv.lifts = b.grad_q.p ? p.q_workgroups : p.delta_blocks;
-        p.norms_bytes = (sizeof(float) * (size_t)(a.batch * a.kv_heads * ((a.states + 63) / 64)) + 255) / 256 * 256;
-        p.largest_bytes = (sizeof(float) * 2 * (size_t)p.kv.lifts + 255) / 256 * 256;
+        p.q.lifts = p.delta.lifts = p.kv.lifts = b.grad_q.p ? p.q.blocks : p.delta.blocks;
+        p.norms_bytes = (sizeof(float) * (size_t)(pairs * ((a.states + 63) / 64)) + 255) / 256 * 256;
+        p.largest_bytes = (sizeof(float) * 2 * (size_t)(pairs * p.kv.lifts) + 255) / 256 * 256;
     }
     p.bytes = p.delta_bytes + p.norms_bytes + p.largest_bytes + sums;
     return p;
@@ -845,10 +873,10 @@ size_t attention_backward_workspace(const AttentionBackward& b) { return plan_of
 int launch_attention_backward(const AttentionBackward& b, void* workspace, hipStream_t s) {
     const Attention& a = b.a;
     Plan p = plan_of(b);
-    p.q.delta = p.kv.delta = (float*)workspace;
+    p.q.delta = p.kv.delta = p.delta.delta = (float*)workspace;
     unsigned char* at = (unsigned char*)workspace + p.delta_bytes;
     p.q.norms = p.kv.norms = (float*)at;
-    p.q.largest = p.kv.largest = (float*)(at += p.norms_bytes);
+    p.q.largest = p.kv.largest = p.delta.largest = (float*)(at += p.norms_bytes);
     p.q.sums = p.kv.sums = (float*)(at += p.largest_bytes);
     const bool states = (b.grad_k.p || b.grad_v.p) && a.k.rows > 0;
     by_dtype(a.dtype, [&](auto t) {
@@ -894,8 +922,8 @@ int launch_attention_backward(const AttentionBackward& b, void* workspace, hipSt
                     join_kernel<T, D><<<join_blocks(a.q.rows * a.heads * a.head), 256, 0, s>>>(
                         p.q.sums, p.q.splits, a.q.rows * a.heads, b.grad_q, a.heads, a.head);
             } else if (a.q.rows && states) {
-                p.kv.first = 0;
-                delta_kernel<T, D><<<(unsigned)p.delta_blocks, 256, 0, s>>>(b, p.kv);
+                in_launches(p.delta, p.delta_workgroups,
+                            [&](unsigned n) { delta_kernel<T, D><<<n, 64 * kWaves, 0, s>>>(b, p.delta); });
             }
             if (!states) return;
             const auto launch = [&](auto what) {
