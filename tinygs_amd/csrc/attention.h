@@ -147,6 +147,36 @@ struct RowTile {
         }
     }
 
+    // The same of the first `rows` rows (1 or more), the others copies of the last: where zeros would be NaN beside an
+    // infinity of the other operand, a copy only is what that row is. pitch: as in begin. WHOLE: heads of whole chunks.
+    template <bool WHOLE>
+    __device__ __forceinline__ void load_first(unsigned char* lds, const unsigned char* base, int64_t end, int64_t rows,
+                                               int64_t pitch, int d, int wave, int lane) const {
+        const i32x4 buffer = buffer_of(base, end);
+        const uint32_t to = lds_address(lds);
+        if (rows >= ROWS && (WHOLE || d % V == 0)) {
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n) load_to_lds(to + (n * WAVES + wave) * 1024, offset[n], buffer);
+            return;
+        }
+        const int last = (int)min(rows, (int64_t)ROWS) - 1;
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const int slot = (n * WAVES + wave) * 64 + lane;
+            const int r = slot / kChunks, c = (slot % kChunks) ^ turn(r);
+            const int some = d - c * V;
+            const uint32_t at = offset[n] - (uint32_t)(max(r - last, 0) * (uint32_t)pitch);
+            if (WHOLE || some >= V || some <= 0) {
+                load_to_lds(to + (n * WAVES + wave) * 1024, some > 0 ? at : kPastEnd, buffer);
+            } else {
+                const T* p = (const T*)(base + at);
+                T* q = (T*)(lds + slot * 16);
+#pragma unroll
+                for (int e = 0; e < V; ++e) q[e] = e < some ? p[e] : (T)0.0f;
+            }
+        }
+    }
+
     // Operand of 32 rows along step s of their columns. lds: the first row, a multiple of 32.
     static __device__ __forceinline__ typename S::Frag along(const unsigned char* lds, int s, int lane) {
         const int r = lane & 31;

@@ -433,12 +433,13 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
             ++h;
         }
         const int64_t r0 = in * QT, left = a.queries - r0;
-        const uint64_t exist = left >= 64 ? ~0ull : (1ull << left) - 1;
-        const uint64_t bits = QT == 64 ? exist : exist & ((1ull << (QT & 63)) - 1);
         const int64_t at = (int64_t)h * d * (int64_t)sizeof(T);
         const int64_t width = d * (int64_t)sizeof(T);
-        tq.load(lds[buffer][0], q0 + at + r0 * q_pitch, (left - 1) * q_pitch + width, bits, d, wave, lane);
-        to.load(lds[buffer][1], o0 + at + r0 * o_pitch, (left - 1) * o_pitch + width, bits, d, wave, lane);
+        // rows past the last are copies of it with an lse of +infinity: their weights are 0
+        tq.template load_first<false>(lds[buffer][0], q0 + at + r0 * q_pitch, (left - 1) * q_pitch + width, left, q_pitch,
+                                      d, wave, lane);
+        to.template load_first<false>(lds[buffer][1], o0 + at + r0 * o_pitch, (left - 1) * o_pitch + width, left, o_pitch,
+                                      d, wave, lane);
         const int64_t row = e * a.queries + r0 + of;
         const int head = kv * g.shared + h;
         if (threadIdx.x < QT)
@@ -616,14 +617,13 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
             ++h;
         }
         const int64_t r0 = in * kOnceRows, left = a.queries - r0;
-        const uint64_t bits = left >= 64 ? ~0ull : (1ull << left) - 1;
         const int head = kv * g.shared + h;
         const int64_t at = (int64_t)head * d * (int64_t)sizeof(T), width = d * (int64_t)sizeof(T);
-        if (wave < kLoaders) {
-            tq.load(lds[buffer][0], (const unsigned char*)a.q.p + at + (first_row + r0) * q_pitch,
-                    (left - 1) * q_pitch + width, bits, d, wave, lane);
-            to.load(lds[buffer][1], (const unsigned char*)b.grad_out.p + at + (first_row + r0) * o_pitch,
-                    (left - 1) * o_pitch + width, bits, d, wave, lane);
+        if (wave < kLoaders) {   // rows past the last: as in grad_kv_kernel
+            tq.template load_first<true>(lds[buffer][0], (const unsigned char*)a.q.p + at + (first_row + r0) * q_pitch,
+                                         (left - 1) * q_pitch + width, left, q_pitch, d, wave, lane);
+            to.template load_first<true>(lds[buffer][1], (const unsigned char*)b.grad_out.p + at + (first_row + r0) * o_pitch,
+                                         (left - 1) * o_pitch + width, left, o_pitch, d, wave, lane);
         }
         // without branches, which would wait for the loads where they meet
         const int64_t x_pitch = a.out.stride * (int64_t)sizeof(T);
