@@ -35,14 +35,15 @@ struct Square {   // halves: 16 of k a step
         for (int e = 0; e < 8; ++e) v[e] = s[8 * u + e];
         return __builtin_convertvector(v, Frag);
     }
-    // What they were rounded by, rounded; nothing beside an infinity.
+    // What they were rounded by, rounded. INFINITE: there may be infinities, beside which it is nothing.
+    template <bool INFINITE>
     static __device__ __forceinline__ Frag rest(const f32x16& s, int u, const Frag& whole) {
         typedef float f32x8 __attribute__((ext_vector_type(8)));
         f32x8 v;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float x = s[8 * u + e] - (float)whole[e];
-            v[e] = fabsf(x) < INFINITY ? x : 0.0f;
+            v[e] = !INFINITE || fabsf(x) < INFINITY ? x : 0.0f;
         }
         return __builtin_convertvector(v, Frag);
     }

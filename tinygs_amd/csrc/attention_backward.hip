@@ -134,10 +134,14 @@ __device__ __forceinline__ void find_largest(const Grid& g, int64_t pair, float&
     workgroup_largest(most, most_delta);
 }
 
-// Whether weights and their gradients are operands in two parts, the second what the first was rounded by: halves of
-// heads up to 32, whose kernels take 10 to 28% longer so (2 x 2e5 rows of 4 heads of 32 halves at 200 states, 2
-// shared, 586 us and 458). Over few columns the sums cancel more than they average the roundings: in one part, heads
-// of 16 are off by 1.6 times what rounding the gradients themselves leaves, heads of 2 by 2.6 and of 64 by 1.4.
+// Whether weights and their gradients are operands in two parts, the second what the first was rounded by: 16-bit heads
+// up to 32, in every kernel, so that the precision does not depend on the number of rows. Over few columns the sums cancel
+// more than they average the roundings: in one part, heads of 16 are off by 1.6 times what rounding the gradients
+// themselves leaves, heads of 2 by 2.6, of 32 by 1.47; in two parts by no more than 1.01. 2 x 2e5 rows of 4 heads of 32
+// halves at 200 states, 2 shared, take 505 us so and 409 in one part; 1e6 of 4 bfloat16 at 256 states in one pass 968 and
+// 595. Wider heads are held in one part, off by 1.37 to 1.47 times: in two, 2 x 8192 rows of 8 heads of 128 halves at 4096
+// states would take 1315 us, 1080 in one, and 1e6 x 4 x 64 bfloat16 at 256 1750 (in two kernels: both parts of the
+// weights do not fit beside the tiles in LDS) and 950.
 template <class T, int D>
 constexpr bool kTwoParts = sizeof(T) == 2 && D == 32;
 
@@ -336,7 +340,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 || sizeof(T) == 2 ? 2 : 1
 #pragma unroll
                     for (int n = 0; n < QB; ++n) {
                         S::multiply(f, w[n], sums[n][c]);
-                        if constexpr (kTwoParts<T, D>) S::multiply(f, S::rest(dp[n], p, w[n]), sums[n][c]);
+                        if constexpr (kTwoParts<T, D>) S::multiply(f, S::template rest<true>(dp[n], p, w[n]), sums[n][c]);
                     }
                 }
             }
@@ -498,8 +502,8 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
                         const auto fo = Tile::across(lo, p * S::kDepth, 0, lane), fq = Tile::across(lq, p * S::kDepth, 0, lane);
                         S::multiply(fo, w, gv[0]);
                         S::multiply(fq, x, gk[0]);
-                        S::multiply(fo, S::rest(s, p, w), gv[0]);
-                        S::multiply(fq, S::rest(dp, p, x), gk[0]);
+                        S::multiply(fo, S::template rest<false>(s, p, w), gv[0]);
+                        S::multiply(fq, S::template rest<true>(dp, p, x), gk[0]);
                         continue;
                     }
                     if constexpr (WHAT & kGradV) S::multiply(Tile::across(lo, p * S::kDepth, 32 * c, lane), w, gv[c]);
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
         }
 }
 
-// ---- up to 256 states of heads of 24 to 64: all three gradients in one pass over
+// ---- up to 256 states of heads up to 64: all three gradients in one pass over
 // the rows. A workgroup's waves hold 32 states each, with the sums of dk and dv;
 // tiles of 64 rows go by. What a tile's ds is to dq needs all states: it goes to LDS
 // as [state][row], and in the next step, behind that tile's barrier, the waves share the
@@ -558,7 +562,8 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
     constexpr int kSteps = D / 16, kCols = D / 32;
     constexpr int kAcross = D / 16, kDown = 4 * kAcross / kOnceWaves;   // 16 x 16 squares of dq across; a wave's
     constexpr int kChunks = D / 8;                                      // of a row's head
-    __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes], weights[2][Weights::kBytes];
+    constexpr int kWeightParts = kTwoParts<T, D> ? 2 : 1;
+    __shared__ __align__(1024) unsigned char lds[2][2][Tile::kBytes], weights[2][kWeightParts][Weights::kBytes];
     __shared__ __align__(16) float row_lse[2][kOnceRows], row_delta[2][kOnceRows];
     const Attention& a = b.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -583,8 +588,8 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
     typename S::Frag kt[kOnceStates / 32];
     {
         using Keys = RowTile<T, D, kOnceStates, kOnceWaves>;
-        static_assert(Keys::kBytes <= 2 * Weights::kBytes, "");
-        unsigned char* const at = weights[0];
+        static_assert(Keys::kBytes <= (int)sizeof(weights), "");
+        unsigned char* const at = weights[0][0];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {   // the lane's row, as it would be loaded
             const int r = (int)j, c = (2 * s + (lane >> 5)) ^ Keys::turn(r);
@@ -642,14 +647,16 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
         return true;
     };
     // dq of the tile whose ds stands in `from`: rows r0 .. of the head
-    const auto add_rows = [&](const unsigned char* from, int head, int64_t r0, bool there) {
+    const auto add_rows = [&](const unsigned char (*from)[Weights::kBytes], int head, int64_t r0, bool there) {
         const int64_t left = there ? a.queries - r0 : 0;
 #pragma unroll
         for (int n = 0; n < kDown; ++n) {
             f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < kOnceStates / 32; ++s)
-                x = multiply(kt[s], Weights::across16(from, 32 * s, 16 * (down + n), lane), x);
+#pragma unroll
+                for (int part = 0; part < kWeightParts; ++part)
+                    x = multiply(kt[s], Weights::across16(from[part], 32 * s, 16 * (down + n), lane), x);
             const int row = 16 * (down + n) + (lane & 15), c0 = 16 * across + 4 * (lane >> 4);
             if (row < left && c0 < d) {   // d is a multiple of 8
                 typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -685,7 +692,7 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
         more = load(buffer ^ 1);
         // the two waves of a SIMD in opposite order: one's products beside the other's exponentials
         if (wave < kOnceWaves / 2) add_rows(weights[buffer ^ 1], last_head, last_row, begun);
-        unsigned char* const to_weights = weights[buffer] + (int)j * Weights::kRowBytes;
+        unsigned char* const to_weights = weights[buffer][0] + (int)j * Weights::kRowBytes;
 #pragma unroll
         for (int u = 0; u < kOnceRows / 32; ++u) {
             const unsigned char *lq = lds[buffer][0] + 32 * u * Tile::kRowBytes, *lo = lq + Tile::kBytes;
@@ -708,17 +715,30 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const auto w = S::rounded(s, p), x = S::rounded(dp, p);
-                typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-                const u32x4 bits = __builtin_bit_cast(u32x4, x) & keep;   // zeros for a state that does not exist
+                const auto leave = [&](const typename S::Frag& f, unsigned char* to) {
+                    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                    const u32x4 bits = __builtin_bit_cast(u32x4, f) & keep;   // zeros for a state that does not exist
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {   // rows 32 u + 16 p + 8 n + 4 (lane / 32) .. + 3
-                    const int c = (4 * u + 2 * p + n) ^ Weights::turn((int)j);
-                    *(u32x2*)(to_weights + (c << 4) + 8 * (lane >> 5)) = u32x2{bits[2 * n], bits[2 * n + 1]};
-                }
+                    for (int n = 0; n < 2; ++n) {   // rows 32 u + 16 p + 8 n + 4 (lane / 32) .. + 3
+                        const int c = (4 * u + 2 * p + n) ^ Weights::turn((int)j);
+                        *(u32x2*)(to + (c << 4) + 8 * (lane >> 5)) = u32x2{bits[2 * n], bits[2 * n + 1]};
+                    }
+                };
+                leave(x, to_weights);
+                if constexpr (kTwoParts<T, D>) {
+                    const auto fo = Tile::across(lo, p * 16, 0, lane), fq = Tile::across(lq, p * 16, 0, lane);
+                    const auto rest = S::template rest<true>(dp, p, x);
+                    leave(rest, to_weights + Weights::kBytes);
+                    S::multiply(fo, w, gv[0]);
+                    S::multiply(fq, x, gk[0]);
+                    S::multiply(fo, S::template rest<false>(s, p, w), gv[0]);
+                    S::multiply(fq, rest, gk[0]);
+                } else {
 #pragma unroll
-                for (int c = 0; c < kCols; ++c) {
-                    S::multiply(Tile::across(lo, p * 16, 32 * c, lane), w, gv[c]);
-                    S::multiply(Tile::across(lq, p * 16, 32 * c, lane), x, gk[c]);
+                    for (int c = 0; c < kCols; ++c) {
+                        S::multiply(Tile::across(lo, p * 16, 32 * c, lane), w, gv[c]);
+                        S::multiply(Tile::across(lq, p * 16, 32 * c, lane), x, gk[c]);
+                    }
                 }
             }
         }
@@ -780,14 +800,13 @@ void split_tiles(int64_t whole, int64_t tiles, int64_t target, int64_t least, in
 // at 448 states 24 us, 30 with 64).
 constexpr int64_t kRowTarget = 256, kRowLeast = 4, kStateTarget = 512, kStateLeast = 64;
 
-// Whether the one-pass kernel takes it: states and heads that it holds, heads that its one part of the weights does for
-// (kTwoParts; of 32 they are off by 1.45 times what rounding leaves, and 1e6 rows of 4 at 256 states take 727 us, 1466 in
-// two parts and two kernels), more states than one wave's, and as many
-// rows as pay for its start and its sums' join.
+// Whether the one-pass kernel takes it: states and heads that it holds, more states than one wave's, and as many rows as
+// pay for its start and its sums' join. 1e6 rows of 4 heads at 256 states, in one pass and in two kernels: of 8 913 us and
+// 1153, of 16 952 and 1227, of 32 968 and 1279, of 64 950 and 1356.
 bool at_once(const AttentionBackward& b) {
     const Attention& a = b.a;
-    return a.dtype == TGS_DTYPE_BFLOAT16 && b.grad_q.p && (b.grad_k.p || b.grad_v.p) && a.head > 16 &&
-           a.head <= 64 && a.head % 8 == 0 && a.states > 32 && a.states <= kOnceStates && a.batch * a.kv_heads <= 1 << 21 &&
+    return a.dtype == TGS_DTYPE_BFLOAT16 && b.grad_q.p && (b.grad_k.p || b.grad_v.p) && a.head <= 64 &&
+           a.head % 8 == 0 && a.states > 32 && a.states <= kOnceStates && a.batch * a.kv_heads <= 1 << 21 &&
            (a.queries + kOnceRows - 1) / kOnceRows * (a.heads / a.kv_heads) * a.batch * a.kv_heads >= 1024;
 }
 
