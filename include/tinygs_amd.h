@@ -567,7 +567,9 @@ typedef struct tgs_attention {
  * [batch x states, kv_heads d], out like q; lse may be NULL: that of row r and
  * head h is at lse[r lse_row_step + h lse_head_step], in rows of heads (steps of
  * at least heads lse_head_step and 1 or more) or heads of rows. Weights of 16-bit matrices are rounded to their dtype ahead of the
- * product with v; their sum is not. No output may overlap an input. */
+ * product with v; their sum is not. Averages of values below 2^95 are finite;
+ * float32 and bfloat16 values above may leave the range of floats on the way.
+ * No output may overlap an input. */
 int tgs_attention_forward(tgs_network* n, const tgs_matrix* q, const tgs_matrix* k, const tgs_matrix* v,
                           const tgs_attention* a, const tgs_matrix* out, float* lse, int64_t lse_row_step,
                           int64_t lse_head_step, void* stream);

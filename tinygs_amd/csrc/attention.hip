@@ -7,9 +7,10 @@
 // exchange between the halves of the wave, and the weights p^T are the second
 // product's operand as they stand. The maximum m is that of a row's first 32
 // states: later scores may pass it by what the weights' type holds, and the sum of
-// the weights tells if they did. Then the wave looks for the maxima of all states and
-// adds them once more. A running maximum takes a tenth more of the vector
-// instructions, and a scaling of the sums on the way, even one that is never reached,
+// the weights tells if they did (halves: the sum of weights times v, which an infinite
+// weight leaves infinite or NaN). Then the wave looks for the maxima of all states and
+// adds them once more where a row's is too far above. A running maximum takes a tenth
+// more of the vector instructions, and a scaling of the sums on the way, even one that is never reached,
 // made the compiler copy them all at every step.
 //
 // 2 x 8192 rows of 8 heads of 128 halves, 2 shared, at 4096 states: 252 to 283 us by
@@ -21,6 +22,8 @@
 // states and their sums are joined by a second kernel.
 #include <math.h>
 
+#include <type_traits>
+
 #include "attention.h"
 #include "row_chunks.h"
 
@@ -30,14 +33,19 @@ namespace {
 
 constexpr float kLn2 = 0.69314718055994531f;
 
-// The sum of a lane's weights up to which none of them can have left its type's
-// range (2^16 for halves), nor their products with values below 2^87 that of floats.
-// Below it a half keeps its bits down to 2^-14 of the first states' largest weight, and is
-// off by at most 2^-25 of that below: with 4096 such states by 2^-13 of the values.
-template <class T>
-constexpr float kMostSum = 0x1p40f;
-template <>
-constexpr float kMostSum<_Float16> = 0x1p15f;
+// The sum of a lane's weights up to which floats and bfloat16 stay relative to the first states' maximum: sums of
+// their products with values below 2^95 are finite then, of 256 parts of the states as well.
+constexpr float kMostSum = 0x1p24f;
+
+// A half keeps its bits down to 2^-14 of what is held as 1, and is off by at most 2^-25 of that below: with 4096 such
+// states by 2^-13 of the values. For more states halves' weights are held times 2^L, with L = log2(states) - 12
+// rounded up, at most 12, so that the bound stays up to 2^24 states; what later scores may be above the first ones (16
+// - L powers of two) shrinks by as much.
+inline int lift_of(int64_t states) {
+    int lift = 0;
+    while (lift < 12 && states > (int64_t)4096 << lift) ++lift;
+    return lift;
+}
 
 struct Grid {
     int64_t first;       // number of the launch's first workgroup
@@ -48,6 +56,7 @@ struct Grid {
     int tiles;           // of a split
     int64_t part;        // held states: blocks of a wave's rows for each workgroup
     float c;             // scale log2(e)
+    float lift;          // halves: L / c, what the maximum is held below its value by
     float* sums;         // of a split's parts: [splits][all rows][D], then m and l
     float* tops;
 };
@@ -56,6 +65,7 @@ struct Grid {
 template <class T, int D, int QB>
 struct WaveRows {
     using S = Square<T>;
+    static constexpr bool kHalves = std::is_same_v<T, _Float16>;
     static constexpr int kSteps = D / S::kDepth;    // of the scores' product
     static constexpr int kParts = 32 / S::kDepth;   // of a square's rows as an operand
     static constexpr int kCols = D / 32;
@@ -63,7 +73,8 @@ struct WaveRows {
     typename S::Frag q[QB][kSteps];
     f32x16 out[QB][kCols];   // sums of weights times v
     float top[QB], sum[QB];  // the maximum that the weights are relative to; of the weights
-    bool low[QB];            // the maximum is to be raised
+    float high[QB];          // the maximum of all states, where it is looked for
+    bool low[QB];            // the maximum may have to be raised
 
     // Rows from number i0 on of batch element b and head kv of the states.
     __device__ __forceinline__ void begin(const Attention& a, const Grid& g, int64_t b, int kv, int64_t i0, int lane) {
@@ -106,10 +117,8 @@ struct WaveRows {
         }
     }
 
-    // Raises the maxima, or only those that do not do, to those of the scores. A NaN
-    // goes into the weights instead.
-    template <bool ALL>
-    __device__ __forceinline__ void raise(const f32x16 (&s)[QB]) {
+    // Raises maxima to those of the scores. A NaN goes into the weights instead.
+    static __device__ __forceinline__ void raise(const f32x16 (&s)[QB], float (&to)[QB]) {
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
             float m = s[n][0];
@@ -117,14 +126,15 @@ struct WaveRows {
             for (int r = 1; r < 16; ++r) m = fmaxf(m, s[n][r]);
             float other = m;
             swap32(m, other);
-            if (ALL || low[n]) top[n] = fmaxf(fmaxf(m, other), top[n]);
+            to[n] = fmaxf(fmaxf(m, other), to[n]);
         }
     }
 
     // Adds 32 states, whose rows start at lk and lv. `first`: the maxima are theirs.
     template <class Tile>
-    __device__ __forceinline__ void add(const unsigned char* lk, const unsigned char* lv, uint32_t bits, bool first, float c,
-                                        int lane) {
+    __device__ __forceinline__ void add(const unsigned char* lk, const unsigned char* lv, uint32_t bits, bool first,
+                                        const Grid& g, int lane) {
+        const float c = g.c;
         f32x16 s[QB];
         typename S::Frag v[kParts][kCols];
         score<Tile>(lk, bits, s, lane);
@@ -133,16 +143,23 @@ struct WaveRows {
         for (int p = 0; p < kParts; ++p)
 #pragma unroll
             for (int k = 0; k < kCols; ++k) v[p][k] = Tile::across(lv, p * S::kDepth, 32 * k, lane);
-        if (first) raise<true>(s);
+        if (first) {
+            raise(s, top);
+            if constexpr (kHalves)
+#pragma unroll
+                for (int n = 0; n < QB; ++n) top[n] -= g.lift;
+        }
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
             const float less = -(top[n] == -INFINITY ? 0.0f : top[n]) * c;
+            float part = 0.0f;   // of the sum: one rounding of the whole for sixteen weights
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 // floats: in two roundings, so that the largest score's weight is 1
                 s[n][r] = __builtin_amdgcn_exp2f(sizeof(T) == 4 ? s[n][r] * c + less : fmaf(s[n][r], c, less));
-                sum[n] += s[n][r];
+                part = r ? part + s[n][r] : s[n][r];
             }
+            sum[n] += part;
         }
 #pragma unroll
         for (int p = 0; p < kParts; ++p)
@@ -154,17 +171,36 @@ struct WaveRows {
             }
     }
 
-    // Whether the maxima of the first states do not do for some row: scores passed it
-    // by more than the weights' range, or its first scores were all -infinity. The other rows keep theirs,
-    // and so their results do not depend on it.
+    // Whether the maxima of the first states may not do for some row: scores passed it
+    // by more than the weights' range, or its first scores were all -infinity.
     __device__ __forceinline__ bool passed() {
         bool any = false;
 #pragma unroll
         for (int n = 0; n < QB; ++n) {
-            float a = sum[n], b = sum[n];
+            float a, b;
+            if constexpr (kHalves) a = b = out[n][0][0] * 0.0f;   // NaN: a weight was infinite, or a value is not finite
+            else a = b = sum[n];
             swap32(a, b);
-            low[n] = a > kMostSum<T> || b > kMostSum<T> || top[n] == -INFINITY;
+            low[n] = (kHalves ? !(a == 0.0f && b == 0.0f) : a > kMostSum || b > kMostSum) || top[n] == -INFINITY;
+            high[n] = -INFINITY;
             any |= low[n];
+        }
+        return ballot(any) != 0;
+    }
+
+    // With the maxima of all states in `high`: raises those that do not do; whether there are any. The other rows keep
+    // theirs, and so their results do not depend on it.
+    __device__ __forceinline__ bool settle(const Grid& g) {
+        bool any = false;
+#pragma unroll
+        for (int n = 0; n < QB; ++n) {
+            bool raised = low[n] && high[n] > top[n];
+            if constexpr (kHalves) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(high[n], g.c, -top[n] * g.c));   // as in add
+                raised = raised && (top[n] == -INFINITY || (float)(T)w == INFINITY);
+            }
+            if (raised) top[n] = high[n] - (kHalves ? g.lift : 0.0f);
+            any |= raised;
         }
         return ballot(any) != 0;
     }
@@ -286,7 +322,7 @@ __global__ void __launch_bounds__(64 * WAVES, (D <= 64 || sizeof(T) == 2 ? 2 : 1
     };
     bool first = true;
     const auto add = [&](const unsigned char* lk, const unsigned char* lv, uint32_t bits) {
-        rows.template add<Tile>(lk, lv, bits, first && bits != 0, g.c, lane);
+        rows.template add<Tile>(lk, lv, bits, first && bits != 0, g, lane);
         first = first && bits == 0;
     };
     rows.clear();
@@ -297,13 +333,14 @@ __global__ void __launch_bounds__(64 * WAVES, (D <= 64 || sizeof(T) == 2 ? 2 : 1
         each([&](const unsigned char* lk, const unsigned char*, uint32_t bits) {
             f32x16 s[QB];
             rows.template score<Tile>(lk, bits, s, lane);
-            rows.template raise<false>(s);
+            rows.raise(s, rows.high);
         });
-        __syncthreads();
-        restart();
-        rows.clear();
-        first = false;
-        each(add);
+        if (__syncthreads_or(rows.settle(g))) {
+            restart();
+            rows.clear();
+            first = false;
+            each(add);
+        }
     }
     if constexpr (SPLIT) rows.store_part(a, g, split, lane);
     else rows.store(a, lane);
@@ -372,13 +409,14 @@ __global__ void __launch_bounds__((64 * kHeldWaves<T, D>)) held_kernel(Attention
             const int u0 = next(-1, bits);
             for (int u = u0; u < squares; u = next(u, bits))
                 rows.template add<Tile>(lk + u * 32 * Tile::kRowBytes, lv + u * 32 * Tile::kRowBytes, bits,
-                                        u == u0 && !again, g.c, lane);
+                                        u == u0 && !again, g, lane);
             if (__builtin_expect(again || !rows.passed(), 1)) break;
             for (int u = next(-1, bits); u < squares; u = next(u, bits)) {
                 f32x16 s[1];
                 rows.template score<Tile>(lk + u * 32 * Tile::kRowBytes, bits, s, lane);
-                rows.template raise<false>(s);
+                rows.raise(s, rows.high);
             }
+            if (!rows.settle(g)) break;
         }
         rows.store(a, lane);
     }
@@ -392,6 +430,7 @@ __global__ void __launch_bounds__((64 * kHeldWaves<T, D>)) held_kernel(Attention
 // together; the scores meet in LDS.
 constexpr int kFewThreads = 1024, kFewAtOnce = kFewThreads / 8, kFewTurns = 4, kFewStates = kFewAtOnce * kFewTurns;
 constexpr int kFewRows = 4;
+constexpr float kFewUnit = 1.0f / kFewStates;
 
 template <class T, int PIECES, int R>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(Attention a, Grid g) {
@@ -409,11 +448,13 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(Attention a, Grid g) {
         for (int n = 0; n < PIECES; ++n) load_chunk<T>(p, l + 8 * n, d, q[r][n]);
     }
     float v[kFewTurns][PIECES][V];
+    int there = 0;   // which of them exist
 #pragma unroll
     for (int t = 0; t < kFewTurns; ++t) {
         const int j = t * kFewAtOnce + (int)threadIdx.x / 8;
         const int64_t at = b * a.states + min(j, states - 1);   // the loads need no branch
         const bool exists = j < states && (!a.mask || a.mask[b * a.mask_stride + j]);
+        there |= (int)exists << t;
         float k[PIECES][V], s[R];
 #pragma unroll
         for (int n = 0; n < PIECES; ++n) {
@@ -448,8 +489,9 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(Attention a, Grid g) {
         float out[PIECES][V] = {};
 #pragma unroll
         for (int t = 0; t < kFewTurns; ++t) {
-            const float s = weights[r][t * kFewAtOnce + (int)threadIdx.x / 8], w = __builtin_amdgcn_exp2f(s - from);
-            if (s == -INFINITY) continue;   // what does not exist may hold anything
+            if (!(there >> t & 1)) continue;   // what does not exist may hold anything
+            // weights of 1 and less times a power of two: the sums stay below the largest value
+            const float w = kFewUnit * __builtin_amdgcn_exp2f(weights[r][t * kFewAtOnce + (int)threadIdx.x / 8] - from);
 #pragma unroll
             for (int n = 0; n < PIECES; ++n)
 #pragma unroll
@@ -484,7 +526,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(Attention a, Grid g) {
         }
         const int64_t row = b * a.queries + r / g.shared;
         const int head = kv * g.shared + r % g.shared;
-        ((T*)a.out.p)[row * a.out.stride + (int64_t)head * d + c] = (T)(of == 0.0f ? 0.0f : x * (1.0f / of));
+        ((T*)a.out.p)[row * a.out.stride + (int64_t)head * d + c] = (T)(of == 0.0f ? 0.0f : x * (1.0f / kFewUnit / of));
         // the maximum is in the exponent's unit, of a scale that is never 0
         if (a.lse && c == 0)
             a.lse[row * a.lse_row_step + head * a.lse_head_step] =
@@ -543,6 +585,7 @@ Plan plan_of(const Attention& a) {
     p.grid.shared = a.heads / a.kv_heads;
     p.grid.rows = a.queries * p.grid.shared;
     p.grid.c = exponent_of(a.scale);
+    p.grid.lift = a.dtype == TGS_DTYPE_FLOAT16 ? fminf((float)lift_of(a.states) / p.grid.c, 0x1p126f) : 0.0f;
     p.grid.splits = 1;
     const int64_t wave_blocks = (p.grid.rows + 31) / 32;
     // where the states fit and every wave has rows; floats of wide heads need too many registers for its eight waves
