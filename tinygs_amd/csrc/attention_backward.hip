@@ -13,7 +13,8 @@
 // two last wait for LDS, whose reads (a row of q and do along and across for each 32
 // states) take as long as their products.
 //
-// Halves: p is held times 2^10, and ds times a power of two that brings the
+// Halves: p is held times 2^13 (down to 2^-27 it keeps the bits of a half; scores of
+// 2^25 and their lse, rounded to floats, leave it below 8), and ds times a power of two that brings the
 // largest it can be, |do| |v| + |delta|, to 2^14: of a row's and all states' in
 // dq, of a state's and all rows' of its element and head in dk, so that small ones
 // keep their bits, and no element's or head's gradients depend on another's.
@@ -34,7 +35,7 @@ constexpr int kWaves = 4;
 template <class T>
 constexpr float kBoost = 0.0f;   // of p, in powers of two
 template <>
-constexpr float kBoost<_Float16> = 10.0f;
+constexpr float kBoost<_Float16> = 13.0f;
 
 struct Grid {
     int64_t first;    // number of the launch's first workgroup
