@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
     const unsigned char* q0 = (const unsigned char*)a.q.p + e * a.queries * q_pitch + (int64_t)kv * g.shared * d * sizeof(T);
     const unsigned char* o0 =
         (const unsigned char*)b.grad_out.p + e * a.queries * o_pitch + (int64_t)kv * g.shared * d * sizeof(T);
-    const int64_t per_head = g.units / g.shared;
+    const int64_t per_head = max(g.units / g.shared, (int64_t)1);   // no queries: no tile of them either
     // a workgroup whose states all do not exist only writes zeros
     const int64_t t1 = __syncthreads_or(exists) ? min((split + 1) * g.part, g.units) : 0;
     // a wave whose states do not exist only loads: 2e5 rows of 4 heads of 64 floats at one state 551 us, 679 without
