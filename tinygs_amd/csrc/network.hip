@@ -252,13 +252,36 @@ int check_clip(const tgs_matrix* grads, const tgs_matrix* clipped, int32_t count
             TGS_TRY(check_shape(&clipped[i], name(x, true, i), grads[i].rows, grads[i].cols, clipped[i].dtype));
         }
     }
-    // no element counts twice, and what is written shares nothing with the rest
-    for (int32_t i = 0; i < count; ++i)
-        for (int32_t j = 0; j < count; ++j) {
-            if (j > i) TGS_TRY(check_apart(&grads[j], name(x, false, j), &grads[i], name(y, false, i)));
-            if (j > i && clipped) TGS_TRY(check_apart(&clipped[j], name(x, true, j), &clipped[i], name(y, true, i)));
-            if (clipped) TGS_TRY(check_apart(&clipped[j], name(x, true, j), &grads[i], name(y, false, i)));
+    // no element counts twice, and what is written shares nothing with the rest: in the order of their addresses, each
+    // is held against those that begin before it ends
+    struct Place {
+        const tgs_matrix* m;
+        int32_t i;
+        bool out;
+    };
+    std::vector<Place> places;
+    try {
+        places.reserve((size_t)count * 2);
+    } catch (...) {
+        return fail(TGS_ERR_STATE, "out of host memory");
+    }
+    for (int32_t i = 0; i < count; ++i) {
+        if (grads[i].rows) places.push_back({&grads[i], i, false});
+        if (clipped && clipped[i].rows) places.push_back({&clipped[i], i, true});
+    }
+    std::sort(places.begin(), places.end(),
+              [](const Place& p, const Place& q) { return (uintptr_t)p.m->data < (uintptr_t)q.m->data; });
+    for (size_t p = 0; p < places.size(); ++p) {
+        const tgs_matrix& a = *places[p].m;
+        const uintptr_t end = (uintptr_t)a.data + (uintptr_t)(((a.rows - 1) * a.stride + a.cols) * element_size(a.dtype));
+        for (size_t q = p + 1; q < places.size() && (uintptr_t)places[q].m->data < end; ++q) {
+            if (!overlap(a, *places[q].m)) continue;
+            // the output, or the later one, comes first
+            const bool turned = places[p].out == places[q].out ? places[p].i > places[q].i : places[p].out;
+            const Place &u = places[turned ? p : q], &v = places[turned ? q : p];
+            return fail(TGS_ERR_INVALID, "%s overlaps %s", name(x, u.out, u.i), name(y, v.out, v.i));
         }
+    }
     return TGS_OK;
 }
 
