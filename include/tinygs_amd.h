@@ -556,7 +556,7 @@ typedef struct tgs_attention {
     int64_t batch;         /* elements: q has batch x queries rows, k and v batch x states */
     int32_t heads;         /* of the queries; d = q's columns / heads, 1 to 128 */
     int32_t kv_heads;      /* of the states; heads is a multiple: head h reads h / (heads / kv_heads) */
-    float scale;           /* of the scores, not negative; 1 / sqrt(d) as a rule */
+    float scale;           /* of the scores, 0 to 2^127; 1 / sqrt(d) as a rule */
     const uint8_t* mask;   /* [batch, states], 0: the state does not exist; NULL: all exist */
     int64_t mask_stride;   /* bytes from an element's mask to the next one's; 0: one for all */
 } tgs_attention;

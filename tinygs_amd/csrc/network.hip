@@ -188,7 +188,8 @@ int check_attention(const tgs_matrix* q, const tgs_matrix* k, const tgs_matrix* 
     if (a->batch < 1 || q->rows % a->batch || k->rows % a->batch)
         return fail(TGS_ERR_INVALID, "a batch of %lld, %lld queries, %lld states", (long long)a->batch,
                     (long long)q->rows, (long long)k->rows);
-    if (!(a->scale >= 0.0f) || !isfinite(a->scale)) return fail(TGS_ERR_INVALID, "scale %g", a->scale);
+    // times log2 e it is still a float
+    if (!(a->scale >= 0.0f) || a->scale > 0x1p127f) return fail(TGS_ERR_INVALID, "scale %g", a->scale);
     TGS_TRY(check_shape(k, "k", k->rows, head * a->kv_heads, q->dtype));
     TGS_TRY(check_shape(v, "v", k->rows, head * a->kv_heads, q->dtype));
     const int64_t states = k->rows / a->batch;
