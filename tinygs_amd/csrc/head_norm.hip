@@ -11,6 +11,8 @@
 // An angle is a sum of up to four products in 64 bits, reduced to half a turn
 // there: at a position of 1e4 and ten radians a unit, 32 bits would leave an
 // error of 0.004. Its sine and cosine are then of a float within half a turn.
+#include <type_traits>
+
 #include "row_chunks.h"
 
 namespace tgs {
@@ -94,6 +96,27 @@ __device__ __forceinline__ void unpack(const typename ChunkOf<T>::type& u, int l
     for (int i = 0; i < kChunk<T>; ++i) v[i] = !WHOLE || lane * kChunk<T> < d ? (float)u[i] : 0.0f;
 }
 
+// The power of two by which a head's elements and epsilon are multiplied where the squares' sum leaves the range of
+// floats or its bits: elements above 2^60, and below 2^-40 where epsilon is below 2^-80. 1 else. Halves hold neither.
+template <class T>
+constexpr bool kLifted = !std::is_same_v<T, _Float16>;
+__device__ __forceinline__ float lift_of(float sum, float eps) {
+    return !(sum <= 0x1p120f) ? 0x1p-70f : sum < 0x1p-80f && eps < 0x1p-80f ? 0x1p100f : 1.0f;
+}
+// 1 / sqrt(mean(x^2) + epsilon) of such heads, whose elements are multiplied; the others' as they are.
+template <int LANES, int V>
+__device__ __forceinline__ float lifted_rstd(float (&v)[V], float by, float eps, float inv) {
+    float sum[1] = {0.0f};
+    int none = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        v[i] *= by;
+        sum[0] = fmaf(v[i], v[i], sum[0]);
+    }
+    group_sum<LANES>(sum, nullptr, none);
+    return 1.0f / sqrtf(fmaf(sum[0], inv, eps * by * by));
+}
+
 template <class T, int LANES, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) forward_kernel(HeadNorm a) {
     constexpr int V = kChunk<T>, kRows = kThreads / LANES;
@@ -121,7 +144,11 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(HeadNorm a) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[0] = fmaf(v[i], v[i], sum[0]);
                 group_sum<LANES>(sum, nullptr, none);
-                const float rstd = 1.0f / sqrtf(fmaf(sum[0], inv, a.eps));
+                float rstd = 1.0f / sqrtf(fmaf(sum[0], inv, a.eps));
+                if constexpr (kLifted<T>) {
+                    const float by = lift_of(sum[0], a.eps);
+                    if (__builtin_expect(__ballot(by != 1.0f) != 0, 0)) rstd = lifted_rstd<LANES>(v, by, a.eps, inv);
+                }
 #pragma unroll
                 for (int i = 0; i < V; ++i) v[i] = v[i] * rstd * gamma[i];
                 turn.template apply<1>(v);
@@ -150,6 +177,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(HeadNorm a, float* p
         T* gx = a.y.p ? (T*)a.y.p + r * a.y.stride : nullptr;
         for (int h0 = 0; h0 < a.heads; h0 += kHeads) {
             typename ChunkOf<T>::type rx[kHeads], rg[kHeads];
+            bool lifted[kHeads] = {};
 #pragma unroll
             for (int k = 0; k < kHeads; ++k) {
                 const int64_t at = (int64_t)min(h0 + k, a.heads - 1) * d;
@@ -170,7 +198,11 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(HeadNorm a, float* p
                     sum[1] = fmaf(g[i] * gamma[i], v[i], sum[1]);
                 }
                 group_sum<LANES>(sum, nullptr, none);
-                const float rstd = 1.0f / sqrtf(fmaf(sum[0], inv, a.eps));
+                float rstd = 1.0f / sqrtf(fmaf(sum[0], inv, a.eps));
+                if constexpr (kLifted<T>) {   // such a head waits: it adds nothing here
+                    lifted[k] = lift_of(sum[0], a.eps) != 1.0f;
+                    rstd = lifted[k] ? 0.0f : rstd;
+                }
                 const float c = sum[1] * rstd * inv;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -178,7 +210,33 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(HeadNorm a, float* p
                     if (SUMS) grad_gamma[i] = fmaf(g[i], h, grad_gamma[i]);
                     v[i] = rstd * fmaf(-h, c, g[i] * gamma[i]);
                 }
-                if (gx) store_chunk<T>(gx + (int64_t)(h0 + k) * d, lane, d, v);
+                if (gx && !(kLifted<T> && lifted[k])) store_chunk<T>(gx + (int64_t)(h0 + k) * d, lane, d, v);
+            }
+            if constexpr (!kLifted<T>) continue;
+            if (__builtin_expect(__ballot(lifted[0] || lifted[1] || lifted[2] || lifted[3]) == 0, 1)) continue;
+#pragma unroll 1
+            for (int k = 0; k < kHeads; ++k) {   // one branch for the heads, and theirs alone once more
+                if (!(k == 0 ? lifted[0] : k == 1 ? lifted[1] : k == 2 ? lifted[2] : lifted[3])) continue;
+                const int64_t at = (int64_t)(h0 + k) * d;
+                float v[V], g[V], sum[1] = {0.0f}, dot[1] = {0.0f};
+                unpack<T, WHOLE>(load_raw<T, WHOLE>(x + at, lane, d), lane, d, v);
+                unpack<T, WHOLE>(load_raw<T, WHOLE>(gy + at, lane, d), lane, d, g);
+                turn.template apply<-1>(g);
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[0] = fmaf(v[i], v[i], sum[0]);
+                group_sum<LANES>(sum, nullptr, none);
+                const float by = lift_of(sum[0], a.eps), rstd = lifted_rstd<LANES>(v, by, a.eps, inv);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    v[i] *= rstd;
+                    dot[0] = fmaf(g[i] * gamma[i], v[i], dot[0]);
+                    if (SUMS) grad_gamma[i] = fmaf(g[i], v[i], grad_gamma[i]);
+                }
+                group_sum<LANES>(dot, nullptr, none);
+                const float c = dot[0] * inv;
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = rstd * fmaf(-v[i], c, g[i] * gamma[i]) * by;
+                if (gx) store_chunk<T>(gx + at, lane, d, v);
             }
         }
     }
