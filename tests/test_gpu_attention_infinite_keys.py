@@ -31,3 +31,26 @@ def test_gradients(ops, dtype, rows, states, d):
     # column 0 of grad_q adds 0 times the infinity: NaN, as the formula says
     for h in (0, d):
         assert bool(torch.isnan(gq[:, h]).all()) and torch.equal(gq[:, h + 1:h + d], wq[:, h + 1:h + d])
+
+
+# the infinite row is the last, beside rows that a tile lacks and beside none
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows, states, d", [(70, 90, 32), (128, 90, 32), (1, 40, 64), (333, 500, 128), (70_003, 90, 64),
+                                             (70_003, 40, 32)])
+def test_infinite_gradients(ops, dtype, rows, states, d):
+    """An infinity in grad_out's last row: that column of grad_v is infinite for every state that has a weight, the others
+    are as beside a finite one; grad_k of its head is what the formula leaves of infinities, no number. 16-bit heads up to
+    32 columns hold a weight as w + r with r of either sign or 0, and an infinity times both is NaN as often."""
+    q, k, v, go = case(rows + d, dtype, 1, rows, states, 2, 2, d, q_scale=0.3)
+    print(f"[attention] infinite gradient {rows} {states} {d} {dtype}", flush=True)
+    out, lse = ops.attention(q, k, v, 2, keep_lse=True)
+    _, wk, wv = ops.attention_backward(go, q, k, v, out, lse, 2)
+    go[rows - 1, 3] = float("-inf")
+    _, gk, gv = ops.attention_backward(go, q, k, v, out, lse, 2)
+    if d <= 32 and dtype != torch.float32:
+        assert not bool(torch.isfinite(gv[:, 3]).any())
+    else:
+        assert bool((gv[:, 3] == float("-inf")).all())
+    gv[:, 3] = wv[:, 3]
+    assert torch.equal(gv, wv)
+    assert torch.equal(gk[:, d:], wk[:, d:]) and not bool(torch.isfinite(gk[:, :d]).any())

@@ -148,9 +148,10 @@ struct RowTile {
         }
     }
 
-    // The same of the first `rows` rows (1 or more), the others copies of the last: where zeros would be NaN beside an
-    // infinity of the other operand, a copy only is what that row is. pitch: as in begin. WHOLE: heads of whole chunks.
-    template <bool WHOLE>
+    // The same of the first `rows` rows (1 or more), the others zeros, or COPIES of the last: where zeros would be NaN
+    // beside an infinity of the other operand, a copy only is what that row is. pitch: as in begin. WHOLE: heads of
+    // whole chunks.
+    template <bool COPIES, bool WHOLE>
     __device__ __forceinline__ void load_first(unsigned char* lds, const unsigned char* base, int64_t end, int64_t rows,
                                                int64_t pitch, int d, int wave, int lane) const {
         const i32x4 buffer = buffer_of(base, end);
@@ -166,9 +167,10 @@ struct RowTile {
             const int slot = (n * WAVES + wave) * 64 + lane;
             const int r = slot / kChunks, c = (slot % kChunks) ^ turn(r);
             const int some = d - c * V;
-            const uint32_t at = offset[n] - (uint32_t)(max(r - last, 0) * (uint32_t)pitch);
-            if (WHOLE || some >= V || some <= 0) {
-                load_to_lds(to + (n * WAVES + wave) * 1024, some > 0 ? at : kPastEnd, buffer);
+            const bool exists = some > 0 && (COPIES || r <= last);
+            const uint32_t at = COPIES ? offset[n] - (uint32_t)max(r - last, 0) * (uint32_t)pitch : offset[n];
+            if (WHOLE || some >= V || !exists) {
+                load_to_lds(to + (n * WAVES + wave) * 1024, exists ? at : kPastEnd, buffer);
             } else {
                 const T* p = (const T*)(base + at);
                 T* q = (T*)(lds + slot * 16);

@@ -440,11 +440,12 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
         const int64_t r0 = in * QT, left = a.queries - r0;
         const int64_t at = (int64_t)h * d * (int64_t)sizeof(T);
         const int64_t width = d * (int64_t)sizeof(T);
-        // rows past the last are copies of it with an lse of +infinity: their weights are 0
-        tq.template load_first<false>(lds[buffer][0], q0 + at + r0 * q_pitch, (left - 1) * q_pitch + width, left, q_pitch,
-                                      d, wave, lane);
-        to.template load_first<false>(lds[buffer][1], o0 + at + r0 * o_pitch, (left - 1) * o_pitch + width, left, o_pitch,
-                                      d, wave, lane);
+        // rows past the last: its q, an lse of +infinity and zeros for do, so that nothing of theirs is but 0 or what
+        // its own is
+        tq.template load_first<true, false>(lds[buffer][0], q0 + at + r0 * q_pitch, (left - 1) * q_pitch + width, left,
+                                            q_pitch, d, wave, lane);
+        to.template load_first<false, false>(lds[buffer][1], o0 + at + r0 * o_pitch, (left - 1) * o_pitch + width, left,
+                                             o_pitch, d, wave, lane);
         const int64_t row = e * a.queries + r0 + of;
         const int head = kv * g.shared + h;
         if (threadIdx.x < QT)
@@ -626,10 +627,12 @@ __global__ void __launch_bounds__(64 * kOnceWaves, 2) once_kernel(AttentionBackw
         const int head = kv * g.shared + h;
         const int64_t at = (int64_t)head * d * (int64_t)sizeof(T), width = d * (int64_t)sizeof(T);
         if (wave < kLoaders) {   // rows past the last: as in grad_kv_kernel
-            tq.template load_first<true>(lds[buffer][0], (const unsigned char*)a.q.p + at + (first_row + r0) * q_pitch,
-                                         (left - 1) * q_pitch + width, left, q_pitch, d, wave, lane);
-            to.template load_first<true>(lds[buffer][1], (const unsigned char*)b.grad_out.p + at + (first_row + r0) * o_pitch,
-                                         (left - 1) * o_pitch + width, left, o_pitch, d, wave, lane);
+            const unsigned char* const from_q = (const unsigned char*)a.q.p + at + (first_row + r0) * q_pitch;
+            const unsigned char* const from_o = (const unsigned char*)b.grad_out.p + at + (first_row + r0) * o_pitch;
+            tq.template load_first<true, true>(lds[buffer][0], from_q, (left - 1) * q_pitch + width, left, q_pitch, d, wave,
+                                               lane);
+            to.template load_first<false, true>(lds[buffer][1], from_o, (left - 1) * o_pitch + width, left, o_pitch, d, wave,
+                                                lane);
         }
         // without branches, which would wait for the loads where they meet
         const int64_t x_pitch = a.out.stride * (int64_t)sizeof(T);
