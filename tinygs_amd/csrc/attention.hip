@@ -13,9 +13,16 @@
 // more of the vector instructions, and a scaling of the sums on the way, even one that is never reached,
 // made the compiler copy them all at every step.
 //
-// 2 x 8192 rows of 8 heads of 128 halves, 2 shared, at 4096 states: 252 to 283 us by
+// 16-bit weights are rounded to the values' type ahead of the second product; their
+// sum is not. An output is off by up to 1.4 times what its own rounding leaves. In two
+// parts (attention_backward.hip, kTwoParts) nothing would be added to that, at a
+// quarter more time: 1e6 x 4 x 64 bfloat16 at 256 states 511 us and 388 in one part,
+// 2 x 8192 x 8 x 128 halves at 4096 333 and 274.
+//
+// 2 x 8192 rows of 8 heads of 128 halves, 2 shared, at 4096 states: 252 to 285 us by
 // card, 0.77 PFLOP/s; wide heads with 32 rows a wave, two waves a SIMD (one wave of 64
-// rows 361).
+// rows 361). Matrix cores busy 37% of the time, vector instructions 41%, LDS 19%: the two
+// waves overlap little, and wait for LDS and the tiles' barriers 39% of theirs.
 //
 // Heads that share the states' are rows side by side, so that a tile is loaded
 // once for all of them. Where there are few rows, workgroups take parts of the
@@ -349,8 +356,8 @@ __global__ void __launch_bounds__(64 * WAVES, (D <= 64 || sizeof(T) == 2 ? 2 : 1
 // All states of a head in LDS, loaded once; the waves go over rows by themselves,
 // without a barrier, while others of the SIMD compute: four of them where a wave's
 // square of rows needs 128 registers. 1e6 rows of 4 heads of 64 bfloat16 at 256
-// states 386 us (0.68 PFLOP/s; 470 with tiles through LDS): a third of the time the
-// matrix cores are busy, two thirds the vector units, half of whose time are the
+// states 388 us (0.68 PFLOP/s; 470 with tiles through LDS): 38% of the time the
+// matrix cores are busy, 77% the vector units, half of whose time are the
 // exponentials.
 constexpr int held_waves(int size, int width) { return width <= (size == 2 ? 64 : 32) ? 16 : 8; }
 template <class T, int D>

@@ -9,9 +9,9 @@
 // in both. The scores are formed twice (seven products in place of five); in
 // one kernel, either sum would have to leave it in as many parts as there are
 // blocks of the other side. 2 x 8192 rows of 8 heads of 128 halves, 2 shared, at 4096
-// states, 2500 of them in one: 1087 to 1100 us, dq 360 to 384, dk 503, dv 400: the
-// two last wait for LDS, whose reads (a row of q and do along and across for each 32
-// states) take as long as their products.
+// states, 2500 of them in one: 1076 us, of which dq 342, dk 385, dv 320 and their
+// joins 21. Matrix cores are busy 48, 44 and 34% of the time, vector instructions 38, 40
+// and 30%, LDS 24, 30 and 22%: two waves a SIMD overlap little, and wait half of theirs.
 //
 // Halves: p is held times 2^13 (down to 2^-27 it keeps the bits of a half; scores of
 // 2^25 and their lse, rounded to floats, leave it below 8), and ds times a power of two that brings the
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(64 * kWaves, D <= 64 || sizeof(T) == 2 ? 2 : 1
 // Tiles of QT rows of one of the shared heads at a time; a wave has 32 states.
 // Both sums of wide heads would leave room for one wave a SIMD: they are formed by
 // a launch each, the scores in both (five products in place of four; 128 columns,
-// 2 x 8192 rows x 8 heads at 4096 shared states: 1018 us together).
+// 2 x 8192 rows x 8 heads at 4096 shared states: 705 us the two, 1018 in one launch).
 enum { kGradK = 1, kGradV = 2 };
 template <class T, int D>
 constexpr bool kApart = sizeof(T) == 2 && D > 64;
@@ -548,10 +548,11 @@ __global__ void __launch_bounds__(64 * kWaves, (D <= 64 || kApart<T, D> ? 2 : 1)
 // tiles of 64 rows go by. What a tile's ds is to dq needs all states: it goes to LDS
 // as [state][row], and in the next step, behind that tile's barrier, the waves share the
 // product k^T ds^T among them, 16 columns by 16 rows at a time, with k^T in registers.
-// 1e6 rows of 4 heads of 64 bfloat16 at 256 states 940 to 956 us (1356 in two kernels),
-// 0.7 PFLOP/s: products 31%, vector instructions 40% and LDS 46% of the time. The two
-// waves that a SIMD has registers for do not fill one another's waits; without its loads it takes
-// 930, without dq 800, without the exponentials 884.
+// 1e6 rows of 4 heads of 64 bfloat16 at 256 states 930 to 995 us by card (1356 in two
+// kernels), 0.7 PFLOP/s: matrix cores busy 32% of the time, vector instructions 39%,
+// LDS 38%. The two waves that a SIMD has registers for do not fill one another's waits,
+// which are half of their time: of 1004 us on one card 930 were left without its loads, 800
+// without dq, 884 without the exponentials.
 constexpr int kOnceWaves = 8, kOnceStates = 32 * kOnceWaves, kOnceRows = 64;
 
 template <class T, int D>
