@@ -11,18 +11,13 @@ from test_gpu_attention import case, forget, mask_of, ops  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 
-def sums(q, k, v, go, out, lse, heads, kv_heads, d, mask=None):
-    """For each head of the states: (columns, heads that share it, the states that exist)."""
-    there = torch.ones(k.shape[0], dtype=torch.bool, device="cuda") if mask is None else mask
-    for g in range(kv_heads):
-        yield slice(g * d, (g + 1) * d), range(g * heads // kv_heads, (g + 1) * heads // kv_heads), there
-
-
 def float64_gradients(q, k, v, go, out, lse, heads, kv_heads, d, mask=None):
     """Each (value, the sum of its terms' sizes, what dp and delta leave of their own roundings), in 64 bits on the
     device. dp and delta are sums of d products each: off by (d + 20) 2^-24 of their terms' sizes."""
     full = [torch.zeros(*t.shape, 3, dtype=torch.float64, device="cuda") for t in (q, k, v)]
-    for cols, group, there in sums(q, k, v, go, out, lse, heads, kv_heads, d, mask):
+    there = torch.ones(k.shape[0], dtype=torch.bool, device="cuda") if mask is None else mask
+    for g in range(kv_heads):
+        cols, group = slice(g * d, (g + 1) * d), range(g * heads // kv_heads, (g + 1) * heads // kv_heads)
         ke, ve = k[:, cols].double()[there], v[:, cols].double()[there]
         part = [torch.zeros(*ke.shape, 3, dtype=torch.float64, device="cuda") for _ in range(2)]
         for h in group:
