@@ -807,12 +807,16 @@ constexpr int64_t kRowTarget = 256, kRowLeast = 4, kStateTarget = 512, kStateLea
 
 // Whether the one-pass kernel takes it: states and heads that it holds, more states than one wave's, and as many rows as
 // pay for its start and its sums' join. 1e6 rows of 4 heads at 256 states, in one pass and in two kernels: of 8 913 us and
-// 1153, of 16 952 and 1227, of 32 968 and 1279, of 64 950 and 1356.
+// 1153, of 16 952 and 1227, of 32 968 and 1279, of 64 950 and 1356. Its eight waves go over all rows whatever states they
+// have, which two parts of the weights make dear: of heads up to 32, up to 128 states of many rows are left to two
+// kernels (5e5 x 4 x 32 at 33 states 494 us in one pass and 397, 2e5 x 4 x 32 at 64 190 and 171; few launches are
+// better for few rows: 70000 x 1 x 32 at 100 50 and 69, 2e4 x 4 x 8 at 40 37 and 40).
 bool at_once(const AttentionBackward& b) {
     const Attention& a = b.a;
+    const int64_t tiles = (a.queries + kOnceRows - 1) / kOnceRows * (a.heads / a.kv_heads) * a.batch * a.kv_heads;
     return a.dtype == TGS_DTYPE_BFLOAT16 && b.grad_q.p && (b.grad_k.p || b.grad_v.p) && a.head <= 64 &&
            a.head % 8 == 0 && a.states > 32 && a.states <= kOnceStates && a.batch * a.kv_heads <= 1 << 21 &&
-           (a.queries + kOnceRows - 1) / kOnceRows * (a.heads / a.kv_heads) * a.batch * a.kv_heads >= 1024;
+           tiles >= 1024 && (a.head > 32 || a.states > 128 || tiles < 4096);
 }
 
 // Rows of a tile of dk's and dv's: 64 but for wide floats (2e5 rows of 4 heads of 64 floats at 256 states 1539 us,
