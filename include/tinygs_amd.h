@@ -490,7 +490,8 @@ int tgs_convert(const void* src, int32_t src_dtype, void* dst, int32_t dst_dtype
  * products, so that infinities, NaN and the largest floats act as in float32.
  * An output may not overlap an input unless its entry says so.
  * A call reads and writes nothing after its last kernel on `stream`; it does
- * not wait for the device, except to grow the handle's workspace. The
+ * not wait for the device, except to grow the handle's workspace, of which it
+ * has one on each device that is current in a call (up to 16). The
  * workspace is shared by the calls on a handle: calls on one handle run on one
  * stream, or the caller orders them. A captured call must not grow it: run one
  * with the same sizes before capturing. A later call that grows it frees what

@@ -13,7 +13,8 @@
 using namespace tgs;
 
 struct tgs_network {
-    DevBuf workspace;
+    static constexpr int kDevices = 16;
+    DevBuf workspaces[kDevices];   // of each device that calls ran on
 };
 
 struct tgs_muon {
@@ -161,6 +162,18 @@ void bind_muon(tgs_muon* m, const tgs_matrix* weights, const tgs_matrix* grads, 
     m->on_device = false;
     m->grad_dtype = grads[0].dtype;
     m->copy_dtype = copies ? copies[0].dtype : TGS_DTYPE_FLOAT32;
+}
+
+// The current device's workspace, of `bytes` or more; NULL for none.
+int workspace_of(tgs_network* n, size_t bytes, void* stream, void*& p) {
+    p = nullptr;
+    if (!bytes) return TGS_OK;
+    int device = 0;
+    TGS_HIP(hipGetDevice(&device));
+    if (device < 0 || device >= tgs_network::kDevices) return fail(TGS_ERR_UNSUPPORTED, "device %d", device);
+    TGS_TRY(ensure(n->workspaces[device], bytes, (hipStream_t)stream));
+    p = n->workspaces[device].p;
+    return TGS_OK;
 }
 
 // out does not lie on the mask's bytes.
@@ -325,7 +338,7 @@ int tgs_network_create(tgs_network** out) {
 
 int tgs_network_destroy(tgs_network* n) {
     if (!n) return TGS_OK;
-    release(n->workspace);
+    for (DevBuf& b : n->workspaces) release(b);
     delete n;
     return TGS_OK;
 }
@@ -355,9 +368,9 @@ int tgs_linear_forward(tgs_network* n, const tgs_matrix* x, const tgs_matrix* w,
     TGS_TRY(check_apart(preact, "preact", y, "y"));
     if (x->rows == 0) return TGS_OK;
     const LinearForward a{view(x), view(w), view(residual), view(preact), view(y), bias, activation, x->dtype};
-    const size_t bytes = linear_forward_workspace(a);
-    if (bytes) TGS_TRY(ensure(n->workspace, bytes, (hipStream_t)stream));
-    return launch_linear_forward(a, n->workspace.p, (hipStream_t)stream);
+    void* workspace;
+    TGS_TRY(workspace_of(n, linear_forward_workspace(a), stream, workspace));
+    return launch_linear_forward(a, workspace, (hipStream_t)stream);
 }
 
 int tgs_linear_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_matrix* x, const tgs_matrix* w,
@@ -386,8 +399,9 @@ int tgs_linear_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_matr
     }
     const LinearBackward a{view(grad_y), view(x), view(w), activation != TGS_ACTIVATION_NONE ? view(preact) : Mat{},
                            view(grad_x), view(grad_w), grad_bias, activation, x->dtype};
-    TGS_TRY(ensure(n->workspace, linear_backward_workspace(a), (hipStream_t)stream));
-    return launch_linear_backward(a, n->workspace.p, (hipStream_t)stream);
+    void* workspace;
+    TGS_TRY(workspace_of(n, linear_backward_workspace(a), stream, workspace));
+    return launch_linear_backward(a, workspace, (hipStream_t)stream);
 }
 
 int tgs_layer_norm_forward(tgs_network* n, const tgs_matrix* x, const float* gamma, const float* beta, float epsilon,
@@ -448,8 +462,9 @@ int tgs_layer_norm_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_
         TGS_TRY(check_apart(grad_x, "grad_x", residual_grad, "residual_grad"));
     const LayerNormBackward a{view(grad_y), view(x), view(residual_grad), view(grad_x), gamma, mean, rstd,
                               grad_gamma, grad_beta, x->dtype};
-    TGS_TRY(ensure(n->workspace, layer_norm_backward_workspace(a), (hipStream_t)stream));
-    return launch_layer_norm_backward(a, n->workspace.p, (hipStream_t)stream);
+    void* workspace;
+    TGS_TRY(workspace_of(n, layer_norm_backward_workspace(a), stream, workspace));
+    return launch_layer_norm_backward(a, workspace, (hipStream_t)stream);
 }
 
 // ------------------------------------------------------------------ attention
@@ -477,9 +492,9 @@ int tgs_attention_forward(tgs_network* n, const tgs_matrix* q, const tgs_matrix*
     to.lse = lse;
     to.lse_row_step = lse_row_step;
     to.lse_head_step = lse_head_step;
-    const size_t bytes = attention_workspace(to);
-    if (bytes) TGS_TRY(ensure(n->workspace, bytes, (hipStream_t)stream));
-    return launch_attention(to, n->workspace.p, (hipStream_t)stream);
+    void* workspace;
+    TGS_TRY(workspace_of(n, attention_workspace(to), stream, workspace));
+    return launch_attention(to, workspace, (hipStream_t)stream);
 }
 
 int tgs_attention_backward(tgs_network* n, const tgs_matrix* grad_out, const tgs_matrix* q, const tgs_matrix* k,
@@ -514,9 +529,9 @@ int tgs_attention_backward(tgs_network* n, const tgs_matrix* grad_out, const tgs
     to.grad_q = view(grad_q);
     to.grad_k = view(grad_k);
     to.grad_v = view(grad_v);
-    const size_t bytes = attention_backward_workspace(to);
-    if (bytes) TGS_TRY(ensure(n->workspace, bytes, (hipStream_t)stream));
-    return launch_attention_backward(to, n->workspace.p, (hipStream_t)stream);
+    void* workspace;
+    TGS_TRY(workspace_of(n, attention_backward_workspace(to), stream, workspace));
+    return launch_attention_backward(to, workspace, (hipStream_t)stream);
 }
 
 int tgs_head_norm_forward(tgs_network* n, const tgs_matrix* x, int32_t heads, const float* gamma, const tgs_turn* turn,
@@ -562,9 +577,9 @@ int tgs_head_norm_backward(tgs_network* n, const tgs_matrix* grad_y, const tgs_m
     to.grad_y = view(grad_y);
     to.y = view(grad_x);
     to.grad_gamma = grad_gamma;
-    const size_t bytes = head_norm_backward_workspace(to);
-    if (bytes) TGS_TRY(ensure(n->workspace, bytes, (hipStream_t)stream));
-    return launch_head_norm_backward(to, n->workspace.p, (hipStream_t)stream);
+    void* workspace;
+    TGS_TRY(workspace_of(n, head_norm_backward_workspace(to), stream, workspace));
+    return launch_head_norm_backward(to, workspace, (hipStream_t)stream);
 }
 
 // ------------------------------------------------------------------ clipping
