@@ -494,8 +494,8 @@ int tgs_convert(const void* src, int32_t src_dtype, void* dst, int32_t dst_dtype
  * has one on each device that is current in a call (up to 16). The
  * workspace is shared by the calls on a handle: calls on one handle run on one
  * stream, or the caller orders them. A captured call must not grow it: run one
- * with the same sizes before capturing. A later call that grows it frees what
- * the captured ones use: larger calls go to a handle of their own, or come first. */
+ * with the same sizes before capturing. What a later call outgrows stays until the
+ * handle is destroyed, which comes after the last replay of what was captured. */
 typedef struct tgs_matrix {
     void* data;
     int64_t rows;

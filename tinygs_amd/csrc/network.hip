@@ -15,6 +15,7 @@ using namespace tgs;
 struct tgs_network {
     static constexpr int kDevices = 16;
     DevBuf workspaces[kDevices];   // of each device that calls ran on
+    std::vector<DevBuf> outgrown;  // which captured calls may still use
 };
 
 struct tgs_muon {
@@ -171,8 +172,17 @@ int workspace_of(tgs_network* n, size_t bytes, void* stream, void*& p) {
     int device = 0;
     TGS_HIP(hipGetDevice(&device));
     if (device < 0 || device >= tgs_network::kDevices) return fail(TGS_ERR_UNSUPPORTED, "device %d", device);
-    TGS_TRY(ensure(n->workspaces[device], bytes, (hipStream_t)stream));
-    p = n->workspaces[device].p;
+    DevBuf& b = n->workspaces[device];
+    if (b.p && b.bytes < bytes) {
+        try {
+            n->outgrown.push_back(b);
+        } catch (...) {
+            return fail(TGS_ERR_STATE, "out of host memory");
+        }
+        b = DevBuf{};
+    }
+    TGS_TRY(ensure(b, bytes, (hipStream_t)stream));
+    p = b.p;
     return TGS_OK;
 }
 
@@ -339,6 +349,7 @@ int tgs_network_create(tgs_network** out) {
 int tgs_network_destroy(tgs_network* n) {
     if (!n) return TGS_OK;
     for (DevBuf& b : n->workspaces) release(b);
+    for (DevBuf& b : n->outgrown) release(b);
     delete n;
     return TGS_OK;
 }
