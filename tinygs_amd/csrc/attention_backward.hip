@@ -14,10 +14,10 @@
 // and 30%, LDS 24, 30 and 22%: two waves a SIMD overlap little, and wait half of theirs.
 //
 // Halves: p is held times 2^13 (down to 2^-27 it keeps the bits of a half; scores of
-// 2^25 and their lse, rounded to floats, leave it below 8), and ds times a power of two that brings the
-// largest it can be, |do| |v| + |delta|, to 2^14: of a row's and all states' in
-// dq, of a state's and all rows' of its element and head in dk, so that small ones
-// keep their bits, and no element's or head's gradients depend on another's.
+// 2^25 and their lse, rounded to floats, leave it below 8), and ds times a power of
+// two that brings the largest it can be, |do| |v| + |delta|, to 2^14: of a row's and
+// all states' in dq, of a state's and all rows' of its element and head in dk, so that
+// small ones keep their bits, and no element's or head's gradients depend on another's.
 #include <math.h>
 
 #include <algorithm>
