@@ -54,3 +54,18 @@ def test_infinite_gradients(ops, dtype, rows, states, d):
     gv[:, 3] = wv[:, 3]
     assert torch.equal(gv, wv)
     assert torch.equal(gk[:, d:], wk[:, d:]) and not bool(torch.isfinite(gk[:, :d]).any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rows, states, d", [(1, 70, 64), (70, 90, 32), (60_000, 200, 64), (20_000, 700, 128), (20, 5000, 96)])
+def test_infinite_values(ops, dtype, rows, states, d):
+    """An infinite value of a state that has a weight makes that column of every average infinite, and no other."""
+    q, k, v, _ = case(rows, dtype, 1, rows, states, 2, 2, d, q_scale=0.3)
+    print(f"[attention] infinite value {rows} {states} {d} {dtype}", flush=True)
+    want = ops.attention(q, k, v, 2)
+    v[states // 2, d + 3] = float("inf")
+    v[3, 2] = float("-inf")
+    got = ops.attention(q, k, v, 2)
+    assert bool((got[:, d + 3] == float("inf")).all()) and bool((got[:, 2] == float("-inf")).all())
+    got[:, d + 3], got[:, 2] = want[:, d + 3], want[:, 2]
+    assert torch.equal(got, want)

@@ -16,8 +16,9 @@
 // 16-bit weights are rounded to the values' type ahead of the second product; their
 // sum is not. An output is off by up to 1.4 times what its own rounding leaves. In two
 // parts (attention_backward.hip, kTwoParts) nothing would be added to that, at a
-// quarter more time: 1e6 x 4 x 64 bfloat16 at 256 states 511 us and 388 in one part,
-// 2 x 8192 x 8 x 128 halves at 4096 333 and 274.
+// quarter more time (1e6 x 4 x 64 bfloat16 at 256 states 511 us and 388 in one part,
+// 2 x 8192 x 8 x 128 halves at 4096 333 and 274), and an infinite value would meet a
+// second part of either sign, or 0: NaN, where its average is infinite.
 //
 // 2 x 8192 rows of 8 heads of 128 halves, 2 shared, at 4096 states: 252 to 285 us by
 // card, 0.77 PFLOP/s; wide heads with 32 rows a wave, two waves a SIMD (one wave of 64
